@@ -75,7 +75,8 @@ int vqm_device_bytes(vqm_runtime *rt, size_t *out);
 /* tensor_info(name) - qwen_runtime.cu:1458-1471 */
 int vqm_tensor_info(vqm_runtime *rt, const char *name, vqm_tensor_info_t *out);
 
-/* alloc(name, n[, elem]) - qwen_runtime.cu:1616-1650: zero-filled buffer of n elements of 4 (fp32) or 2 bytes. */
+/* alloc(name, n[, elem]) - qwen_runtime.cu:1616-1650: zero-filled buffer of n elements of 4 (fp32), 2 (fp16)
+ * or 1 (int8) bytes. */
 int vqm_alloc(vqm_runtime *rt, const char *name, size_t n, int elem);
 /* Registers caller-owned device memory under a buffer name (the runtime will not free it).  Lets a second
  * runtime or a torch tensor share memory, the use the reference makes of buffer_ptr (qwen_runtime.cu:1473-1483). */
@@ -144,6 +145,53 @@ int vqm_set_argmax_row_base(vqm_runtime *rt, const char *weight, int row_base);
  * exposes the block decoders the matvec uses so that they can be checked bit for bit against the
  * reference dequantiser (engine/src/vinf/gguf/dequant.py:17-57). */
 int vqm_dequantize(vqm_runtime *rt, const char *weight, const char *out);
+
+/* ---- Passes in 8-bit integers (no counterpart in the reference) ----
+ * A weight tensor of 8-bit integer rows holds W[r][k] = scales[r] * w[r][k], w int8; activations are int8 rows with one fp32 scale
+ * per row.  Rows of 8-bit values lie `pitch` bytes apart, a multiple of 16: activations at round_up(cols, 16).  1 <= cols <= 131071 (with
+ * more a 32-bit sum could overflow).  Buffers of 8-bit values are allocated or bound with elem = 1.  has / free / tensor_info
+ * (type VQM_I8_ROWS, row_bytes = pitch) / device_bytes know these tensors; the matvec entry points refuse them (VQM_ERR_VALUE).
+ *
+ * vqm_upload_i8   w: rows * cols int8 in host memory, densely packed; scales: rows floats.  Synchronous; re-upload replaces.
+ * vqm_bind_i8     the same in device memory that the caller keeps: 16-byte aligned, `pitch` bytes from row to row (0: round_up(cols, 16));
+ *                 what lies behind a row's last column is ignored.
+ * vqm_convert_i8  makes the tensor `name` from any GGUF tensor: scales[r] = max |row r| / 127, values to the nearest integer.  Synchronous.
+ */
+#define VQM_I8_ROWS 24
+int vqm_upload_i8(vqm_runtime *rt, const char *name, const void *data, size_t nbytes, const float *scales, size_t scale_bytes, int cols, int rows);
+int vqm_bind_i8(vqm_runtime *rt, const char *name, const void *device_ptr, size_t pitch, const float *scales, int cols, int rows);
+int vqm_convert_i8(vqm_runtime *rt, const char *weight, const char *name);
+/* Activation rows as 8-bit integers: x [ntok][cols] (fp32 or fp16 buffer) -> q (int8 buffer, ntok * round_up(cols, 16) bytes, zeros behind the
+ * last column) and scales (fp32 buffer, ntok).  Asynchronous.  Per row
+ *   v = x;  VQM_FUSE_SILU_MUL: v = silu(x) * x2;  VQM_FUSE_ADD: v = x + residual, rounded to the buffers' type and stored in `total` (a buffer
+ *   that may be x or residual; NULL: residual);
+ *   VQM_FUSE_NORM: n = v * rsqrt(mean(v^2) + eps) * norm_weight (an fp32 buffer or F32 tensor of cols values), else n = v;
+ *   scale = max |n| / 127 in fp32, q = n / scale to the nearest integer, ties to even, as the exact values of n and the stored scale have it.
+ * A row of zeros has scale 0 and q = 0.  A row with an infinite or undefined n, or whose scale is beyond fp32, has an undefined (NaN)
+ * scale and q = 0, which makes its products undefined.  x, x2, residual and total share one type.  Buffers do not overlap otherwise. */
+int vqm_rows_i8(vqm_runtime *rt, const char *x, const char *q, const char *scales, int cols, int ntok, int flags, const char *x2, const char *residual,
+                const char *total, const char *norm_weight, float eps);
+/* y[t][r] = scales[t] * W scales[r] * sum_k q[t][k] w[r][k] (VQM_FUSE_ADD: +=) for a tensor of 8-bit integer rows; sums are exact, y is an fp32 or
+ * fp16 buffer.  Asynchronous; any ntok >= 1. */
+int vqm_qmm_i8(vqm_runtime *rt, const char *weight, const char *q, const char *scales, const char *y, int ntok, int flags);
+
+/* Verification of drafted tokens against the target's probabilities (no counterpart in the reference, whose speculative decoder compares greedy
+ * tokens on the host).  Per sequence: logits of the target at `drafts` + 1 positions, target [seqs][drafts + 1][vocab]; the drafted
+ * tokens [seqs][drafts] (int32 in a buffer of 4-byte elements) with the logits they were drawn from, draft [seqs][drafts][vocab] (NULL: drafts
+ * without probabilities, q = 1 at the token); random numbers from [0, 1), uniforms [seqs][drafts + 1].  Optional: lens [seqs] (int32), how many
+ * of a sequence's drafts count (clamped to 0..drafts; the target's row lens[s] is the one behind them); temperature [seqs] (NULL: 1).
+ *   p = softmax(target / T), q = softmax(draft / T); draft i is accepted if u[i] q(token) < p(token), up to the first that is not;
+ *   the next token is the smallest one up to which the sum of r = max(p - q, 0) at the refused draft (behind the last draft: r = p) is above
+ *   u[drafts] times r's whole sum.  So the tokens are distributed as p.  T <= 0 (or NaN): p and q are 1 at their rows' largest logit, the
+ *   lowest index on ties: greedy verification.
+ * Decisions are those of 64-bit arithmetic.  Logits of -inf and NaN have no probability; a row without any refuses its draft, and the
+ * token drawn from such a row is -1.  A token outside [0, vocab) is refused, and where drafts have no probabilities nothing is taken off p then.
+ * out [seqs][drafts + 2] (int32): the number of accepted drafts a, the accepted tokens, the next token, then -1.  out_host (seqs * (drafts + 2)
+ * ints) may be NULL: then the call is asynchronous.  target and draft are both fp32 or both fp16.  drafts = 0 samples from the target.
+ * 0 <= drafts <= VQM_MAX_DRAFTS. */
+#define VQM_MAX_DRAFTS 255
+int vqm_verify(vqm_runtime *rt, const char *target, const char *draft, const char *tokens, const char *lens, const char *uniforms, const char *temperature,
+               int vocab, int seqs, int drafts, const char *out, int *out_host);
 
 /* set_gemm_min_rows(n) - qwen_runtime.cu:2324-2330: passes of n or more activation rows take the tensor-core GEMM
  * (fp16 operands, fp32 accumulation, like the reference's prompt kernel); 0 = never, every pass is fp32 matvecs. */

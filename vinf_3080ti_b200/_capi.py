@@ -60,6 +60,12 @@ SIGNATURES: dict[str, list] = {
     "vqm_argmax_fetch": [c_void_p, c_int, POINTER(c_int), POINTER(ctypes.c_float)],
     "vqm_set_argmax_row_base": [c_void_p, c_char_p, c_int],
     "vqm_dequantize": [c_void_p, c_char_p, c_char_p],
+    "vqm_upload_i8": [c_void_p, c_char_p, c_void_p, c_size_t, c_void_p, c_size_t, c_int, c_int],
+    "vqm_bind_i8": [c_void_p, c_char_p, c_void_p, c_size_t, c_void_p, c_int, c_int],
+    "vqm_convert_i8": [c_void_p, c_char_p, c_char_p],
+    "vqm_rows_i8": [c_void_p, c_char_p, c_char_p, c_char_p, c_int, c_int, c_int, c_char_p, c_char_p, c_char_p, c_char_p, ctypes.c_float],
+    "vqm_qmm_i8": [c_void_p, c_char_p, c_char_p, c_char_p, c_char_p, c_int, c_int],
+    "vqm_verify": [c_void_p, c_char_p, c_char_p, c_char_p, c_char_p, c_char_p, c_char_p, c_int, c_int, c_int, c_char_p, POINTER(c_int)],
     "vqm_set_gemm_min_rows": [c_void_p, c_int],
     "vqm_synchronize": [c_void_p],
     "vqm_mem_info": [POINTER(c_size_t), POINTER(c_size_t)],

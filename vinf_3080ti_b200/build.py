@@ -115,6 +115,9 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False, d
     work += [("vqm_tcmv_type.cu", [f"-DVQM_TYPE={tid}", f"-DVQM_TYPE_NAME={tname}"], OBJ / f"tcmv_{tname}.o") for tid, tname in TC_TYPES]
     work.append(("vqm_tcmv_maps.cu", [], OBJ / "tcmv_maps.o"))
     work.append(("vqm_aux.cu", [], OBJ / "aux.o"))
+    work.append(("vqm_rows_i8.cu", [], OBJ / "rows_i8.o"))
+    work.append(("vqm_qmm_i8.cu", [], OBJ / "qmm_i8.o"))
+    work.append(("vqm_verify.cu", [], OBJ / "verify.o"))
     work.append(("vqm_probe.cu", [], OBJ / "probe.o"))
     work.append(("vqm_gemm.cu", [], OBJ / "gemm.o"))
     work.append(("vqm_gemm_tc5.cu", [], OBJ / "gemm_tc5.o"))

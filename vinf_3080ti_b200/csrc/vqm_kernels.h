@@ -167,6 +167,51 @@ cudaError_t launch_qgemm_tc5(int type, const uint8_t *w, const void *xh, float *
 
 // n16 16-byte words from pinned host memory
 cudaError_t launch_fetch(const void *from, void *to, int n16, cudaStream_t stream);
+
+// ---- 8-bit integer passes (vqm_rows_i8.cu, vqm_qmm_i8.cu) and the verification of drafted tokens (vqm_verify.cu) ----
+
+constexpr int kI8Rows = 24;          // type id of a weight tensor of 8-bit integer rows with a scale each (VQM_I8_ROWS)
+constexpr int kI8MaxCols = 131071;   // (2^17 - 1) * 2^14 still fits into a 32-bit sum
+__host__ __device__ constexpr long long i8_pitch(int cols) { return (static_cast<long long>(cols) + 15) / 16 * 16; }  // bytes from one row of 8-bit values to the next
+
+struct RowsI8Args {
+    const void *x;         // [ntok][cols] of `elem` bytes
+    const void *x2;        // the values are silu(x) * x2; or null
+    const void *residual;  // the values are x + residual, and go to `total` as well (which may be either of them); or null
+    void *total;
+    const float *norm_w;   // rmsnorm over the columns times these; or null
+    int8_t *q;             // [ntok][i8_pitch(cols)], zeros behind the last column
+    float *scales;         // [ntok]
+    int cols, ntok, elem;
+    float eps;
+};
+cudaError_t launch_rows_i8(const RowsI8Args &a, cudaStream_t stream);
+
+struct QmmI8Args {
+    const int8_t *w;       // [rows][w_pitch], 16-byte aligned, w_pitch a multiple of 16
+    const float *w_scales;
+    const int8_t *q;       // [ntok][i8_pitch(cols)]
+    const float *q_scales;
+    void *y;               // [ntok][rows] of y_elem bytes
+    long long w_pitch;
+    int rows, cols, ntok, y_elem;
+    bool add;              // y += instead of y =
+    unsigned *status;      // device word that receives a code if a bounded wait expires
+};
+cudaError_t launch_qmm_i8(const QmmI8Args &a, int sm_count, cudaStream_t stream);
+
+struct VerifyArgs {
+    const void *target;        // [seqs][drafts + 1][vocab] of `elem` bytes
+    const void *draft;         // [seqs][drafts][vocab], or null: the drafts have no probabilities of their own
+    const int *tokens;         // [seqs][drafts]
+    const int *lens;           // [seqs] drafts of each sequence; or null: all
+    const float *uniforms;     // [seqs][drafts + 1]
+    const float *temperature;  // [seqs]; or null: 1
+    int *out;                  // [seqs][drafts + 2]
+    int vocab, seqs, drafts, elem;
+};
+cudaError_t launch_verify(const VerifyArgs &a, int sm_count, cudaStream_t stream);
+
 cudaError_t launch_argmax_rows(const float *x, int n, int ntok, int *out, cudaStream_t stream);
 cudaError_t launch_dequant(int type, const uint8_t *w, float *out, long long numel, const uint8_t *codebook,
                            cudaStream_t stream);

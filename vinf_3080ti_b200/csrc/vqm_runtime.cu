@@ -15,7 +15,9 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
+#include <new>
 #include <string>
 #include <thread>
 #include <unordered_map>
@@ -53,6 +55,7 @@ struct Tensor {
     bool owned = true;
     bool mapped = false;
     CUtensorMap maps[8];  // of the tensor-core matvec, if `mapped`
+    const float *scales = nullptr;  // of 8-bit integer rows (kI8Rows), else null
 };
 
 struct Buffer {
@@ -162,13 +165,31 @@ bool codebook_fits(const vqm_runtime *rt, int type) {
     return false;
 }
 
-Tensor *find_tensor(vqm_runtime *rt, const char *name, int *status) {
+Tensor *find_any_tensor(vqm_runtime *rt, const char *name, int *status) {
     auto it = rt->tensors.find(name);
     if (it == rt->tensors.end()) {
         *status = fail(VQM_ERR_KEY, "weight tensor %s is not loaded", name);
         return nullptr;
     }
     return &it->second;
+}
+// A tensor of GGUF blocks ...
+Tensor *find_tensor(vqm_runtime *rt, const char *name, int *status) {
+    Tensor *t = find_any_tensor(rt, name, status);
+    if (t != nullptr && t->type == vqm::kI8Rows) {
+        *status = fail(VQM_ERR_VALUE, "weight tensor %s holds 8-bit integer rows (qmm_i8 multiplies by those)", name);
+        return nullptr;
+    }
+    return t;
+}
+// ... and one of 8-bit integer rows.
+Tensor *find_i8_tensor(vqm_runtime *rt, const char *name, int *status) {
+    Tensor *t = find_any_tensor(rt, name, status);
+    if (t != nullptr && t->type != vqm::kI8Rows) {
+        *status = fail(VQM_ERR_VALUE, "weight tensor %s holds GGUF blocks, not 8-bit integer rows (convert_i8 makes those)", name);
+        return nullptr;
+    }
+    return t;
 }
 
 Buffer *find_any_buffer(vqm_runtime *rt, const char *name, int *status) {
@@ -185,7 +206,7 @@ float *find_f32(vqm_runtime *rt, const char *name, size_t min_n, int *status) {
     Buffer *b = find_any_buffer(rt, name, status);
     if (b == nullptr) return nullptr;
     if (b->elem != 4) {
-        *status = fail(VQM_ERR_TYPE, "device buffer %s is fp16 (KV cache), not fp32", name);
+        *status = fail(VQM_ERR_TYPE, b->elem == 1 ? "device buffer %s is int8, not fp32" : "device buffer %s is fp16 (KV cache), not fp32", name);
         return nullptr;
     }
     if (b->n < min_n) {
@@ -193,6 +214,34 @@ float *find_f32(vqm_runtime *rt, const char *name, size_t min_n, int *status) {
         return nullptr;
     }
     return static_cast<float *>(b->data);
+}
+// fp32 or fp16 buffer; *elem: the bytes it must have per element, 0: any, which becomes what it has
+void *find_real(vqm_runtime *rt, const char *name, size_t min_n, int *elem, int *status) {
+    Buffer *b = find_any_buffer(rt, name, status);
+    if (b == nullptr) return nullptr;
+    if (b->elem == 1 || (*elem != 0 && b->elem != *elem)) {
+        *status = fail(VQM_ERR_TYPE, "device buffer %s has %d-byte elements, need %s", name, b->elem, *elem == 0 ? "fp32 or fp16" : *elem == 4 ? "fp32" : "fp16");
+        return nullptr;
+    }
+    if (b->n < min_n) {
+        *status = fail(VQM_ERR_VALUE, "device buffer %s has %zu elements, need %zu", name, b->n, min_n);
+        return nullptr;
+    }
+    *elem = b->elem;
+    return b->data;
+}
+int8_t *find_i8(vqm_runtime *rt, const char *name, size_t min_n, int *status) {
+    Buffer *b = find_any_buffer(rt, name, status);
+    if (b == nullptr) return nullptr;
+    if (b->elem != 1) {
+        *status = fail(VQM_ERR_TYPE, "device buffer %s is not int8", name);
+        return nullptr;
+    }
+    if (b->n < min_n) {
+        *status = fail(VQM_ERR_VALUE, "device buffer %s has %zu bytes, need %zu", name, b->n, min_n);
+        return nullptr;
+    }
+    return static_cast<int8_t *>(b->data);
 }
 
 void release(Tensor &t) {
@@ -1031,7 +1080,7 @@ int vqm_device_bytes(vqm_runtime *rt, size_t *out) {
 
 int vqm_tensor_info(vqm_runtime *rt, const char *name, vqm_tensor_info_t *out) {
     int rc = VQM_OK;
-    Tensor *t = find_tensor(rt, name, &rc);
+    Tensor *t = find_any_tensor(rt, name, &rc);
     if (t == nullptr) return rc;
     out->addr = reinterpret_cast<uintptr_t>(t->data);
     out->type = t->type;
@@ -1045,7 +1094,7 @@ int vqm_tensor_info(vqm_runtime *rt, const char *name, vqm_tensor_info_t *out) {
 
 int vqm_alloc(vqm_runtime *rt, const char *name, size_t n, int elem) {
     if (n == 0 || n > (static_cast<size_t>(1) << 62)) return fail(VQM_ERR_VALUE, "buffer %s size must be positive", name);
-    if (elem != 4 && elem != 2) return fail(VQM_ERR_VALUE, "element size must be 4 (fp32) or 2 (fp16)");
+    if (elem != 4 && elem != 2 && elem != 1) return fail(VQM_ERR_VALUE, "element size must be 4 (fp32), 2 (fp16) or 1 (int8)");
     const int rc = no_capture(rt, "alloc");
     if (rc != VQM_OK) return rc;
     auto it = rt->buffers.find(name);
@@ -1070,7 +1119,7 @@ int vqm_alloc(vqm_runtime *rt, const char *name, size_t n, int elem) {
 
 int vqm_bind(vqm_runtime *rt, const char *name, void *device_ptr, size_t n, int elem) {
     if (n == 0) return fail(VQM_ERR_VALUE, "buffer %s size must be positive", name);
-    if (elem != 4 && elem != 2) return fail(VQM_ERR_VALUE, "element size must be 4 (fp32) or 2 (fp16)");
+    if (elem != 4 && elem != 2 && elem != 1) return fail(VQM_ERR_VALUE, "element size must be 4 (fp32), 2 (fp16) or 1 (int8)");
     if (device_ptr == nullptr || (reinterpret_cast<uintptr_t>(device_ptr) & 15u) != 0)
         return fail(VQM_ERR_VALUE, "%s: device pointer must be 16-byte aligned", name);
     auto it = rt->buffers.find(name);
@@ -1359,6 +1408,7 @@ int vqm_matvec(vqm_runtime *rt, const char *weight, const float *x_host, size_t 
     auto it = rt->tensors.find(weight);
     if (it == rt->tensors.end()) return fail(VQM_ERR_KEY, "%s is not resident on the GPU", weight);
     Tensor &t = it->second;
+    if (t.type == vqm::kI8Rows) return fail(VQM_ERR_VALUE, "weight tensor %s holds 8-bit integer rows (qmm_i8 multiplies by those)", weight);
     if (x_bytes != static_cast<size_t>(t.cols) * sizeof(float))
         return fail(VQM_ERR_VALUE, "%s: x has %zu bytes, expected %d float32", weight, x_bytes, t.cols);
     if (y_bytes < static_cast<size_t>(t.rows) * sizeof(float))
@@ -1427,6 +1477,267 @@ int vqm_dequantize(vqm_runtime *rt, const char *weight, const char *out) {
     if (err != cudaSuccess) return cuda_fail("dequantize launch", err);
     count_launch(rt);
     return VQM_OK;
+}
+
+}  // extern "C"
+// ---- 8-bit integer passes and the verification of drafted tokens ---------------------------------------------
+
+namespace {
+
+// What every entry point below begins with: names that must be there, the device, and no C++ exception past the C boundary.
+template <typename F>
+int entry(vqm_runtime *rt, std::initializer_list<const char *> names, F &&body) {
+    if (rt == nullptr) return fail(VQM_ERR_VALUE, "the runtime must not be NULL");
+    for (const char *name : names)
+        if (name == nullptr) return fail(VQM_ERR_VALUE, "a name must not be NULL");
+    int dev = -1;
+    if (const cudaError_t err = cudaGetDevice(&dev); err != cudaSuccess) return cuda_fail("cudaGetDevice", err);
+    if (dev != rt->device) return fail(VQM_ERR_VALUE, "the runtime is on device %d, the current device is %d", rt->device, dev);
+    try {
+        return body();
+    } catch (const std::bad_alloc &) {
+        return fail(VQM_ERR_MEMORY, "out of host memory");
+    } catch (const std::exception &e) {
+        return fail(VQM_ERR_VALUE, "%s", e.what());
+    }
+}
+
+int check_i8_shape(const char *name, int cols, int rows) {
+    if (cols < 1 || rows < 1) return fail(VQM_ERR_VALUE, "%s: rows and columns must be positive", name);
+    if (cols > vqm::kI8MaxCols) return fail(VQM_ERR_VALUE, "%s: 8-bit integer rows have at most %d columns (32-bit sums)", name, vqm::kI8MaxCols);
+    return VQM_OK;
+}
+
+void put_tensor(vqm_runtime *rt, const char *name, const Tensor &t) {
+    auto it = rt->tensors.find(name);
+    if (it != rt->tensors.end()) {
+        cudaStreamSynchronize(rt->stream);
+        release(it->second);
+        rt->tensors.erase(it);
+    }
+    rt->tensors[name] = t;
+}
+
+// Rows of i8_pitch(cols) bytes, zeros behind their last columns, and behind them the scales.
+cudaError_t alloc_i8(Tensor &t, int cols, int rows) {
+    const size_t pitch = static_cast<size_t>(vqm::i8_pitch(cols)), values = pitch * static_cast<size_t>(rows), at = (values + 255) / 256 * 256;
+    const cudaError_t err = cudaMalloc(&t.data, at + sizeof(float) * static_cast<size_t>(rows));
+    if (err != cudaSuccess) {
+        t.data = nullptr;
+        return err;
+    }
+    t.scales = reinterpret_cast<const float *>(t.data + at);
+    t.type = vqm::kI8Rows;
+    t.rows = rows;
+    t.cols = cols;
+    t.row_bytes = pitch;
+    t.nbytes = values + sizeof(float) * static_cast<size_t>(rows);
+    return cudaSuccess;
+}
+
+// The norm weights of `cols` columns: an fp32 buffer, or an F32 tensor.
+const float *find_norm(vqm_runtime *rt, const char *name, int cols, int *status) {
+    auto wt = rt->tensors.find(name);
+    if (wt == rt->tensors.end()) return find_f32(rt, name, static_cast<size_t>(cols), status);
+    if (wt->second.type != vqm::kF32 || static_cast<long long>(wt->second.rows) * wt->second.cols != cols) {
+        *status = fail(VQM_ERR_VALUE, "%s: norm weights must be F32 with %d elements", name, cols);
+        return nullptr;
+    }
+    return reinterpret_cast<const float *>(wt->second.data);
+}
+
+}  // namespace
+
+extern "C" {
+
+int vqm_upload_i8(vqm_runtime *rt, const char *name, const void *data, size_t nbytes, const float *scales, size_t scale_bytes, int cols, int rows) {
+    return entry(rt, {name}, [&]() -> int {
+        int rc = check_i8_shape(name, cols, rows);
+        if (rc != VQM_OK) return rc;
+        const size_t want = static_cast<size_t>(cols) * rows;
+        if (data == nullptr || nbytes != want) return fail(VQM_ERR_VALUE, "%s: got %zu bytes, expected %zu", name, data == nullptr ? size_t{0} : nbytes, want);
+        if (scales == nullptr || scale_bytes != sizeof(float) * static_cast<size_t>(rows))
+            return fail(VQM_ERR_VALUE, "%s: got %zu bytes of scales, expected %zu", name, scales == nullptr ? size_t{0} : scale_bytes, sizeof(float) * static_cast<size_t>(rows));
+        if ((rc = no_capture(rt, "upload_i8")) != VQM_OK) return rc;
+        Tensor t;
+        cudaError_t err = alloc_i8(t, cols, rows);
+        if (err == cudaSuccess && t.row_bytes != static_cast<size_t>(cols)) err = cudaMemset(t.data, 0, t.row_bytes * rows);
+        if (err == cudaSuccess) err = cudaMemcpy2D(t.data, t.row_bytes, data, cols, cols, rows, cudaMemcpyHostToDevice);
+        if (err == cudaSuccess) err = cudaMemcpy(const_cast<float *>(t.scales), scales, scale_bytes, cudaMemcpyHostToDevice);
+        if (err != cudaSuccess) {
+            release(t);
+            return cuda_fail("upload_i8", err);
+        }
+        put_tensor(rt, name, t);
+        return VQM_OK;
+    });
+}
+
+int vqm_bind_i8(vqm_runtime *rt, const char *name, const void *device_ptr, size_t pitch, const float *scales, int cols, int rows) {
+    return entry(rt, {name}, [&]() -> int {
+        const int rc = check_i8_shape(name, cols, rows);
+        if (rc != VQM_OK) return rc;
+        if (device_ptr == nullptr || (reinterpret_cast<uintptr_t>(device_ptr) & 15u) != 0)
+            return fail(VQM_ERR_VALUE, "%s: device pointer must be 16-byte aligned", name);
+        if (scales == nullptr || (reinterpret_cast<uintptr_t>(scales) & 3u) != 0)
+            return fail(VQM_ERR_VALUE, "%s: the scales' device pointer must be 4-byte aligned", name);
+        if (pitch == 0) pitch = static_cast<size_t>(vqm::i8_pitch(cols));
+        if (pitch % 16 != 0 || pitch < static_cast<size_t>(cols) || pitch >= (static_cast<size_t>(1) << 40))
+            return fail(VQM_ERR_VALUE, "%s: the rows' pitch must be a multiple of 16 bytes and no less than the columns", name);
+        Tensor t;
+        t.data = const_cast<uint8_t *>(static_cast<const uint8_t *>(device_ptr));
+        t.owned = false;
+        t.scales = scales;
+        t.type = vqm::kI8Rows;
+        t.rows = rows;
+        t.cols = cols;
+        t.row_bytes = pitch;
+        t.nbytes = pitch * static_cast<size_t>(rows) + sizeof(float) * static_cast<size_t>(rows);
+        put_tensor(rt, name, t);
+        return VQM_OK;
+    });
+}
+
+int vqm_convert_i8(vqm_runtime *rt, const char *weight, const char *name) {
+    return entry(rt, {weight, name}, [&]() -> int {
+        int rc = VQM_OK;
+        Tensor *from = find_tensor(rt, weight, &rc);
+        if (from == nullptr) return rc;
+        if ((rc = check_i8_shape(weight, from->cols, from->rows)) != VQM_OK) return rc;
+        const size_t numel = static_cast<size_t>(from->rows) * from->cols;
+        if (numel % 8 != 0) return fail(VQM_ERR_VALUE, "%s: element count must be a multiple of 8", weight);
+        const uint8_t *cb = codebook_for(rt, from->type);
+        if (vqm::grid_is_codebook(from->type) && cb == nullptr)
+            return fail(VQM_ERR_VALUE, "the codebook for GGUF type %d has not been set (vqm_set_codebook)", from->type);
+        if ((rc = no_capture(rt, "convert_i8")) != VQM_OK) return rc;
+        // a part of the rows at a time, a multiple of 8 of them, in 64 MB or so of fp32
+        size_t part = (static_cast<size_t>(1) << 24) / from->cols / 8 * 8;
+        if (part < 8) part = 8;
+        if (part > static_cast<size_t>(from->rows)) part = from->rows;
+        Tensor t;
+        float *values = nullptr;
+        cudaError_t err = alloc_i8(t, from->cols, from->rows);
+        if (err == cudaSuccess) err = cudaMalloc(&values, sizeof(float) * part * from->cols);
+        for (size_t r = 0; r < static_cast<size_t>(from->rows) && err == cudaSuccess; r += part) {
+            const size_t n = part < from->rows - r ? part : from->rows - r;
+            err = vqm::launch_dequant(from->type, from->data + r * from->row_bytes, values, static_cast<long long>(n * from->cols), cb, rt->stream);
+            vqm::RowsI8Args a{};
+            a.x = values;
+            a.q = reinterpret_cast<int8_t *>(t.data) + r * t.row_bytes;
+            a.scales = const_cast<float *>(t.scales) + r;
+            a.cols = from->cols;
+            a.ntok = static_cast<int>(n);
+            a.elem = 4;
+            if (err == cudaSuccess) err = vqm::launch_rows_i8(a, rt->stream);
+            if (err == cudaSuccess) count_launch(rt, 2);
+        }
+        const cudaError_t done = cudaStreamSynchronize(rt->stream);  // (products fetch weights ahead of the stream's order)
+        if (err == cudaSuccess) err = done;
+        cudaFree(values);
+        if (err != cudaSuccess) {
+            release(t);
+            return cuda_fail("convert_i8", err);
+        }
+        put_tensor(rt, name, t);
+        return VQM_OK;
+    });
+}
+
+int vqm_rows_i8(vqm_runtime *rt, const char *x, const char *q, const char *scales, int cols, int ntok, int flags, const char *x2, const char *residual,
+                const char *total, const char *norm_weight, float eps) {
+    return entry(rt, {x, q, scales}, [&]() -> int {
+        if (ntok < 1) return fail(VQM_ERR_VALUE, "ntok must be positive");
+        if (cols < 1 || cols > vqm::kI8MaxCols) return fail(VQM_ERR_VALUE, "cols must be in [1, %d]", vqm::kI8MaxCols);
+        if ((flags & ~(VQM_FUSE_ADD | VQM_FUSE_NORM | VQM_FUSE_SILU_MUL)) != 0) return fail(VQM_ERR_VALUE, "unknown flag bits %d", flags);
+        if ((flags & VQM_FUSE_ADD) && (flags & VQM_FUSE_SILU_MUL)) return fail(VQM_ERR_VALUE, "a residual is added to x itself, not to silu(x) * x2");
+        const size_t n = static_cast<size_t>(ntok) * cols;
+        int rc = VQM_OK;
+        vqm::RowsI8Args a{};
+        a.cols = cols;
+        a.ntok = ntok;
+        a.eps = eps;
+        if ((a.x = find_real(rt, x, n, &a.elem, &rc)) == nullptr) return rc;
+        if ((a.q = find_i8(rt, q, static_cast<size_t>(vqm::i8_pitch(cols)) * ntok, &rc)) == nullptr) return rc;
+        if ((a.scales = find_f32(rt, scales, static_cast<size_t>(ntok), &rc)) == nullptr) return rc;
+        if (flags & VQM_FUSE_SILU_MUL) {
+            if (x2 == nullptr) return fail(VQM_ERR_VALUE, "VQM_FUSE_SILU_MUL needs x2");
+            if ((a.x2 = find_real(rt, x2, n, &a.elem, &rc)) == nullptr) return rc;
+        }
+        if (flags & VQM_FUSE_ADD) {
+            if (residual == nullptr) return fail(VQM_ERR_VALUE, "VQM_FUSE_ADD needs the residual");
+            if ((a.residual = find_real(rt, residual, n, &a.elem, &rc)) == nullptr) return rc;
+            if ((a.total = find_real(rt, total != nullptr ? total : residual, n, &a.elem, &rc)) == nullptr) return rc;
+        } else if (total != nullptr) {
+            return fail(VQM_ERR_VALUE, "a buffer for the sums without VQM_FUSE_ADD");
+        }
+        if (flags & VQM_FUSE_NORM) {
+            if (norm_weight == nullptr) return fail(VQM_ERR_VALUE, "VQM_FUSE_NORM needs norm_weight");
+            if ((a.norm_w = find_norm(rt, norm_weight, cols, &rc)) == nullptr) return rc;
+            if (!(eps >= 0.0f)) return fail(VQM_ERR_VALUE, "eps must be >= 0");
+        }
+        const cudaError_t err = vqm::launch_rows_i8(a, rt->stream);
+        if (err != cudaSuccess) return cuda_fail("rows_i8 launch", err);
+        count_launch(rt);
+        return VQM_OK;
+    });
+}
+
+int vqm_qmm_i8(vqm_runtime *rt, const char *weight, const char *q, const char *scales, const char *y, int ntok, int flags) {
+    return entry(rt, {weight, q, scales, y}, [&]() -> int {
+        if (ntok < 1) return fail(VQM_ERR_VALUE, "ntok must be positive");
+        if ((flags & ~VQM_FUSE_ADD) != 0) return fail(VQM_ERR_VALUE, "unknown flag bits %d", flags);
+        int rc = VQM_OK;
+        Tensor *t = find_i8_tensor(rt, weight, &rc);
+        if (t == nullptr) return rc;
+        vqm::QmmI8Args a{};
+        if ((a.q = find_i8(rt, q, static_cast<size_t>(vqm::i8_pitch(t->cols)) * ntok, &rc)) == nullptr) return rc;
+        if ((a.q_scales = find_f32(rt, scales, static_cast<size_t>(ntok), &rc)) == nullptr) return rc;
+        if ((a.y = find_real(rt, y, static_cast<size_t>(t->rows) * ntok, &a.y_elem, &rc)) == nullptr) return rc;
+        a.w = reinterpret_cast<const int8_t *>(t->data);
+        a.w_scales = t->scales;
+        a.w_pitch = static_cast<long long>(t->row_bytes);
+        a.rows = t->rows;
+        a.cols = t->cols;
+        a.ntok = ntok;
+        a.add = (flags & VQM_FUSE_ADD) != 0;
+        a.status = rt->status;
+        const cudaError_t err = vqm::launch_qmm_i8(a, rt->sm_count, rt->stream);
+        if (err != cudaSuccess) return cuda_fail("qmm_i8 launch", err);
+        count_launch(rt);
+        return VQM_OK;
+    });
+}
+
+int vqm_verify(vqm_runtime *rt, const char *target, const char *draft, const char *tokens, const char *lens, const char *uniforms, const char *temperature,
+               int vocab, int seqs, int drafts, const char *out, int *out_host) {
+    return entry(rt, {target, uniforms, out}, [&]() -> int {
+        if (vocab < 1 || seqs < 1) return fail(VQM_ERR_VALUE, "vocab and the number of sequences must be positive");
+        if (drafts < 0 || drafts > VQM_MAX_DRAFTS) return fail(VQM_ERR_VALUE, "drafts must be in [0, %d]", VQM_MAX_DRAFTS);
+        if (drafts > 0 && tokens == nullptr) return fail(VQM_ERR_VALUE, "drafts without tokens");
+        const size_t s = static_cast<size_t>(seqs), k = static_cast<size_t>(drafts);
+        int rc = VQM_OK, word = 4;
+        vqm::VerifyArgs a{};
+        a.vocab = vocab;
+        a.seqs = seqs;
+        a.drafts = drafts;
+        if ((a.target = find_real(rt, target, s * (k + 1) * static_cast<size_t>(vocab), &a.elem, &rc)) == nullptr) return rc;
+        if (drafts > 0 && draft != nullptr && (a.draft = find_real(rt, draft, s * k * static_cast<size_t>(vocab), &a.elem, &rc)) == nullptr) return rc;
+        if (drafts > 0 && (a.tokens = static_cast<const int *>(find_real(rt, tokens, s * k, &word, &rc))) == nullptr) return rc;
+        if (lens != nullptr && (a.lens = static_cast<const int *>(find_real(rt, lens, s, &word, &rc))) == nullptr) return rc;
+        if ((a.uniforms = find_f32(rt, uniforms, s * (k + 1), &rc)) == nullptr) return rc;
+        if (temperature != nullptr && (a.temperature = find_f32(rt, temperature, s, &rc)) == nullptr) return rc;
+        if ((a.out = static_cast<int *>(find_real(rt, out, s * (k + 2), &word, &rc))) == nullptr) return rc;
+        if (out_host != nullptr && (rc = no_capture(rt, "a blocking verify")) != VQM_OK) return rc;
+        cudaError_t err = vqm::launch_verify(a, rt->sm_count, rt->stream);
+        if (err != cudaSuccess) return cuda_fail("verify launch", err);
+        count_launch(rt);
+        if (out_host != nullptr) {
+            err = cudaMemcpyAsync(out_host, a.out, sizeof(int) * s * (k + 2), cudaMemcpyDeviceToHost, rt->stream);
+            if (err == cudaSuccess) err = cudaStreamSynchronize(rt->stream);
+            if (err != cudaSuccess) return cuda_fail("verify", err);
+        }
+        return VQM_OK;
+    });
 }
 
 int vqm_set_gemm_min_rows(vqm_runtime *rt, int n) {

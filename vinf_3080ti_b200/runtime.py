@@ -20,6 +20,7 @@ import numpy as np
 from . import _capi
 from .gguf_types import CODEBOOK_BYTES
 
+MAX_DRAFTS = 255  # of a sequence, in one verification
 MAX_ARGMAX_ROWS = 256  # engine/csrc/megakernel/qwen_runtime.cu:573
 
 
@@ -170,9 +171,9 @@ class Runtime:
         return out.tobytes()
 
     def read_array(self, name: str, n: int = -1, offset: int = 0) -> np.ndarray:
-        """read() as a float32 / float16 numpy array (no reference counterpart; saves a copy)."""
+        """read() as a float32 / float16 / int8 numpy array (no reference counterpart; saves a copy)."""
         data = self.read(name, n, offset)
-        return np.frombuffer(data, dtype=np.float32 if self.buffer_elem(name) == 4 else np.float16)
+        return np.frombuffer(data, dtype={4: np.float32, 2: np.float16, 1: np.int8}[self.buffer_elem(name)])
 
     def copy(self, dst: str, dst_off: int, src: str, src_off: int, n: int) -> None:
         if dst_off < 0 or src_off < 0 or n < 0:
@@ -275,6 +276,49 @@ class Runtime:
     def dequantize(self, weight: str, out: str) -> None:
         """Exact fp32 values of a weight tensor into an fp32 buffer (rows * cols elements)."""
         _capi.check(self._lib.vqm_dequantize(self._h, _name(weight), _name(out)))
+
+    # ---- passes in 8-bit integers, verification of drafted tokens (no reference counterpart; see include/vinf_b200.h) -----------
+    def upload_i8(self, name: str, data, scales, cols: int, rows: int) -> None:
+        """A weight tensor of 8-bit integer rows: rows * cols int8, densely packed, and one fp32 scale per row."""
+        keep, addr, n = _ptr(data)
+        keep_scales, scale_addr, scale_n = _ptr(scales)
+        _capi.check(self._lib.vqm_upload_i8(self._h, _name(name), addr, n, scale_addr, scale_n, int(cols), int(rows)))
+
+    def bind_i8(self, name: str, device_ptr: int, scales_ptr: int, cols: int, rows: int, pitch: int = 0) -> None:
+        """The same in device memory (not freed by the runtime); rows `pitch` bytes apart, 0: cols rounded up to 16."""
+        if pitch < 0:
+            raise ValueError("pitch must not be negative")
+        _capi.check(self._lib.vqm_bind_i8(self._h, _name(name), ctypes.c_void_p(device_ptr), int(pitch), ctypes.c_void_p(scales_ptr), int(cols), int(rows)))
+
+    def convert_i8(self, weight: str, name: str) -> None:
+        """Makes the 8-bit tensor `name` from the GGUF tensor `weight`, a scale per row."""
+        _capi.check(self._lib.vqm_convert_i8(self._h, _name(weight), _name(name)))
+
+    def rows_i8(self, x: str, q: str, scales: str, cols: int, ntok: int = 1, *, residual: str | None = None, total: str | None = None,
+                norm: str | None = None, eps: float = 1e-6, silu_mul: str | None = None) -> None:
+        """Activation rows as 8-bit integers `q` with a scale per row, after the residual's addition (the sum goes to `total`, or back to
+        `residual`) or silu(x) * silu_mul, and the rms norm with the weights `norm`, where given.  Asynchronous."""
+        flags = (1 if residual is not None else 0) | (2 if norm is not None else 0) | (8 if silu_mul is not None else 0)
+        _capi.check(self._lib.vqm_rows_i8(self._h, _name(x), _name(q), _name(scales), int(cols), int(ntok), flags, _name(silu_mul), _name(residual),
+                                          _name(total), _name(norm), float(eps)))
+
+    def qmm_i8(self, weight: str, q: str, scales: str, y: str, ntok: int = 1, *, add: bool = False) -> None:
+        """y (+)= W x for a tensor of 8-bit integer rows and activations from rows_i8.  Asynchronous."""
+        _capi.check(self._lib.vqm_qmm_i8(self._h, _name(weight), _name(q), _name(scales), _name(y), int(ntok), 1 if add else 0))
+
+    def verify(self, target: str, draft: str | None, tokens: str | None, uniforms: str, vocab: int, seqs: int, drafts: int, *, out: str,
+               lens: str | None = None, temperature: str | None = None, blocking: bool = True) -> list[list[int]] | None:
+        """Speculative decoding's decision: which drafted tokens are kept, and the token after them.  Returns per sequence the kept tokens
+        followed by the next one (blocking), or leaves [count, tokens..., -1...] in the buffer `out`."""
+        if seqs < 1 or drafts < 0 or drafts > MAX_DRAFTS:
+            raise ValueError(f"seqs must be positive and drafts in [0, {MAX_DRAFTS}]")
+        host = (ctypes.c_int * (seqs * (drafts + 2)))() if blocking else None
+        _capi.check(self._lib.vqm_verify(self._h, _name(target), _name(draft), _name(tokens), _name(lens), _name(uniforms), _name(temperature),
+                                         int(vocab), int(seqs), int(drafts), _name(out), host))
+        if host is None:
+            return None
+        rows = [list(host[i * (drafts + 2):(i + 1) * (drafts + 2)]) for i in range(seqs)]
+        return [row[1:row[0] + 2] for row in rows]
 
     def set_gemm_min_rows(self, n: int) -> None:
         _capi.check(self._lib.vqm_set_gemm_min_rows(self._h, int(n)))
