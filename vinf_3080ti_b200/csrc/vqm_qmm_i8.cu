@@ -1,52 +1,416 @@
-// Product of 8-bit integers:  y[t][r] = sx[t] sw[r] sum_k q[t][k] W[r][k],  sums in 32-bit integers, exact.
+// Product of 8-bit integers on the 5th-generation tensor cores:  y[t][r] = sx[t] sw[r] sum_k q[t][k] W[r][k],  sums in 32-bit integers, exact.
+//
+// The weight rows are the rows of the accumulator (lanes of tensor memory), the activation rows its columns: an output row of 32 lanes is
+// then 128 consecutive bytes, and a lane needs one weight scale.  Both operands come by TMA in 128-byte swizzled tiles of 128 columns, go
+// through a ring of stages, and are multiplied by tcgen05.mma (kind::i8).
+//   warp 0      one thread issues the copies
+//   warp 1      one thread issues the MMAs (in the second block of a pair: passes "full" on to the first)
+//   warp 2      tensor memory
+//   warps 4-11  outputs: two warps for each 32 lanes
+// PAIR: two blocks of a cluster multiply 256 weight rows by up to 256 activation rows together (cta_group::2), each holding half of both.
+// SPLIT: the blocks (pairs) of a cluster share the columns of a tile; sums are integers, so how they are split does not show in the result.
+// Every output is the same whatever else is in its launch.
+//
+// Every wait is bounded: on expiry the block records a status code and everybody falls through to the end.
+#include <cuda.h>
 #include <cuda_fp16.h>
 
 #include "vqm_kernels.h"
+#include "vqm_tcmv.cuh"
 
 namespace vqm {
 namespace {
 
-constexpr int kGroup = 8;  // activation rows that a warp carries along
+constexpr int kQRows = 128, kQCols = 128;           // weight rows of a block's tile, columns of a stage
+constexpr int kQA = kQRows * kQCols;                // bytes of a stage's weights
+constexpr int kQMaxN = 256, kQMaxStages = 12, kQMaxSplit = 8;
+constexpr int kQRing = 216 * 1024;                  // shared memory of the stages
+constexpr int kQWriters = 8, kQThreads = 128 + 32 * kQWriters;
 
-__global__ void __launch_bounds__(256) qmm_i8_kernel(const QmmI8Args a) {
-    const int row = static_cast<int>(blockIdx.x * 8 + (threadIdx.x >> 5)), lane = threadIdx.x & 31;
-    if (row >= a.rows) return;
-    const int t0 = blockIdx.y * kGroup, m = min(kGroup, a.ntok - t0);
-    const long long pitch = i8_pitch(a.cols);
-    const int8_t *w = a.w + static_cast<size_t>(row) * a.w_pitch;
-    int sum[kGroup] = {};
-    for (int c = lane * 4; c < a.cols; c += 128) {
-        int word = *reinterpret_cast<const int *>(w + c);
-        if (c + 4 > a.cols) word &= (1 << (8 * (a.cols - c))) - 1;  // what lies behind the last column counts nothing
-#pragma unroll
-        for (int t = 0; t < kGroup; ++t)
-            if (t < m) sum[t] = __dp4a(word, *reinterpret_cast<const int *>(a.q + static_cast<size_t>(t0 + t) * pitch + c), sum[t]);
+struct QmmTc {
+    const float *w_scales, *q_scales;
+    void *y;
+    unsigned *status;
+    int rows, ntok, n_k;               // n_k: stages of a whole row
+    int n, row_tiles, tok_tiles;       // activation rows of a tile, a multiple of 16 (pairs: 32)
+    int stages, b_bytes;               // of the ring; bytes of a block's activations in a stage
+    int acc_cols, tmem_cols;           // tensor-memory columns from one accumulator to the next, and in all
+    int split;                         // blocks (pairs) that share a tile's columns
+    int y_elem, add;
+};
+
+using tc::bar_arrive, tc::bar_init, tc::bar_try, tc::bar_wait, tc::bar_wait_cluster, tc::in_block, tc::s32;
+
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {  // K-major, 128-byte swizzle, groups of 8 rows 1024 bytes apart
+    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void copy_tile(uint32_t to, const CUtensorMap *map, int x, int row, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to), "l"(map), "r"(x), "r"(row), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void arrive_in(uint32_t cluster_addr) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory"); }
+__device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (PAIR)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                     : "memory");
+}
+// Arrives on the barrier (in both blocks of pair `pair`) once the MMAs issued so far are done.
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t pair) {
+    if constexpr (PAIR) {
+        const uint16_t both = static_cast<uint16_t>(3u << (2 * pair));
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(both) : "memory");
+    } else {
+        tc::commit(bar);
     }
+}
+__device__ __forceinline__ void load8(uint32_t at, int (&v)[8]) {
+    __syncwarp();
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// 8 activation rows from `tok` on of this lane's weight row.
+__device__ __forceinline__ void write8(const QmmTc &a, const int (&v)[8], int row, int tok, float w_scale) {
+    if (row >= a.rows) return;
 #pragma unroll
-    for (int t = 0; t < kGroup; ++t)
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], off);
-    if (lane != 0) return;
-    for (int t = 0; t < m; ++t) {
-        const size_t at = static_cast<size_t>(t0 + t) * a.rows + row;
-        const float v = static_cast<float>(sum[t]) * a.q_scales[t0 + t] * a.w_scales[row];
+    for (int j = 0; j < 8; ++j) {
+        if (tok + j >= a.ntok) break;
+        const float out = static_cast<float>(v[j]) * a.q_scales[tok + j] * w_scale;
+        const size_t at = static_cast<size_t>(tok + j) * a.rows + row;
         if (a.y_elem == 2) {
             __half *y = static_cast<__half *>(a.y) + at;
-            *y = __float2half_rn(a.add ? __half2float(*y) + v : v);
+            *y = __float2half_rn(a.add ? __half2float(*y) + out : out);
         } else {
             float *y = static_cast<float *>(a.y) + at;
-            *y = a.add ? *y + v : v;
+            *y = a.add ? *y + out : out;
         }
     }
 }
 
+template <bool PAIR, bool SPLIT>
+__global__ void __launch_bounds__(kQThreads, 1) qmm_i8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap q_map, const QmmTc a) {
+    constexpr int GROUP = PAIR ? 2 : 1;
+    extern __shared__ uint8_t ring_raw[];
+    __shared__ __align__(8) uint64_t s_full[kQMaxStages], s_empty[kQMaxStages], s_acc_full[2], s_acc_empty[2];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_failed;
+    const uint32_t ring = (s32(ring_raw) + 1023u) & ~1023u;  // (the swizzle works on address bits)
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t in_cluster = 0;
+    if constexpr (PAIR || SPLIT) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(in_cluster));
+    const int rank = PAIR ? static_cast<int>(in_cluster & 1u) : 0, part = static_cast<int>(in_cluster) / GROUP;  // place in the pair, share of the columns
+    const uint32_t leader = in_cluster & ~1u;
+    const int cluster = static_cast<int>(blockIdx.x) / (GROUP * a.split), n_clusters = static_cast<int>(gridDim.x) / (GROUP * a.split);
+    const int k0 = SPLIT ? part * a.n_k / a.split : 0, k1 = SPLIT ? (part + 1) * a.n_k / a.split : a.n_k;
+    const int n_tiles = a.row_tiles * a.tok_tiles;
+    const uint32_t stage_bytes = kQA + a.b_bytes;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < a.stages; ++s) {
+            bar_init(s32(&s_full[s]), PAIR && rank == 0 ? 2 : 1);  // the first block of a pair hears of the second's stage
+            bar_init(s32(&s_empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            bar_init(s32(&s_acc_full[b]), 1);
+            bar_init(s32(&s_acc_empty[b]), kQWriters * GROUP);
+        }
+        s_failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&s_tmem)), "r"(a.tmem_cols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&s_tmem)), "r"(a.tmem_cols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if constexpr (PAIR || SPLIT) cluster_sync();  // the other blocks' barriers and tensor memory exist
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = s_tmem;
+    volatile int *failed = &s_failed;
+
+    // Tiles go to clusters in turn; 8 tiles of weight rows by all tiles of activation rows follow one another, so that what is multiplied at one
+    // time is a block of both that stays in L2.
+    auto place = [&](int tile, int &row_tile, int &tok_tile) {
+        constexpr int kBand = 8;
+        const int band = tile / (kBand * a.tok_tiles), first = band * kBand, height = min(kBand, a.row_tiles - first), in_band = tile - band * kBand * a.tok_tiles;
+        tok_tile = in_band / height;
+        row_tile = first + in_band - tok_tile * height;
+    };
+
+    if (warp == 0) {
+        if (tc::elect_one()) {
+            auto copy_w = [&](int stage, int k, int row_tile) { copy_tile(ring + stage * stage_bytes, &w_map, k * kQCols, (row_tile * GROUP + rank) * kQRows, s32(&s_full[stage])); };
+            auto copy_q = [&](int stage, int k, int tok_tile) {
+                copy_tile(ring + stage * stage_bytes + kQA, &q_map, k * kQCols, tok_tile * a.n + rank * (a.n / 2), s32(&s_full[stage]));
+            };
+            int it = 0, issued = 0;
+            bool ok = true;
+            for (int tile = cluster; tile < n_tiles && ok; tile += n_clusters) {
+                int row_tile, tok_tile;
+                place(tile, row_tile, tok_tile);
+                int k = k0;
+                if (it == 0) {
+                    // Weights are in place before the launch; what the kernel before this one in the stream makes, the activations, is waited for.
+                    const int ahead = min(a.stages, k1 - k0);
+                    for (int i = 0; i < ahead; ++i) {
+                        expect(s32(&s_full[i]), stage_bytes);
+                        copy_w(i, k0 + i, row_tile);
+                    }
+                    asm volatile("griddepcontrol.wait;" ::: "memory");
+                    for (int i = 0; i < ahead; ++i) copy_q(i, k0 + i, tok_tile);
+                    it = issued = ahead;
+                    k += ahead;
+                }
+                for (; k < k1; ++k, ++it) {
+                    const int stage = it % a.stages, use = it / a.stages;
+                    if (use > 0) {
+                        bar_wait(s32(&s_empty[stage]), (use - 1) & 1, failed);
+                        if (*failed) {
+                            ok = false;
+                            break;
+                        }
+                    }
+                    expect(s32(&s_full[stage]), stage_bytes);
+                    copy_w(stage, k, row_tile);
+                    copy_q(stage, k, tok_tile);
+                    issued = it + 1;
+                }
+            }
+            if (!ok)  // the last copies land before the block may leave
+                for (int last = max(0, issued - a.stages); last < issued; ++last)
+                    for (int i = 0; i < (1 << 16) && !bar_try(s32(&s_full[last % a.stages]), (last / a.stages) & 1); ++i) __nanosleep(64);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        const bool first = rank == 0;
+        // D s32, A and B s8, K-major
+        const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(a.n >> 3) << 17) | (static_cast<uint32_t>(GROUP * kQRows >> 4) << 24);
+        int it = 0, done = 0;
+        for (int tile = cluster; tile < n_tiles; tile += n_clusters, ++done) {
+            const int buf = SPLIT ? 0 : done & 1;
+            if (first && done >= 2) {
+                if constexpr (PAIR) bar_wait_cluster(s32(&s_acc_empty[buf]), ((done >> 1) - 1) & 1, failed);
+                else bar_wait(s32(&s_acc_empty[buf]), ((done >> 1) - 1) & 1, failed);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            }
+            for (int k = k0; k < k1; ++k, ++it) {
+                const int stage = it % a.stages;
+                const uint32_t full = s32(&s_full[stage]), parity = (it / a.stages) & 1;
+                if (PAIR && first) bar_wait_cluster(full, parity, failed);
+                else bar_wait(full, parity, failed);
+                if (__any_sync(0xFFFFFFFFu, *failed)) break;
+                if (first) {
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (tc::elect_one()) {
+                        const uint64_t w_desc = tile_desc(ring + stage * stage_bytes), q_desc = tile_desc(ring + stage * stage_bytes + kQA);
+#pragma unroll
+                        for (int j = 0; j < kQCols / 32; ++j) mma_i8<PAIR>(tmem + buf * a.acc_cols, w_desc + 2 * j, q_desc + 2 * j, idesc, (k > k0 || j > 0) ? 1u : 0u);
+                        commit<PAIR>(s32(&s_empty[stage]), static_cast<uint32_t>(part));
+                    }
+                    __syncwarp();
+                } else if (lane == 0) {
+                    arrive_in(in_block(full, static_cast<int>(leader)));
+                }
+            }
+            if (__any_sync(0xFFFFFFFFu, *failed)) break;
+            if (first && tc::elect_one()) commit<PAIR>(s32(&s_acc_full[buf]), static_cast<uint32_t>(part));
+            __syncwarp();
+        }
+    }
+
+    if constexpr (!SPLIT) {
+        if (warp >= 4) {
+            const int lanes = warp & 3, half = (warp - 4) >> 2;  // (a warp may read the 32 lanes (warp % 4) * 32 onwards)
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            int done = 0;
+            for (int tile = cluster; tile < n_tiles; tile += n_clusters, ++done) {
+                int row_tile, tok_tile;
+                place(tile, row_tile, tok_tile);
+                const int buf = done & 1, row = (row_tile * GROUP + rank) * kQRows + lanes * 32 + lane;
+                const float w_scale = row < a.rows ? __ldg(a.w_scales + row) : 0.0f;
+                bar_wait(s32(&s_acc_full[buf]), (done >> 1) & 1, failed);
+                if (__any_sync(0xFFFFFFFFu, *failed)) break;
+                if (tile + n_clusters >= n_tiles) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t at = tmem + buf * a.acc_cols + (static_cast<uint32_t>(lanes * 32) << 16);
+                for (int c = half * 8; c < a.n; c += 16) {
+                    int v[8];
+                    load8(at + c, v);
+                    loaded();
+                    write8(a, v, row, tok_tile * a.n + c, w_scale);
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (PAIR) arrive_in(in_block(s32(&s_acc_empty[buf]), static_cast<int>(leader)));
+                    else bar_arrive(s32(&s_acc_empty[buf]));
+                }
+            }
+        }
+    } else {
+        // One tile; its sums go, 8 columns of 32 lanes at a time, to the block that writes them: unit u to part u % split.
+        const int lanes = warp & 3, half = (warp - 4) >> 2;
+        const uint32_t at = tmem + (static_cast<uint32_t>(lanes * 32) << 16);
+        if (warp >= 4) {
+            bar_wait(s32(&s_acc_full[0]), 0, failed);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
+        cluster_sync();  // every block's MMAs are done with its stages
+        if (warp >= 4) {
+            for (int c = half; c < a.n / 8; c += 2) {
+                const int unit = c * 4 + lanes, owner = unit % a.split;
+                if (owner == part) continue;
+                int v[8];
+                load8(at + c * 8, v);
+                loaded();
+                const uint32_t to = in_block(ring + ((unit / a.split) * (a.split - 1) + (part < owner ? part : part - 1)) * 1024 + lane * 16, owner * GROUP + rank);
+                asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+                asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 512), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+            }
+        }
+        cluster_sync();
+        if (warp >= 4) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+            int row_tile, tok_tile;
+            place(cluster, row_tile, tok_tile);
+            const int row = (row_tile * GROUP + rank) * kQRows + lanes * 32 + lane;
+            const float w_scale = row < a.rows ? __ldg(a.w_scales + row) : 0.0f;
+            for (int c = half; c < a.n / 8; c += 2) {
+                const int unit = c * 4 + lanes;
+                if (unit % a.split != part) continue;
+                int v[8];
+                load8(at + c * 8, v);
+                loaded();
+                for (int p = 0; p < a.split - 1; ++p) {
+                    const uint32_t from = ring + ((unit / a.split) * (a.split - 1) + p) * 1024 + lane * 16;
+                    const uint4 x = lds128u(from), z = lds128u(from + 512);
+                    v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += z.x, v[5] += z.y, v[6] += z.z, v[7] += z.w;
+                }
+                if (!*failed) write8(a, v, row, tok_tile * a.n + c * 8, w_scale);
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if constexpr (PAIR || SPLIT) cluster_sync();  // no block's shared or tensor memory goes away under another
+    if (warp == 2) {
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+        if (lane == 0 && s_failed) atomicExch(a.status, kStatusWaitExpired);
+    }
+}
+
+// 8-bit rows as a 2-D tensor; a tile is 128 columns of `box_rows` rows.  Columns and rows beyond the last arrive as zeros.
+cudaError_t encode_rows(CUtensorMap *map, const int8_t *rows_at, int cols, long long pitch, int rows, int box_rows) {
+    TcEncode encode = nullptr;
+    if (const cudaError_t err = tc_encoder(&encode); err != cudaSuccess) return err;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(pitch)};
+    const cuuint32_t box[2] = {kQCols, static_cast<cuuint32_t>(box_rows)}, elem[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(rows_at), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? cudaSuccess
+               : cudaErrorInvalidValue;
+}
+
+template <bool PAIR, bool SPLIT>
+struct Variant {
+    static constexpr int kSmem = kQRing + 1024;
+    static constexpr int kGroup = PAIR ? 2 : 1;
+    static constexpr auto kKernel = qmm_i8_kernel<PAIR, SPLIT>;
+    static void configure(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int clusters, int split, cudaStream_t stream) {
+        cfg.gridDim = dim3(static_cast<unsigned>(clusters * split * kGroup));
+        cfg.blockDim = dim3(kQThreads);
+        cfg.dynamicSmemBytes = kSmem;
+        cfg.stream = stream;
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = static_cast<unsigned>(split * kGroup);
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+    }
+    // clusters that fit on the GPU at once (cached; one device per process), 0 if the kernel cannot run
+    static int clusters(int split) {
+        static int cached[kQMaxSplit + 1] = {};
+        if (cached[split] == 0) {
+            int n = 0;
+            cudaLaunchConfig_t cfg{};
+            cudaLaunchAttribute attr[2];
+            configure(cfg, attr, 1024, split, nullptr);
+            if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kKernel, &cfg) != cudaSuccess) {
+                (void)cudaGetLastError();
+                n = 0;
+            }
+            cached[split] = n > 0 ? n : -1;
+        }
+        return cached[split] < 0 ? 0 : cached[split];
+    }
+    static cudaError_t launch(const CUtensorMap &w, const CUtensorMap &q, const QmmTc &a, cudaStream_t stream) {
+        const int fit = clusters(a.split), tiles = a.row_tiles * a.tok_tiles;
+        if (fit == 0) return cudaErrorInvalidConfiguration;
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute attr[2];
+        configure(cfg, attr, SPLIT ? tiles : (tiles < fit ? tiles : fit), a.split, stream);
+        return cudaLaunchKernelEx(&cfg, kKernel, w, q, a);
+    }
+};
+
 }  // namespace
 
-cudaError_t launch_qmm_i8(const QmmI8Args &a, int sm_count, cudaStream_t stream) {
-    (void)sm_count;
-    const dim3 grid((a.rows + 7) / 8, (a.ntok + kGroup - 1) / kGroup);
-    qmm_i8_kernel<<<grid, 256, 0, stream>>>(a);
-    return cudaGetLastError();
+cudaError_t launch_qmm_i8(const QmmI8Args &in, int sm_count, cudaStream_t stream) {
+    QmmTc a{};
+    a.w_scales = in.w_scales;
+    a.q_scales = in.q_scales;
+    a.y = in.y;
+    a.status = in.status;
+    a.rows = in.rows;
+    a.ntok = in.ntok;
+    a.n_k = (in.cols + kQCols - 1) / kQCols;
+    a.y_elem = in.y_elem;
+    a.add = in.add;
+    const bool pair = in.ntok > 256;
+    const int group = pair ? 2 : 1, step = pair ? 32 : 16;
+    a.tok_tiles = (in.ntok + kQMaxN - 1) / kQMaxN;
+    a.n = ((in.ntok + a.tok_tiles - 1) / a.tok_tiles + step - 1) / step * step;
+    a.tok_tiles = (in.ntok + a.n - 1) / a.n;
+    a.row_tiles = (in.rows + group * kQRows - 1) / (group * kQRows);
+    a.split = 1;
+    const int tiles = a.row_tiles * a.tok_tiles;
+    while (a.split < (pair ? 4 : kQMaxSplit) && tiles * group * (a.split + 1) <= sm_count && a.n_k / (a.split + 1) >= 2) ++a.split;
+    a.b_bytes = a.n / group * kQCols;
+    a.stages = kQRing / (kQA + a.b_bytes);
+    if (a.stages > kQMaxStages) a.stages = kQMaxStages;
+    a.acc_cols = 32;
+    while (a.acc_cols < a.n) a.acc_cols *= 2;
+    a.tmem_cols = (a.split > 1 ? 1 : 2) * a.acc_cols;
+    CUtensorMap w, q;
+    cudaError_t err = encode_rows(&w, in.w, in.cols, in.w_pitch, in.rows, kQRows);
+    if (err == cudaSuccess) err = encode_rows(&q, in.q, in.cols, i8_pitch(in.cols), in.ntok, a.n / group);
+    if (err != cudaSuccess) return err;
+    if (pair) return a.split > 1 ? Variant<true, true>::launch(w, q, a, stream) : Variant<true, false>::launch(w, q, a, stream);
+    return a.split > 1 ? Variant<false, true>::launch(w, q, a, stream) : Variant<false, false>::launch(w, q, a, stream);
 }
 
 }  // namespace vqm
