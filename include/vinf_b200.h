@@ -184,12 +184,14 @@ int vqm_qmm_i8(vqm_runtime *rt, const char *weight, const char *q, const char *s
  *   the next token is the smallest one up to which the sum of r = max(p - q, 0) at the refused draft (behind the last draft: r = p) is above
  *   u[drafts] times r's whole sum.  So the tokens are distributed as p.  T <= 0 (or NaN): p and q are 1 at their rows' largest logit, the
  *   lowest index on ties: greedy verification.
- * Decisions are those of 64-bit arithmetic.  Logits of -inf and NaN have no probability; a row without any refuses its draft, and the
+ * Decisions are those of 64-bit arithmetic; where p - q is within its rounding (2^-44 p) it is nothing, and where nothing is left of p - q the
+ * token is drawn from p.  Logits of -inf and NaN have no probability; a row without any refuses its draft, and the
  * token drawn from such a row is -1.  A token outside [0, vocab) is refused, and where drafts have no probabilities nothing is taken off p then.
  * out [seqs][drafts + 2] (int32): the number of accepted drafts a, the accepted tokens, the next token, then -1.  out_host (seqs * (drafts + 2)
  * ints) may be NULL: then the call is asynchronous.  target and draft are both fp32 or both fp16.  drafts = 0 samples from the target.
- * 0 <= drafts <= VQM_MAX_DRAFTS. */
+ * 0 <= drafts <= VQM_MAX_DRAFTS, vocab <= VQM_MAX_VOCAB. */
 #define VQM_MAX_DRAFTS 255
+#define VQM_MAX_VOCAB 1073741824
 int vqm_verify(vqm_runtime *rt, const char *target, const char *draft, const char *tokens, const char *lens, const char *uniforms, const char *temperature,
                int vocab, int seqs, int drafts, const char *out, int *out_host);
 

@@ -210,7 +210,7 @@ struct VerifyArgs {
     int *out;                  // [seqs][drafts + 2]
     int vocab, seqs, drafts, elem;
 };
-cudaError_t launch_verify(const VerifyArgs &a, int sm_count, cudaStream_t stream);
+cudaError_t launch_verify(const VerifyArgs &a, cudaStream_t stream);
 
 cudaError_t launch_argmax_rows(const float *x, int n, int ntok, int *out, cudaStream_t stream);
 cudaError_t launch_dequant(int type, const uint8_t *w, float *out, long long numel, const uint8_t *codebook,

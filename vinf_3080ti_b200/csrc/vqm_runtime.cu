@@ -1711,7 +1711,7 @@ int vqm_qmm_i8(vqm_runtime *rt, const char *weight, const char *q, const char *s
 int vqm_verify(vqm_runtime *rt, const char *target, const char *draft, const char *tokens, const char *lens, const char *uniforms, const char *temperature,
                int vocab, int seqs, int drafts, const char *out, int *out_host) {
     return entry(rt, {target, uniforms, out}, [&]() -> int {
-        if (vocab < 1 || seqs < 1) return fail(VQM_ERR_VALUE, "vocab and the number of sequences must be positive");
+        if (vocab < 1 || vocab > VQM_MAX_VOCAB || seqs < 1) return fail(VQM_ERR_VALUE, "vocab must be in [1, %d], the number of sequences positive", VQM_MAX_VOCAB);
         if (drafts < 0 || drafts > VQM_MAX_DRAFTS) return fail(VQM_ERR_VALUE, "drafts must be in [0, %d]", VQM_MAX_DRAFTS);
         if (drafts > 0 && tokens == nullptr) return fail(VQM_ERR_VALUE, "drafts without tokens");
         const size_t s = static_cast<size_t>(seqs), k = static_cast<size_t>(drafts);
@@ -1728,7 +1728,7 @@ int vqm_verify(vqm_runtime *rt, const char *target, const char *draft, const cha
         if (temperature != nullptr && (a.temperature = find_f32(rt, temperature, s, &rc)) == nullptr) return rc;
         if ((a.out = static_cast<int *>(find_real(rt, out, s * (k + 2), &word, &rc))) == nullptr) return rc;
         if (out_host != nullptr && (rc = no_capture(rt, "a blocking verify")) != VQM_OK) return rc;
-        cudaError_t err = vqm::launch_verify(a, rt->sm_count, rt->stream);
+        cudaError_t err = vqm::launch_verify(a, rt->stream);
         if (err != cudaSuccess) return cuda_fail("verify launch", err);
         count_launch(rt);
         if (out_host != nullptr) {
