@@ -184,8 +184,9 @@ struct RowsI8Args {
     float *scales;         // [ntok]
     int cols, ntok, elem;
     float eps;
+    double inv_cols;       // 1 / cols, filled in by the launcher
 };
-cudaError_t launch_rows_i8(const RowsI8Args &a, cudaStream_t stream);
+cudaError_t launch_rows_i8(const RowsI8Args &a, int sm_count, cudaStream_t stream);
 
 struct QmmI8Args {
     const int8_t *w;       // [rows][w_pitch], 16-byte aligned, w_pitch a multiple of 16

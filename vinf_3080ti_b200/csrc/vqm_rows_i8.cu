@@ -1,8 +1,12 @@
 // Activation rows as 8-bit integers with a scale per row, after what a layer does to them on the way to a projection:
 //   v = x,  or silu(x) * x2,  or h = x + residual (rounded to its type and stored);   n = v * g / sqrt(mean(v^2) + eps), or v;
 //   s = max |n| / 127 in fp32,   q = n / s rounded to the nearest whole number, ties to even.
-// All of it is done in 64 bits: which of two whole numbers a value goes to is then decided by the formula, not by the order of 32-bit
-// roundings.
+// Which of two whole numbers a value goes to is decided by the formula, not by the order of 32-bit roundings: the mean and the largest value are
+// taken in 64 bits (the mean's square root cancels out of n / s but for the rounding of s), the values in 32, and a value that 32 bits leave next to a
+// half is worked out again in 64.
+//
+// A block per row, its values in registers between the two passes: memory is read and written once, which is what bounds it.
+// Rows too long for that, a norm of gated values, and rows whose largest value is out of fp32's middle range are worked out in 64 bits throughout.
 #include <cuda_fp16.h>
 
 #include "vqm_kernels.h"
@@ -10,21 +14,69 @@
 namespace vqm {
 namespace {
 
-constexpr int kRowThreads = 512;
-
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ void put(float *p, float v) { *p = v; }
 __device__ __forceinline__ void put(__half *p, float v) { *p = __float2half_rn(v); }
 
+template <int VEC>
+__device__ __forceinline__ void load(const float *p, float (&v)[VEC]) {
+    if constexpr (VEC == 4) {
+        const float4 w = *reinterpret_cast<const float4 *>(p);
+        v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+    } else {
+        v[0] = *p;
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void load(const __half *p, float (&v)[VEC]) {
+    if constexpr (VEC == 4) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(p);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
+        v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+    } else {
+        v[0] = __half2float(*p);
+    }
+}
+// stores v rounded to the buffer's type, and leaves that in v
+template <int VEC>
+__device__ __forceinline__ void store(float *p, float (&v)[VEC]) {
+    if constexpr (VEC == 4) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    else *p = v[0];
+}
+template <int VEC>
+__device__ __forceinline__ void store(__half *p, float (&v)[VEC]) {
+    if constexpr (VEC == 4) {
+        const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+        *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+        const float2 c = __half22float2(a), d = __half22float2(b);
+        v[0] = c.x, v[1] = c.y, v[2] = d.x, v[3] = d.y;
+    } else {
+        const __half a = __float2half_rn(v[0]);
+        *p = a;
+        v[0] = __half2float(a);
+    }
+}
+
+constexpr float kUndefined = __builtin_nanf("");
+constexpr double kMostScale = 3.4028235677973366e38;  // half a step above fp32's largest: rounds to infinity from here on
+
+struct RowShared {
+    double d[32];
+    float a[32];
+    int bad;
+    unsigned long long largest;  // bits of a positive number, which are in its order
+    double r, scale;
+    float factor;
+};
+
+// One row by the whole block, in 64 bits.
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) rows_i8_kernel(const RowsI8Args a) {
-    __shared__ double s_red[kRowThreads / 32];
-    __shared__ int s_bad;
-    const size_t row = blockIdx.x, at = row * a.cols;
+static __device__ __noinline__ void exact_row(const RowsI8Args &a, size_t row, bool total_is_there, RowShared &s) {
+    const size_t at = row * a.cols;
     const T *x = static_cast<const T *>(a.x) + at, *x2 = static_cast<const T *>(a.x2) + at, *res = static_cast<const T *>(a.residual) + at;
     T *total = static_cast<T *>(a.total) + at;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, threads = static_cast<int>(blockDim.x);
     auto value = [&](int c) -> double {
         if (a.residual != nullptr) return as_float(total[c]);  // (by the thread that wrote it)
         const double v = as_float(x[c]);
@@ -34,56 +86,342 @@ __global__ void __launch_bounds__(kRowThreads) rows_i8_kernel(const RowsI8Args a
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, off));
         __syncthreads();
-        if (lane == 0) s_red[warp] = v;
+        if (lane == 0) s.d[warp] = v;
         __syncthreads();
-        v = s_red[0];
-        for (int i = 1; i < kRowThreads / 32; ++i) v = op(v, s_red[i]);
+        v = s.d[0];
+        for (int i = 1; i < threads / 32; ++i) v = op(v, s.d[i]);
         return v;
     };
-    if (a.residual != nullptr)
-        for (int c = threadIdx.x; c < a.cols; c += kRowThreads) put(total + c, as_float(x[c]) + as_float(res[c]));
+    if (total_is_there) __syncthreads();  // (the threads of the fast pass hold other columns)
+    else if (a.residual != nullptr)
+        for (int c = threadIdx.x; c < a.cols; c += threads) put(total + c, as_float(x[c]) + as_float(res[c]));
     double r = 1.0;
     if (a.norm_w != nullptr) {
         double sum = 0.0;
-        for (int c = threadIdx.x; c < a.cols; c += kRowThreads) {
+        for (int c = threadIdx.x; c < a.cols; c += threads) {
             const double v = value(c);
             sum += v * v;
         }
         sum = combine(sum, [](double p, double q) { return p + q; });
         r = 1.0 / sqrt(sum / a.cols + static_cast<double>(a.eps));
     }
-    if (threadIdx.x == 0) s_bad = 0;
+    if (threadIdx.x == 0) s.bad = 0;
     double top = 0.0;
     bool bad = false;
-    for (int c = threadIdx.x; c < a.cols; c += kRowThreads) {
+    for (int c = threadIdx.x; c < a.cols; c += threads) {
         const double n = a.norm_w != nullptr ? value(c) * r * static_cast<double>(a.norm_w[c]) : value(c);
         bad |= !(fabs(n) <= 1e300);
         top = fmax(top, fabs(n));
     }
     top = combine(top, [](double p, double q) { return fmax(p, q); });
-    if (bad) s_bad = 1;
+    if (bad) s.bad = 1;
     __syncthreads();
-    float s = static_cast<float>(top / 127.0);
     // a value that is infinite or undefined makes the row's outputs undefined
-    if (s_bad || !(s <= 3.4028235e38f)) s = __int_as_float(0x7fc00000);
-    if (threadIdx.x == 0) a.scales[row] = s;
+    const float scale = s.bad || top / 127.0 >= kMostScale ? kUndefined : static_cast<float>(top / 127.0);
+    if (threadIdx.x == 0) a.scales[row] = scale;
     const long long pitch = i8_pitch(a.cols);
-    for (int c = threadIdx.x; c < pitch; c += kRowThreads) {
+    for (int c = threadIdx.x; c < pitch; c += threads) {
         int q = 0;
-        if (c < a.cols && s > 0.0f) {
+        if (c < a.cols && scale > 0.0f) {
             const double n = a.norm_w != nullptr ? value(c) * r * static_cast<double>(a.norm_w[c]) : value(c);
-            q = min(127, max(-127, __double2int_rn(n / static_cast<double>(s))));
+            q = min(127, max(-127, __double2int_rn(n / static_cast<double>(scale))));
         }
         a.q[row * pitch + c] = static_cast<int8_t>(q);
     }
 }
 
+template <typename T>
+__global__ void __launch_bounds__(512) exact_rows_kernel(const RowsI8Args a) {
+    __shared__ RowShared s;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    exact_row<T>(a, blockIdx.x, false, s);
+}
+
+// silu(x) * y in 64 bits
+static __device__ __noinline__ double exact_gate(float x, float y) { return static_cast<double>(x) / (1.0 + exp(-static_cast<double>(x))) * static_cast<double>(y); }
+
+__device__ __forceinline__ float largest_of(float a, float b) {  // undefined if either is
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+
+// r such that r r m = 1, in 64 bits: two steps of Newton's method from 22 bits
+__device__ __forceinline__ double inverse_root(double m) {
+    if (!(m > 1e-30 && m < 1e30)) return 1.0 / sqrt(m);
+    double r = static_cast<double>(rsqrtf(static_cast<float>(m)));
+    const double half = 0.5 * m;
+    r = fma(r, fma(-half * r, r, 0.5), r);
+    return fma(r, fma(-half * r, r, 0.5), r);
+}
+
+// VEC values in registers: as they come, or as floats where they are no longer of the buffer's type.
+template <typename T, int VEC, bool WIDE>
+struct Kept {
+    float f[VEC];
+    __device__ __forceinline__ void fetch(const T *p) { load<VEC>(p, f); }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int l = 0; l < VEC; ++l) f[l] = 0.0f;
+    }
+    __device__ __forceinline__ void values(float (&v)[VEC]) const {
+#pragma unroll
+        for (int l = 0; l < VEC; ++l) v[l] = f[l];
+    }
+    __device__ __forceinline__ void keep(const float (&v)[VEC]) {
+#pragma unroll
+        for (int l = 0; l < VEC; ++l) f[l] = v[l];
+    }
+    __device__ __forceinline__ void put_to(T *p) { store<VEC>(p, f); }
+};
+template <>
+struct Kept<__half, 4, false> {
+    uint2 w;
+    __device__ __forceinline__ void fetch(const __half *p) { w = *reinterpret_cast<const uint2 *>(p); }
+    __device__ __forceinline__ void clear() { w = make_uint2(0, 0); }
+    __device__ __forceinline__ void values(float (&v)[4]) const {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
+        v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+    }
+    __device__ __forceinline__ void keep(const float (&v)[4]) {
+        const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+        w = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    }
+    __device__ __forceinline__ void put_to(__half *p) const { *reinterpret_cast<uint2 *>(p) = w; }
+};
+
+// A block per row.  A thread holds NV vectors of VEC neighbouring columns (VEC 4 where rows start at multiples of 16 bytes), vector i at
+// (thread + i * threads) * VEC: v before the norm's weights, which come from the caches both times.
+template <typename T, int VEC, int NV, int THREADS, bool GATED>
+__global__ void __launch_bounds__(THREADS, THREADS != 256 ? 1 : VEC == 1 ? 4 : 3) rows_i8_kernel(const RowsI8Args a) {
+    __shared__ RowShared s;
+    constexpr int WARPS = THREADS / 32;
+    const size_t row = blockIdx.x, at = row * a.cols;
+    const T *x = static_cast<const T *>(a.x) + at, *second = static_cast<const T *>(a.x2 != nullptr ? a.x2 : a.residual) + at;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool norm = !GATED && a.norm_w != nullptr;
+    auto column = [&](int i) { return (static_cast<int>(threadIdx.x) + i * THREADS) * VEC; };
+    if (threadIdx.x == 0) s.largest = 0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    Kept<T, VEC, GATED> v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (column(i) < a.cols) v[i].fetch(x + column(i));
+        else v[i].clear();
+    float top = 0.0f;
+    if (GATED || a.residual != nullptr) {
+        Kept<T, VEC, false> y[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (column(i) < a.cols) y[i].fetch(second + column(i));
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (column(i) >= a.cols) continue;
+            float e[VEC], d[VEC];
+            v[i].values(e);
+            y[i].values(d);
+#pragma unroll
+            for (int l = 0; l < VEC; ++l) {
+                if (GATED) {
+                    // silu(-inf) is undefined; silu(-80) = -1e-33 may have lost digits, which shows if y is large: not this way
+                    if (e[l] < -80.0f && (fabsf(d[l]) > 1e3f || e[l] == -INFINITY)) top = INFINITY;
+                    e[l] = __fdividef(e[l], 1.0f + __expf(-e[l])) * d[l];
+                } else {
+                    e[l] += d[l];
+                }
+            }
+            v[i].keep(e);
+            if (!GATED) v[i].put_to(static_cast<T *>(a.total) + at + column(i));
+        }
+    }
+    double sum = 0.0;
+    if (norm) {
+        double part[2] = {};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (column(i) >= a.cols) continue;
+            float g[VEC], e[VEC];
+            load<VEC>(a.norm_w + column(i), g);
+            v[i].values(e);
+#pragma unroll
+            for (int l = 0; l < VEC; ++l) {
+                const double d = static_cast<double>(e[l]);
+                part[l & 1] = fma(d, d, part[l & 1]);
+                top = largest_of(top, fabsf(e[l] * g[l]));
+            }
+        }
+        sum = part[0] + part[1];
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float e[VEC];
+            v[i].values(e);
+#pragma unroll
+            for (int l = 0; l < VEC; ++l) top = largest_of(top, fabsf(e[l]));
+        }
+    }
+    const float own = top;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = largest_of(top, __shfl_xor_sync(0xffffffffu, top, off));
+    if (lane == 0) s.d[warp] = sum, s.a[warp] = top;
+    __syncthreads();
+    top = lane < WARPS ? s.a[lane] : 0.0f;
+#pragma unroll
+    for (int off = WARPS > 16 ? 16 : WARPS / 2; off > 0; off >>= 1) top = largest_of(top, __shfl_xor_sync(0xffffffffu, top, off));
+    top = __shfl_sync(0xffffffffu, top, 0);
+    if (!(top > (GATED ? 1e-20f : 1e-30f) && top < 1e30f)) {  // (the same in every thread: zero, tiny, huge, undefined)
+        exact_row<T>(a, row, true, s);
+        return;
+    }
+    // The largest in 64 bits.  Rounding keeps the order: of products with the norm's weights it is one whose rounded value is the largest.  Gated
+    // values: __expf and the division leave 2e-6, and 6e-8 |x| where the exponential counts (|x| < 90), so it is one within 2e-5 of it.
+    if (GATED || norm) {
+        const float least = GATED ? top * (1.0f - 2e-5f) : top;
+        if (own >= least) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (column(i) >= a.cols) continue;
+                float g[VEC], e[VEC];
+#pragma unroll
+                for (int l = 0; l < VEC; ++l) g[l] = 1.0f;
+                if (norm) load<VEC>(a.norm_w + column(i), g);
+                v[i].values(e);
+#pragma unroll
+                for (int l = 0; l < VEC; ++l)
+                    if (fabsf(e[l] * g[l]) >= least) {
+                        const double d = GATED ? exact_gate(as_float(x[column(i) + l]), as_float(second[column(i) + l])) : static_cast<double>(e[l]) * static_cast<double>(g[l]);
+                        atomicMax(&s.largest, static_cast<unsigned long long>(__double_as_longlong(fabs(d))));
+                    }
+            }
+        }
+    }
+    // One thread does what is left in 64 bits: that pipe is shared by the warps of all rows on the SM.
+    double r = 1.0;
+    if (norm && warp == 0) {
+        sum = lane < WARPS ? s.d[lane] : 0.0;
+#pragma unroll
+        for (int off = WARPS > 16 ? 16 : WARPS / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        r = inverse_root(fma(sum, a.inv_cols, static_cast<double>(a.eps)));
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const double largest = GATED || norm ? __longlong_as_double(static_cast<long long>(s.largest)) : static_cast<double>(top);
+        const double wide = norm ? largest * r * (1.0 / 127.0) : largest / 127.0;
+        const float scale = wide >= kMostScale ? kUndefined : static_cast<float>(wide);
+        s.r = r;
+        s.scale = static_cast<double>(scale);
+        s.factor = scale > 1e-37f ? __fdividef(static_cast<float>(r), scale) : 0.0f;
+        a.scales[row] = scale;
+    }
+    __syncthreads();
+    const float f = s.factor;  // about 127 / largest
+    if (f == 0.0f) {  // (a norm can take the scale out of the middle range; so can an undefined one)
+        exact_row<T>(a, row, true, s);
+        return;
+    }
+
+    // To whole numbers: the sum with 1.5 * 2^23 rounds to the nearest, and holds it in its last bits.  32 bits leave a value off by 6 * 2^-24 |t| (the product
+    // with the norm's weights, r, two of the division, the product with the factor), gated ones by up to 6e-6 |t| more; whoever is that near to a half is
+    // worked out in 64.
+    constexpr float kWhole = 12582912.0f, kOff = GATED ? 6.5e-6f : 4e-7f;
+    const long long pitch = i8_pitch(a.cols);
+    int8_t *out = a.q + row * pitch;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (column(i) >= a.cols) continue;
+        float g[VEC], t[VEC], e[VEC];
+        if (norm) load<VEC>(a.norm_w + column(i), g);
+        v[i].values(e);
+        uint32_t bits[VEC];
+        bool near = false;
+#pragma unroll
+        for (int l = 0; l < VEC; ++l) {
+            t[l] = (norm ? e[l] * g[l] : e[l]) * f;  // |t| < 127.1
+            const float k = t[l] + kWhole;
+            bits[l] = __float_as_uint(k);
+            const float sure = fmaf(fabsf(t[l]), -kOff, 0.5f);
+            t[l] = fabsf(t[l] - (k - kWhole)) - sure;
+            near |= t[l] > 0.0f;
+        }
+        if (near) {
+#pragma unroll
+            for (int l = 0; l < VEC; ++l)
+                if (t[l] > 0.0f) {
+                    double d = static_cast<double>(e[l]);
+                    if (GATED) d = exact_gate(as_float(x[column(i) + l]), as_float(second[column(i) + l]));
+                    else if (norm) d *= static_cast<double>(g[l]);
+                    bits[l] = static_cast<uint32_t>(__double2int_rn(d * s.r / s.scale));  // (divided: a tie stays a tie)
+                }
+        }
+        if constexpr (VEC == 4) *reinterpret_cast<uint32_t *>(out + column(i)) = __byte_perm(__byte_perm(bits[0], bits[1], 0x0040), __byte_perm(bits[2], bits[3], 0x0040), 0x5410);
+        else out[column(i)] = static_cast<int8_t>(bits[0]);
+    }
+    if (threadIdx.x < pitch - a.cols) out[a.cols + threadIdx.x] = 0;
+}
+
+template <typename K>
+cudaError_t launch_kernel(K kernel, const RowsI8Args &a, int threads, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(static_cast<unsigned>(a.ntok));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.stream = stream;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+template <typename T, int VEC, int NV, int THREADS>
+cudaError_t launch_variant(const RowsI8Args &a, cudaStream_t stream) {
+    return a.x2 != nullptr ? launch_kernel(rows_i8_kernel<T, VEC, NV, THREADS, true>, a, THREADS, stream)
+                           : launch_kernel(rows_i8_kernel<T, VEC, NV, THREADS, false>, a, THREADS, stream);
+}
+template <typename T, int THREADS>
+cudaError_t launch_vectors(const RowsI8Args &a, cudaStream_t stream) {  // at most 12 vectors of 4 columns per thread
+    const int n = (a.cols / 4 + THREADS - 1) / THREADS;
+    if (n <= 2) return launch_variant<T, 4, 2, THREADS>(a, stream);
+    if (n <= 5) return launch_variant<T, 4, 5, THREADS>(a, stream);
+    if (n <= 8) return launch_variant<T, 4, 8, THREADS>(a, stream);
+    if (n <= 10) return launch_variant<T, 4, 10, THREADS>(a, stream);
+    return launch_variant<T, 4, 12, THREADS>(a, stream);
+}
+template <typename T, int THREADS>
+cudaError_t launch_columns(const RowsI8Args &a, cudaStream_t stream) {  // at most 32 columns per thread
+    const int n = (a.cols + THREADS - 1) / THREADS;
+    if (n <= 4) return launch_variant<T, 1, 4, THREADS>(a, stream);
+    if (n <= 12) return launch_variant<T, 1, 12, THREADS>(a, stream);
+    return launch_variant<T, 1, 32, THREADS>(a, stream);
+}
+
+template <typename T>
+cudaError_t launch_t(const RowsI8Args &a, int sm_count, cudaStream_t stream) {
+    if (a.cols > 32768 || (a.x2 != nullptr && a.norm_w != nullptr)) return launch_kernel(exact_rows_kernel<T>, a, 512, stream);
+    const bool many = a.ntok > sm_count;  // few rows: as many threads on each as there are
+    if (a.cols % 4 == 0) {
+        if (a.cols <= 1024 && many) return launch_vectors<T, 32>(a, stream);
+        if (a.cols <= (sizeof(T) == 2 ? 6144 : 4096) && many) return launch_vectors<T, 128>(a, stream);
+        if (a.cols <= 12288 && many) return launch_vectors<T, 256>(a, stream);
+        if (a.cols <= 24576) return launch_vectors<T, 512>(a, stream);
+        return launch_variant<T, 4, 8, 1024>(a, stream);
+    }
+    if (a.cols <= 1024 && many) return launch_columns<T, 32>(a, stream);
+    if (a.cols <= 8192 && many) return launch_columns<T, 256>(a, stream);
+    return launch_columns<T, 1024>(a, stream);
+}
+
 }  // namespace
 
-cudaError_t launch_rows_i8(const RowsI8Args &a, cudaStream_t stream) {
-    if (a.elem == 2) rows_i8_kernel<__half><<<a.ntok, kRowThreads, 0, stream>>>(a);
-    else rows_i8_kernel<float><<<a.ntok, kRowThreads, 0, stream>>>(a);
-    return cudaGetLastError();
+cudaError_t launch_rows_i8(const RowsI8Args &in, int sm_count, cudaStream_t stream) {
+    RowsI8Args a = in;
+    a.inv_cols = 1.0 / a.cols;
+    return a.elem == 2 ? launch_t<__half>(a, sm_count, stream) : launch_t<float>(a, sm_count, stream);
 }
 
 }  // namespace vqm

@@ -1628,7 +1628,7 @@ int vqm_convert_i8(vqm_runtime *rt, const char *weight, const char *name) {
             a.cols = from->cols;
             a.ntok = static_cast<int>(n);
             a.elem = 4;
-            if (err == cudaSuccess) err = vqm::launch_rows_i8(a, rt->stream);
+            if (err == cudaSuccess) err = vqm::launch_rows_i8(a, rt->sm_count, rt->stream);
             if (err == cudaSuccess) count_launch(rt, 2);
         }
         const cudaError_t done = cudaStreamSynchronize(rt->stream);  // (products fetch weights ahead of the stream's order)
@@ -1675,7 +1675,7 @@ int vqm_rows_i8(vqm_runtime *rt, const char *x, const char *q, const char *scale
             if ((a.norm_w = find_norm(rt, norm_weight, cols, &rc)) == nullptr) return rc;
             if (!(eps >= 0.0f)) return fail(VQM_ERR_VALUE, "eps must be >= 0");
         }
-        const cudaError_t err = vqm::launch_rows_i8(a, rt->stream);
+        const cudaError_t err = vqm::launch_rows_i8(a, rt->sm_count, rt->stream);
         if (err != cudaSuccess) return cuda_fail("rows_i8 launch", err);
         count_launch(rt);
         return VQM_OK;
