@@ -75,3 +75,47 @@ def test_verification_on_small_numbers():
     assert F.verify(target, None, tokens, np.array([[0.29, 0.0]])).tolist() == [[1, 1, 0]]
     assert F.verify(target, None, tokens, np.array([[0.31, 0.75]])).tolist() == [[0, 2, -1]]
     assert F.verify(target, None, tokens, np.array([[0.31, 0.7]])).tolist() == [[0, 0, -1]]
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["native", "ctypes"])
+def test_calls_hand_their_arguments_on(lib, native, monkeypatch):
+    got = []
+    P, S, I, Fl = ctypes.c_void_p, ctypes.c_char_p, ctypes.c_int, ctypes.c_float
+
+    def fake(*kinds):
+        @ctypes.CFUNCTYPE(I, P, *kinds)
+        def fn(*args):
+            got.append(args)
+            return 4
+
+        return fn
+
+    fakes = {"rows_i8": fake(S, S, S, I, I, I, S, S, S, S, Fl), "qmm_i8": fake(S, S, S, S, I, I), "verify": fake(S, S, S, S, S, S, I, I, I, S, P)}
+    if native:
+        call = {n: lambda *a, n=n: getattr(_capi.pycall(), n)(ctypes.cast(fakes[n], P).value, *a) for n in fakes}
+    else:
+        monkeypatch.setattr(_capi, "_callers", {})
+        monkeypatch.setattr(_capi, "pycall", lambda: None)
+        monkeypatch.setattr(_capi, "load", lambda: type("Lib", (), {"vqm_" + n: staticmethod(f) for n, f in fakes.items()}))
+        call = {n: _capi.caller(n) for n in fakes}
+    host = (ctypes.c_int * 4)()
+    at = ctypes.addressof(host)
+    assert call["rows_i8"](123, "x", "größe", "s", 5120, np.int64(3), 9, None, "r", None, "g", 0.5) == 4
+    assert call["qmm_i8"](123, "w", "q", "s", "y", 2**32 + 9, True) == 4
+    assert call["verify"](123, "t", None, "k", None, "u", "temp", 9, 2, 1, "o", at) == 4
+    assert call["verify"](123, "t", "d", None, "l", "u", None, 9, 2, 0, "o", 0) == 4
+    assert got == [(123, b"x", "größe".encode(), b"s", 5120, 3, 9, None, b"r", None, b"g", 0.5), (123, b"w", b"q", b"s", b"y", 9, 1),
+                   (123, b"t", None, b"k", None, b"u", b"temp", 9, 2, 1, b"o", at), (123, b"t", b"d", None, b"l", b"u", None, 9, 2, 0, b"o", None)]
+    for name, args in (("rows_i8", (None, "x", "q", "s", 1, 1, 0, None, None, None, None, 0.0)), ("qmm_i8", (None, "w", "q", "s", "y", 1, 0))):
+        with pytest.raises((TypeError, ValueError)):  # a closed runtime
+            call[name](*args)
+    if native:
+        for name, args in (("rows_i8", (1, b"x", "q", "s", 1, 1, 0, None, None, None, None, 0.0)), ("rows_i8", (1, "x", "q", "s", 1, 1, 0, None, None, None, 5, 0.0)),
+                           ("qmm_i8", (1, "w", None, "s", "y", 1, 0)), ("verify", (1, None, "d", None, "l", "u", None, 9, 2, 0, "o", 0))):
+            with pytest.raises(AttributeError):
+                call[name](*args)
+        for name, args in (("rows_i8", (1, "x", "q", "s", "a", 1, 0, None, None, None, None, 0.0)), ("rows_i8", (1, "x", "q", "s", 1, 1, 0, None, None, None, None, "e")),
+                           ("qmm_i8", (1, "w", "q", "s", "y", None, 0)), ("qmm_i8", (1, "w", "q", "s", "y", 1))):
+            with pytest.raises((TypeError, ValueError)):
+                call[name](*args)
+    assert len(got) == 4

@@ -6,6 +6,7 @@ CPU or PyTorch fallback.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from ctypes import POINTER, c_char_p, c_int, c_size_t, c_uint64, c_void_p
 from pathlib import Path
@@ -113,6 +114,29 @@ def qmv_caller():
         return fn(handle, weight.encode("utf-8"), x.encode("utf-8"), y.encode("utf-8"), int(ntok))
 
     return call, None
+
+
+_callers: dict = {}
+
+
+def caller(name: str):
+    """vqm_<name> on Python's str (or None), int and float, without ctypes where that can be."""
+    call = _callers.get(name)
+    if call is None:
+        fn, native = getattr(load(), "vqm_" + name), getattr(pycall(), name, None)
+        if native is not None:
+            call = functools.partial(native, ctypes.cast(fn, c_void_p).value)
+        else:
+            def call(handle, *args):
+                if not handle:
+                    raise ValueError("the runtime is closed")
+                # (the same Python errors as without ctypes: names are str, addresses of answers stand last)
+                args = [a.encode("utf-8") if isinstance(a, str) else a for a in args]
+                kinds = SIGNATURES["vqm_" + name][1:]
+                return fn(handle, *(ctypes.cast(a or None, k) if issubclass(k, ctypes._Pointer) else int(a) if k is c_int else float(a) if k is ctypes.c_float else a
+                                    for a, k in zip(args, kinds)))
+        _callers[name] = call
+    return call
 
 
 def load() -> ctypes.CDLL:

@@ -39,7 +39,25 @@ struct QmmTc {
     int y_elem, add;
 };
 
-using tc::bar_arrive, tc::bar_init, tc::bar_try, tc::bar_wait, tc::bar_wait_cluster, tc::in_block, tc::s32;
+using tc::bar_arrive, tc::bar_init, tc::bar_try, tc::bar_try_cluster, tc::in_block, tc::s32;
+
+// Bounded; false once this or another wait of the block has given up.  A wait that succeeds looks at nothing but its barrier: the loops below have some
+// 500 cycles per stage.
+template <bool CLUSTER>
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *failed) {
+    unsigned long long began = 0;
+#pragma unroll 1
+    for (uint32_t i = 1;; ++i) {
+        if (CLUSTER ? bar_try_cluster(bar, parity) : bar_try(bar, parity)) return true;
+        if ((i & 255u) == 0 && tc::give_up(&began, failed)) return false;
+    }
+}
+// The same by one lane for its warp.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *failed) {
+    int ok = 1;
+    if ((threadIdx.x & 31) == 0) ok = wait<false>(bar, parity, failed) ? 1 : 0;
+    return __shfl_sync(0xFFFFFFFFu, ok, 0) != 0;
+}
 
 __device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {  // K-major, 128-byte swizzle, groups of 8 rows 1024 bytes apart
     return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
@@ -163,13 +181,14 @@ __global__ void __launch_bounds__(kQThreads, 1) qmm_i8_kernel(const __grid_const
             auto copy_q = [&](int stage, int k, int tok_tile) {
                 copy_tile(ring + stage * stage_bytes + kQA, &q_map, k * kQCols, tok_tile * a.n + rank * (a.n / 2), s32(&s_full[stage]));
             };
-            int it = 0, issued = 0;
+            int issued = 0, stage = 0;
+            uint32_t parity = 1;  // of the wait for a stage that is being used again
             bool ok = true;
             for (int tile = cluster; tile < n_tiles && ok; tile += n_clusters) {
                 int row_tile, tok_tile;
                 place(tile, row_tile, tok_tile);
                 int k = k0;
-                if (it == 0) {
+                if (issued == 0) {
                     // Weights are in place before the launch; what the kernel before this one in the stream makes, the activations, is waited for.
                     const int ahead = min(a.stages, k1 - k0);
                     for (int i = 0; i < ahead; ++i) {
@@ -178,22 +197,21 @@ __global__ void __launch_bounds__(kQThreads, 1) qmm_i8_kernel(const __grid_const
                     }
                     asm volatile("griddepcontrol.wait;" ::: "memory");
                     for (int i = 0; i < ahead; ++i) copy_q(i, k0 + i, tok_tile);
-                    it = issued = ahead;
+                    issued = ahead;
                     k += ahead;
+                    if (ahead == a.stages) parity = 0;
+                    else stage = ahead;
                 }
-                for (; k < k1; ++k, ++it) {
-                    const int stage = it % a.stages, use = it / a.stages;
-                    if (use > 0) {
-                        bar_wait(s32(&s_empty[stage]), (use - 1) & 1, failed);
-                        if (*failed) {
-                            ok = false;
-                            break;
-                        }
+                for (; k < k1; ++k) {
+                    if (issued >= a.stages && !wait<false>(s32(&s_empty[stage]), parity, failed)) {
+                        ok = false;
+                        break;
                     }
                     expect(s32(&s_full[stage]), stage_bytes);
                     copy_w(stage, k, row_tile);
                     copy_q(stage, k, tok_tile);
-                    issued = it + 1;
+                    ++issued;
+                    if (++stage == a.stages) stage = 0, parity ^= 1;
                 }
             }
             if (!ok)  // the last copies land before the block may leave
@@ -202,40 +220,39 @@ __global__ void __launch_bounds__(kQThreads, 1) qmm_i8_kernel(const __grid_const
         }
         __syncwarp();
     } else if (warp == 1) {
-        const bool first = rank == 0;
-        // D s32, A and B s8, K-major
-        const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(a.n >> 3) << 17) | (static_cast<uint32_t>(GROUP * kQRows >> 4) << 24);
-        int it = 0, done = 0;
-        for (int tile = cluster; tile < n_tiles; tile += n_clusters, ++done) {
-            const int buf = SPLIT ? 0 : done & 1;
-            if (first && done >= 2) {
-                if constexpr (PAIR) bar_wait_cluster(s32(&s_acc_empty[buf]), ((done >> 1) - 1) & 1, failed);
-                else bar_wait(s32(&s_acc_empty[buf]), ((done >> 1) - 1) & 1, failed);
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            }
-            for (int k = k0; k < k1; ++k, ++it) {
-                const int stage = it % a.stages;
-                const uint32_t full = s32(&s_full[stage]), parity = (it / a.stages) & 1;
-                if (PAIR && first) bar_wait_cluster(full, parity, failed);
-                else bar_wait(full, parity, failed);
-                if (__any_sync(0xFFFFFFFFu, *failed)) break;
-                if (first) {
+        if (tc::elect_one()) {
+            // D s32, A and B s8, K-major
+            const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(a.n >> 3) << 17) | (static_cast<uint32_t>(GROUP * kQRows >> 4) << 24);
+            int stage = 0, done = 0;
+            uint32_t parity = 0;
+            bool ok = true;
+            for (int tile = cluster; tile < n_tiles && ok; tile += n_clusters, ++done) {
+                const int buf = SPLIT ? 0 : done & 1;
+                if (rank == 0 && done >= 2) {
+                    ok = wait<PAIR>(s32(&s_acc_empty[buf]), ((done >> 1) - 1) & 1, failed);
+                    if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (tc::elect_one()) {
+                }
+                const uint32_t acc = tmem + buf * a.acc_cols;
+                for (int k = k0; k < k1; ++k) {
+                    const uint32_t full = s32(&s_full[stage]);
+                    ok = PAIR && rank == 0 ? wait<true>(full, parity, failed) : wait<false>(full, parity, failed);
+                    if (!ok) break;
+                    if (rank == 0) {
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         const uint64_t w_desc = tile_desc(ring + stage * stage_bytes), q_desc = tile_desc(ring + stage * stage_bytes + kQA);
 #pragma unroll
-                        for (int j = 0; j < kQCols / 32; ++j) mma_i8<PAIR>(tmem + buf * a.acc_cols, w_desc + 2 * j, q_desc + 2 * j, idesc, (k > k0 || j > 0) ? 1u : 0u);
+                        for (int j = 0; j < kQCols / 32; ++j) mma_i8<PAIR>(acc, w_desc + 2 * j, q_desc + 2 * j, idesc, (k > k0 || j > 0) ? 1u : 0u);
                         commit<PAIR>(s32(&s_empty[stage]), static_cast<uint32_t>(part));
+                    } else {
+                        arrive_in(in_block(full, static_cast<int>(leader)));
                     }
-                    __syncwarp();
-                } else if (lane == 0) {
-                    arrive_in(in_block(full, static_cast<int>(leader)));
+                    if (++stage == a.stages) stage = 0, parity ^= 1;
                 }
+                if (ok && rank == 0) commit<PAIR>(s32(&s_acc_full[buf]), static_cast<uint32_t>(part));
             }
-            if (__any_sync(0xFFFFFFFFu, *failed)) break;
-            if (first && tc::elect_one()) commit<PAIR>(s32(&s_acc_full[buf]), static_cast<uint32_t>(part));
-            __syncwarp();
         }
+        __syncwarp();
     }
 
     if constexpr (!SPLIT) {
@@ -248,8 +265,7 @@ __global__ void __launch_bounds__(kQThreads, 1) qmm_i8_kernel(const __grid_const
                 place(tile, row_tile, tok_tile);
                 const int buf = done & 1, row = (row_tile * GROUP + rank) * kQRows + lanes * 32 + lane;
                 const float w_scale = row < a.rows ? __ldg(a.w_scales + row) : 0.0f;
-                bar_wait(s32(&s_acc_full[buf]), (done >> 1) & 1, failed);
-                if (__any_sync(0xFFFFFFFFu, *failed)) break;
+                if (!warp_wait(s32(&s_acc_full[buf]), (done >> 1) & 1, failed)) break;
                 if (tile + n_clusters >= n_tiles) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t at = tmem + buf * a.acc_cols + (static_cast<uint32_t>(lanes * 32) << 16);
@@ -272,7 +288,7 @@ __global__ void __launch_bounds__(kQThreads, 1) qmm_i8_kernel(const __grid_const
         const int lanes = warp & 3, half = (warp - 4) >> 2;
         const uint32_t at = tmem + (static_cast<uint32_t>(lanes * 32) << 16);
         if (warp >= 4) {
-            bar_wait(s32(&s_acc_full[0]), 0, failed);
+            (void)warp_wait(s32(&s_acc_full[0]), 0, failed);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
         cluster_sync();  // every block's MMAs are done with its stages

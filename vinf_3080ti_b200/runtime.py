@@ -299,12 +299,15 @@ class Runtime:
         """Activation rows as 8-bit integers `q` with a scale per row, after the residual's addition (the sum goes to `total`, or back to
         `residual`) or silu(x) * silu_mul, and the rms norm with the weights `norm`, where given.  Asynchronous."""
         flags = (1 if residual is not None else 0) | (2 if norm is not None else 0) | (8 if silu_mul is not None else 0)
-        _capi.check(self._lib.vqm_rows_i8(self._h, _name(x), _name(q), _name(scales), int(cols), int(ntok), flags, _name(silu_mul), _name(residual),
-                                          _name(total), _name(norm), float(eps)))
+        status = _capi.caller("rows_i8")(self._h.value, x, q, scales, cols, ntok, flags, silu_mul, residual, total, norm, eps)
+        if status:
+            _capi.check(status)
 
     def qmm_i8(self, weight: str, q: str, scales: str, y: str, ntok: int = 1, *, add: bool = False) -> None:
         """y (+)= W x for a tensor of 8-bit integer rows and activations from rows_i8.  Asynchronous."""
-        _capi.check(self._lib.vqm_qmm_i8(self._h, _name(weight), _name(q), _name(scales), _name(y), int(ntok), 1 if add else 0))
+        status = _capi.caller("qmm_i8")(self._h.value, weight, q, scales, y, ntok, 1 if add else 0)
+        if status:
+            _capi.check(status)
 
     def verify(self, target: str, draft: str | None, tokens: str | None, uniforms: str, vocab: int, seqs: int, drafts: int, *, out: str,
                lens: str | None = None, temperature: str | None = None, blocking: bool = True) -> list[list[int]] | None:
@@ -313,8 +316,10 @@ class Runtime:
         if seqs < 1 or drafts < 0 or drafts > MAX_DRAFTS:
             raise ValueError(f"seqs must be positive and drafts in [0, {MAX_DRAFTS}]")
         host = (ctypes.c_int * (seqs * (drafts + 2)))() if blocking else None
-        _capi.check(self._lib.vqm_verify(self._h, _name(target), _name(draft), _name(tokens), _name(lens), _name(uniforms), _name(temperature),
-                                         int(vocab), int(seqs), int(drafts), _name(out), host))
+        status = _capi.caller("verify")(self._h.value, target, draft, tokens, lens, uniforms, temperature, vocab, seqs, drafts, out,
+                                        ctypes.addressof(host) if blocking else 0)
+        if status:
+            _capi.check(status)
         if host is None:
             return None
         rows = [list(host[i * (drafts + 2):(i + 1) * (drafts + 2)]) for i in range(seqs)]
