@@ -24,7 +24,10 @@ namespace {
 constexpr int kQRows = 128, kQCols = 128;           // weight rows of a block's tile, columns of a stage
 constexpr int kQA = kQRows * kQCols;                // bytes of a stage's weights
 constexpr int kQMaxN = 256, kQMaxStages = 12, kQMaxSplit = 8;
-constexpr int kQRing = 216 * 1024;                  // shared memory of the stages
+// Shared memory of the stages.  Blocks of few activation rows, which wait for memory, take half an SM: those of the next launch are there already, with
+// their first weights on the way, while the last outputs are written.
+constexpr int kQRing = 216 * 1024, kQHalfRing = 104 * 1024;
+constexpr int kQHalfMost = 80;  // activation rows up to which half an SM holds four stages
 constexpr int kQWriters = 8, kQThreads = 128 + 32 * kQWriters;
 
 struct QmmTc {
@@ -37,6 +40,7 @@ struct QmmTc {
     int acc_cols, tmem_cols;           // tensor-memory columns from one accumulator to the next, and in all
     int split;                         // blocks (pairs) that share a tile's columns
     int y_elem, add;
+    int half_sm;                       // two blocks per SM
 };
 
 using tc::bar_arrive, tc::bar_init, tc::bar_try, tc::bar_try_cluster, tc::in_block, tc::s32;
@@ -93,35 +97,47 @@ __device__ __forceinline__ void commit(uint32_t bar, uint32_t pair) {
         tc::commit(bar);
     }
 }
-__device__ __forceinline__ void load8(uint32_t at, int (&v)[8]) {
+template <int N>
+__device__ __forceinline__ void load_sums(uint32_t at, int (&v)[N]) {
     __syncwarp();
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                 : "r"(at)
-                 : "memory");
+    if constexpr (N == 8)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                     : "r"(at)
+                     : "memory");
+    else
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
+                       "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                     : "r"(at)
+                     : "memory");
 }
 __device__ __forceinline__ void loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// 8 activation rows from `tok` on of this lane's weight row.
-__device__ __forceinline__ void write8(const QmmTc &a, const int (&v)[8], int row, int tok, float w_scale) {
-    if (row >= a.rows) return;
+__device__ __forceinline__ void put(float *y, float v, bool add) { *y = add ? *y + v : v; }
+__device__ __forceinline__ void put(__half *y, float v, bool add) { *y = __float2half_rn(add ? __half2float(*y) + v : v); }
+
+// Outputs of this lane's weight row for N activation rows from `tok` on.  The activation rows' scales are read by one lane each.
+template <typename Y, bool ADD, int N>
+__device__ __forceinline__ void write_rows(const QmmTc &a, const int (&v)[N], int row, int tok, float w_scale) {
+    const int lane = threadIdx.x & 31, left = a.ntok - tok;
+    const float scales = lane < N && lane < left ? a.q_scales[tok + lane] : 0.0f;
+    Y *y = static_cast<Y *>(a.y) + static_cast<size_t>(tok) * a.rows + row;
+    const bool mine = row < a.rows;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        if (tok + j >= a.ntok) break;
-        const float out = static_cast<float>(v[j]) * a.q_scales[tok + j] * w_scale;
-        const size_t at = static_cast<size_t>(tok + j) * a.rows + row;
-        if (a.y_elem == 2) {
-            __half *y = static_cast<__half *>(a.y) + at;
-            *y = __float2half_rn(a.add ? __half2float(*y) + out : out);
-        } else {
-            float *y = static_cast<float *>(a.y) + at;
-            *y = a.add ? *y + out : out;
-        }
+    for (int j = 0; j < N; ++j, y += a.rows) {
+        const float out = static_cast<float>(v[j]) * __shfl_sync(0xFFFFFFFFu, scales, j) * w_scale;
+        if (mine && j < left) put(y, out, ADD);
     }
+}
+template <int N>
+__device__ __forceinline__ void write_any(const QmmTc &a, const int (&v)[N], int row, int tok, float w_scale) {
+    if (a.y_elem == 2) a.add ? write_rows<__half, true>(a, v, row, tok, w_scale) : write_rows<__half, false>(a, v, row, tok, w_scale);
+    else a.add ? write_rows<float, true>(a, v, row, tok, w_scale) : write_rows<float, false>(a, v, row, tok, w_scale);
 }
 
 template <bool PAIR, bool SPLIT>
-__global__ void __launch_bounds__(kQThreads, 1) qmm_i8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap q_map, const QmmTc a) {
+__global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap q_map, const QmmTc a) {
     constexpr int GROUP = PAIR ? 2 : 1;
     extern __shared__ uint8_t ring_raw[];
     __shared__ __align__(8) uint64_t s_full[kQMaxStages], s_empty[kQMaxStages], s_acc_full[2], s_acc_empty[2];
@@ -138,6 +154,7 @@ __global__ void __launch_bounds__(kQThreads, 1) qmm_i8_kernel(const __grid_const
     const int n_tiles = a.row_tiles * a.tok_tiles;
     const uint32_t stage_bytes = kQA + a.b_bytes;
 
+    if (a.half_sm) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; ++s) {
             bar_init(s32(&s_full[s]), PAIR && rank == 0 ? 2 : 1);  // the first block of a pair hears of the second's stage
@@ -269,12 +286,17 @@ __global__ void __launch_bounds__(kQThreads, 1) qmm_i8_kernel(const __grid_const
                 if (tile + n_clusters >= n_tiles) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t at = tmem + buf * a.acc_cols + (static_cast<uint32_t>(lanes * 32) << 16);
-                for (int c = half * 8; c < a.n; c += 16) {
-                    int v[8];
-                    load8(at + c, v);
+                int v[16], next[16];
+                load_sums(at + half * 16, v);  // (pairs' tiles and those of more than 16 rows are wide enough; of 16 the second warp reads and writes nothing)
+#pragma unroll 1
+                for (int c = half * 16; c < a.n; c += 32) {
                     loaded();
-                    write8(a, v, row, tok_tile * a.n + c, w_scale);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) next[j] = v[j];
+                    if (c + 32 < a.n) load_sums(at + c + 32, v);  // (on its way while these are written)
+                    write_any(a, next, row, tok_tile * a.n + c, w_scale);
                 }
+                loaded();
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
@@ -287,7 +309,13 @@ __global__ void __launch_bounds__(kQThreads, 1) qmm_i8_kernel(const __grid_const
         // One tile; its sums go, 8 columns of 32 lanes at a time, to the block that writes them: unit u to part u % split.
         const int lanes = warp & 3, half = (warp - 4) >> 2;
         const uint32_t at = tmem + (static_cast<uint32_t>(lanes * 32) << 16);
+        int row_tile, tok_tile;
+        place(cluster, row_tile, tok_tile);
+        const int row = (row_tile * GROUP + rank) * kQRows + lanes * 32 + lane;
+        float w_scale = 0.0f;
         if (warp >= 4) {
+            if (row < a.rows) w_scale = __ldg(a.w_scales + row);
+            asm volatile("griddepcontrol.wait;" ::: "memory");
             (void)warp_wait(s32(&s_acc_full[0]), 0, failed);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
@@ -297,7 +325,7 @@ __global__ void __launch_bounds__(kQThreads, 1) qmm_i8_kernel(const __grid_const
                 const int unit = c * 4 + lanes, owner = unit % a.split;
                 if (owner == part) continue;
                 int v[8];
-                load8(at + c * 8, v);
+                load_sums(at + c * 8, v);
                 loaded();
                 const uint32_t to = in_block(ring + ((unit / a.split) * (a.split - 1) + (part < owner ? part : part - 1)) * 1024 + lane * 16, owner * GROUP + rank);
                 asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
@@ -306,24 +334,19 @@ __global__ void __launch_bounds__(kQThreads, 1) qmm_i8_kernel(const __grid_const
         }
         cluster_sync();
         if (warp >= 4) {
-            asm volatile("griddepcontrol.wait;" ::: "memory");
             asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-            int row_tile, tok_tile;
-            place(cluster, row_tile, tok_tile);
-            const int row = (row_tile * GROUP + rank) * kQRows + lanes * 32 + lane;
-            const float w_scale = row < a.rows ? __ldg(a.w_scales + row) : 0.0f;
             for (int c = half; c < a.n / 8; c += 2) {
                 const int unit = c * 4 + lanes;
                 if (unit % a.split != part) continue;
                 int v[8];
-                load8(at + c * 8, v);
+                load_sums(at + c * 8, v);
                 loaded();
                 for (int p = 0; p < a.split - 1; ++p) {
                     const uint32_t from = ring + ((unit / a.split) * (a.split - 1) + p) * 1024 + lane * 16;
                     const uint4 x = lds128u(from), z = lds128u(from + 512);
                     v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += z.x, v[5] += z.y, v[6] += z.z, v[7] += z.w;
                 }
-                if (!*failed) write8(a, v, row, tok_tile * a.n + c * 8, w_scale);
+                if (!*failed) write_any(a, v, row, tok_tile * a.n + c * 8, w_scale);
             }
         }
     }
@@ -351,13 +374,13 @@ cudaError_t encode_rows(CUtensorMap *map, const int8_t *rows_at, int cols, long 
 
 template <bool PAIR, bool SPLIT>
 struct Variant {
-    static constexpr int kSmem = kQRing + 1024;
+    static constexpr int smem(bool half) { return (half ? kQHalfRing : kQRing) + 1024; }
     static constexpr int kGroup = PAIR ? 2 : 1;
     static constexpr auto kKernel = qmm_i8_kernel<PAIR, SPLIT>;
-    static void configure(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int clusters, int split, cudaStream_t stream) {
+    static void configure(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int clusters, int split, bool half, cudaStream_t stream) {
         cfg.gridDim = dim3(static_cast<unsigned>(clusters * split * kGroup));
         cfg.blockDim = dim3(kQThreads);
-        cfg.dynamicSmemBytes = kSmem;
+        cfg.dynamicSmemBytes = smem(half);
         cfg.stream = stream;
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -367,15 +390,15 @@ struct Variant {
         cfg.attrs = attr;
         cfg.numAttrs = 2;
     }
-    // clusters that fit on the GPU at once (cached; one device per process), 0 if the kernel cannot run
+    // clusters that fit on the GPU at once, one block per SM (cached; one device per process), 0 if the kernel cannot run
     static int clusters(int split) {
         static int cached[kQMaxSplit + 1] = {};
         if (cached[split] == 0) {
             int n = 0;
             cudaLaunchConfig_t cfg{};
             cudaLaunchAttribute attr[2];
-            configure(cfg, attr, 1024, split, nullptr);
-            if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kKernel, &cfg) != cudaSuccess) {
+            configure(cfg, attr, 1024, split, false, nullptr);
+            if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem(false)) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kKernel, &cfg) != cudaSuccess) {
                 (void)cudaGetLastError();
                 n = 0;
             }
@@ -388,7 +411,7 @@ struct Variant {
         if (fit == 0) return cudaErrorInvalidConfiguration;
         cudaLaunchConfig_t cfg{};
         cudaLaunchAttribute attr[2];
-        configure(cfg, attr, SPLIT ? tiles : (tiles < fit ? tiles : fit), a.split, stream);
+        configure(cfg, attr, SPLIT ? tiles : (tiles < fit ? tiles : fit), a.split, a.half_sm != 0, stream);
         return cudaLaunchKernelEx(&cfg, kKernel, w, q, a);
     }
 };
@@ -412,11 +435,14 @@ cudaError_t launch_qmm_i8(const QmmI8Args &in, int sm_count, cudaStream_t stream
     a.n = ((in.ntok + a.tok_tiles - 1) / a.tok_tiles + step - 1) / step * step;
     a.tok_tiles = (in.ntok + a.n - 1) / a.n;
     a.row_tiles = (in.rows + group * kQRows - 1) / (group * kQRows);
+    a.half_sm = !pair && a.n <= kQHalfMost;
+    // As many parts of the columns as leave every cluster room beside the others, of two stages at least.
     a.split = 1;
     const int tiles = a.row_tiles * a.tok_tiles;
-    while (a.split < (pair ? 4 : kQMaxSplit) && tiles * group * (a.split + 1) <= sm_count && a.n_k / (a.split + 1) >= 2) ++a.split;
+    for (int split = 2; split <= (pair ? kQMaxSplit / 2 : kQMaxSplit) && a.n_k >= 2 * split; ++split)
+        if (tiles <= (pair ? Variant<true, true>::clusters(split) : Variant<false, true>::clusters(split))) a.split = split;
     a.b_bytes = a.n / group * kQCols;
-    a.stages = kQRing / (kQA + a.b_bytes);
+    a.stages = (a.half_sm ? kQHalfRing : kQRing) / (kQA + a.b_bytes);
     if (a.stages > kQMaxStages) a.stages = kQMaxStages;
     a.acc_cols = 32;
     while (a.acc_cols < a.n) a.acc_cols *= 2;
