@@ -26,8 +26,7 @@ constexpr int kQA = kQRows * kQCols;                // bytes of a stage's weight
 constexpr int kQMaxN = 256, kQMaxStages = 12, kQMaxSplit = 8;
 // Shared memory of the stages.  Blocks of few activation rows, which wait for memory, take half an SM: those of the next launch are there already, with
 // their first weights on the way, while the last outputs are written.
-constexpr int kQRing = 216 * 1024, kQHalfRing = 104 * 1024;
-constexpr int kQHalfMost = 80;  // activation rows up to which half an SM holds four stages
+constexpr int kQRing = 216 * 1024, kQHalfRing = 108 * 1024;
 constexpr int kQWriters = 8, kQThreads = 128 + 32 * kQWriters;
 
 struct QmmTc {
@@ -39,6 +38,7 @@ struct QmmTc {
     int stages, b_bytes;               // of the ring; bytes of a block's activations in a stage
     int acc_cols, tmem_cols;           // tensor-memory columns from one accumulator to the next, and in all
     int split;                         // blocks (pairs) that share a tile's columns
+    int exchange;                      // where in the ring's memory they leave sums for one another, if not where the stages are (0)
     int y_elem, add;
     int half_sm;                       // two blocks per SM
 };
@@ -60,6 +60,7 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *failed) {
     int ok = 1;
     if ((threadIdx.x & 31) == 0) ok = wait<false>(bar, parity, failed) ? 1 : 0;
+    __syncwarp();
     return __shfl_sync(0xFFFFFFFFu, ok, 0) != 0;
 }
 
@@ -117,23 +118,28 @@ __device__ __forceinline__ void loaded() { asm volatile("tcgen05.wait::ld.sync.a
 __device__ __forceinline__ void put(float *y, float v, bool add) { *y = add ? *y + v : v; }
 __device__ __forceinline__ void put(__half *y, float v, bool add) { *y = __float2half_rn(add ? __half2float(*y) + v : v); }
 
-// Outputs of this lane's weight row for N activation rows from `tok` on.  The activation rows' scales are read by one lane each.
+// Outputs of this lane's weight row for N activation rows from `tok` on, whose scales are in shared memory.
 template <typename Y, bool ADD, int N>
-__device__ __forceinline__ void write_rows(const QmmTc &a, const int (&v)[N], int row, int tok, float w_scale) {
-    const int lane = threadIdx.x & 31, left = a.ntok - tok;
-    const float scales = lane < N && lane < left ? a.q_scales[tok + lane] : 0.0f;
+__device__ __forceinline__ void write_rows(const QmmTc &a, const int (&v)[N], int row, int tok, float w_scale, const float *scales) {
+    const int left = a.ntok - tok;
     Y *y = static_cast<Y *>(a.y) + static_cast<size_t>(tok) * a.rows + row;
     const bool mine = row < a.rows;
 #pragma unroll
     for (int j = 0; j < N; ++j, y += a.rows) {
-        const float out = static_cast<float>(v[j]) * __shfl_sync(0xFFFFFFFFu, scales, j) * w_scale;
+        const float out = static_cast<float>(v[j]) * scales[j] * w_scale;
         if (mine && j < left) put(y, out, ADD);
     }
 }
 template <int N>
-__device__ __forceinline__ void write_any(const QmmTc &a, const int (&v)[N], int row, int tok, float w_scale) {
-    if (a.y_elem == 2) a.add ? write_rows<__half, true>(a, v, row, tok, w_scale) : write_rows<__half, false>(a, v, row, tok, w_scale);
-    else a.add ? write_rows<float, true>(a, v, row, tok, w_scale) : write_rows<float, false>(a, v, row, tok, w_scale);
+__device__ __forceinline__ void write_any(const QmmTc &a, const int (&v)[N], int row, int tok, float w_scale, const float *scales) {
+    if (a.y_elem == 2) a.add ? write_rows<__half, true>(a, v, row, tok, w_scale, scales) : write_rows<__half, false>(a, v, row, tok, w_scale, scales);
+    else a.add ? write_rows<float, true>(a, v, row, tok, w_scale, scales) : write_rows<float, false>(a, v, row, tok, w_scale, scales);
+}
+// A tile's activation scales, by the writers (256 threads), and a barrier among them.
+__device__ __forceinline__ void fetch_scales(const QmmTc &a, int tok, float *to) {
+    const int i = static_cast<int>(threadIdx.x) - 128;
+    if (i < a.n) to[i] = tok + i < a.ntok ? a.q_scales[tok + i] : 0.0f;
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kQWriters) : "memory");
 }
 
 template <bool PAIR, bool SPLIT>
@@ -141,6 +147,8 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
     constexpr int GROUP = PAIR ? 2 : 1;
     extern __shared__ uint8_t ring_raw[];
     __shared__ __align__(8) uint64_t s_full[kQMaxStages], s_empty[kQMaxStages], s_acc_full[2], s_acc_empty[2];
+    __shared__ __align__(8) uint64_t s_sums;
+    __shared__ float s_scales[2][kQMaxN];
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed;
     const uint32_t ring = (s32(ring_raw) + 1023u) & ~1023u;  // (the swizzle works on address bits)
@@ -164,6 +172,7 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
             bar_init(s32(&s_acc_full[b]), 1);
             bar_init(s32(&s_acc_empty[b]), kQWriters * GROUP);
         }
+        bar_init(s32(&s_sums), 1);
         s_failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -277,12 +286,15 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
             const int lanes = warp & 3, half = (warp - 4) >> 2;  // (a warp may read the 32 lanes (warp % 4) * 32 onwards)
             asm volatile("griddepcontrol.wait;" ::: "memory");
             int done = 0;
+            bool ok = true;  // (once a wait has given up the writers go on to the end without writing: they meet at a barrier for every tile)
             for (int tile = cluster; tile < n_tiles; tile += n_clusters, ++done) {
                 int row_tile, tok_tile;
                 place(tile, row_tile, tok_tile);
                 const int buf = done & 1, row = (row_tile * GROUP + rank) * kQRows + lanes * 32 + lane;
                 const float w_scale = row < a.rows ? __ldg(a.w_scales + row) : 0.0f;
-                if (!warp_wait(s32(&s_acc_full[buf]), (done >> 1) & 1, failed)) break;
+                fetch_scales(a, tok_tile * a.n, s_scales[buf]);
+                ok = ok && warp_wait(s32(&s_acc_full[buf]), (done >> 1) & 1, failed);
+                if (!ok) continue;
                 if (tile + n_clusters >= n_tiles) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t at = tmem + buf * a.acc_cols + (static_cast<uint32_t>(lanes * 32) << 16);
@@ -294,7 +306,7 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
 #pragma unroll
                     for (int j = 0; j < 16; ++j) next[j] = v[j];
                     if (c + 32 < a.n) load_sums(at + c + 32, v);  // (on its way while these are written)
-                    write_any(a, next, row, tok_tile * a.n + c, w_scale);
+                    write_any(a, next, row, tok_tile * a.n + c, w_scale, s_scales[buf] + c);
                 }
                 loaded();
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -316,10 +328,13 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
         if (warp >= 4) {
             if (row < a.rows) w_scale = __ldg(a.w_scales + row);
             asm volatile("griddepcontrol.wait;" ::: "memory");
+            fetch_scales(a, tok_tile * a.n, s_scales[0]);
             (void)warp_wait(s32(&s_acc_full[0]), 0, failed);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
-        cluster_sync();  // every block's MMAs are done with its stages
+        const uint32_t sums = s32(&s_sums), room = ring + a.exchange;
+        const bool own_room = a.exchange != 0;
+        if (!own_room) cluster_sync();  // every block's MMAs are done with its stages, where the sums go
         if (warp >= 4) {
             for (int c = half; c < a.n / 8; c += 2) {
                 const int unit = c * 4 + lanes, owner = unit % a.split;
@@ -327,14 +342,23 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
                 int v[8];
                 load_sums(at + c * 8, v);
                 loaded();
-                const uint32_t to = in_block(ring + ((unit / a.split) * (a.split - 1) + (part < owner ? part : part - 1)) * 1024 + lane * 16, owner * GROUP + rank);
-                asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-                asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 512), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+                // stores that count their bytes on a barrier of the block that they go to
+                const uint32_t to = in_block(room + ((unit / a.split) * (a.split - 1) + (part < owner ? part : part - 1)) * 1024 + lane * 16, owner * GROUP + rank);
+                const uint32_t bar = in_block(sums, owner * GROUP + rank);
+                asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(bar)
+                             : "memory");
+                asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to + 512), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(bar)
+                             : "memory");
             }
         }
-        cluster_sync();
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (its other half is at the end: until then others may still send)
         if (warp >= 4) {
             asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+            const int units = a.n / 2, mine = units / a.split + (part < units % a.split ? 1 : 0);  // of this block
+            if (warp == 4 && lane == 0) expect(sums, static_cast<uint32_t>(mine * (a.split - 1)) * 1024);
+            const bool ok = wait<true>(sums, 0, failed);  // (by every lane: it reads what others have stored)
+            __syncwarp();
             for (int c = half; c < a.n / 8; c += 2) {
                 const int unit = c * 4 + lanes;
                 if (unit % a.split != part) continue;
@@ -342,17 +366,19 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
                 load_sums(at + c * 8, v);
                 loaded();
                 for (int p = 0; p < a.split - 1; ++p) {
-                    const uint32_t from = ring + ((unit / a.split) * (a.split - 1) + p) * 1024 + lane * 16;
+                    const uint32_t from = room + ((unit / a.split) * (a.split - 1) + p) * 1024 + lane * 16;
                     const uint4 x = lds128u(from), z = lds128u(from + 512);
                     v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += z.x, v[5] += z.y, v[6] += z.z, v[7] += z.w;
                 }
-                if (!*failed) write_any(a, v, row, tok_tile * a.n + c * 8, w_scale);
+                if (ok && !*failed) write_any(a, v, row, tok_tile * a.n + c * 8, w_scale, s_scales[0] + c * 8);
             }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if constexpr (PAIR || SPLIT) cluster_sync();  // no block's shared or tensor memory goes away under another
+    // no block's shared or tensor memory goes away under another
+    if constexpr (SPLIT) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    else if constexpr (PAIR) cluster_sync();
     if (warp == 2) {
         if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
         else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
@@ -435,14 +461,19 @@ cudaError_t launch_qmm_i8(const QmmI8Args &in, int sm_count, cudaStream_t stream
     a.n = ((in.ntok + a.tok_tiles - 1) / a.tok_tiles + step - 1) / step * step;
     a.tok_tiles = (in.ntok + a.n - 1) / a.n;
     a.row_tiles = (in.rows + group * kQRows - 1) / (group * kQRows);
-    a.half_sm = !pair && a.n <= kQHalfMost;
     // As many parts of the columns as leave every cluster room beside the others, of two stages at least.
     a.split = 1;
     const int tiles = a.row_tiles * a.tok_tiles;
     for (int split = 2; split <= (pair ? kQMaxSplit / 2 : kQMaxSplit) && a.n_k >= 2 * split; ++split)
         if (tiles <= (pair ? Variant<true, true>::clusters(split) : Variant<false, true>::clusters(split))) a.split = split;
+    const bool brief = a.n_k <= 8 * a.split;  // a few stages for each block: what counts is how soon it begins and ends
+    a.half_sm = !pair && a.n <= (brief ? 80 : 32);
     a.b_bytes = a.n / group * kQCols;
-    a.stages = (a.half_sm ? kQHalfRing : kQRing) / (kQA + a.b_bytes);
+    // Sums have memory of their own where that costs no stage or the stages are few, else they go where the stages were, one barrier of the cluster later.
+    const int ring = a.half_sm ? kQHalfRing : kQRing, units = a.n / 2, room = a.split > 1 ? (units + a.split - 1) / a.split * (a.split - 1) * 1024 : 0;
+    a.stages = ring / (kQA + a.b_bytes);
+    const int beside = (ring - room) / (kQA + a.b_bytes);
+    if (a.split > 1 && (beside == a.stages || (brief && beside >= 3))) a.exchange = ring - room, a.stages = beside;
     if (a.stages > kQMaxStages) a.stages = kQMaxStages;
     a.acc_cols = 32;
     while (a.acc_cols < a.n) a.acc_cols *= 2;
