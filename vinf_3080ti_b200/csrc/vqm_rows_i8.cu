@@ -238,6 +238,9 @@ __global__ void __launch_bounds__(THREADS, THREADS != 256 ? 1 : VEC == 1 ? 4 : 3
         }
     }
     double sum = 0.0;
+    float best = -1.0f;  // the thread's largest product with the norm's weights, the vector it is in, whether it is there twice
+    int best_at = 0;
+    bool twice = false;
     if (norm) {
         double part[2] = {};
 #pragma unroll
@@ -250,8 +253,14 @@ __global__ void __launch_bounds__(THREADS, THREADS != 256 ? 1 : VEC == 1 ? 4 : 3
             for (int l = 0; l < VEC; ++l) {
                 const double d = static_cast<double>(e[l]);
                 part[l & 1] = fma(d, d, part[l & 1]);
-                top = largest_of(top, fabsf(e[l] * g[l]));
+                g[l] = fabsf(e[l] * g[l]);
             }
+            float most = g[0];
+#pragma unroll
+            for (int l = 1; l < VEC; ++l) most = largest_of(most, g[l]);
+            top = largest_of(top, most);
+            if (most > best) best = most, best_at = i, twice = false;
+            else if (most == best) twice = true;
         }
         sum = part[0] + part[1];
 #pragma unroll
@@ -282,7 +291,17 @@ __global__ void __launch_bounds__(THREADS, THREADS != 256 ? 1 : VEC == 1 ? 4 : 3
     // values: __expf and the division leave 2e-6, and 6e-8 |x| where the exponential counts (|x| < 90), so it is one within 2e-5 of it.
     if (GATED || norm) {
         const float least = GATED ? top * (1.0f - 2e-5f) : top;
-        if (own >= least) {
+        auto offer = [&](double d) { atomicMax(&s.largest, static_cast<unsigned long long>(__double_as_longlong(fabs(d)))); };
+        if (own >= least && norm && !twice) {
+            // (one thread, for which all the others wait: it looks at one vector only)
+            const int c = (static_cast<int>(threadIdx.x) + best_at * THREADS) * VEC;
+            float e[VEC], g[VEC];
+            load<VEC>((a.residual != nullptr ? static_cast<const T *>(a.total) + at : x) + c, e);
+            load<VEC>(a.norm_w + c, g);
+#pragma unroll
+            for (int l = 0; l < VEC; ++l)
+                if (fabsf(e[l] * g[l]) >= least) offer(static_cast<double>(e[l]) * static_cast<double>(g[l]));
+        } else if (own >= least) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 if (column(i) >= a.cols) continue;
@@ -293,10 +312,8 @@ __global__ void __launch_bounds__(THREADS, THREADS != 256 ? 1 : VEC == 1 ? 4 : 3
                 v[i].values(e);
 #pragma unroll
                 for (int l = 0; l < VEC; ++l)
-                    if (fabsf(e[l] * g[l]) >= least) {
-                        const double d = GATED ? exact_gate(as_float(x[column(i) + l]), as_float(second[column(i) + l])) : static_cast<double>(e[l]) * static_cast<double>(g[l]);
-                        atomicMax(&s.largest, static_cast<unsigned long long>(__double_as_longlong(fabs(d))));
-                    }
+                    if (fabsf(e[l] * g[l]) >= least)
+                        offer(GATED ? exact_gate(as_float(x[column(i) + l]), as_float(second[column(i) + l])) : static_cast<double>(e[l]) * static_cast<double>(g[l]));
             }
         }
     }
