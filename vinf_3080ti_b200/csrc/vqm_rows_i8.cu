@@ -19,45 +19,12 @@ __device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ void put(float *p, float v) { *p = v; }
 __device__ __forceinline__ void put(__half *p, float v) { *p = __float2half_rn(v); }
 
-template <int VEC>
-__device__ __forceinline__ void load(const float *p, float (&v)[VEC]) {
-    if constexpr (VEC == 4) {
-        const float4 w = *reinterpret_cast<const float4 *>(p);
-        v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
-    } else {
-        v[0] = *p;
-    }
-}
-template <int VEC>
-__device__ __forceinline__ void load(const __half *p, float (&v)[VEC]) {
-    if constexpr (VEC == 4) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(p);
-        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
-        v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
-    } else {
-        v[0] = __half2float(*p);
-    }
-}
-// stores v rounded to the buffer's type, and leaves that in v
-template <int VEC>
-__device__ __forceinline__ void store(float *p, float (&v)[VEC]) {
-    if constexpr (VEC == 4) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    else *p = v[0];
-}
-template <int VEC>
-__device__ __forceinline__ void store(__half *p, float (&v)[VEC]) {
-    if constexpr (VEC == 4) {
-        const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
-        *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
-        const float2 c = __half22float2(a), d = __half22float2(b);
-        v[0] = c.x, v[1] = c.y, v[2] = d.x, v[3] = d.y;
-    } else {
-        const __half a = __float2half_rn(v[0]);
-        *p = a;
-        v[0] = __half2float(a);
-    }
+__device__ __forceinline__ void load4(const float *p, float (&v)[4]) {
+    const float4 w = *reinterpret_cast<const float4 *>(p);
+    v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
 }
 
+constexpr int kMostFast = 24564;  // columns of a row that 512 threads hold in 12 vectors each, wherever it begins
 constexpr float kUndefined = __builtin_nanf("");
 constexpr double kMostScale = 3.4028235677973366e38;  // half a step above fp32's largest: rounds to infinity from here on
 
@@ -156,30 +123,25 @@ __device__ __forceinline__ double inverse_root(double m) {
     return fma(r, fma(-half * r, r, 0.5), r);
 }
 
-// VEC values in registers: as they come, or as floats where they are no longer of the buffer's type.
-template <typename T, int VEC, bool WIDE>
+// Four values in registers: as they come, or as floats where they are no longer of the buffer's type.
+template <typename T, bool WIDE>
 struct Kept {
-    float f[VEC];
-    __device__ __forceinline__ void fetch(const T *p) { load<VEC>(p, f); }
-    __device__ __forceinline__ void clear() {
+    float f[4];
+    __device__ __forceinline__ void fetch(const T *p);
+    __device__ __forceinline__ void values(float (&v)[4]) const {
 #pragma unroll
-        for (int l = 0; l < VEC; ++l) f[l] = 0.0f;
+        for (int l = 0; l < 4; ++l) v[l] = f[l];
     }
-    __device__ __forceinline__ void values(float (&v)[VEC]) const {
+    __device__ __forceinline__ void keep(const float (&v)[4]) {
 #pragma unroll
-        for (int l = 0; l < VEC; ++l) v[l] = f[l];
+        for (int l = 0; l < 4; ++l) f[l] = v[l];
     }
-    __device__ __forceinline__ void keep(const float (&v)[VEC]) {
-#pragma unroll
-        for (int l = 0; l < VEC; ++l) f[l] = v[l];
-    }
-    __device__ __forceinline__ void put_to(T *p) { store<VEC>(p, f); }
+    __device__ __forceinline__ void put_to(float *p) const { *reinterpret_cast<float4 *>(p) = make_float4(f[0], f[1], f[2], f[3]); }
 };
 template <>
-struct Kept<__half, 4, false> {
+struct Kept<__half, false> {
     uint2 w;
     __device__ __forceinline__ void fetch(const __half *p) { w = *reinterpret_cast<const uint2 *>(p); }
-    __device__ __forceinline__ void clear() { w = make_uint2(0, 0); }
     __device__ __forceinline__ void values(float (&v)[4]) const {
         const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
         v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
@@ -190,42 +152,76 @@ struct Kept<__half, 4, false> {
     }
     __device__ __forceinline__ void put_to(__half *p) const { *reinterpret_cast<uint2 *>(p) = w; }
 };
+template <typename T, bool WIDE>
+__device__ __forceinline__ void Kept<T, WIDE>::fetch(const T *p) {
+    if constexpr (sizeof(T) == 4) {
+        load4(reinterpret_cast<const float *>(p), f);
+    } else {
+        Kept<__half, false> half;
+        half.fetch(reinterpret_cast<const __half *>(p));
+        half.values(f);
+    }
+}
 
-// A block per row.  A thread holds NV vectors of VEC neighbouring columns (VEC 4 where rows start at multiples of 16 bytes), vector i at
-// (thread + i * threads) * VEC: v before the norm's weights, which come from the caches both times.
-template <typename T, int VEC, int NV, int THREADS, bool GATED>
-__global__ void __launch_bounds__(THREADS, THREADS != 256 ? 1 : VEC == 1 ? 4 : 3) rows_i8_kernel(const RowsI8Args a) {
+// A block per row.  A thread holds NV vectors of 4 neighbouring columns, vector i at (thread + i * threads) * 4: v before the norm's weights, which come
+// from the caches both times.  LOOSE: rows of any length, whose vectors lie on the buffers' grid, not the row's: the first and the last may be
+// partly outside of the row, and the norm's weights and the outputs, which lie on other grids, go one by one.
+template <typename T, int NV, int THREADS, bool GATED, bool LOOSE>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rows_i8_kernel(const RowsI8Args a) {
     __shared__ RowShared s;
     constexpr int WARPS = THREADS / 32;
     const size_t row = blockIdx.x, at = row * a.cols;
     const T *x = static_cast<const T *>(a.x) + at, *second = static_cast<const T *>(a.x2 != nullptr ? a.x2 : a.residual) + at;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool norm = !GATED && a.norm_w != nullptr;
-    auto column = [&](int i) { return (static_cast<int>(threadIdx.x) + i * THREADS) * VEC; };
+    const int ahead = LOOSE ? static_cast<int>(at & 3) : 0;  // columns between the grid's line and the row's first
+    auto column = [&](int i) { return (static_cast<int>(threadIdx.x) + i * THREADS) * 4 - ahead; };
+    auto in = [&](int c) { return !LOOSE || (c >= 0 && c < a.cols); };
+    auto whole = [&](int i) { return !LOOSE || (column(i) >= 0 && column(i) + 4 <= a.cols); };
+    auto fetch = [&](auto &kept, const T *from, int i) {
+        if (whole(i)) {
+            kept.fetch(from + column(i));
+        } else {
+            float e[4];
+#pragma unroll
+            for (int l = 0; l < 4; ++l) e[l] = in(column(i) + l) ? as_float(from[column(i) + l]) : 0.0f;
+            kept.keep(e);
+        }
+    };
+    auto weights = [&](int c, float (&g)[4]) {
+        if (!LOOSE) {
+            load4(a.norm_w + c, g);
+        } else {
+#pragma unroll
+            for (int l = 0; l < 4; ++l) g[l] = in(c + l) ? a.norm_w[c + l] : 0.0f;
+        }
+    };
     if (threadIdx.x == 0) s.largest = 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    Kept<T, VEC, GATED> v[NV];
+    Kept<T, GATED> v[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (column(i) < a.cols) v[i].fetch(x + column(i));
-        else v[i].clear();
+    for (int i = 0; i < NV; ++i) {
+        const float none[4] = {};
+        if (column(i) < a.cols) fetch(v[i], x, i);
+        else v[i].keep(none);
+    }
     float top = 0.0f;
     if (GATED || a.residual != nullptr) {
-        Kept<T, VEC, false> y[NV];
+        Kept<T, false> y[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (column(i) < a.cols) y[i].fetch(second + column(i));
+            if (column(i) < a.cols) fetch(y[i], second, i);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (column(i) >= a.cols) continue;
-            float e[VEC], d[VEC];
+            float e[4], d[4];
             v[i].values(e);
             y[i].values(d);
 #pragma unroll
-            for (int l = 0; l < VEC; ++l) {
-                if (GATED) {
+            for (int l = 0; l < 4; ++l) {
+                if constexpr (GATED) {
                     // silu(-inf) is undefined; silu(-80) = -1e-33 may have lost digits, which shows if y is large: not this way
                     if (e[l] < -80.0f && (fabsf(d[l]) > 1e3f || e[l] == -INFINITY)) top = INFINITY;
                     e[l] = __fdividef(e[l], 1.0f + __expf(-e[l])) * d[l];
@@ -234,7 +230,16 @@ __global__ void __launch_bounds__(THREADS, THREADS != 256 ? 1 : VEC == 1 ? 4 : 3
                 }
             }
             v[i].keep(e);
-            if (!GATED) v[i].put_to(static_cast<T *>(a.total) + at + column(i));
+            if constexpr (!GATED) {
+                T *const to = static_cast<T *>(a.total) + at + column(i);
+                if (whole(i)) {
+                    v[i].put_to(to);
+                } else {
+#pragma unroll
+                    for (int l = 0; l < 4; ++l)
+                        if (in(column(i) + l)) put(to + l, e[l]);
+                }
+            }
         }
     }
     double sum = 0.0;
@@ -246,18 +251,18 @@ __global__ void __launch_bounds__(THREADS, THREADS != 256 ? 1 : VEC == 1 ? 4 : 3
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (column(i) >= a.cols) continue;
-            float g[VEC], e[VEC];
-            load<VEC>(a.norm_w + column(i), g);
+            float g[4], e[4];
+            weights(column(i), g);
             v[i].values(e);
 #pragma unroll
-            for (int l = 0; l < VEC; ++l) {
+            for (int l = 0; l < 4; ++l) {
                 const double d = static_cast<double>(e[l]);
                 part[l & 1] = fma(d, d, part[l & 1]);
                 g[l] = fabsf(e[l] * g[l]);
             }
             float most = g[0];
 #pragma unroll
-            for (int l = 1; l < VEC; ++l) most = largest_of(most, g[l]);
+            for (int l = 1; l < 4; ++l) most = largest_of(most, g[l]);
             top = largest_of(top, most);
             if (most > best) best = most, best_at = i, twice = false;
             else if (most == best) twice = true;
@@ -268,10 +273,10 @@ __global__ void __launch_bounds__(THREADS, THREADS != 256 ? 1 : VEC == 1 ? 4 : 3
     } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            float e[VEC];
+            float e[4];
             v[i].values(e);
 #pragma unroll
-            for (int l = 0; l < VEC; ++l) top = largest_of(top, fabsf(e[l]));
+            for (int l = 0; l < 4; ++l) top = largest_of(top, fabsf(e[l]));
         }
     }
     const float own = top;
@@ -294,24 +299,26 @@ __global__ void __launch_bounds__(THREADS, THREADS != 256 ? 1 : VEC == 1 ? 4 : 3
         auto offer = [&](double d) { atomicMax(&s.largest, static_cast<unsigned long long>(__double_as_longlong(fabs(d)))); };
         if (own >= least && norm && !twice) {
             // (one thread, for which all the others wait: it looks at one vector only)
-            const int c = (static_cast<int>(threadIdx.x) + best_at * THREADS) * VEC;
-            float e[VEC], g[VEC];
-            load<VEC>((a.residual != nullptr ? static_cast<const T *>(a.total) + at : x) + c, e);
-            load<VEC>(a.norm_w + c, g);
+            const int c = column(best_at);
+            float e[4], g[4];
+            Kept<T, false> again;
+            fetch(again, a.residual != nullptr ? static_cast<const T *>(a.total) + at : x, best_at);
+            again.values(e);
+            weights(c, g);
 #pragma unroll
-            for (int l = 0; l < VEC; ++l)
+            for (int l = 0; l < 4; ++l)
                 if (fabsf(e[l] * g[l]) >= least) offer(static_cast<double>(e[l]) * static_cast<double>(g[l]));
         } else if (own >= least) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 if (column(i) >= a.cols) continue;
-                float g[VEC], e[VEC];
+                float g[4], e[4];
 #pragma unroll
-                for (int l = 0; l < VEC; ++l) g[l] = 1.0f;
-                if (norm) load<VEC>(a.norm_w + column(i), g);
+                for (int l = 0; l < 4; ++l) g[l] = 1.0f;
+                if (norm) weights(column(i), g);
                 v[i].values(e);
 #pragma unroll
-                for (int l = 0; l < VEC; ++l)
+                for (int l = 0; l < 4; ++l)
                     if (fabsf(e[l] * g[l]) >= least)
                         offer(GATED ? exact_gate(as_float(x[column(i) + l]), as_float(second[column(i) + l])) : static_cast<double>(e[l]) * static_cast<double>(g[l]));
             }
@@ -351,13 +358,13 @@ __global__ void __launch_bounds__(THREADS, THREADS != 256 ? 1 : VEC == 1 ? 4 : 3
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         if (column(i) >= a.cols) continue;
-        float g[VEC], t[VEC], e[VEC];
-        if (norm) load<VEC>(a.norm_w + column(i), g);
+        float g[4], t[4], e[4];
+        if (norm) weights(column(i), g);
         v[i].values(e);
-        uint32_t bits[VEC];
+        uint32_t bits[4];
         bool near = false;
 #pragma unroll
-        for (int l = 0; l < VEC; ++l) {
+        for (int l = 0; l < 4; ++l) {
             t[l] = (norm ? e[l] * g[l] : e[l]) * f;  // |t| < 127.1
             const float k = t[l] + kWhole;
             bits[l] = __float_as_uint(k);
@@ -367,7 +374,7 @@ __global__ void __launch_bounds__(THREADS, THREADS != 256 ? 1 : VEC == 1 ? 4 : 3
         }
         if (near) {
 #pragma unroll
-            for (int l = 0; l < VEC; ++l)
+            for (int l = 0; l < 4; ++l)
                 if (t[l] > 0.0f) {
                     double d = static_cast<double>(e[l]);
                     if (GATED) d = exact_gate(as_float(x[column(i) + l]), as_float(second[column(i) + l]));
@@ -375,8 +382,13 @@ __global__ void __launch_bounds__(THREADS, THREADS != 256 ? 1 : VEC == 1 ? 4 : 3
                     bits[l] = static_cast<uint32_t>(__double2int_rn(d * s.r / s.scale));  // (divided: a tie stays a tie)
                 }
         }
-        if constexpr (VEC == 4) *reinterpret_cast<uint32_t *>(out + column(i)) = __byte_perm(__byte_perm(bits[0], bits[1], 0x0040), __byte_perm(bits[2], bits[3], 0x0040), 0x5410);
-        else out[column(i)] = static_cast<int8_t>(bits[0]);
+        if (!LOOSE) {
+            *reinterpret_cast<uint32_t *>(out + column(i)) = __byte_perm(__byte_perm(bits[0], bits[1], 0x0040), __byte_perm(bits[2], bits[3], 0x0040), 0x5410);
+        } else {
+#pragma unroll
+            for (int l = 0; l < 4; ++l)
+                if (in(column(i) + l)) out[column(i) + l] = static_cast<int8_t>(bits[l]);
+        }
     }
     if (threadIdx.x < pitch - a.cols) out[a.cols + threadIdx.x] = 0;
 }
@@ -395,42 +407,33 @@ cudaError_t launch_kernel(K kernel, const RowsI8Args &a, int threads, cudaStream
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-template <typename T, int VEC, int NV, int THREADS>
+template <typename T, int NV, int THREADS, bool LOOSE>
 cudaError_t launch_variant(const RowsI8Args &a, cudaStream_t stream) {
-    return a.x2 != nullptr ? launch_kernel(rows_i8_kernel<T, VEC, NV, THREADS, true>, a, THREADS, stream)
-                           : launch_kernel(rows_i8_kernel<T, VEC, NV, THREADS, false>, a, THREADS, stream);
+    return a.x2 != nullptr ? launch_kernel(rows_i8_kernel<T, NV, THREADS, true, LOOSE>, a, THREADS, stream)
+                           : launch_kernel(rows_i8_kernel<T, NV, THREADS, false, LOOSE>, a, THREADS, stream);
 }
-template <typename T, int THREADS>
-cudaError_t launch_vectors(const RowsI8Args &a, cudaStream_t stream) {  // at most 12 vectors of 4 columns per thread
-    const int n = (a.cols / 4 + THREADS - 1) / THREADS;
-    if (n <= 2) return launch_variant<T, 4, 2, THREADS>(a, stream);
-    if (n <= 5) return launch_variant<T, 4, 5, THREADS>(a, stream);
-    if (n <= 8) return launch_variant<T, 4, 8, THREADS>(a, stream);
-    if (n <= 10) return launch_variant<T, 4, 10, THREADS>(a, stream);
-    return launch_variant<T, 4, 12, THREADS>(a, stream);
-}
-template <typename T, int THREADS>
-cudaError_t launch_columns(const RowsI8Args &a, cudaStream_t stream) {  // at most 32 columns per thread
-    const int n = (a.cols + THREADS - 1) / THREADS;
-    if (n <= 4) return launch_variant<T, 1, 4, THREADS>(a, stream);
-    if (n <= 12) return launch_variant<T, 1, 12, THREADS>(a, stream);
-    return launch_variant<T, 1, 32, THREADS>(a, stream);
+template <typename T, int THREADS, bool LOOSE>
+cudaError_t launch_vectors(const RowsI8Args &a, cudaStream_t stream) {  // at most 12 vectors per thread
+    const int n = ((a.cols + (LOOSE ? 6 : 3)) / 4 + THREADS - 1) / THREADS;
+    if (n <= 2) return launch_variant<T, 2, THREADS, LOOSE>(a, stream);
+    if (n <= 5) return launch_variant<T, 5, THREADS, LOOSE>(a, stream);
+    if (n <= 8) return launch_variant<T, 8, THREADS, LOOSE>(a, stream);
+    if (n <= 10) return launch_variant<T, 10, THREADS, LOOSE>(a, stream);
+    return launch_variant<T, 12, THREADS, LOOSE>(a, stream);
 }
 
+template <typename T, bool LOOSE>
+cudaError_t launch_size(const RowsI8Args &a, int sm_count, cudaStream_t stream) {
+    const bool many = a.ntok > sm_count;  // few rows: as many threads on each as there are
+    if (a.cols <= 1024 && many) return launch_vectors<T, 32, LOOSE>(a, stream);
+    if (a.cols <= (sizeof(T) == 2 ? 6138 : 4096) && many) return launch_vectors<T, 128, LOOSE>(a, stream);
+    if (a.cols <= 12282 && many) return launch_vectors<T, 256, LOOSE>(a, stream);
+    return launch_vectors<T, 512, LOOSE>(a, stream);
+}
 template <typename T>
 cudaError_t launch_t(const RowsI8Args &a, int sm_count, cudaStream_t stream) {
-    if (a.cols > 32768 || (a.x2 != nullptr && a.norm_w != nullptr)) return launch_kernel(exact_rows_kernel<T>, a, 512, stream);
-    const bool many = a.ntok > sm_count;  // few rows: as many threads on each as there are
-    if (a.cols % 4 == 0) {
-        if (a.cols <= 1024 && many) return launch_vectors<T, 32>(a, stream);
-        if (a.cols <= (sizeof(T) == 2 ? 6144 : 4096) && many) return launch_vectors<T, 128>(a, stream);
-        if (a.cols <= 12288 && many) return launch_vectors<T, 256>(a, stream);
-        if (a.cols <= 24576) return launch_vectors<T, 512>(a, stream);
-        return launch_variant<T, 4, 8, 1024>(a, stream);
-    }
-    if (a.cols <= 1024 && many) return launch_columns<T, 32>(a, stream);
-    if (a.cols <= 8192 && many) return launch_columns<T, 256>(a, stream);
-    return launch_columns<T, 1024>(a, stream);
+    if (a.cols > kMostFast || (a.x2 != nullptr && a.norm_w != nullptr)) return launch_kernel(exact_rows_kernel<T>, a, 512, stream);
+    return a.cols % 4 == 0 ? launch_size<T, false>(a, sm_count, stream) : launch_size<T, true>(a, sm_count, stream);
 }
 
 }  // namespace
