@@ -6,7 +6,7 @@
 // half is worked out again in 64.
 //
 // A block per row, its values in registers between the two passes: memory is read and written once, which is what bounds it.
-// Rows too long for that, a norm of gated values, and rows whose largest value is out of fp32's middle range are worked out in 64 bits throughout.
+// Rows too long for that, norms of gated values, and rows whose largest value is out of fp32's middle range are worked out in 64 bits throughout.
 #include <cuda_fp16.h>
 
 #include "vqm_kernels.h"
@@ -103,6 +103,57 @@ __global__ void __launch_bounds__(512) exact_rows_kernel(const RowsI8Args a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     exact_row<T>(a, blockIdx.x, false, s);
+}
+
+// The norm of gated values, whose mean wants more digits than 32 bits leave of silu: in 64 bits too, but each value is made once and kept.
+template <typename T, int NV>
+__global__ void __launch_bounds__(512) gated_norm_kernel(const RowsI8Args a) {
+    __shared__ double s_sum[16], s_top[16];
+    const size_t row = blockIdx.x, at = row * a.cols;
+    const T *x = static_cast<const T *>(a.x) + at, *x2 = static_cast<const T *>(a.x2) + at;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    double v[NV], sum = 0.0, top = 0.0;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = static_cast<int>(threadIdx.x) + i * 512;
+        v[i] = 0.0;
+        if (c < a.cols) {
+            const double e = static_cast<double>(as_float(x[c]));
+            v[i] = e / (1.0 + exp(-e)) * static_cast<double>(as_float(x2[c]));
+        }
+        sum = fma(v[i], v[i], sum);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = static_cast<int>(threadIdx.x) + i * 512;
+        if (c < a.cols) v[i] *= static_cast<double>(a.norm_w[c]);
+        bad |= !(fabs(v[i]) <= 1e300);
+        top = fmax(top, fabs(v[i]));
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off), top = fmax(top, __shfl_xor_sync(0xffffffffu, top, off));
+    if (__any_sync(0xffffffffu, bad)) top = __longlong_as_double(0x7ff0000000000000ll);
+    if (lane == 0) s_sum[warp] = sum, s_top[warp] = top;
+    __syncthreads();
+    sum = lane < 16 ? s_sum[lane] : 0.0, top = lane < 16 ? s_top[lane] : 0.0;
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off), top = fmax(top, __shfl_xor_sync(0xffffffffu, top, off));
+    sum = __shfl_sync(0xffffffffu, sum, 0), top = __shfl_sync(0xffffffffu, top, 0);
+    const double r = 1.0 / sqrt(sum / a.cols + static_cast<double>(a.eps)), wide = top * r / 127.0;
+    const float scale = wide < kMostScale ? static_cast<float>(wide) : kUndefined;  // (not so for undefined ones)
+    if (threadIdx.x == 0) a.scales[row] = scale;
+    const double factor = r / static_cast<double>(scale);
+    const long long pitch = i8_pitch(a.cols);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = static_cast<int>(threadIdx.x) + i * 512;
+        if (c >= pitch) continue;
+        const int q = scale > 0.0f && c < a.cols ? min(127, max(-127, __double2int_rn(v[i] * factor))) : 0;
+        a.q[row * pitch + c] = static_cast<int8_t>(q);
+    }
 }
 
 // silu(x) * y in 64 bits
@@ -432,6 +483,11 @@ cudaError_t launch_size(const RowsI8Args &a, int sm_count, cudaStream_t stream) 
 }
 template <typename T>
 cudaError_t launch_t(const RowsI8Args &a, int sm_count, cudaStream_t stream) {
+    if (a.x2 != nullptr && a.norm_w != nullptr && i8_pitch(a.cols) <= 512 * 40) {
+        if (i8_pitch(a.cols) <= 512 * 4) return launch_kernel(gated_norm_kernel<T, 4>, a, 512, stream);
+        if (i8_pitch(a.cols) <= 512 * 16) return launch_kernel(gated_norm_kernel<T, 16>, a, 512, stream);
+        return launch_kernel(gated_norm_kernel<T, 40>, a, 512, stream);
+    }
     if (a.cols > kMostFast || (a.x2 != nullptr && a.norm_w != nullptr)) return launch_kernel(exact_rows_kernel<T>, a, 512, stream);
     return a.cols % 4 == 0 ? launch_size<T, false>(a, sm_count, stream) : launch_size<T, true>(a, sm_count, stream);
 }
