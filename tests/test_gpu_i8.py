@@ -106,6 +106,62 @@ def test_many_rows(rt, ntok, cols):
 
 
 @pytest.mark.parametrize("kind", [np.float32, np.float16])
+@pytest.mark.parametrize("cols", [1, 5, 33, 997, 1023, 1025, 2047, 4095, 4097, 5121, 6138, 6139, 6142, 8191])
+def test_many_rows_of_any_length(rt, cols, kind):
+    """More rows than SMs; rows that begin anywhere on a line."""
+    rng = np.random.default_rng(cols)
+    ntok = 203
+    x, res = (rng.standard_normal((2, ntok, cols)) * 2).astype(kind)
+    g = rng.uniform(0.5, 1.5, cols).astype(np.float32)
+    check_rows(rt, x, residual=res, norm=g)
+    check_rows(rt, x, residual=res, norm=g, total="t")
+    check_rows(rt, x)
+    check_rows(rt, x, x2=res)
+    check_rows(rt, x, x2=res, norm=g)
+
+
+@pytest.mark.parametrize("cols,ntok", [(12282, 170), (12283, 170), (12288, 1), (20464, 2), (20481, 2), (20496, 160), (24560, 3), (24564, 3), (24565, 3), (24568, 150)])
+def test_lengths_at_which_another_kernel_takes_over(rt, cols, ntok):
+    rng = np.random.default_rng(cols)
+    x, res = rng.standard_normal((2, ntok, cols)).astype(np.float32)
+    g = rng.uniform(0.5, 1.5, cols).astype(np.float32)
+    check_rows(rt, x, residual=res, norm=g)
+    check_rows(rt, x[:5], x2=res[:5])
+    check_rows(rt, x[:5], x2=res[:5], norm=g)
+
+
+def test_equal_largest_values_and_equal_rows(rt):
+    """The largest product more than once: in one thread's vectors, in several; products that round to the same 32 bits."""
+    rng = np.random.default_rng(12)
+    for cols in (64, 5120, 5121, 20000):
+        x = np.full((3, cols), 0.7, np.float32)
+        x[1] = rng.choice(np.float32([0.1, -0.3, 0.3]), cols)
+        g = np.full(cols, 1.3, np.float32)
+        g[cols // 2:] = np.nextafter(np.float32(1.3), np.float32(2))
+        x[2] = np.where(np.arange(cols) < cols // 2, np.float32(0.9), np.nextafter(np.float32(0.9), np.float32(0)))
+        check_rows(rt, x, norm=g, eps=1e-3)
+        check_rows(rt, x, x2=np.ascontiguousarray(x[:, ::-1]))
+        check_rows(rt, x)
+
+
+def test_gated_values_far_from_zero(rt):
+    """Large negative x, whose silu is all but nothing, beside ordinary ones and beside large x2."""
+    rng = np.random.default_rng(13)
+    x = np.concatenate([np.linspace(-120, 120, 601), [-88.5, -87.0, -103.0, -200.0, 1e4, -1e4]]).astype(np.float32)
+    x = np.tile(x, (6, 1))
+    x2 = rng.standard_normal(x.shape).astype(np.float32)
+    x[1] = np.minimum(x[1], -79)
+    x[2] = np.minimum(x[2], -95)
+    x2[3, ::7] = 1e20
+    x2[4] *= np.float32(1e-25)
+    x[5, x[5] > -60] = 0
+    x2[5, ::5] = 1e30
+    check_rows(rt, x, x2=x2)
+    check_rows(rt, x, x2=x2, norm=np.ones(x.shape[1], np.float32))
+    check_rows(rt, np.tile(x, (40, 1)), x2=np.tile(x2, (40, 1)))
+
+
+@pytest.mark.parametrize("kind", [np.float32, np.float16])
 def test_halves_go_to_even(rt, kind):
     x = np.zeros((2, 260), kind)
     x[0, :127], x[0, 127] = np.arange(127) + 0.5, 127  # scale 1
@@ -243,6 +299,15 @@ def test_product_on_shapes_of_models(rt, rows, cols, ntok):
     w, ws, q, qs = make(rng, rows, cols, ntok)
     check_product(rt, w, ws, q, qs)
     check_product(rt, w, ws, q, qs, kind=np.float16)
+
+
+@pytest.mark.parametrize("rows,cols,ntok", [(600, 17408, 30), (600, 17408, 40), (600, 17408, 70), (600, 17408, 130), (600, 17408, 256), (300, 20000, 300), (3000, 9000, 600), (1100, 2050, 48),
+                                            (1100, 2050, 49), (1100, 2050, 80), (1100, 2050, 81), (20000, 300, 33), (20000, 300, 300), (40000, 130, 257), (256, 256, 4097)])
+def test_product_split_by_columns_and_not(rt, rows, cols, ntok):
+    """Columns shared by the blocks of a cluster, with memory of their own for the sums and without; tiles that blocks take one after the other."""
+    rng = np.random.default_rng(ntok)
+    w, ws, q, qs = make(rng, rows, cols, ntok)
+    check_product(rt, w, ws, q, qs, kind=np.float16 if ntok in (40, 600) else np.float32)
 
 
 @pytest.mark.parametrize("ntok", [1, 40])

@@ -210,3 +210,46 @@ def test_between_matvecs_of_gguf_blocks(codebooks):
         rt.zero("z")
         assert np.array_equal(go(False), want)
     rt.close()
+
+
+FIRST_IN_A_CAPTURE = """
+import sys
+import numpy as np
+sys.path.insert(0, {repo!r})
+from vinf_3080ti_b200.runtime import Runtime
+rt = Runtime()
+rng = np.random.default_rng(0)
+cols, vocab = 640, 40000
+w = rng.integers(-127, 128, (vocab, cols), dtype=np.int8)
+rt.upload_i8("w", w, np.full(vocab, 1e-3, np.float32), cols, vocab)
+rt.upload_i8("few", w[:300], np.full(300, 1e-3, np.float32), cols, 300)
+for name, n, e in (("x", 300 * cols, 4), ("q", 300 * cols, 1), ("s", 300, 4), ("y", 300 * 300, 4), ("logits", 4 * vocab, 4), ("u", 4, 4), ("k", 3, 4), ("out", 5, 4)):
+    rt.alloc(name, n, e)
+rt.write("x", rng.standard_normal((300, cols)).astype(np.float32))
+def go():
+    for ntok in (2, 300):
+        rt.rows_i8("x", "q", "s", cols, ntok)
+        rt.qmm_i8("few", "q", "s", "y", ntok)
+    rt.qmm_i8("w", "q", "s", "logits", 4)
+    rt.verify("logits", None, "k", "u", vocab, 1, 3, out="out", blocking=False)
+rt.capture_begin()
+go()
+graph = rt.capture_end()
+rt.graph_launch(graph)
+first = [rt.read(n) for n in ("q", "s", "y", "logits", "out")]
+for n in ("q", "s", "y", "logits", "out"):
+    rt.zero(n)
+go()
+assert first == [rt.read(n) for n in ("q", "s", "y", "logits", "out")]
+rt.synchronize()
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    repo = str(Path(__file__).resolve().parent.parent)
+    done = subprocess.run([sys.executable, "-c", FIRST_IN_A_CAPTURE.format(repo=repo)], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
