@@ -7,9 +7,18 @@
 //   warp 1      one thread issues the MMAs (in the second block of a pair: passes "full" on to the first)
 //   warp 2      tensor memory
 //   warps 4-11  outputs: two warps for each 32 lanes
-// PAIR: two blocks of a cluster multiply 256 weight rows by up to 256 activation rows together (cta_group::2), each holding half of both.
-// SPLIT: the blocks (pairs) of a cluster share the columns of a tile; sums are integers, so how they are split does not show in the result.
+// PAIR (more than 256 activation rows): two blocks of a cluster multiply 256 weight rows by up to 256 activation rows together (cta_group::2), each holding
+// half of both; they take tile after tile, and the outputs of one are written while the next is multiplied (two accumulators).
+// SPLIT (few tiles): the blocks (pairs) of a cluster share the columns of a tile; sums are integers, so how they are split does not show in the result.
 // Every output is the same whatever else is in its launch.
+//
+// What bounds it.  Few rows: memory, and 3 us of start and end (17408 x 5120 with 1 row: 16.6 us of one stream, 5390 GB/s; 151936 x 5120 with 4: 124 us, 6300).
+// Many: the MMAs, 512 cycles a stage of a pair, at 73 % of their rate for 2048 rows, 56 % for 512 (two rounds of tiles, start and end), and the power cap:
+// 17408 x 5120 x 4096 takes 225 us (3240 TOP/s) in a burst and 265 at the 1530 MHz that 1000 W leave.  1024 x 5120 with 4 rows: 6.6 us, of which 2 are
+// the exchange of sums.  What it took: the loop that issues the MMAs in one thread, with waits that look at their barrier only (4096 rows: 307 and 299
+// us); outputs loaded 16 columns ahead, scales in shared memory, no choice of types inside (a tile's outputs took 10 us, as long as its MMAs: 299 and
+// 262); two blocks per SM for few rows (5120 x 17408 with 24: 15.6 and 13.9).  Tried: weights fetched into L2 8 or 24 stages ahead of their copies, 16.6
+// and 19.7 or 22.0 us for one row.
 //
 // Every wait is bounded: on expiry the block records a status code and everybody falls through to the end.
 #include <cuda.h>
