@@ -183,7 +183,7 @@ int vqm_qmm_i8(vqm_runtime *rt, const char *weight, const char *q, const char *s
  *   p = softmax(target / T), q = softmax(draft / T); draft i is accepted if u[i] q(token) < p(token), up to the first that is not;
  *   the next token is the smallest one up to which the sum of r = max(p - q, 0) at the refused draft (behind the last draft: r = p) is above
  *   u[drafts] times r's whole sum.  So the tokens are distributed as p.  T <= 0 (or NaN): p and q are 1 at their rows' largest logit, the
- *   lowest index on ties: greedy verification.
+ *   lowest index on ties: greedy verification.  T above 1e30 counts as infinite: all tokens that are not masked are equally likely.
  * Decisions are those of 64-bit arithmetic; where p - q is within its rounding (2^-44 p) it is nothing, and where nothing is left of p - q the
  * token is drawn from p.  Logits of -inf and NaN have no probability; a row without any refuses its draft, and the
  * token drawn from such a row is -1.  A token outside [0, vocab) is refused, and where drafts have no probabilities nothing is taken off p then.

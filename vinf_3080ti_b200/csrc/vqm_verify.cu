@@ -103,7 +103,7 @@ struct Shared {
     float top[kVMaxRows], sum[kVMaxRows];          // this block's (greedy: lowest index of the largest, as int bits)
     float all_top[kVMaxRows], all_sum[kVMaxRows];  // the whole row's
     unsigned char verdict[256];                    // of the drafts
-    double warp_sum[2][kVWarps];                // of the warps; of the row(s) being summed
+    double warp_sum[3][kVWarps];                   // of the warps; of the row(s) being summed, of one warp's part
     double block_sum[2][2];                        // this block's, for the others; two buffers in turn
 };
 enum : unsigned char { kAccept, kRefuse, kUnsure };
@@ -112,12 +112,20 @@ enum : unsigned char { kAccept, kRefuse, kUnsure };
 struct Weights {
     double scale, magic;  // log2(e) / T, kVMagic - shift
     float least;          // a smaller logit weighs 2^-1000, which counts as nothing (and so does a masked or undefined one)
-    bool plain;           // everything above is within its bounds
     float top;
-    double inv_t;
+    int kind;             // of the row
 };
+// Rows whose logits are not taken as they are, but as 0 or -inf: only the largest count (it is infinite, or the lowest number there is), all that are not masked
+// do (T above 1e30), none do.
+enum : int { kOrdinary, kLargestOnly, kAllEqual, kNone };
 constexpr double kTiny = 0x1p-960;
 
+template <int N>
+__device__ __forceinline__ void ordinary(const Weights &w, float *x) {
+    if (w.kind == kOrdinary) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = (w.kind == kLargestOnly ? x[i] == w.top : w.kind == kAllEqual && x[i] > -INFINITY) ? 0.0f : -INFINITY;
+}
 // 2^y with y = x scale - shift: y = j / 128 + r, |r| <= 1 / 256; 2^(j / 128) by table, 2^r by the series of exp up to the fourth power of
 // r ln 2 < 0.00271, which leaves 1.2e-15 (table-driven exponential: P. Tang, ACM TOMS 15, 1989).  Eight instructions of the 64-bit pipe.
 template <int N>
@@ -129,7 +137,7 @@ __device__ __forceinline__ void powers(const float *x, const Weights &w, const d
     for (int i = 0; i < N; ++i) t[i] = fma(out[i], w.scale, w.magic);  // kVMagic + j / 128
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int n = __double2loint(t[i]);
+        const int n = max(__double2loint(t[i]), -1000 * kVTable);  // (the logit below which nothing counts is rounded: y may be lower)
         const double two = table[(n & (kVTable - 1)) * kVCopies];
         f[i] = __hiloint2double(__double2hiint(two) + (n & -kVTable) * ((1 << 20) / kVTable), __double2loint(two));
         r[i] = fma(out[i], w.scale, w.magic - t[i]);  // (the difference is exact)
@@ -145,25 +153,29 @@ __device__ __forceinline__ void powers(const float *x, const Weights &w, const d
 #pragma unroll
     for (int i = 0; i < N; ++i) out[i] *= f[i];
 }
-// Rows whose largest logit or temperature is out of the ordinary; not inlined: cold code costs every launch its fetch.
-static __device__ __noinline__ double rare_weight(float x, float top, double inv_t) {
-    return !(x > -INFINITY) ? 0.0 : x == top ? 1.0 : exp((static_cast<double>(x) - static_cast<double>(top)) * inv_t);
-}
 __device__ __forceinline__ double weight(float x, const Weights &w, const double *table) {
     double p;
-    if (w.plain) powers<1>(&x, w, table, &p);
-    else p = rare_weight(x, w.top, w.inv_t);
+    ordinary<1>(w, &x);
+    powers<1>(&x, w, table, &p);
     return p > kTiny ? p : 0.0;
 }
-__device__ __forceinline__ Weights weights_of(float top, float temperature) {
+// scale, reach: log2(e) / T and 1000 over that, which a sequence's rows have in common
+__device__ __forceinline__ Weights weights_of(float top, double scale, double reach) {
+    constexpr float kMost = 3.402823466e38f;
     Weights w;
     w.top = top;
-    w.inv_t = fmax(1.0 / static_cast<double>(temperature), 1e-300);
-    w.scale = w.inv_t * kLog2e;
-    const double shift = static_cast<double>(top) * w.scale;
-    w.magic = kVMagic - shift;  // (rounds the shift)
-    w.least = static_cast<float>(static_cast<double>(top) - 1000.0 / w.scale);
-    w.plain = fabs(shift) < 1e7 && w.scale > 1e-30 && w.scale < 1e30;
+    w.kind = top == -INFINITY ? kNone : top == INFINITY || top <= -kMost ? kLargestOnly : scale < 1e-30 ? kAllEqual : kOrdinary;
+    double at = static_cast<double>(top);
+    if (w.kind != kOrdinary) {
+        at = 0.0, scale = 1.0, reach = 1000.0;
+    } else if (fabs(at) * scale > 4e12) {
+        // the next lower number is 2^-24 of the largest away, which is 2^-200000 then: a smaller scale gives the same weights, 1 and 0
+        scale = 4e12 / fabs(at);
+        reach = 1000.0 / scale;
+    }
+    w.scale = scale;
+    w.magic = kVMagic - at * scale;  // (rounds the shift)
+    w.least = fmaxf(__double2float_rd(at - reach), -kMost);
     return w;
 }
 
@@ -172,121 +184,6 @@ __device__ __forceinline__ double warp_total(double v) {
     for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
     return v;
 }
-// The one or two rows that the token behind is drawn from.
-template <typename T>
-struct Rest {
-    const T *x, *y;      // target's and (or null) draft's
-    Weights wp, wq;
-    double inv_p, inv_q;  // 1 / sums
-    const double *table;
-    int n, first, token;  // token: drafted without probabilities, its weight is taken off (or -1)
-    enum { kSums, kRise, kTarget } what;  // sums of both rows; weights max(p - q, 0); weights p
-
-    template <bool BOTH>
-    __device__ __forceinline__ void load(int v, uint4 &e, uint4 &d) const {
-        load_vec(x, n, first, v, e);
-        if (!BOTH || y == nullptr) return;
-        if (first_of(y) == first) {
-            load_vec(y, n, first, v, d);
-        } else {  // the draft's row lies on another grid
-            uint32_t r[4] = {};
-#pragma unroll
-            for (int i = 0; i < kVec<T>; ++i) {
-                const int at = first + v * kVec<T> + i;
-                const bool in = at >= 0 && at < n;
-                if constexpr (sizeof(T) == 4) r[i] = in ? __float_as_uint(as_float(y[at])) : kNothing<T>;
-                else r[i / 2] |= (in ? static_cast<uint32_t>(__half_as_ushort(y[at])) : 0xFC00u) << (16 * (i & 1));
-            }
-            d = make_uint4(r[0], r[1], r[2], r[3]);
-        }
-    }
-    __device__ __forceinline__ double of(float e, float d, int at) const {
-        const double p = weight(e, wp, table);
-        if (what == kTarget) return at == token ? 0.0 : p;
-        const double a = __dmul_rn(p, inv_p), rise = a - __dmul_rn(weight(d, wq, table), inv_q);
-        return rise > a * kNoise ? rise : 0.0;
-    }
-    // this warp's sums over vectors [v0, v1), in every lane
-    __device__ __noinline__ double2 sums(int v0, int v1) const {
-        if (!wp.plain || !wq.plain) return rare_sums(v0, v1);
-        return what == kRise ? plain_sums<true, true>(v0, v1) : y != nullptr && what == kSums ? plain_sums<true, false>(v0, v1) : plain_sums<false, false>(v0, v1);
-    }
-    template <bool BOTH, bool RISE>
-    __device__ __forceinline__ double2 plain_sums(int v0, int v1) const {
-        double a = 0.0, b = 0.0;
-        const Weights p = wp, q = wq;
-        const double by_p = inv_p, by_q = inv_q;
-        const double *const powers_of = table;
-        const int skip = what == kTarget && token >= 0 ? token : -1;
-        auto take = [&](int v, const uint4 &e_raw, const uint4 &d_raw) {
-            float e[kVec<T>], d[kVec<T>];
-            values_of(e_raw, e);
-            if (BOTH) values_of(d_raw, d);
-            if (!BOTH) {
-                const unsigned at = static_cast<unsigned>(skip - (first + v * kVec<T>));
-                if (at < kVec<T>) {
-#pragma unroll
-                    for (int l = 0; l < kVec<T>; ++l)
-                        if (at == l) e[l] = -INFINITY;
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < kVec<T>; i += 4) {  // four elements of one or two rows side by side
-                double w[4], z[4];
-                powers<4>(e + i, p, powers_of, w);
-                if (BOTH) powers<4>(d + i, q, powers_of, z);
-                if (RISE) {
-#pragma unroll
-                    for (int l = 0; l < 4; ++l) {
-                        const double x = __dmul_rn(w[l], by_p), diff = x - __dmul_rn(z[l], by_q);
-                        w[l] = diff > x * kNoise ? diff : 0.0;
-                    }
-                }
-                a += (w[0] + w[1]) + (w[2] + w[3]);
-                if (BOTH && !RISE) b += (z[0] + z[1]) + (z[2] + z[3]);
-            }
-        };
-        auto fetch = [&](int v, uint4 &e, uint4 &d) {
-            if (v < v1) load<BOTH>(v, e, d);
-        };
-        uint4 e0, d0, e1, d1;
-        int v = v0 + static_cast<int>(threadIdx.x & 31);
-        fetch(v, e0, d0);
-        fetch(v + 32, e1, d1);
-        for (; v < v1; v += 64) {  // (the next two are on their way)
-            take(v, e0, d0);
-            fetch(v + 64, e0, d0);
-            if (v + 32 >= v1) break;
-            take(v + 32, e1, d1);
-            fetch(v + 96, e1, d1);
-        }
-        return make_double2(warp_total(a), warp_total(b));
-    }
-    __device__ __noinline__ double2 rare_sums(int v0, int v1) const {
-        double a = 0.0, b = 0.0;
-        for (int v = v0 + static_cast<int>(threadIdx.x & 31); v < v1; v += 32) {
-            uint4 e_raw, d_raw = make_uint4(0, 0, 0, 0);
-            load<true>(v, e_raw, d_raw);
-            float e[kVec<T>], d[kVec<T>];
-            values_of(e_raw, e);
-            values_of(d_raw, d);
-#pragma unroll 1
-            for (int i = 0; i < kVec<T>; ++i) {
-                const float ei = element(e, i), di = element(d, i);
-                if (what == kSums) a += weight(ei, wp, table), b += y != nullptr ? weight(di, wq, table) : 0.0;
-                else a += of(ei, di, first + v * kVec<T> + i);
-            }
-        }
-        return make_double2(warp_total(a), warp_total(b));
-    }
-    __device__ __forceinline__ static float element(const float (&e)[kVec<T>], int i) {
-        float v = e[0];
-#pragma unroll
-        for (int l = 1; l < kVec<T>; ++l) v = l == i ? e[l] : v;
-        return v;
-    }
-};
-
 template <typename T>
 __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const VerifyArgs a) {
     __shared__ Shared s;
@@ -320,7 +217,8 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const VerifyArgs a
 
     // ---- 1. largest and sum of every row.  The block's shares of all rows, one behind the other, are dealt to its warps in equal parts: a
     //      warp has one or two ends of a row to reduce, and reads in between without a pause.
-    const float c = static_cast<float>(kLog2e / static_cast<double>(temperature));
+    const double scale = fmax(kLog2e / static_cast<double>(temperature), 1e-300), reach = 1000.0 * kLn2 * fmin(static_cast<double>(temperature), 1e300);
+    const float c = static_cast<float>(scale);
     const long long total = static_cast<long long>(n_rows) * share;
     // (largest, sum) of two parts; greedy: (largest, its lowest index)
     auto join = [&](float &top, float &sum, float t, float v) {
@@ -449,12 +347,17 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const VerifyArgs a
                 verdict = my_token == __float_as_int(s.all_sum[r]) ? kAccept : kRefuse;
             } else {
                 // u wq / Sq < wp / Sp; the sums are of exp((x - top) / T), the weights have a factor of their own
-                const Weights wp = weights_of(s.all_top[r], temperature), wq = weights_of(s.all_top[with_draft ? r + 1 : r], temperature);
-                const float other = s.all_sum[with_draft ? r + 1 : r];
-                bool sure = wp.plain && wq.plain && s.all_sum[r] > 0.0f && s.all_sum[r] < INFINITY && other > 0.0f && other < INFINITY;
-                double left = static_cast<double>(my_u) * static_cast<double>(s.all_sum[r]), right = weight(my_x, wp, table);
-                left *= weight(wp.top, wp, table);
-                if (with_draft) left *= weight(my_y, wq, table), right *= static_cast<double>(other) * weight(wq.top, wq, table);
+                double left = static_cast<double>(my_u), right = 1.0;
+                bool sure = true;
+#pragma unroll 1
+                for (int side = 0; side < per_step; ++side) {
+                    const float sum = s.all_sum[r + side];
+                    const Weights w = weights_of(s.all_top[r + side], scale, reach);
+                    sure = sure && w.kind == kOrdinary && sum > 0.0f && sum < INFINITY;
+                    const double token_weight = weight(side ? my_y : my_x, w, table), whole = static_cast<double>(sum) * weight(w.top, w, table);
+                    left *= side ? token_weight : whole;
+                    right *= side ? whole : token_weight;
+                }
                 sure = sure && !(fabs(left - right) <= 1e-4 * fmax(fabs(left), fabs(right)));
                 verdict = !sure ? kUnsure : left < right ? kAccept : kRefuse;
             }
@@ -463,7 +366,8 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const VerifyArgs a
     }
     __syncthreads();
 
-    // ---- 3. the token behind, and what of the drafts is not sure yet
+    // ---- 3. the token behind, and what of the drafts is not sure yet.  No part of this may live in local memory: a barrier of the cluster empties
+    //      the L1 cache, and each access after it costs 600 cycles.  So there is one loop for all passes over the one or two rows, not a function.
     int j = 0, next = -1;
     while (j < len && s.verdict[j] == kAccept) ++j;
     bool mine = block == 0;  // whether this block writes the answer
@@ -471,135 +375,200 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const VerifyArgs a
         const int at = __float_as_int(s.all_sum[j]);
         next = at < n ? at : -1;
     } else {
-        const double last_u = static_cast<double>(u[k]);
-        Rest<T> rest;
-        rest.table = table;
-        rest.n = n;
-        rest.inv_p = rest.inv_q = 1.0;
-        auto look_at = [&] {  // row j
-            rest.x = target + static_cast<size_t>(j) * n;
-            rest.y = with_draft && j < len ? draft + static_cast<size_t>(j) * n : nullptr;
-            rest.first = first_of(rest.x);
-            rest.wp = weights_of(s.all_top[j * per_step], temperature);
-            rest.wq = rest.y != nullptr ? weights_of(s.all_top[j * per_step + 1], temperature) : rest.wp;
-            rest.token = j < len && !with_draft ? tokens[j] : -1;
-            rest.what = rest.y != nullptr || (j < len && s.verdict[j] == kUnsure) ? Rest<T>::kSums : Rest<T>::kTarget;
+        enum { kSums, kRise, kTarget };  // passes: sums of both rows; weights max(p - q, 0); weights p
+        int pass = kSums, turn = 0, skip = -1, first = 0;
+        bool again = true, fine = false;  // a new row j; the last pass, over one warp's part
+        const T *x = nullptr, *y = nullptr;
+        Weights wp{}, wq{};
+        double inv_p = 1.0, inv_q = 1.0, before = 0.0, point = 0.0;
+        int v0 = 0, v1 = 0, part0 = 0, part_size = 0;
+        auto above = [&](double p, double q) -> double {  // max(p - q, 0) of two weights
+            const double a = __dmul_rn(p, inv_p), rise = a - __dmul_rn(q, inv_q);
+            return rise > a * kNoise ? rise : 0.0;
         };
-        look_at();
-        int v0 = 0, v1 = 0, turn = 0;  // this warp's vectors
-        auto deal = [&](int w) {
-            const int n_vec = min((n - rest.first + VEC - 1) / VEC, from + share), size = max(0, n_vec - from);
-            v0 = from + static_cast<int>(static_cast<long long>(size) * w / WARPS);
-            v1 = from + static_cast<int>(static_cast<long long>(size) * (w + 1) / WARPS);
+        // the first of the lanes' sums that passes the point, else the last with a weight; what is before it is added up
+        auto pick = [&](double p) -> int {
+            double up_to = p;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const double t = __shfl_up_sync(0xffffffffu, up_to, off);
+                if (lane >= off) up_to += t;
+            }
+            const unsigned passed = __ballot_sync(0xffffffffu, p > kTiny && before + up_to > point), some = __ballot_sync(0xffffffffu, p > kTiny);
+            const int found = passed != 0 ? __ffs(static_cast<int>(passed)) - 1 : max(0, 31 - __clz(static_cast<int>(some)));
+            before += __shfl_sync(0xffffffffu, up_to - p, found);
+            return found;
         };
-        double whole = 0.0;
+        auto load = [&](int v, bool both, uint4 &e, uint4 &d) {
+            load_vec(x, n, first, v, e);
+            if (!both) return;
+            if (first_of(y) == first) {
+                load_vec(y, n, first, v, d);
+            } else {  // the draft's row lies on another grid
+                uint32_t r[4] = {};
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const int at = first + v * VEC + i;
+                    const bool in = at >= 0 && at < n;
+                    if constexpr (sizeof(T) == 4) r[i] = in ? __float_as_uint(as_float(y[at])) : kNothing<T>;
+                    else r[i / 2] |= (in ? static_cast<uint32_t>(__half_as_ushort(y[at])) : 0xFC00u) << (16 * (i & 1));
+                }
+                d = make_uint4(r[0], r[1], r[2], r[3]);
+            }
+        };
+        // weights of vector v, four at a time
+        auto weights = [&](int v, bool both, const uint4 &e_raw, const uint4 &d_raw, auto use) {
+            float e[VEC], d[VEC];
+            values_of(e_raw, e);
+            if (skip >= 0 && pass == kTarget) {
+                const int at = skip - (first + v * VEC);
+#pragma unroll
+                for (int l = 0; l < VEC; ++l)
+                    if (at == l) e[l] = -INFINITY;
+            }
+            ordinary<VEC>(wp, e);
+            if (both) {
+                values_of(d_raw, d);
+                ordinary<VEC>(wq, d);
+            }
+#pragma unroll
+            for (int i = 0; i < VEC; i += 4) {
+                double p[4], q[4] = {};
+                powers<4>(e + i, wp, table, p);
+                if (both) powers<4>(d + i, wq, table, q);
+                use(i, p, q);
+            }
+        };
 #pragma unroll 1
         for (;;) {
-            deal(warp);
-            const double2 sums = rest.sums(v0, v1);
-            if (lane == 0) s.warp_sum[0][warp] = sums.x, s.warp_sum[1][warp] = sums.y;
+            if (again) {
+                x = target + static_cast<size_t>(j) * n;
+                y = with_draft && j < len ? draft + static_cast<size_t>(j) * n : nullptr;
+                first = first_of(x);
+                wp = weights_of(s.all_top[j * per_step], scale, reach);
+                wq = y != nullptr ? weights_of(s.all_top[j * per_step + 1], scale, reach) : wp;
+                skip = j < len && !with_draft ? tokens[j] : -1;
+                pass = y != nullptr || (j < len && s.verdict[j] == kUnsure) ? kSums : kTarget;
+                const int n_vec = min((n - first + VEC - 1) / VEC, from + share);
+                part0 = from, part_size = max(0, n_vec - from);
+                again = false;
+            }
+            v0 = part0 + static_cast<int>(static_cast<long long>(part_size) * warp / WARPS);
+            v1 = part0 + static_cast<int>(static_cast<long long>(part_size) * (warp + 1) / WARPS);
+            const bool both = y != nullptr && pass != kTarget;
+            double sum_p = 0.0, sum_q = 0.0;
+            {
+                uint4 e0, d0, e1, d1;
+                e0 = d0 = e1 = d1 = make_uint4(0, 0, 0, 0);
+                int v = v0 + lane;
+                if (v < v1) load(v, both, e0, d0);
+                if (v + 32 < v1) load(v + 32, both, e1, d1);
+#pragma unroll 1
+                for (; v < v1; v += 32) {  // (two vectors on their way)
+                    const uint4 e = e0, d = d0;
+                    e0 = e1, d0 = d1;
+                    if (v + 64 < v1) load(v + 64, both, e1, d1);
+                    weights(v, both, e, d, [&](int, const double (&p)[4], const double (&q)[4]) {
+                        if (pass == kRise) {
+                            sum_p += (above(p[0], q[0]) + above(p[1], q[1])) + (above(p[2], q[2]) + above(p[3], q[3]));
+                        } else {
+                            sum_p += (p[0] + p[1]) + (p[2] + p[3]);
+                            if (both) sum_q += (q[0] + q[1]) + (q[2] + q[3]);
+                        }
+                    });
+                }
+            }
+            sum_p = warp_total(sum_p);
+            sum_q = warp_total(sum_q);
+            if (lane == 0) s.warp_sum[fine ? 2 : 0][warp] = sum_p, s.warp_sum[1][warp] = sum_q;
             __syncthreads();
+            if (fine) {
+                if (warp != 0) break;
+                const int w = pick(lane < WARPS ? s.warp_sum[2][lane] : 0.0), end = part0 + static_cast<int>(static_cast<long long>(part_size) * (w + 1) / WARPS);
+#pragma unroll 1
+                for (int v = part0 + static_cast<int>(static_cast<long long>(part_size) * w / WARPS); v < end; v += 32) {
+                    double r[VEC], ahead = 0.0;
+                    uint4 e = make_uint4(0, 0, 0, 0), d = e;
+                    const bool in = v + lane < end;
+                    if (in) load(v + lane, both, e, d);
+                    weights(v + lane, both, e, d, [&](int i, const double (&p)[4], const double (&q)[4]) {
+#pragma unroll
+                        for (int l = 0; l < 4; ++l) {
+                            const double w = pass == kRise ? above(p[l] > kTiny ? p[l] : 0.0, q[l] > kTiny ? q[l] : 0.0) : p[l] > kTiny ? p[l] : 0.0;
+                            r[i + l] = in ? w : 0.0;
+                            ahead += r[i + l];
+                        }
+                    });
+                    double up_to = ahead;
+#pragma unroll
+                    for (int off = 1; off < 32; off <<= 1) {
+                        const double t = __shfl_up_sync(0xffffffffu, up_to, off);
+                        if (lane >= off) up_to += t;
+                    }
+                    double t = before + (up_to - ahead);
+                    int passed = -1, some = -1;  // first weight that passes the point, last weight
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        t += r[i];
+                        if (r[i] > 0.0) {
+                            some = first + (v + lane) * VEC + i;
+                            if (passed < 0 && t > point) passed = some;
+                        }
+                    }
+                    const unsigned have = __ballot_sync(0xffffffffu, passed >= 0), any = __ballot_sync(0xffffffffu, some >= 0);
+                    if (have != 0) {
+                        next = __shfl_sync(0xffffffffu, passed, __ffs(static_cast<int>(have)) - 1);
+                        break;
+                    }
+                    if (any != 0) next = __shfl_sync(0xffffffffu, some, 31 - __clz(static_cast<int>(any)));
+                    before += __shfl_sync(0xffffffffu, up_to, 31);
+                }
+                break;
+            }
             if (warp == 0) {
                 const double p = warp_total(lane < WARPS ? s.warp_sum[0][lane] : 0.0), q = warp_total(lane < WARPS ? s.warp_sum[1][lane] : 0.0);
                 if (lane == 0) s.block_sum[turn][0] = p, s.block_sum[turn][1] = q;
             }
             sync_cluster();
-            double sum_p = 0.0, sum_q = 0.0;
+            double block_p = 0.0, block_q = 0.0;
             if (lane < static_cast<int>(n_blocks)) {
                 const uint32_t at = tc::in_block(tc::s32(&s.block_sum[turn][0]), lane);
-                sum_p = cluster_load_double(at);
-                sum_q = cluster_load_double(at + 8);
+                block_p = cluster_load_double(at);
+                block_q = cluster_load_double(at + 8);
             }
-            sum_p = warp_total(sum_p);
-            sum_q = warp_total(sum_q);
-            if (rest.what == Rest<T>::kSums) {
-                // (the buffer of the next turn was last read before this turn's barrier)
-                turn ^= 1;
-                rest.inv_p = sum_p > kTiny ? 1.0 / sum_p : 0.0;
-                rest.inv_q = sum_q > kTiny ? 1.0 / sum_q : 0.0;
+            sum_p = warp_total(block_p);
+            sum_q = warp_total(block_q);
+            turn ^= 1;  // (the other buffer was last read before this turn's barrier)
+            if (pass == kSums) {
+                inv_p = sum_p > kTiny ? 1.0 / sum_p : 0.0;
+                inv_q = sum_q > kTiny ? 1.0 / sum_q : 0.0;
                 if (s.verdict[j] == kUnsure) {  // (only where j < len)
                     const int token = tokens[j];
-                    const double p = weight(as_float(rest.x[token]), rest.wp, table) * rest.inv_p;
-                    const double q = with_draft ? weight(as_float(rest.y[token]), rest.wq, table) * rest.inv_q : 1.0;
+                    const double p = weight(as_float(x[token]), wp, table) * inv_p, q = with_draft ? weight(as_float(y[token]), wq, table) * inv_q : 1.0;
                     if (static_cast<double>(u[j]) * q < p) {
                         do ++j;
                         while (j < len && s.verdict[j] == kAccept);
-                        look_at();
+                        again = true;
                         continue;
                     }
                 }
-                rest.what = with_draft ? Rest<T>::kRise : Rest<T>::kTarget;
+                pass = with_draft ? kRise : kTarget;
                 continue;
             }
-            whole = sum_p;
-            if (whole > kTiny || (rest.what == Rest<T>::kTarget && rest.token < 0)) break;
-            turn ^= 1;
-            rest.what = Rest<T>::kTarget;  // nothing is left of p: p itself
-            rest.token = -1;
-        }
-        const double point = last_u * whole;
-        if (whole > kTiny) {
-            // The block, the warp's part, a part of that, the element: the first whose sums pass the point, else the last with a weight.
-            double before = 0.0;
-            auto pick = [&](double p) -> int {  // of the lanes' sums
-                double up_to = p;
-#pragma unroll
-                for (int off = 1; off < 32; off <<= 1) {
-                    const double t = __shfl_up_sync(0xffffffffu, up_to, off);
-                    if (lane >= off) up_to += t;
-                }
-                const unsigned passed = __ballot_sync(0xffffffffu, p > kTiny && before + up_to > point), some = __ballot_sync(0xffffffffu, p > kTiny);
-                const int found = passed != 0 ? __ffs(static_cast<int>(passed)) - 1 : max(0, 31 - __clz(static_cast<int>(some)));
-                before += __shfl_sync(0xffffffffu, up_to - p, found);
-                return found;
-            };
-            const int chosen = pick(lane < static_cast<int>(n_blocks) ? cluster_load_double(tc::in_block(tc::s32(&s.block_sum[turn][0]), lane)) : 0.0);
-            mine = static_cast<int>(block) == chosen;
-            if (mine) {  // (the whole block)
-                deal(pick(lane < WARPS ? s.warp_sum[0][lane] : 0.0));
-                const int w0 = v0, size = v1 - v0;
-                const double2 sums = rest.sums(w0 + size * warp / WARPS, w0 + size * (warp + 1) / WARPS);
-                if (lane == 0) s.warp_sum[1][warp] = sums.x;
-                __syncthreads();
-                if (warp == 0) {
-                    const int w = pick(lane < WARPS ? s.warp_sum[1][lane] : 0.0), end = w0 + size * (w + 1) / WARPS;
-#pragma unroll 1
-                    for (int v = w0 + size * w / WARPS; v < end; v += 32) {
-                        double r[VEC], ahead = 0.0;
-                        float e[VEC], d[VEC];
-                        uint4 e_raw = make_uint4(0, 0, 0, 0), d_raw = e_raw;
-                        const bool in = v + lane < end;
-                        if (in) rest.template load<true>(v + lane, e_raw, d_raw);
-                        values_of(e_raw, e);
-                        values_of(d_raw, d);
-#pragma unroll
-                        for (int i = 0; i < VEC; ++i) r[i] = in ? rest.of(e[i], d[i], rest.first + (v + lane) * VEC + i) : 0.0, ahead += r[i];
-                        double up_to = ahead;
-#pragma unroll
-                        for (int off = 1; off < 32; off <<= 1) {
-                            const double t = __shfl_up_sync(0xffffffffu, up_to, off);
-                            if (lane >= off) up_to += t;
-                        }
-                        double t = before + (up_to - ahead);
-                        int passed = -1, some = -1;  // first weight that passes the point, last weight
-#pragma unroll
-                        for (int i = 0; i < VEC; ++i) {
-                            t += r[i];
-                            if (r[i] > 0.0) {
-                                some = rest.first + (v + lane) * VEC + i;
-                                if (passed < 0 && t > point) passed = some;
-                            }
-                        }
-                        const unsigned have = __ballot_sync(0xffffffffu, passed >= 0), any = __ballot_sync(0xffffffffu, some >= 0);
-                        if (have != 0) {
-                            next = __shfl_sync(0xffffffffu, passed, __ffs(static_cast<int>(have)) - 1);
-                            break;
-                        }
-                        if (any != 0) next = __shfl_sync(0xffffffffu, some, 31 - __clz(static_cast<int>(any)));
-                        before += __shfl_sync(0xffffffffu, up_to, 31);
-                    }
-                }
+            if (!(sum_p > kTiny)) {
+                if (pass == kTarget && skip < 0) break;  // an empty row
+                pass = kTarget;                          // nothing is left of p: p itself
+                skip = -1;
+                continue;
             }
+            point = static_cast<double>(u[k]) * sum_p;
+            mine = static_cast<int>(block) == pick(block_p);
+            if (!mine) break;
+            // (the whole block) one warp's part again, in as many parts
+            const int w = pick(lane < WARPS ? s.warp_sum[0][lane] : 0.0);
+            const int begin = part0 + static_cast<int>(static_cast<long long>(part_size) * w / WARPS), end = part0 + static_cast<int>(static_cast<long long>(part_size) * (w + 1) / WARPS);
+            part0 = begin, part_size = end - begin;
+            fine = true;
         }
     }
     if (mine && warp == 0) {
