@@ -212,6 +212,47 @@ def test_between_matvecs_of_gguf_blocks(codebooks):
     rt.close()
 
 
+@pytest.mark.parametrize("ntok", [1, 8, 24])
+def test_products_and_matvecs_that_begin_before_the_last_one_ends(codebooks, ntok):
+    """Captured products of few rows and matvecs by turns: blocks of two launches share SMs and their tensor memory."""
+    from vinf_3080ti_b200.runtime import Runtime
+
+    rt = Runtime(codebooks["iq3s_grid"], codebooks)
+    rng = np.random.default_rng(6)
+    rt.upload("a", synthetic_blocks(T.Q4_K, 2048, 1024, rng), int(T.Q4_K), 1024, 2048)
+    for name, rows in (("few", 384), ("many", 19000)):
+        w = rng.integers(-127, 128, (rows, 1024), dtype=np.int8)
+        rt.upload_i8(name, w, np.full(rows, 1e-3, np.float32), 1024, rows)
+    for name, n, e in (("x", ntok * 1024, 4), ("q", ntok * 1024, 1), ("s", ntok, 4), ("y", ntok * 2048, 4), ("few_y", ntok * 384, 4), ("many_y", ntok * 19000, 4)):
+        rt.alloc(name, n, e)
+    rt.write("x", rng.standard_normal((ntok, 1024)).astype(np.float32))
+    rt.rows_i8("x", "q", "s", 1024, ntok)
+
+    def go(wait):
+        for _ in range(1 if wait else 25):
+            for call in (lambda: rt.qmm_i8("few", "q", "s", "few_y", ntok), lambda: rt.qmv("a", "x", "y", ntok), lambda: rt.qmm_i8("many", "q", "s", "many_y", ntok),
+                         lambda: rt.qmv("a", "x", "y", ntok)):
+                call()
+                if wait:
+                    rt.synchronize()
+
+    def seen():
+        return [rt.read(n) for n in ("y", "few_y", "many_y")]
+
+    go(True)
+    want = seen()
+    rt.capture_begin()
+    go(False)
+    graph = rt.capture_end()
+    for _ in range(4):
+        for n in ("y", "few_y", "many_y"):
+            rt.zero(n)
+        rt.graph_launch(graph)
+        assert seen() == want
+    rt.graph_destroy(graph)
+    rt.close()
+
+
 FIRST_IN_A_CAPTURE = """
 import sys
 import numpy as np

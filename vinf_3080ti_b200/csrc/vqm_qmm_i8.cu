@@ -171,7 +171,6 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
     const int n_tiles = a.row_tiles * a.tok_tiles;
     const uint32_t stage_bytes = kQA + a.b_bytes;
 
-    if (a.half_sm) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; ++s) {
             bar_init(s32(&s_full[s]), PAIR && rank == 0 ? 2 : 1);  // the first block of a pair hears of the second's stage
@@ -196,6 +195,8 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    // Not before this block has its tensor memory: a block of the next launch, which waits for this one's end, could take all that the SM has.
+    if (a.half_sm) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if constexpr (PAIR || SPLIT) cluster_sync();  // the other blocks' barriers and tensor memory exist
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = s_tmem;
