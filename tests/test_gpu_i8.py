@@ -198,6 +198,16 @@ def test_zero_tiny_and_huge_rows(rt):
     check_rows(rt, x, x2=np.ones((8, 96), np.float32))
 
 
+@pytest.mark.parametrize("cols", [64, 67, 1536])
+def test_norms_of_values_at_the_ends_of_fp32(rt, cols):
+    """Root mean squares whose reciprocal fp32 does not hold, and weights that bring the products back."""
+    rng = np.random.default_rng(cols)
+    g = rng.uniform(0.5, 1.5, cols)
+    x = rng.standard_normal((40, cols))
+    for size, weight in ((1e-40, 1e20), (1e-38, 1e18), (1e-42, 1e30), (8e37, 1e-20), (8e37, 1e-8), (3e37, 1.0)):
+        check_rows(rt, (x.clip(-4, 4) * size).astype(np.float32), norm=(g * weight).astype(np.float32), eps=0.0)
+
+
 def test_undefined_rows_have_an_undefined_scale_and_leave_the_others_alone(rt):
     rng = np.random.default_rng(5)
     x = rng.standard_normal((6, 333)).astype(np.float32)

@@ -395,12 +395,12 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rows_i8_kerne
         const float scale = wide >= kMostScale ? kUndefined : static_cast<float>(wide);
         s.r = r;
         s.scale = static_cast<double>(scale);
-        s.factor = scale > 1e-37f ? __fdividef(static_cast<float>(r), scale) : 0.0f;
+        s.factor = scale > 1e-37f && r > 1.2e-38 && r < 1e38 ? __fdividef(static_cast<float>(r), scale) : 0.0f;  // (r as a normal fp32 number)
         a.scales[row] = scale;
     }
     __syncthreads();
     const float f = s.factor;  // about 127 / largest
-    if (f == 0.0f) {  // (a norm can take the scale out of the middle range; so can an undefined one)
+    if (f == 0.0f) {  // (a norm can take the scale or its own factor out of the middle range; so can an undefined one)
         exact_row<T>(a, row, true, s);
         return;
     }
