@@ -149,12 +149,12 @@ int vqm_dequantize(vqm_runtime *rt, const char *weight, const char *out);
 /* ---- Passes in 8-bit integers (no counterpart in the reference) ----
  * A weight tensor of 8-bit integer rows holds W[r][k] = scales[r] * w[r][k], w int8; activations are int8 rows with one fp32 scale
  * per row.  Rows of 8-bit values lie `pitch` bytes apart, a multiple of 16: activations at round_up(cols, 16).  1 <= cols <= 131071 (with
- * more a 32-bit sum could overflow).  Buffers of 8-bit values are allocated or bound with elem = 1.  has / free / tensor_info
+ * more a 32-bit sum could overflow); rows and a product's ntok are at most 2^30.  Buffers of 8-bit values are allocated or bound with elem = 1.  has / free / tensor_info
  * (type VQM_I8_ROWS, row_bytes = pitch) / device_bytes know these tensors; the matvec entry points refuse them (VQM_ERR_VALUE).
  *
  * vqm_upload_i8   w: rows * cols int8 in host memory, densely packed; scales: rows floats.  Synchronous; re-upload replaces.
- * vqm_bind_i8     the same in device memory that the caller keeps and has filled (products fetch weights ahead of the stream's order): 16-byte aligned, `pitch` bytes from row to row (0: round_up(cols, 16));
- *                 what lies behind a row's last column is ignored.
+ * vqm_bind_i8     the same in device memory that the caller keeps and has filled (products fetch weights ahead of the stream's order): 16-byte
+ *                 aligned, `pitch` bytes from row to row (0: round_up(cols, 16)); what lies behind a row's last column is ignored.
  * vqm_convert_i8  makes the tensor `name` from any GGUF tensor: scales[r] = max |row r| / 127, values to the nearest integer.  Synchronous.
  */
 #define VQM_I8_ROWS 24
@@ -171,8 +171,9 @@ int vqm_convert_i8(vqm_runtime *rt, const char *weight, const char *name);
  * scale and q = 0, which makes its products undefined.  x, x2, residual and total share one type.  Buffers do not overlap otherwise. */
 int vqm_rows_i8(vqm_runtime *rt, const char *x, const char *q, const char *scales, int cols, int ntok, int flags, const char *x2, const char *residual,
                 const char *total, const char *norm_weight, float eps);
-/* y[t][r] = scales[t] * W scales[r] * sum_k q[t][k] w[r][k] (VQM_FUSE_ADD: +=) for a tensor of 8-bit integer rows; sums are exact, y is an fp32 or
- * fp16 buffer.  Asynchronous; any ntok >= 1. */
+/* y[t][r] = sum_k q[t][k] w[r][k] * scales[t] * W scales[r] (VQM_FUSE_ADD: +=) for a tensor of 8-bit integer rows; sums are exact, the two products
+ * are fp32, in this order; y is an fp32 or fp16 buffer that overlaps
+ * none of the others.  Asynchronous. */
 int vqm_qmm_i8(vqm_runtime *rt, const char *weight, const char *q, const char *scales, const char *y, int ntok, int flags);
 
 /* Verification of drafted tokens against the target's probabilities (no counterpart in the reference, whose speculative decoder compares greedy
@@ -188,7 +189,8 @@ int vqm_qmm_i8(vqm_runtime *rt, const char *weight, const char *q, const char *s
  * token is drawn from p.  Logits of -inf and NaN have no probability; a row without any refuses its draft, and the
  * token drawn from such a row is -1.  A token outside [0, vocab) is refused, and where drafts have no probabilities nothing is taken off p then.
  * out [seqs][drafts + 2] (int32): the number of accepted drafts a, the accepted tokens, the next token, then -1.  out_host (seqs * (drafts + 2)
- * ints) may be NULL: then the call is asynchronous.  target and draft are both fp32 or both fp16.  drafts = 0 samples from the target.
+ * ints) may be NULL: then the call is asynchronous.  target and draft are both fp32 or both fp16; `out` overlaps none
+ * of the others.  drafts = 0 samples from the target.
  * 0 <= drafts <= VQM_MAX_DRAFTS, vocab <= VQM_MAX_VOCAB. */
 #define VQM_MAX_DRAFTS 255
 #define VQM_MAX_VOCAB 1073741824

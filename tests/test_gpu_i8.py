@@ -538,6 +538,35 @@ def test_refusals(rt):
     rt.synchronize()
 
 
+def test_what_is_written_has_a_buffer_of_its_own(rt):
+    rt.upload_i8("w8", np.zeros((2, 4), np.int8), np.ones(2, np.float32), 4, 2)
+    for name, n, elem in (("x", 8, 4), ("r", 8, 4), ("q", 32, 1), ("s", 4, 4), ("g", 4, 4), ("y", 4, 4)):
+        rt.alloc(name, n, elem)
+    for kw in (dict(x="s", scales="s", ntok=1), dict(silu_mul="s", ntok=1), dict(norm="s"), dict(residual="s", total="r", ntok=1), dict(residual="r", total="s", ntok=1),
+               dict(residual="g", norm="g", ntok=1)):
+        a = {**dict(x="x", q="q", scales="s", cols=4, ntok=2), **kw}
+        with pytest.raises(ValueError, match="of their own"):
+            rt.rows_i8(a.pop("x"), a.pop("q"), a.pop("scales"), a.pop("cols"), a.pop("ntok"), **a)
+    with pytest.raises(ValueError, match="of their own"):
+        rt.qmm_i8("w8", "q", "s", "s", 2)
+    rt.rows_i8("x", "q", "s", 4, 2, residual="r", total="x", norm="g")
+    rt.qmm_i8("w8", "q", "s", "y", 2)
+    rt.synchronize()
+
+
+def test_more_rows_than_an_integer_counts_by_tiles_are_refused(rt):
+    rt.alloc("x", 4)
+    at = rt.buffer_ptr("x")[0]
+    for rows in (2**30 + 1, 2**31 - 1):
+        with pytest.raises(ValueError, match="at most"):
+            rt.bind_i8("n", at, at, 16, rows)
+    rt.upload_i8("w8", np.zeros((2, 4), np.int8), np.ones(2, np.float32), 4, 2)
+    rt.alloc("q", 32, 1)
+    for ntok in (2**30 + 1, 2**31 - 1):
+        with pytest.raises(ValueError, match="ntok"):
+            rt.qmm_i8("w8", "q", "x", "x", ntok)
+
+
 def test_bytes_are_written_copied_and_read(rt):
     data = np.arange(-100, 100, dtype=np.int8)
     rt.alloc("b", 200, 1)

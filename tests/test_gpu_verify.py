@@ -252,3 +252,12 @@ def test_refusals(rt):
         rt.verify(**ok, blocking=False)
     finally:
         rt.graph_destroy(rt.capture_end())
+
+
+@pytest.mark.parametrize("name", ["target", "draft", "tokens", "u", "lens", "temp"])
+def test_answers_have_a_buffer_of_their_own(rt, name):
+    for buffer in ("target", "draft", "tokens", "u", "lens", "temp", "out"):
+        rt.alloc(buffer, 60)
+    with pytest.raises(ValueError, match="of their own"):
+        rt.verify("target", "draft", "tokens", "u", 10, 2, 2, lens="lens", temperature="temp", out=name)
+    rt.verify("target", "draft", "tokens", "u", 10, 2, 2, lens="lens", temperature="temp", out="out")

@@ -172,6 +172,7 @@ cudaError_t launch_fetch(const void *from, void *to, int n16, cudaStream_t strea
 
 constexpr int kI8Rows = 24;          // type id of a weight tensor of 8-bit integer rows with a scale each (VQM_I8_ROWS)
 constexpr int kI8MaxCols = 131071;   // (2^17 - 1) * 2^14 still fits into a 32-bit sum
+constexpr int kI8MaxRows = 1 << 30;  // (sums of a row and a tile fit into 32 bits)
 __host__ __device__ constexpr long long i8_pitch(int cols) { return (static_cast<long long>(cols) + 15) / 16 * 16; }  // bytes from one row of 8-bit values to the next
 
 struct RowsI8Args {

@@ -1502,9 +1502,17 @@ int entry(vqm_runtime *rt, std::initializer_list<const char *> names, F &&body) 
     }
 }
 
+// What is written by blocks while others still read lies in a buffer of its own.
+int check_apart(const char *what, const void *written, std::initializer_list<const void *> read) {
+    for (const void *p : read)
+        if (p == written) return fail(VQM_ERR_VALUE, "%s need a buffer of their own", what);
+    return VQM_OK;
+}
+
 int check_i8_shape(const char *name, int cols, int rows) {
     if (cols < 1 || rows < 1) return fail(VQM_ERR_VALUE, "%s: rows and columns must be positive", name);
     if (cols > vqm::kI8MaxCols) return fail(VQM_ERR_VALUE, "%s: 8-bit integer rows have at most %d columns (32-bit sums)", name, vqm::kI8MaxCols);
+    if (rows > vqm::kI8MaxRows) return fail(VQM_ERR_VALUE, "%s: at most %d rows", name, vqm::kI8MaxRows);
     return VQM_OK;
 }
 
@@ -1564,6 +1572,7 @@ int vqm_upload_i8(vqm_runtime *rt, const char *name, const void *data, size_t nb
         if (err == cudaSuccess && t.row_bytes != static_cast<size_t>(cols)) err = cudaMemset(t.data, 0, t.row_bytes * rows);
         if (err == cudaSuccess) err = cudaMemcpy2D(t.data, t.row_bytes, data, cols, cols, rows, cudaMemcpyHostToDevice);
         if (err == cudaSuccess) err = cudaMemcpy(const_cast<float *>(t.scales), scales, scale_bytes, cudaMemcpyHostToDevice);
+        if (err == cudaSuccess) err = cudaStreamSynchronize(nullptr);  // (a copy from pageable memory may return while its last part is on its way)
         if (err != cudaSuccess) {
             release(t);
             return cuda_fail("upload_i8", err);
@@ -1675,6 +1684,8 @@ int vqm_rows_i8(vqm_runtime *rt, const char *x, const char *q, const char *scale
             if ((a.norm_w = find_norm(rt, norm_weight, cols, &rc)) == nullptr) return rc;
             if (!(eps >= 0.0f)) return fail(VQM_ERR_VALUE, "eps must be >= 0");
         }
+        if ((rc = check_apart("the scales", a.scales, {a.x, a.x2, a.residual, a.total, a.norm_w})) != VQM_OK) return rc;
+        if (a.total != nullptr && (rc = check_apart("the sums", a.total, {a.norm_w})) != VQM_OK) return rc;
         const cudaError_t err = vqm::launch_rows_i8(a, rt->sm_count, rt->stream);
         if (err != cudaSuccess) return cuda_fail("rows_i8 launch", err);
         count_launch(rt);
@@ -1684,7 +1695,7 @@ int vqm_rows_i8(vqm_runtime *rt, const char *x, const char *q, const char *scale
 
 int vqm_qmm_i8(vqm_runtime *rt, const char *weight, const char *q, const char *scales, const char *y, int ntok, int flags) {
     return entry(rt, {weight, q, scales, y}, [&]() -> int {
-        if (ntok < 1) return fail(VQM_ERR_VALUE, "ntok must be positive");
+        if (ntok < 1 || ntok > vqm::kI8MaxRows) return fail(VQM_ERR_VALUE, "ntok must be in [1, %d]", vqm::kI8MaxRows);
         if ((flags & ~VQM_FUSE_ADD) != 0) return fail(VQM_ERR_VALUE, "unknown flag bits %d", flags);
         int rc = VQM_OK;
         Tensor *t = find_i8_tensor(rt, weight, &rc);
@@ -1693,6 +1704,7 @@ int vqm_qmm_i8(vqm_runtime *rt, const char *weight, const char *q, const char *s
         if ((a.q = find_i8(rt, q, static_cast<size_t>(vqm::i8_pitch(t->cols)) * ntok, &rc)) == nullptr) return rc;
         if ((a.q_scales = find_f32(rt, scales, static_cast<size_t>(ntok), &rc)) == nullptr) return rc;
         if ((a.y = find_real(rt, y, static_cast<size_t>(t->rows) * ntok, &a.y_elem, &rc)) == nullptr) return rc;
+        if ((rc = check_apart("the outputs", a.y, {a.q_scales})) != VQM_OK) return rc;
         a.w = reinterpret_cast<const int8_t *>(t->data);
         a.w_scales = t->scales;
         a.w_pitch = static_cast<long long>(t->row_bytes);
@@ -1727,6 +1739,7 @@ int vqm_verify(vqm_runtime *rt, const char *target, const char *draft, const cha
         if ((a.uniforms = find_f32(rt, uniforms, s * (k + 1), &rc)) == nullptr) return rc;
         if (temperature != nullptr && (a.temperature = find_f32(rt, temperature, s, &rc)) == nullptr) return rc;
         if ((a.out = static_cast<int *>(find_real(rt, out, s * (k + 2), &word, &rc))) == nullptr) return rc;
+        if ((rc = check_apart("the answers", a.out, {a.target, a.draft, a.tokens, a.lens, a.uniforms, a.temperature})) != VQM_OK) return rc;
         if (out_host != nullptr && (rc = no_capture(rt, "a blocking verify")) != VQM_OK) return rc;
         cudaError_t err = vqm::launch_verify(a, rt->stream);
         if (err != cudaSuccess) return cuda_fail("verify launch", err);
