@@ -198,6 +198,24 @@ def test_zero_tiny_and_huge_rows(rt):
     check_rows(rt, x, x2=np.ones((8, 96), np.float32))
 
 
+@pytest.mark.parametrize("kind", [np.float32, np.float16])
+@pytest.mark.parametrize("ntok", [3, 150])
+@pytest.mark.parametrize("cols", [1018, 1019, 1024, 1028, 4090, 4091, 4096, 4100, 5120, 5121, 6138, 6140, 10232, 10234, 10236, 12281, 12284, 16384, 17406, 18432, 18435, 20474, 20480, 24563])
+def test_lengths_and_numbers_of_rows_at_which_blocks_change(rt, cols, ntok, kind):
+    rng = np.random.default_rng(cols + ntok)
+    x, y = (rng.standard_normal((ntok, cols)).astype(kind) for _ in range(2))
+    check_rows(rt, x, residual=y, norm=rng.uniform(0.5, 1.5, cols).astype(np.float32), total="t")
+    check_rows(rt, x, x2=y)
+
+
+def test_gates_that_are_subnormal_or_far_below_zero(rt):
+    """Their sigmoid or their product with it has few digits left, their values count all the same."""
+    rng = np.random.default_rng(8)
+    for low, high, size in ((1e-42, 1e-39, 1e30), (1e-38, 1e-37, 1e28), (-79.9, -60.0, 1e32), (-80.0, -1.0, 1.0), (-120.0, -70.0, 1e3), (-85.0, -79.0, 2e3)):
+        x = rng.uniform(low, high, (30, 999)).astype(np.float32)
+        check_rows(rt, x, x2=(rng.standard_normal((30, 999)) * size).astype(np.float32))
+
+
 @pytest.mark.parametrize("cols", [64, 67, 1536])
 def test_norms_of_values_at_the_ends_of_fp32(rt, cols):
     """Root mean squares whose reciprocal fp32 does not hold, and weights that bring the products back."""

@@ -5,13 +5,15 @@
 // taken in 64 bits (the mean's square root cancels out of n / s but for the rounding of s), the values in 32, and a value that 32 bits leave next to a
 // half is worked out again in 64.
 //
-// A block per row (of 32 to 512 threads), its values in registers: memory is read and written once.
+// A block per row (of 32 to 1024 threads), its values in registers: memory is read and written once.
 // Rows too long for that, norms of gated values, and rows whose largest value is out of fp32's middle range are worked out in 64 bits throughout.
 //
-// What bounds it: 4001 rows of 5120 with residual and norm take 53 us in fp32 (4980 GB/s of the 6550 that a copy gets) and 40 in fp16 (3550 GB/s): there the
-// instructions, 36 per element of which half are conversions, the mean's 64 bits and the norm's weights, and a row's steps one after the other (13000 cycles,
-// seven rows at a time on an SM).  1000 gated rows of 17408: 57 us (2730 GB/s), two of ex2 and a reciprocal per element and the rows' steps.  One row: 3.3 us.
-// Tried: rows copied ahead into shared memory by blocks that stay (71 us for 47), five or six blocks of 256 threads per SM (spills, 53 and 69).
+// What bounds it: 4001 rows of 5120 with residual and norm take 51 us in fp32 (5200 GB/s of the 6550 that a copy gets) and 36 in fp16 (3980 GB/s): there the
+// instructions, 33 per element, the mean's 64 bits and the norm's weights, and a row's steps one after the other.  1000 gated rows of 17408: 48.5 us in
+// fp32 (3230 GB/s), 36 in fp16; 4001 of 5120: 37 and 38, ex2 and a reciprocal per element and the rows' steps.  One row: 3.4 us.
+// What it took: more rows at a time on an SM (below); an error bound of the gate that looks at the values, so that fewer of them are worked out in 64 bits (1000
+// gated rows of 17408 57 and 52 us, 4001 of 5120 in fp16 53 and 38).
+// Tried: rows copied ahead into shared memory by blocks that stay (71 us for 47), four values looked at together for nearness to a half (no gain).
 #include <cuda_fp16.h>
 
 #include "vqm_kernels.h"
@@ -29,7 +31,7 @@ __device__ __forceinline__ void load4(const float *p, float (&v)[4]) {
     v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
 }
 
-constexpr int kMostFast = 24564;  // columns of a row that 512 threads hold in 12 vectors each, wherever it begins
+constexpr int kMostFast = 24564;  // columns of a row that 512 threads hold in 12 vectors each, or 1024 in 6, wherever it begins
 constexpr float kUndefined = __builtin_nanf("");
 constexpr double kMostScale = 3.4028235677973366e38;  // half a step above fp32's largest: rounds to infinity from here on
 
@@ -164,6 +166,18 @@ __global__ void __launch_bounds__(512) gated_norm_kernel(const RowsI8Args a) {
 // silu(x) * y in 64 bits
 static __device__ __noinline__ double exact_gate(float x, float y) { return static_cast<double>(x) / (1.0 + exp(-static_cast<double>(x))) * static_cast<double>(y); }
 
+// n / s as a whole number, n = d r, in 64 bits (divided: a tie stays a tie)
+static __device__ __noinline__ int exact_whole(double d, double r, double scale) { return __double2int_rn(d * r / scale); }
+
+// 1 / (1 + exp(-x)), off by no more than 5e-7 + 7.5e-8 max(-x, 0): 2^-22 of ex2, 2^-24 |x| of its argument and 1.4e-8 |x| of the constant in it, 2^-24 of the
+// sum, 2^-23 of the reciprocal.
+__device__ __forceinline__ float sigmoid(float x) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.44269504f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return r;
+}
+
 __device__ __forceinline__ float largest_of(float a, float b) {  // undefined if either is
     float m;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
@@ -193,6 +207,10 @@ struct Kept {
         for (int l = 0; l < 4; ++l) f[l] = v[l];
     }
     __device__ __forceinline__ void put_to(float *p) const { *reinterpret_cast<float4 *>(p) = make_float4(f[0], f[1], f[2], f[3]); }
+    __device__ __forceinline__ void add(const Kept &y) {
+#pragma unroll
+        for (int l = 0; l < 4; ++l) f[l] += y.f[l];
+    }
 };
 template <>
 struct Kept<__half, false> {
@@ -207,6 +225,12 @@ struct Kept<__half, false> {
         w = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
     }
     __device__ __forceinline__ void put_to(__half *p) const { *reinterpret_cast<uint2 *>(p) = w; }
+    // (one rounding, as of the fp32 sum: its 24 bits are twice 11 and two more)
+    __device__ __forceinline__ void add(const Kept &y) {
+        const __half2 a = __hadd2_rn(*reinterpret_cast<const __half2 *>(&w.x), *reinterpret_cast<const __half2 *>(&y.w.x));
+        const __half2 b = __hadd2_rn(*reinterpret_cast<const __half2 *>(&w.y), *reinterpret_cast<const __half2 *>(&y.w.y));
+        w = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    }
 };
 template <typename T, bool WIDE>
 __device__ __forceinline__ void Kept<T, WIDE>::fetch(const T *p) {
@@ -219,11 +243,21 @@ __device__ __forceinline__ void Kept<T, WIDE>::fetch(const T *p) {
     }
 }
 
+// Blocks that an SM holds at least, which bounds the registers: while some rows wait for memory, others are worked on.  Measured, against one block less or
+// more: fp16, 128 threads 35.8 us (6: 37.1; 8, with spills: 41.9; 4001 rows of 5120), 256 threads 19.2 (3: 20.5; 1000 of 8192), 512 threads 27.1 (1: 32.6;
+// 600 of 17408); fp32, 256 threads with 5 vectors 51.2 (3: 53.4; 4001 of 5120), with more of them 3 (5 or 6 spill).
+template <typename T, int NV, int THREADS>
+constexpr int blocks_per_sm() {
+    if (THREADS == 512) return 2;
+    if (THREADS == 256) return sizeof(T) == 2 || NV <= 5 ? 4 : 3;
+    return THREADS == 128 && sizeof(T) == 2 ? 7 : 1;
+}
+
 // A block per row.  A thread holds NV vectors of 4 neighbouring columns, vector i at (thread + i * threads) * 4: v before the norm's weights, which come
 // from the caches both times.  LOOSE: rows of any length, whose vectors lie on the buffers' grid, not the row's: the first and the last may be
 // partly outside of the row, and the norm's weights and the outputs, which lie on other grids, go one by one.
 template <typename T, int NV, int THREADS, bool GATED, bool LOOSE>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rows_i8_kernel(const RowsI8Args a) {
+__global__ void __launch_bounds__(THREADS, blocks_per_sm<T, NV, THREADS>()) rows_i8_kernel(const RowsI8Args a) {
     __shared__ RowShared s;
     constexpr int WARPS = THREADS / 32;
     const size_t row = blockIdx.x, at = row * a.cols;
@@ -263,7 +297,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rows_i8_kerne
         if (column(i) < a.cols) fetch(v[i], x, i);
         else v[i].keep(none);
     }
-    float top = 0.0f;
+    float top = 0.0f, lowest = 0.0f;
     if (GATED || a.residual != nullptr) {
         Kept<T, false> y[NV];
 #pragma unroll
@@ -272,25 +306,28 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rows_i8_kerne
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (column(i) >= a.cols) continue;
-            float e[4], d[4];
-            v[i].values(e);
-            y[i].values(d);
+            if constexpr (GATED) {
+                float e[4], d[4];
+                v[i].values(e);
+                y[i].values(d);
+                const float least = fminf(fminf(e[0], e[1]), fminf(e[2], e[3]));
+                lowest = fminf(lowest, least);
+                if (least < -80.0f) {
 #pragma unroll
-            for (int l = 0; l < 4; ++l) {
-                if constexpr (GATED) {
-                    // silu(-inf) is undefined; silu(-80) = -1e-33 may have lost digits, which shows if y is large: not this way
-                    if (e[l] < -80.0f && (fabsf(d[l]) > 1e3f || e[l] == -INFINITY)) top = INFINITY;
-                    e[l] = __fdividef(e[l], 1.0f + __expf(-e[l])) * d[l];
-                } else {
-                    e[l] += d[l];
+                    for (int l = 0; l < 4; ++l)  // silu(-inf) is undefined; silu(-80) = -1e-33 may have lost digits, which shows if y is large: not this way
+                        if (e[l] < -80.0f && (fabsf(d[l]) > 1e3f || e[l] == -INFINITY)) top = INFINITY;
                 }
-            }
-            v[i].keep(e);
-            if constexpr (!GATED) {
+#pragma unroll
+                for (int l = 0; l < 4; ++l) e[l] = e[l] * d[l] * sigmoid(e[l]);  // (x y first: the product of a tiny x with the sigmoid would lose digits)
+                v[i].keep(e);
+            } else {
+                v[i].add(y[i]);
                 T *const to = static_cast<T *>(a.total) + at + column(i);
                 if (whole(i)) {
                     v[i].put_to(to);
                 } else {
+                    float e[4];
+                    v[i].values(e);
 #pragma unroll
                     for (int l = 0; l < 4; ++l)
                         if (in(column(i) + l)) put(to + l, e[l]);
@@ -349,7 +386,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rows_i8_kerne
         return;
     }
     // The largest in 64 bits.  Rounding keeps the order: of products with the norm's weights it is one whose rounded value is the largest.  Gated
-    // values: __expf and the division leave 2e-6, and 6e-8 |x| where the exponential counts (|x| < 90), so it is one within 2e-5 of it.
+    // values are off by 8e-6 at most (x = -80), so it is one within 2e-5 of it.
     if (GATED || norm) {
         const float least = GATED ? top * (1.0f - 2e-5f) : top;
         auto offer = [&](double d) { atomicMax(&s.largest, static_cast<unsigned long long>(__double_as_longlong(fabs(d)))); };
@@ -406,9 +443,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rows_i8_kerne
     }
 
     // To whole numbers: the sum with 1.5 * 2^23 rounds to the nearest, and holds it in its last bits.  32 bits leave a value off by 6 * 2^-24 |t| (the product
-    // with the norm's weights, r, two of the division, the product with the factor), gated ones by up to 6e-6 |t| more; whoever is that near to a half is
-    // worked out in 64.
-    constexpr float kWhole = 12582912.0f, kOff = GATED ? 6.5e-6f : 4e-7f;
+    // with the norm's weights, r, two of the division, the product with the factor), gated ones by 5 * 2^-24 (two of them products), the sigmoid's 5e-7 and
+    // 7.5e-8 times the largest -x of the thread; whoever is that near to a half is worked out in 64.
+    constexpr float kWhole = 12582912.0f;
+    const float off = GATED ? fmaf(fmaxf(lowest, -80.0f), -8e-8f, 1e-6f) : 4e-7f;
     const long long pitch = i8_pitch(a.cols);
     int8_t *out = a.q + row * pitch;
 #pragma unroll
@@ -424,7 +462,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rows_i8_kerne
             t[l] = (norm ? e[l] * g[l] : e[l]) * f;  // |t| < 127.1
             const float k = t[l] + kWhole;
             bits[l] = __float_as_uint(k);
-            const float sure = fmaf(fabsf(t[l]), -kOff, 0.5f);
+            const float sure = fmaf(fabsf(t[l]), -off, 0.5f);
             t[l] = fabsf(t[l] - (k - kWhole)) - sure;
             near |= t[l] > 0.0f;
         }
@@ -435,7 +473,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rows_i8_kerne
                     double d = static_cast<double>(e[l]);
                     if (GATED) d = exact_gate(as_float(x[column(i) + l]), as_float(second[column(i) + l]));
                     else if (norm) d *= static_cast<double>(g[l]);
-                    bits[l] = static_cast<uint32_t>(__double2int_rn(d * s.r / s.scale));  // (divided: a tie stays a tie)
+                    bits[l] = static_cast<uint32_t>(exact_whole(d, s.r, s.scale));
                 }
         }
         if (!LOOSE) {
@@ -468,23 +506,32 @@ cudaError_t launch_variant(const RowsI8Args &a, cudaStream_t stream) {
     return a.x2 != nullptr ? launch_kernel(rows_i8_kernel<T, NV, THREADS, true, LOOSE>, a, THREADS, stream)
                            : launch_kernel(rows_i8_kernel<T, NV, THREADS, false, LOOSE>, a, THREADS, stream);
 }
-template <typename T, int THREADS, bool LOOSE>
-cudaError_t launch_vectors(const RowsI8Args &a, cudaStream_t stream) {  // at most 12 vectors per thread
-    const int n = ((a.cols + (LOOSE ? 6 : 3)) / 4 + THREADS - 1) / THREADS;
-    if (n <= 2) return launch_variant<T, 2, THREADS, LOOSE>(a, stream);
-    if (n <= 5) return launch_variant<T, 5, THREADS, LOOSE>(a, stream);
-    if (n <= 8) return launch_variant<T, 8, THREADS, LOOSE>(a, stream);
-    if (n <= 10) return launch_variant<T, 10, THREADS, LOOSE>(a, stream);
-    return launch_variant<T, 12, THREADS, LOOSE>(a, stream);
+// Threads of a row: many rows have an SM to share, few rows wait for their own steps only (4 gated rows of 17408: 512 threads 6.2 us, 1024 5.2).  fp32
+// rows of more than 12282 values fit twice on an SM only with spills (47 us for 40 with 512 threads each), so they take one block of 1024 (1000 gated rows of
+// 17408: 52.7 us with one block of 512, 48.5).  fp16 rows of 4097 to 6138 values: 128 threads 36.1, 256 39.3 us.
+// The smallest of the given numbers of vectors per thread that holds a row.
+template <typename T, int THREADS, bool LOOSE, int NV, int... MORE>
+cudaError_t launch_vectors(const RowsI8Args &a, cudaStream_t stream) {
+    if constexpr (sizeof...(MORE) > 0)
+        if ((a.cols + (LOOSE ? 6 : 3)) / 4 > NV * THREADS) return launch_vectors<T, THREADS, LOOSE, MORE...>(a, stream);
+    return launch_variant<T, NV, THREADS, LOOSE>(a, stream);
 }
 
 template <typename T, bool LOOSE>
 cudaError_t launch_size(const RowsI8Args &a, int sm_count, cudaStream_t stream) {
-    const bool many = a.ntok > sm_count;  // few rows: as many threads on each as there are
-    if (a.cols <= 1024 && many) return launch_vectors<T, 32, LOOSE>(a, stream);
-    if (a.cols <= (sizeof(T) == 2 ? 6138 : 4096) && many) return launch_vectors<T, 128, LOOSE>(a, stream);
-    if (a.cols <= 12282 && many) return launch_vectors<T, 256, LOOSE>(a, stream);
-    return launch_vectors<T, 512, LOOSE>(a, stream);
+    if (a.ntok <= sm_count)  // few rows: as many threads on each as there are
+        return a.cols <= 10234 ? launch_vectors<T, 512, LOOSE, 2, 5>(a, stream) : launch_vectors<T, 1024, LOOSE, 5, 6>(a, stream);
+    constexpr int kMore = LOOSE ? 6 : 0;  // columns that a row may need room for, because it does not begin with a vector
+    if (a.cols <= 1024 - kMore) return launch_vectors<T, 32, LOOSE, 2, 5, 8>(a, stream);
+    if constexpr (sizeof(T) == 2) {
+        if (a.cols <= 6138) return launch_vectors<T, 128, LOOSE, 5, 8, 10, 12>(a, stream);
+        if (a.cols <= 12282) return launch_vectors<T, 256, LOOSE, 8, 10, 12>(a, stream);
+        return launch_vectors<T, 512, LOOSE, 8, 9, 10, 12>(a, stream);
+    } else {
+        if (a.cols <= 4096 - kMore) return launch_vectors<T, 128, LOOSE, 5, 8>(a, stream);
+        if (a.cols <= 12282) return launch_vectors<T, 256, LOOSE, 5, 8, 10, 12>(a, stream);
+        return launch_vectors<T, 1024, LOOSE, 5, 6>(a, stream);
+    }
 }
 template <typename T>
 cudaError_t launch_t(const RowsI8Args &a, int sm_count, cudaStream_t stream) {
