@@ -9,7 +9,7 @@
 // Rows too long for that, norms of gated values, and rows whose largest value is out of fp32's middle range are worked out in 64 bits throughout.
 //
 // What bounds it: 4001 rows of 5120 with residual and norm take 51 us in fp32 (5200 GB/s of the 6550 that a copy gets) and 36 in fp16 (3980 GB/s): there the
-// instructions, 33 per element, the mean's 64 bits and the norm's weights, and a row's steps one after the other.  1000 gated rows of 17408: 48.5 us in
+// instructions, 32 per element, the mean's 64 bits and the norm's weights, and a row's steps one after the other.  1000 gated rows of 17408: 48.5 us in
 // fp32 (3230 GB/s), 36 in fp16; 4001 of 5120: 37 and 38, ex2 and a reciprocal per element and the rows' steps.  One row: 3.4 us.
 // What it took: more rows at a time on an SM (below); an error bound of the gate that looks at the values, so that fewer of them are worked out in 64 bits (1000
 // gated rows of 17408 57 and 52 us, 4001 of 5120 in fp16 53 and 38).

@@ -12,7 +12,7 @@
 //      takes are summed in 64 bits: both rows' sums, then the weights by blocks and warps, then within one warp's part.
 // Nothing is kept in device memory between the steps: launches on several streams and in several graphs do not meet.
 //
-// What bounds it: 64 sequences x 4 drafts x 151936 in fp32 take 142 us of one stream (2460 GB/s; three streams: 77 us a call, 4520 GB/s): 60 us are step 1, near
+// What bounds it: 64 sequences x 4 drafts x 151936 in fp32 take 142 us of one stream (2460 GB/s; three streams: 73.5 us a call, 4760 GB/s): 60 us are step 1, near
 // the copy bandwidth, the rest the exponentials in 64 bits of two rows (eight instructions of that pipe and some twenty others each: 45 cycles per 32 of them
 // and scheduler, whatever of loads, table or series is left out).  One sequence x 3 drafts: 28 us on 16 SMs, as many as a cluster takes.  Of that, half
 // is the steps' latency: a vocabulary of 1000 takes 14 us.  Tried: 1024 threads, two blocks of 256 or 512 per SM (spills), a second round of
