@@ -185,17 +185,15 @@ cudaError_t launch_t(const uint8_t *w, const __half *xh, float *y, int rows, int
 
 int gemm_token_tile() { return kBN; }
 
-cudaError_t launch_f32_to_f16_rows(const float *x, void *xh, long long n_valid, long long n_total, cudaStream_t stream) {
+cudaError_t launch_f32_to_f16_rows(const float *x, void *xh, long long n_valid, long long n_total, bool overlap, cudaStream_t stream) {
     const bool wide = n_valid % 8 == 0 && n_total % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(xh) % 16 == 0;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
     cfg.gridDim = dim3(static_cast<unsigned>((n_total / (wide ? 8 : 1) + 255) / 256));
     cfg.blockDim = dim3(256);
     cfg.stream = stream;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = launch_attributes(attr, overlap, 0);
     if (wide)
         return cudaLaunchKernelEx(&cfg, f32_to_f16_rows8_kernel, reinterpret_cast<const float4 *>(x), static_cast<uint4 *>(xh), n_valid / 8, n_total / 8);
     return cudaLaunchKernelEx(&cfg, f32_to_f16_rows_kernel, x, static_cast<__half *>(xh), n_valid, n_total);

@@ -631,20 +631,15 @@ struct Tc5Variant {
     static_assert(kSmem - table_bytes16(TYPE) - 1024 >= (kMaxPairs - 1) * (kTNMax / kXChunk / kMaxPairs) * kXBytes, "room for the exchange");
     static constexpr auto kKernel = qgemm_tc5_kernel<TYPE, NH>;
 
-    static void configure(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int row_tiles, int tok_tiles, int pairs, cudaStream_t stream) {
+    static void configure(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int row_tiles, int tok_tiles, int pairs, bool overlap, cudaStream_t stream) {
         cfg.gridDim = dim3(static_cast<unsigned>(row_tiles * pairs * 2), static_cast<unsigned>(tok_tiles));
         cfg.blockDim = dim3(kTThreads);
         cfg.dynamicSmemBytes = kSmem;
         cfg.stream = stream;
         // May start while the kernel before it in the stream (the fp32 -> fp16 conversion of the activations) still runs: the
         // set-up, the first weight copies and the first decoded tiles overlap it; the thread that feeds the activations waits.
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        attr[1].id = cudaLaunchAttributeClusterDimension;
-        attr[1].val.clusterDim.x = static_cast<unsigned>(pairs * 2);
-        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
         cfg.attrs = attr;
-        cfg.numAttrs = 2;
+        cfg.numAttrs = launch_attributes(attr, overlap, pairs * 2);
     }
     // clusters of `pairs` pairs that fit on the GPU at once (cached; one device per process), 0 if the kernel cannot run
     static int clusters(int pairs) {
@@ -653,7 +648,7 @@ struct Tc5Variant {
             int n = 0;
             cudaLaunchConfig_t cfg{};
             cudaLaunchAttribute attr[2];
-            configure(cfg, attr, 1024, 1, pairs, nullptr);
+            configure(cfg, attr, 1024, 1, pairs, true, nullptr);
             if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
                 cudaOccupancyMaxActiveClusters(&n, kKernel, &cfg) != cudaSuccess) {
                 (void)cudaGetLastError();
@@ -696,7 +691,7 @@ Tc5Plan plan_t(int rows, int cols, int ntok) {
 
 template <int TYPE>
 cudaError_t launch_t(const uint8_t *w, const __half *xh, float *y, int rows, int cols, long long row_bytes, int ntok, const uint8_t *codebook,
-                     unsigned *status, cudaStream_t stream) {
+                     unsigned *status, bool overlap, cudaStream_t stream) {
     const Tc5Plan plan = plan_t<TYPE>(rows, cols, ntok);
     if (plan.nh == 0) return cudaErrorInvalidConfiguration;
     Tc5Maps maps{};
@@ -708,10 +703,10 @@ cudaError_t launch_t(const uint8_t *w, const __half *xh, float *y, int rows, int
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[2];
     if (plan.nh == 1) {
-        Tc5Variant<TYPE, 1>::configure(cfg, attr, row_tiles, plan.tok_tiles, plan.pairs, stream);
+        Tc5Variant<TYPE, 1>::configure(cfg, attr, row_tiles, plan.tok_tiles, plan.pairs, overlap, stream);
         return cudaLaunchKernelEx(&cfg, Tc5Variant<TYPE, 1>::kKernel, maps, w, y, rows, cols, row_bytes, ntok, plan.n_acc, shift, codebook, status);
     }
-    Tc5Variant<TYPE, 2>::configure(cfg, attr, row_tiles, plan.tok_tiles, plan.pairs, stream);
+    Tc5Variant<TYPE, 2>::configure(cfg, attr, row_tiles, plan.tok_tiles, plan.pairs, overlap, stream);
     return cudaLaunchKernelEx(&cfg, Tc5Variant<TYPE, 2>::kKernel, maps, w, y, rows, cols, row_bytes, ntok, plan.n_acc, shift, codebook, status);
 }
 
@@ -720,11 +715,11 @@ cudaError_t launch_t(const uint8_t *w, const __half *xh, float *y, int rows, int
 bool gemm_tc5_supports(int cols) { return cols % kTK == 0; }
 
 cudaError_t launch_qgemm_tc5(int type, const uint8_t *w, const void *xh, float *y, int rows, int cols, long long row_bytes, int ntok,
-                             const uint8_t *codebook, unsigned *status, cudaStream_t stream) {
+                             const uint8_t *codebook, unsigned *status, bool overlap, cudaStream_t stream) {
     const __half *x = static_cast<const __half *>(xh);
     switch (type) {
 #define VQM_CASE(id, name) \
-    case id: return launch_t<id>(w, x, y, rows, cols, row_bytes, ntok, codebook, status, stream);
+    case id: return launch_t<id>(w, x, y, rows, cols, row_bytes, ntok, codebook, status, overlap, stream);
         VQM_FOR_EACH_TYPE(VQM_CASE)
 #undef VQM_CASE
         default: return cudaErrorInvalidValue;

@@ -8,6 +8,25 @@
 
 namespace vqm {
 
+// Attributes of a launch, of which `attr` holds two; returns how many there are.  overlap: programmatic stream serialization, with which the blocks
+// may begin while the kernel before them in the stream still runs (they wait for its end themselves, but for weights, which are in place).
+// cluster: blocks of a cluster, 0 for none.
+inline unsigned launch_attributes(cudaLaunchAttribute *attr, bool overlap, int cluster) {
+    unsigned n = 0;
+    if (overlap) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    if (cluster > 0) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = static_cast<unsigned>(cluster);
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    return n;
+}
+
 constexpr int kMaxParts = 4;  // tensors one launch can cover (they share the activations, the type and the columns)
 
 // Row-sharded matvec across GPUs: where a launch stores its outputs inside every rank's exchange region (plain remote
@@ -154,7 +173,8 @@ constexpr int kMaxGrid = 4096;  // upper bound on the matvec grid (sizes the arg
 
 // Prompt-pass GEMM on the tensor cores (vqm_gemm.cu).  xh: fp16 activations [ntok padded to gemm_token_tile()][cols].
 int gemm_token_tile();
-cudaError_t launch_f32_to_f16_rows(const float *x, void *xh, long long n_valid, long long n_total, cudaStream_t stream);
+// overlap: see launch_attributes
+cudaError_t launch_f32_to_f16_rows(const float *x, void *xh, long long n_valid, long long n_total, bool overlap, cudaStream_t stream);
 cudaError_t launch_qgemm(int type, const uint8_t *w, const void *xh, float *y, int rows, int cols, long long row_bytes, int ntok,
                          const uint8_t *codebook, cudaStream_t stream);
 
@@ -163,7 +183,7 @@ cudaError_t launch_qgemm(int type, const uint8_t *w, const void *xh, float *y, i
 // wait expires.
 bool gemm_tc5_supports(int cols);
 cudaError_t launch_qgemm_tc5(int type, const uint8_t *w, const void *xh, float *y, int rows, int cols, long long row_bytes, int ntok,
-                             const uint8_t *codebook, unsigned *status, cudaStream_t stream);
+                             const uint8_t *codebook, unsigned *status, bool overlap, cudaStream_t stream);
 
 // n16 16-byte words from pinned host memory
 cudaError_t launch_fetch(const void *from, void *to, int n16, cudaStream_t stream);
@@ -186,6 +206,7 @@ struct RowsI8Args {
     int cols, ntok, elem;
     float eps;
     double inv_cols;       // 1 / cols, filled in by the launcher
+    bool overlap;          // host only, see launch_attributes
 };
 cudaError_t launch_rows_i8(const RowsI8Args &a, int sm_count, cudaStream_t stream);
 
@@ -198,6 +219,7 @@ struct QmmI8Args {
     long long w_pitch;
     int rows, cols, ntok, y_elem;
     bool add;              // y += instead of y =
+    bool overlap;          // see launch_attributes
     unsigned *status;      // device word that receives a code if a bounded wait expires
 };
 cudaError_t launch_qmm_i8(const QmmI8Args &a, int sm_count, cudaStream_t stream);
@@ -211,6 +233,7 @@ struct VerifyArgs {
     const float *temperature;  // [seqs]; or null: 1
     int *out;                  // [seqs][drafts + 2]
     int vocab, seqs, drafts, elem;
+    bool overlap;              // host only, see launch_attributes
 };
 cudaError_t launch_verify(const VerifyArgs &a, cudaStream_t stream);
 

@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
                 place(tile, row_tile, tok_tile);
                 int k = k0;
                 if (issued == 0) {
-                    // Weights are in place before the launch; what the kernel before this one in the stream makes, the activations, is waited for.
+                    // Weights are in place before the launch (where they may not be, the caller has turned overlap off); what the kernel before this one in the stream makes, the activations, is waited for.
                     const int ahead = min(a.stages, k1 - k0);
                     for (int i = 0; i < ahead; ++i) {
                         expect(s32(&s_full[i]), stage_bytes);
@@ -413,18 +413,13 @@ struct Variant {
     static constexpr int smem(bool half) { return (half ? kQHalfRing : kQRing) + 1024; }
     static constexpr int kGroup = PAIR ? 2 : 1;
     static constexpr auto kKernel = qmm_i8_kernel<PAIR, SPLIT>;
-    static void configure(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int clusters, int split, bool half, cudaStream_t stream) {
+    static void configure(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int clusters, int split, bool half, bool overlap, cudaStream_t stream) {
         cfg.gridDim = dim3(static_cast<unsigned>(clusters * split * kGroup));
         cfg.blockDim = dim3(kQThreads);
         cfg.dynamicSmemBytes = smem(half);
         cfg.stream = stream;
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        attr[1].id = cudaLaunchAttributeClusterDimension;
-        attr[1].val.clusterDim.x = static_cast<unsigned>(split * kGroup);
-        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
         cfg.attrs = attr;
-        cfg.numAttrs = 2;
+        cfg.numAttrs = launch_attributes(attr, overlap, split * kGroup);
     }
     // clusters that fit on the GPU at once, one block per SM (cached; one device per process), 0 if the kernel cannot run
     static int clusters(int split) {
@@ -433,7 +428,7 @@ struct Variant {
             int n = 0;
             cudaLaunchConfig_t cfg{};
             cudaLaunchAttribute attr[2];
-            configure(cfg, attr, 1024, split, false, nullptr);
+            configure(cfg, attr, 1024, split, false, true, nullptr);
             if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem(false)) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kKernel, &cfg) != cudaSuccess) {
                 (void)cudaGetLastError();
                 n = 0;
@@ -442,12 +437,12 @@ struct Variant {
         }
         return cached[split] < 0 ? 0 : cached[split];
     }
-    static cudaError_t launch(const CUtensorMap &w, const CUtensorMap &q, const QmmTc &a, cudaStream_t stream) {
+    static cudaError_t launch(const CUtensorMap &w, const CUtensorMap &q, const QmmTc &a, bool overlap, cudaStream_t stream) {
         const int fit = clusters(a.split), tiles = a.row_tiles * a.tok_tiles;
         if (fit == 0) return cudaErrorInvalidConfiguration;
         cudaLaunchConfig_t cfg{};
         cudaLaunchAttribute attr[2];
-        configure(cfg, attr, SPLIT ? tiles : (tiles < fit ? tiles : fit), a.split, a.half_sm != 0, stream);
+        configure(cfg, attr, SPLIT ? tiles : (tiles < fit ? tiles : fit), a.split, a.half_sm != 0, overlap, stream);
         return cudaLaunchKernelEx(&cfg, kKernel, w, q, a);
     }
 };
@@ -492,8 +487,8 @@ cudaError_t launch_qmm_i8(const QmmI8Args &in, int sm_count, cudaStream_t stream
     cudaError_t err = encode_rows(&w, in.w, in.cols, in.w_pitch, in.rows, kQRows);
     if (err == cudaSuccess) err = encode_rows(&q, in.q, in.cols, i8_pitch(in.cols), in.ntok, a.n / group);
     if (err != cudaSuccess) return err;
-    if (pair) return a.split > 1 ? Variant<true, true>::launch(w, q, a, stream) : Variant<true, false>::launch(w, q, a, stream);
-    return a.split > 1 ? Variant<false, true>::launch(w, q, a, stream) : Variant<false, false>::launch(w, q, a, stream);
+    if (pair) return a.split > 1 ? Variant<true, true>::launch(w, q, a, in.overlap, stream) : Variant<true, false>::launch(w, q, a, in.overlap, stream);
+    return a.split > 1 ? Variant<false, true>::launch(w, q, a, in.overlap, stream) : Variant<false, false>::launch(w, q, a, in.overlap, stream);
 }
 
 }  // namespace vqm

@@ -494,10 +494,8 @@ cudaError_t launch_kernel(K kernel, const RowsI8Args &a, int threads, cudaStream
     cfg.gridDim = dim3(static_cast<unsigned>(a.ntok));
     cfg.blockDim = dim3(static_cast<unsigned>(threads));
     cfg.stream = stream;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = launch_attributes(attr, a.overlap, 0);
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 

@@ -138,7 +138,7 @@ struct vqm_runtime {
     int exchange_slots = 0;
     int gemm_min_rows = 0;
     int gemm_tcgen05 = 1;    // prompt passes run on the tcgen05 kernel (VINF_B200_GEMM=mma: warp-level MMA only)
-    int overlap_launch = 1;  // programmatic dependent launch of consecutive matvecs (VINF_B200_NO_PDL=1 turns it off)
+    int overlap_launch = 1;  // programmatic dependent launch of consecutive kernels (VINF_B200_NO_PDL=1 turns it off)
     bool capturing = false;
     uint64_t launches = 0, capture_launches = 0;
     uint64_t memory_exchanges = 0;  // launches that exchanged partial sums through memory
@@ -1275,11 +1275,11 @@ int vqm_qmv(vqm_runtime *rt, const char *weight, const char *x, const char *y, i
             if (err != cudaSuccess) return cuda_fail("prompt-pass activation buffer", err);
             rt->gemm_x_len = need;
         }
-        err = vqm::launch_f32_to_f16_rows(xp, rt->gemm_x, static_cast<long long>(ntok) * t->cols, static_cast<long long>(need), rt->stream);
+        err = vqm::launch_f32_to_f16_rows(xp, rt->gemm_x, static_cast<long long>(ntok) * t->cols, static_cast<long long>(need), rt->overlap_launch != 0, rt->stream);
         if (err == cudaSuccess) {
             if (tc5)
                 err = vqm::launch_qgemm_tc5(t->type, t->data, rt->gemm_x, yp, t->rows, t->cols, static_cast<long long>(t->row_bytes), ntok, cb,
-                                            rt->status, rt->stream);
+                                            rt->status, rt->overlap_launch != 0, rt->stream);
             else
                 err = vqm::launch_qgemm(t->type, t->data, rt->gemm_x, yp, t->rows, t->cols, static_cast<long long>(t->row_bytes), ntok, cb, rt->stream);
         }
@@ -1637,6 +1637,7 @@ int vqm_convert_i8(vqm_runtime *rt, const char *weight, const char *name) {
             a.cols = from->cols;
             a.ntok = static_cast<int>(n);
             a.elem = 4;
+            a.overlap = rt->overlap_launch != 0;
             if (err == cudaSuccess) err = vqm::launch_rows_i8(a, rt->sm_count, rt->stream);
             if (err == cudaSuccess) count_launch(rt, 2);
         }
@@ -1665,6 +1666,7 @@ int vqm_rows_i8(vqm_runtime *rt, const char *x, const char *q, const char *scale
         a.cols = cols;
         a.ntok = ntok;
         a.eps = eps;
+        a.overlap = rt->overlap_launch != 0;
         if ((a.x = find_real(rt, x, n, &a.elem, &rc)) == nullptr) return rc;
         if ((a.q = find_i8(rt, q, static_cast<size_t>(vqm::i8_pitch(cols)) * ntok, &rc)) == nullptr) return rc;
         if ((a.scales = find_f32(rt, scales, static_cast<size_t>(ntok), &rc)) == nullptr) return rc;
@@ -1712,6 +1714,7 @@ int vqm_qmm_i8(vqm_runtime *rt, const char *weight, const char *q, const char *s
         a.cols = t->cols;
         a.ntok = ntok;
         a.add = (flags & VQM_FUSE_ADD) != 0;
+        a.overlap = rt->overlap_launch != 0;
         a.status = rt->status;
         const cudaError_t err = vqm::launch_qmm_i8(a, rt->sm_count, rt->stream);
         if (err != cudaSuccess) return cuda_fail("qmm_i8 launch", err);
@@ -1732,6 +1735,7 @@ int vqm_verify(vqm_runtime *rt, const char *target, const char *draft, const cha
         a.vocab = vocab;
         a.seqs = seqs;
         a.drafts = drafts;
+        a.overlap = rt->overlap_launch != 0;
         if ((a.target = find_real(rt, target, s * (k + 1) * static_cast<size_t>(vocab), &a.elem, &rc)) == nullptr) return rc;
         if (drafts > 0 && draft != nullptr && (a.draft = find_real(rt, draft, s * k * static_cast<size_t>(vocab), &a.elem, &rc)) == nullptr) return rc;
         if (drafts > 0 && (a.tokens = static_cast<const int *>(find_real(rt, tokens, s * k, &word, &rc))) == nullptr) return rc;

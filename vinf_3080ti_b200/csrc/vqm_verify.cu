@@ -580,17 +580,12 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const VerifyArgs a
 template <typename T>
 struct Launcher {
     static constexpr auto kKernel = verify_kernel<T>;
-    static void configure(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int seqs, int blocks, cudaStream_t stream) {
+    static void configure(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int seqs, int blocks, bool overlap, cudaStream_t stream) {
         cfg.gridDim = dim3(static_cast<unsigned>(seqs) * static_cast<unsigned>(blocks));
         cfg.blockDim = dim3(kVThreads);
         cfg.stream = stream;
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        attr[1].id = cudaLaunchAttributeClusterDimension;
-        attr[1].val.clusterDim.x = static_cast<unsigned>(blocks);
-        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
         cfg.attrs = attr;
-        cfg.numAttrs = 2;
+        cfg.numAttrs = launch_attributes(attr, overlap, blocks);
     }
     // clusters of so many blocks that fit on the GPU at once (cached; one device per process)
     static int fit(int blocks) {
@@ -599,7 +594,7 @@ struct Launcher {
             int n = 0;
             cudaLaunchConfig_t cfg{};
             cudaLaunchAttribute attr[2];
-            configure(cfg, attr, 1024, blocks, nullptr);
+            configure(cfg, attr, 1024, blocks, true, nullptr);
             if ((blocks > 8 && cudaFuncSetAttribute(kKernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
                 cudaOccupancyMaxActiveClusters(&n, kKernel, &cfg) != cudaSuccess) {
                 (void)cudaGetLastError();
@@ -616,7 +611,7 @@ struct Launcher {
         while (blocks > 1 && (a.seqs > fit(blocks) || a.vocab < blocks * 2048)) --blocks;
         cudaLaunchConfig_t cfg{};
         cudaLaunchAttribute attr[2];
-        configure(cfg, attr, a.seqs, blocks, stream);
+        configure(cfg, attr, a.seqs, blocks, a.overlap, stream);
         return cudaLaunchKernelEx(&cfg, kKernel, a);
     }
 };
