@@ -236,6 +236,12 @@ struct VerifyArgs {
     bool overlap;              // host only, see launch_attributes
 };
 cudaError_t launch_verify(const VerifyArgs &a, cudaStream_t stream);
+// How far from one another, relative to the larger, the two sides of a draft's test may be if they are equal but come from fp32 sums of exponentials, of
+// which a lane adds up `adds` parts.  In units of 2^-24: a part is added with one rounding, and where it has a new largest the sum before it is scaled, 4 of
+// ex2 and 1 of the product; both sides have such a sum, and the products of so many factors add less than 5 %.  The rest is 2e-5: 4 of each ex2, 3 times
+// its argument (over a row at most the logarithm of its length, 22, on average), 10 of the additions within a part, 90 of 15 joins of lanes, warps and blocks.
+// Beyond 32768 parts (16.7 million logits to a block) nothing is taken for sure.
+__host__ __device__ constexpr double verify_band(long long adds) { return adds > 32768 ? 2.0 : 1e-4 + 1.05 * 12.0 / (1 << 24) * static_cast<double>(adds); }
 
 cudaError_t launch_argmax_rows(const float *x, int n, int ntok, int *out, cudaStream_t stream);
 cudaError_t launch_dequant(int type, const uint8_t *w, float *out, long long numel, const uint8_t *codebook,

@@ -4,9 +4,9 @@
 // own holds for any q; a draft without probabilities is q = 1 at its token.
 //
 // One cluster per sequence, each block a slice of the vocabulary.
-//   1. One pass over the logits: every row's largest and the sum of exp over it, in fp32 (exponentials by ex2, sums of at most some hundred terms
-//      per lane).  The blocks exchange (largest, sum) of each row through distributed shared memory.
-//   2. Every block decides on all drafts.  fp32 leaves the two sides of a test uncertain by about 1e-6; where they are within 1e-4 of one another, and for rows
+//   1. One pass over the logits: every row's largest and the sum of exp over it, in fp32 (exponentials by ex2, sums of one part of 16 or 32 terms after the
+//      other per lane).  The blocks exchange (largest, sum) of each row through distributed shared memory.
+//   2. Every block decides on all drafts.  fp32 leaves the two sides of a test uncertain by about 1e-6; where they are within a bound of that (verify_band, 1e-4 and some), and for rows
 //      with values that fp32 cannot hold (infinite, undefined, too large over T), the cluster sums the row's exponentials again in 64 bits.
 //   3. The token behind: which of 150000 intervals the random number falls into hangs on the 12th digit of the sums, so the one or two rows it
 //      takes are summed in 64 bits: both rows' sums, then the weights by blocks and warps, then within one warp's part.
@@ -26,6 +26,7 @@ namespace vqm {
 namespace {
 
 constexpr int kVThreads = 512, kVWarps = kVThreads / 32, kVMaxCluster = 16, kVMaxRows = 2 * 255 + 1;
+constexpr int kVPart = 4;  // vectors that a lane adds up before they go to its sum
 constexpr int kVTable = 128, kVCopies = 16;  // entries of 2^(j / 128), and copies: lanes that look up at random do not meet in a bank
 constexpr double kVMagic = 6755399441055744.0 / kVTable;  // 1.5 * 2^52 / 128: adding it rounds to a multiple of 1 / 128
 constexpr double kNoise = 1.0 / (1ull << 44);  // p - q within the rounding of the rows' sums is nothing: equal rows leave no rest
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const VerifyArgs a
             const int v0 = from + static_cast<int>(f - base), v1 = min(n_vec, from + static_cast<int>(min(f_end - base, static_cast<long long>(share))));
             f = base + share;
             float top = -INFINITY, sum = none;
-            constexpr int U = 4;
+            constexpr int U = kVPart;
             uint4 raw[2][U];  // what is being added up, and the next on its way
             auto fetch = [&](int v, uint4 (&to)[U]) {
 #pragma unroll
@@ -349,6 +350,7 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const VerifyArgs a
                 // u wq / Sq < wp / Sp; the sums are of exp((x - top) / T), the weights have a factor of their own
                 double left = static_cast<double>(my_u), right = 1.0;
                 bool sure = true;
+                const double band = verify_band(share / (32 * kVPart) + 2);  // (a warp has at most a block's share of a row)
 #pragma unroll 1
                 for (int side = 0; side < per_step; ++side) {
                     const float sum = s.all_sum[r + side];
@@ -358,7 +360,7 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const VerifyArgs a
                     left *= side ? token_weight : whole;
                     right *= side ? whole : token_weight;
                 }
-                sure = sure && !(fabs(left - right) <= 1e-4 * fmax(fabs(left), fabs(right)));
+                sure = sure && !(fabs(left - right) <= band * fmax(fabs(left), fabs(right)));
                 verdict = !sure ? kUnsure : left < right ? kAccept : kRefuse;
             }
         }
