@@ -188,7 +188,9 @@ int vqm_qmm_i8(vqm_runtime *rt, const char *weight, const char *q, const char *s
  * Decisions are those of 64-bit arithmetic; where p - q is within its rounding (2^-44 p) it is nothing, and where nothing is left of p - q the
  * token is drawn from p.  Logits of -inf and NaN have no probability; a row without any refuses its draft, and the
  * token drawn from such a row is -1.  A token outside [0, vocab) is refused, and where drafts have no probabilities nothing is taken off p then.
- * out [seqs][drafts + 2] (int32): the number of accepted drafts a, the accepted tokens, the next token, then -1.  out_host (seqs * (drafts + 2)
+ * out [seqs][drafts + 2] (int32): the number of accepted drafts a, the accepted tokens, the next token, then -1.  Where a kernel of the runtime has given up a
+ * bounded wait that nobody has been told of yet, the logits may not be complete: out is -1 throughout (a = -1), and a call with out_host reports the
+ * failure as vqm_synchronize does (VQM_ERR_CUDA).  out_host (seqs * (drafts + 2)
  * ints) may be NULL: then the call is asynchronous.  target and draft are both fp32 or both fp16; `out` overlaps none
  * of the others.  drafts = 0 samples from the target.
  * 0 <= drafts <= VQM_MAX_DRAFTS, vocab <= VQM_MAX_VOCAB. */

@@ -231,7 +231,8 @@ struct VerifyArgs {
     const int *lens;           // [seqs] drafts of each sequence; or null: all
     const float *uniforms;     // [seqs][drafts + 1]
     const float *temperature;  // [seqs]; or null: 1
-    int *out;                  // [seqs][drafts + 2]
+    int *out;                  // [seqs][drafts + 2]; all -1 if the status word is not 0
+    const unsigned *status;    // device word with the code of a wait that has expired: the logits may not be what they should
     int vocab, seqs, drafts, elem;
     bool overlap;              // host only, see launch_attributes
 };

@@ -1744,6 +1744,7 @@ int vqm_verify(vqm_runtime *rt, const char *target, const char *draft, const cha
         if (temperature != nullptr && (a.temperature = find_f32(rt, temperature, s, &rc)) == nullptr) return rc;
         if ((a.out = static_cast<int *>(find_real(rt, out, s * (k + 2), &word, &rc))) == nullptr) return rc;
         if ((rc = check_apart("the answers", a.out, {a.target, a.draft, a.tokens, a.lens, a.uniforms, a.temperature})) != VQM_OK) return rc;
+        a.status = rt->status;
         if (out_host != nullptr && (rc = no_capture(rt, "a blocking verify")) != VQM_OK) return rc;
         cudaError_t err = vqm::launch_verify(a, rt->stream);
         if (err != cudaSuccess) return cuda_fail("verify launch", err);
@@ -1752,6 +1753,9 @@ int vqm_verify(vqm_runtime *rt, const char *target, const char *draft, const cha
             err = cudaMemcpyAsync(out_host, a.out, sizeof(int) * s * (k + 2), cudaMemcpyDeviceToHost, rt->stream);
             if (err == cudaSuccess) err = cudaStreamSynchronize(rt->stream);
             if (err != cudaSuccess) return cuda_fail("verify", err);
+            // no count is negative but of answers that a failure before them has taken back
+            for (size_t i = 0; i < s; ++i)
+                if (out_host[i * (k + 2)] < 0) return (rc = check_status_word(rt, "verify")) != VQM_OK ? rc : fail(VQM_ERR_CUDA, "verify failed: its logits are not complete");
         }
         return VQM_OK;
     });

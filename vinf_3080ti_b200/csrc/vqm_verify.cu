@@ -106,6 +106,7 @@ struct Shared {
     unsigned char verdict[256];                    // of the drafts
     double warp_sum[3][kVWarps];                   // of the warps; of the row(s) being summed, of one warp's part
     double block_sum[2][2];                        // this block's, for the others; two buffers in turn
+    unsigned status;
 };
 enum : unsigned char { kAccept, kRefuse, kUnsure };
 
@@ -199,6 +200,7 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const VerifyArgs a
     }
     const double *const table = &s.table[0][lane % kVCopies];
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (threadIdx.x == 0) s.status = *a.status;  // (not needed before the end: nobody waits for it there)
     const float temperature = a.temperature != nullptr ? a.temperature[seq] : 1.0f;
     const bool greedy = !(temperature > 0.0f);
     const float *u = a.uniforms + static_cast<size_t>(seq) * (k + 1);
@@ -574,7 +576,7 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const VerifyArgs a
         }
     }
     if (mine && warp == 0) {
-        for (int i = lane; i < k + 2; i += 32) out[i] = i == 0 ? j : i <= j ? tokens[i - 1] : i == j + 1 ? next : -1;
+        for (int i = lane; i < k + 2; i += 32) out[i] = s.status != 0 ? -1 : i == 0 ? j : i <= j ? tokens[i - 1] : i == j + 1 ? next : -1;
     }
     sync_cluster();  // no block's shared memory goes away under another
 }

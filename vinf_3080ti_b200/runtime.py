@@ -312,7 +312,8 @@ class Runtime:
     def verify(self, target: str, draft: str | None, tokens: str | None, uniforms: str, vocab: int, seqs: int, drafts: int, *, out: str,
                lens: str | None = None, temperature: str | None = None, blocking: bool = True) -> list[list[int]] | None:
         """Speculative decoding's decision: which drafted tokens are kept, and the token after them.  Returns per sequence the kept tokens
-        followed by the next one (blocking), or leaves [count, tokens..., -1...] in the buffer `out`."""
+        followed by the next one (blocking), or leaves [count, tokens..., -1...] in the buffer `out` (count -1: an earlier launch has failed,
+        which synchronize() reports)."""
         if seqs < 1 or drafts < 0 or drafts > MAX_DRAFTS:
             raise ValueError(f"seqs must be positive and drafts in [0, {MAX_DRAFTS}]")
         host = (ctypes.c_int * (seqs * (drafts + 2)))() if blocking else None
