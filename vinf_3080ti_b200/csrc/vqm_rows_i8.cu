@@ -442,11 +442,10 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<T, NV, THREADS>()) rows
         return;
     }
 
-    // To whole numbers: the sum with 1.5 * 2^23 rounds to the nearest, and holds it in its last bits.  32 bits leave a value off by 6 * 2^-24 |t| (the product
-    // with the norm's weights, r, two of the division, the product with the factor), gated ones by 5 * 2^-24 (two of them products), the sigmoid's 5e-7 and
-    // 7.5e-8 times the largest -x of the thread; whoever is that near to a half is worked out in 64.
+    // To whole numbers: the sum with 1.5 * 2^23 rounds to the nearest, and holds it in its last bits.  Whoever is so near to a half that fp32 leaves it
+    // open (kI8Off) is worked out in 64 bits.
     constexpr float kWhole = 12582912.0f;
-    const float off = GATED ? fmaf(fmaxf(lowest, -80.0f), -8e-8f, 1e-6f) : 4e-7f;
+    const float off = GATED ? fmaf(fmaxf(lowest, -80.0f), -kI8GatedOffPerX, kI8GatedOff) : kI8Off;
     const long long pitch = i8_pitch(a.cols);
     int8_t *out = a.q + row * pitch;
 #pragma unroll
