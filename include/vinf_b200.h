@@ -168,12 +168,13 @@ int vqm_convert_i8(vqm_runtime *rt, const char *weight, const char *name);
  *   VQM_FUSE_NORM: n = v * rsqrt(mean(v^2) + eps) * norm_weight (an fp32 buffer or F32 tensor of cols values), else n = v;
  *   scale = max |n| / 127 in fp32, q = n / scale to the nearest integer, ties to even, as the exact values of n and the stored scale have it.
  * A row of zeros has scale 0 and q = 0.  A row with an infinite or undefined n, or whose scale is beyond fp32, has an undefined (NaN)
- * scale and q = 0, which makes its products undefined.  x, x2, residual and total share one type.  Buffers do not overlap otherwise. */
+ * scale and q = 0, which makes its products undefined.  x, x2, residual and total share one type.  Where what is written overlaps
+ * anything else in device memory, under whatever names (total is exactly x or the residual, or apart from them), the call is refused (VQM_ERR_VALUE). */
 int vqm_rows_i8(vqm_runtime *rt, const char *x, const char *q, const char *scales, int cols, int ntok, int flags, const char *x2, const char *residual,
                 const char *total, const char *norm_weight, float eps);
 /* y[t][r] = sum_k q[t][k] w[r][k] * scales[t] * W scales[r] (VQM_FUSE_ADD: +=) for a tensor of 8-bit integer rows; sums are exact, the two products
- * are fp32, in this order; y is an fp32 or fp16 buffer that overlaps
- * none of the others.  Asynchronous. */
+ * are fp32, in this order; y is an fp32 or fp16 buffer; a call
+ * whose y overlaps q, the scales or the weights in device memory is refused (VQM_ERR_VALUE).  Asynchronous. */
 int vqm_qmm_i8(vqm_runtime *rt, const char *weight, const char *q, const char *scales, const char *y, int ntok, int flags);
 
 /* Verification of drafted tokens against the target's probabilities (no counterpart in the reference, whose speculative decoder compares greedy
@@ -191,8 +192,8 @@ int vqm_qmm_i8(vqm_runtime *rt, const char *weight, const char *q, const char *s
  * out [seqs][drafts + 2] (int32): the number of accepted drafts a, the accepted tokens, the next token, then -1.  Where a kernel of the runtime has given up a
  * bounded wait that nobody has been told of yet, the logits may not be complete: out is -1 throughout (a = -1), and a call with out_host reports the
  * failure as vqm_synchronize does (VQM_ERR_CUDA).  out_host (seqs * (drafts + 2)
- * ints) may be NULL: then the call is asynchronous.  target and draft are both fp32 or both fp16; `out` overlaps none
- * of the others.  drafts = 0 samples from the target.
+ * ints) may be NULL: then the call is asynchronous.  target and draft are both fp32 or both fp16; a call whose `out`
+ * overlaps any of the others in device memory is refused (VQM_ERR_VALUE).  drafts = 0 samples from the target.
  * 0 <= drafts <= VQM_MAX_DRAFTS, vocab <= VQM_MAX_VOCAB. */
 #define VQM_MAX_DRAFTS 255
 #define VQM_MAX_VOCAB 1073741824

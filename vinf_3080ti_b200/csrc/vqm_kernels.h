@@ -8,6 +8,17 @@
 
 namespace vqm {
 
+// Memory that a call reads or writes; none: at a null pointer.
+struct Extent {
+    const void *at;
+    size_t bytes;
+};
+constexpr Extent kNoExtent{nullptr, 0};
+inline bool overlap(const Extent &a, const Extent &b) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(a.at), q = reinterpret_cast<uintptr_t>(b.at);
+    return a.at != nullptr && b.at != nullptr && (p <= q ? q - p < a.bytes && b.bytes > 0 : p - q < b.bytes && a.bytes > 0);
+}
+
 // Attributes of a launch, of which `attr` holds two; returns how many there are.  overlap: programmatic stream serialization, with which the blocks
 // may begin while the kernel before them in the stream still runs (they wait for its end themselves, but for weights, which are in place).
 // cluster: blocks of a cluster, 0 for none.

@@ -1502,10 +1502,10 @@ int entry(vqm_runtime *rt, std::initializer_list<const char *> names, F &&body) 
     }
 }
 
-// What is written by blocks while others still read lies in a buffer of its own.
-int check_apart(const char *what, const void *written, std::initializer_list<const void *> read) {
-    for (const void *p : read)
-        if (p == written) return fail(VQM_ERR_VALUE, "%s need a buffer of their own", what);
+// What is written by blocks while others still read lies in memory of its own.
+int check_apart(const char *what, const vqm::Extent &written, std::initializer_list<vqm::Extent> others) {
+    for (const vqm::Extent &e : others)
+        if (vqm::overlap(written, e)) return fail(VQM_ERR_VALUE, "%s need a buffer of their own", what);
     return VQM_OK;
 }
 
@@ -1591,7 +1591,7 @@ int vqm_bind_i8(vqm_runtime *rt, const char *name, const void *device_ptr, size_
         if (scales == nullptr || (reinterpret_cast<uintptr_t>(scales) & 3u) != 0)
             return fail(VQM_ERR_VALUE, "%s: the scales' device pointer must be 4-byte aligned", name);
         if (pitch == 0) pitch = static_cast<size_t>(vqm::i8_pitch(cols));
-        if (pitch % 16 != 0 || pitch < static_cast<size_t>(cols) || pitch >= (static_cast<size_t>(1) << 40))
+        if (pitch % 16 != 0 || pitch < static_cast<size_t>(cols) || pitch >= (static_cast<size_t>(1) << 40) || pitch > (static_cast<size_t>(1) << 62) / static_cast<size_t>(rows))
             return fail(VQM_ERR_VALUE, "%s: the rows' pitch must be a multiple of 16 bytes and no less than the columns", name);
         Tensor t;
         t.data = const_cast<uint8_t *>(static_cast<const uint8_t *>(device_ptr));
@@ -1686,8 +1686,13 @@ int vqm_rows_i8(vqm_runtime *rt, const char *x, const char *q, const char *scale
             if ((a.norm_w = find_norm(rt, norm_weight, cols, &rc)) == nullptr) return rc;
             if (!(eps >= 0.0f)) return fail(VQM_ERR_VALUE, "eps must be >= 0");
         }
-        if ((rc = check_apart("the scales", a.scales, {a.x, a.x2, a.residual, a.total, a.norm_w})) != VQM_OK) return rc;
-        if (a.total != nullptr && (rc = check_apart("the sums", a.total, {a.norm_w})) != VQM_OK) return rc;
+        const size_t bytes = n * static_cast<size_t>(a.elem);
+        const vqm::Extent ex{a.x, bytes}, ex2{a.x2, bytes}, er{a.residual, bytes}, et{a.total, bytes}, eg{a.norm_w, sizeof(float) * static_cast<size_t>(cols)};
+        const vqm::Extent es{a.scales, sizeof(float) * static_cast<size_t>(ntok)}, eq{a.q, static_cast<size_t>(vqm::i8_pitch(cols)) * ntok};
+        if ((rc = check_apart("the scales", es, {ex, ex2, er, et, eg})) != VQM_OK) return rc;
+        if ((rc = check_apart("the 8-bit rows", eq, {ex, ex2, er, et, eg, es})) != VQM_OK) return rc;
+        // (sums may lie where x or the residual does, value for value)
+        if ((rc = check_apart("the sums", et, {a.total == a.x ? vqm::kNoExtent : ex, a.total == a.residual ? vqm::kNoExtent : er, eg})) != VQM_OK) return rc;
         const cudaError_t err = vqm::launch_rows_i8(a, rt->sm_count, rt->stream);
         if (err != cudaSuccess) return cuda_fail("rows_i8 launch", err);
         count_launch(rt);
@@ -1706,7 +1711,10 @@ int vqm_qmm_i8(vqm_runtime *rt, const char *weight, const char *q, const char *s
         if ((a.q = find_i8(rt, q, static_cast<size_t>(vqm::i8_pitch(t->cols)) * ntok, &rc)) == nullptr) return rc;
         if ((a.q_scales = find_f32(rt, scales, static_cast<size_t>(ntok), &rc)) == nullptr) return rc;
         if ((a.y = find_real(rt, y, static_cast<size_t>(t->rows) * ntok, &a.y_elem, &rc)) == nullptr) return rc;
-        if ((rc = check_apart("the outputs", a.y, {a.q_scales})) != VQM_OK) return rc;
+        const size_t rows = static_cast<size_t>(t->rows), tok = static_cast<size_t>(ntok);
+        const vqm::Extent w{t->data, (rows - 1) * t->row_bytes + static_cast<size_t>(t->cols)}, ws{t->scales, sizeof(float) * rows};
+        const vqm::Extent eq{a.q, static_cast<size_t>(vqm::i8_pitch(t->cols)) * tok}, es{a.q_scales, sizeof(float) * tok};
+        if ((rc = check_apart("the outputs", vqm::Extent{a.y, rows * tok * static_cast<size_t>(a.y_elem)}, {eq, es, w, ws})) != VQM_OK) return rc;
         a.w = reinterpret_cast<const int8_t *>(t->data);
         a.w_scales = t->scales;
         a.w_pitch = static_cast<long long>(t->row_bytes);
@@ -1743,7 +1751,11 @@ int vqm_verify(vqm_runtime *rt, const char *target, const char *draft, const cha
         if ((a.uniforms = find_f32(rt, uniforms, s * (k + 1), &rc)) == nullptr) return rc;
         if (temperature != nullptr && (a.temperature = find_f32(rt, temperature, s, &rc)) == nullptr) return rc;
         if ((a.out = static_cast<int *>(find_real(rt, out, s * (k + 2), &word, &rc))) == nullptr) return rc;
-        if ((rc = check_apart("the answers", a.out, {a.target, a.draft, a.tokens, a.lens, a.uniforms, a.temperature})) != VQM_OK) return rc;
+        const size_t row = static_cast<size_t>(vocab) * static_cast<size_t>(a.elem);
+        if ((rc = check_apart("the answers", vqm::Extent{a.out, 4 * s * (k + 2)},
+                              {vqm::Extent{a.target, s * (k + 1) * row}, vqm::Extent{a.draft, s * k * row}, vqm::Extent{a.tokens, 4 * s * k}, vqm::Extent{a.lens, 4 * s},
+                               vqm::Extent{a.uniforms, 4 * s * (k + 1)}, vqm::Extent{a.temperature, 4 * s}})) != VQM_OK)
+            return rc;
         a.status = rt->status;
         if (out_host != nullptr && (rc = no_capture(rt, "a blocking verify")) != VQM_OK) return rc;
         cudaError_t err = vqm::launch_verify(a, rt->stream);
