@@ -154,7 +154,8 @@ int vqm_dequantize(vqm_runtime *rt, const char *weight, const char *out);
  *
  * vqm_upload_i8   w: rows * cols int8 in host memory, densely packed; scales: rows floats.  Synchronous; re-upload replaces.
  * vqm_bind_i8     the same in device memory that the caller keeps and has filled (products fetch weights ahead of the stream's order, but
- *                 with VINF_B200_NO_PDL=1 in the environment when the runtime is created): 16-byte aligned, `pitch` bytes from row to row (0: round_up(cols, 16)); what lies behind a row's last column is ignored.
+ *                 with VINF_B200_NO_PDL=1 in the environment when the runtime is created): 16-byte aligned, `pitch` bytes from row to row (0: round_up(cols, 16)); what lies behind a row's
+ *                 last column is ignored.  Not to replace a tensor while a graph is being captured.
  * vqm_convert_i8  makes the tensor `name` from any GGUF tensor: scales[r] = max |row r| / 127, values to the nearest integer.  Synchronous.
  */
 #define VQM_I8_ROWS 24

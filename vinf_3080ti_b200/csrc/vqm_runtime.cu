@@ -1584,7 +1584,7 @@ int vqm_upload_i8(vqm_runtime *rt, const char *name, const void *data, size_t nb
 
 int vqm_bind_i8(vqm_runtime *rt, const char *name, const void *device_ptr, size_t pitch, const float *scales, int cols, int rows) {
     return entry(rt, {name}, [&]() -> int {
-        const int rc = check_i8_shape(name, cols, rows);
+        int rc = check_i8_shape(name, cols, rows);
         if (rc != VQM_OK) return rc;
         if (device_ptr == nullptr || (reinterpret_cast<uintptr_t>(device_ptr) & 15u) != 0)
             return fail(VQM_ERR_VALUE, "%s: device pointer must be 16-byte aligned", name);
@@ -1593,6 +1593,8 @@ int vqm_bind_i8(vqm_runtime *rt, const char *name, const void *device_ptr, size_
         if (pitch == 0) pitch = static_cast<size_t>(vqm::i8_pitch(cols));
         if (pitch % 16 != 0 || pitch < static_cast<size_t>(cols) || pitch >= (static_cast<size_t>(1) << 40) || pitch > (static_cast<size_t>(1) << 62) / static_cast<size_t>(rows))
             return fail(VQM_ERR_VALUE, "%s: the rows' pitch must be a multiple of 16 bytes and no less than the columns", name);
+        // (a new name is only noted; for another tensor of that name the stream is waited for, and its memory freed)
+        if (rt->tensors.count(name) != 0 && (rc = no_capture(rt, "to replace a tensor")) != VQM_OK) return rc;
         Tensor t;
         t.data = const_cast<uint8_t *>(static_cast<const uint8_t *>(device_ptr));
         t.owned = false;
