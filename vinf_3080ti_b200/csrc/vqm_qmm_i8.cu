@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
     __shared__ __align__(8) uint64_t s_sums;
     __shared__ float s_scales[2][kQMaxN];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_failed;
+    __shared__ int s_failed, s_issued;
     const uint32_t ring = (s32(ring_raw) + 1023u) & ~1023u;  // (the swizzle works on address bits)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t in_cluster = 0;
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
             bar_init(s32(&s_acc_empty[b]), kQWriters * GROUP);
         }
         bar_init(s32(&s_sums), 1);
-        s_failed = 0;
+        s_failed = s_issued = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 2) {
@@ -250,9 +250,7 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
                     if (++stage == a.stages) stage = 0, parity ^= 1;
                 }
             }
-            if (!ok)  // the last copies land before the block may leave
-                for (int last = max(0, issued - a.stages); last < issued; ++last)
-                    for (int i = 0; i < (1 << 16) && !bar_try(s32(&s_full[last % a.stages]), (last / a.stages) & 1); ++i) __nanosleep(64);
+            s_issued = issued;
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -386,6 +384,12 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (s_failed && threadIdx.x == 0) {  // whichever wait gave up: the last copies land before the block may leave (this wait has a limit too)
+        int left = 1 << 16;
+        for (int last = max(0, s_issued - a.stages); last < s_issued; ++last)
+            while (!bar_try(s32(&s_full[last % a.stages]), (last / a.stages) & 1) && --left > 0) __nanosleep(64);
+    }
+    __syncwarp();
     // no block's shared or tensor memory goes away under another
     if constexpr (SPLIT) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     else if constexpr (PAIR) cluster_sync();
