@@ -217,9 +217,9 @@ struct RowsI8Args {
     int cols, ntok, elem;
     float eps;
     double inv_cols;       // 1 / cols, filled in by the launcher
-    bool overlap;          // host only, see launch_attributes
 };
-cudaError_t launch_rows_i8(const RowsI8Args &a, int sm_count, cudaStream_t stream);
+// overlap: see launch_attributes
+cudaError_t launch_rows_i8(const RowsI8Args &a, bool overlap, int sm_count, cudaStream_t stream);
 // How far fp32 leaves t = n / s from its value, relative to t: whoever is that near to a half is rounded in 64 bits.  In units of 2^-24: the product with the
 // norm's weights 1, its factor r 1, the division of r by s 4 (2 steps at most, which are 2 units each behind a power of two), the product with that 1, and the
 // rounding of the bound itself, half a unit at |t| = 1/2.  Gated values have two products before the division instead, and the sigmoid: 4 of ex2, 1 of
@@ -250,9 +250,9 @@ struct VerifyArgs {
     int *out;                  // [seqs][drafts + 2]; all -1 if the status word is not 0
     const unsigned *status;    // device word with the code of a wait that has expired: the logits may not be what they should
     int vocab, seqs, drafts, elem;
-    bool overlap;              // host only, see launch_attributes
 };
-cudaError_t launch_verify(const VerifyArgs &a, cudaStream_t stream);
+// overlap: see launch_attributes
+cudaError_t launch_verify(const VerifyArgs &a, bool overlap, cudaStream_t stream);
 // How far from one another, relative to the larger, the two sides of a draft's test may be if they are equal but come from fp32 sums of exponentials, of
 // which a lane adds up `adds` parts.  In units of 2^-24: a part is added with one rounding, and where it has a new largest the sum before it is scaled, 4 of
 // ex2 and 1 of the product; both sides have such a sum, and the products of so many factors add less than 5 %.  The rest is 2e-5: 4 of each ex2, 3 times

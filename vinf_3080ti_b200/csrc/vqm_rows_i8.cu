@@ -486,67 +486,75 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<T, NV, THREADS>()) rows
     if (threadIdx.x < pitch - a.cols) out[a.cols + threadIdx.x] = 0;
 }
 
+// (`overlap` is not among the kernel's parameters: with 8 bytes more of them 4001 rows of 5120 in fp16 take 34.2 instead of 33.6 us)
+struct Place {
+    bool overlap;
+    int sm_count;
+    cudaStream_t stream;
+};
+
 template <typename K>
-cudaError_t launch_kernel(K kernel, const RowsI8Args &a, int threads, cudaStream_t stream) {
+cudaError_t launch_kernel(K kernel, const RowsI8Args &a, int threads, const Place &at) {
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
     cfg.gridDim = dim3(static_cast<unsigned>(a.ntok));
     cfg.blockDim = dim3(static_cast<unsigned>(threads));
-    cfg.stream = stream;
+    cfg.stream = at.stream;
     cfg.attrs = attr;
-    cfg.numAttrs = launch_attributes(attr, a.overlap, 0);
+    cfg.numAttrs = launch_attributes(attr, at.overlap, 0);
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
 template <typename T, int NV, int THREADS, bool LOOSE>
-cudaError_t launch_variant(const RowsI8Args &a, cudaStream_t stream) {
-    return a.x2 != nullptr ? launch_kernel(rows_i8_kernel<T, NV, THREADS, true, LOOSE>, a, THREADS, stream)
-                           : launch_kernel(rows_i8_kernel<T, NV, THREADS, false, LOOSE>, a, THREADS, stream);
+cudaError_t launch_variant(const RowsI8Args &a, const Place &at) {
+    return a.x2 != nullptr ? launch_kernel(rows_i8_kernel<T, NV, THREADS, true, LOOSE>, a, THREADS, at)
+                           : launch_kernel(rows_i8_kernel<T, NV, THREADS, false, LOOSE>, a, THREADS, at);
 }
 // Threads of a row: many rows have an SM to share, few rows wait for their own steps only (4 gated rows of 17408: 512 threads 6.2 us, 1024 5.2).  fp32
 // rows of more than 12282 values fit twice on an SM only with spills (47 us for 40 with 512 threads each), so they take one block of 1024 (1000 gated rows of
 // 17408: 52.7 us with one block of 512, 48.5).  fp16 rows of 4097 to 6138 values: 128 threads 36.1, 256 39.3 us.
 // The smallest of the given numbers of vectors per thread that holds a row.
 template <typename T, int THREADS, bool LOOSE, int NV, int... MORE>
-cudaError_t launch_vectors(const RowsI8Args &a, cudaStream_t stream) {
+cudaError_t launch_vectors(const RowsI8Args &a, const Place &at) {
     if constexpr (sizeof...(MORE) > 0)
-        if ((a.cols + (LOOSE ? 6 : 3)) / 4 > NV * THREADS) return launch_vectors<T, THREADS, LOOSE, MORE...>(a, stream);
-    return launch_variant<T, NV, THREADS, LOOSE>(a, stream);
+        if ((a.cols + (LOOSE ? 6 : 3)) / 4 > NV * THREADS) return launch_vectors<T, THREADS, LOOSE, MORE...>(a, at);
+    return launch_variant<T, NV, THREADS, LOOSE>(a, at);
 }
 
 template <typename T, bool LOOSE>
-cudaError_t launch_size(const RowsI8Args &a, int sm_count, cudaStream_t stream) {
-    if (a.ntok <= sm_count)  // few rows: as many threads on each as there are
-        return a.cols <= 10234 ? launch_vectors<T, 512, LOOSE, 2, 5>(a, stream) : launch_vectors<T, 1024, LOOSE, 5, 6>(a, stream);
+cudaError_t launch_size(const RowsI8Args &a, const Place &at) {
+    if (a.ntok <= at.sm_count)  // few rows: as many threads on each as there are
+        return a.cols <= 10234 ? launch_vectors<T, 512, LOOSE, 2, 5>(a, at) : launch_vectors<T, 1024, LOOSE, 5, 6>(a, at);
     constexpr int kMore = LOOSE ? 6 : 0;  // columns that a row may need room for, because it does not begin with a vector
-    if (a.cols <= 1024 - kMore) return launch_vectors<T, 32, LOOSE, 2, 5, 8>(a, stream);
+    if (a.cols <= 1024 - kMore) return launch_vectors<T, 32, LOOSE, 2, 5, 8>(a, at);
     if constexpr (sizeof(T) == 2) {
-        if (a.cols <= 6138) return launch_vectors<T, 128, LOOSE, 5, 8, 10, 12>(a, stream);
-        if (a.cols <= 12282) return launch_vectors<T, 256, LOOSE, 8, 10, 12>(a, stream);
-        return launch_vectors<T, 512, LOOSE, 8, 9, 10, 12>(a, stream);
+        if (a.cols <= 6138) return launch_vectors<T, 128, LOOSE, 5, 8, 10, 12>(a, at);
+        if (a.cols <= 12282) return launch_vectors<T, 256, LOOSE, 8, 10, 12>(a, at);
+        return launch_vectors<T, 512, LOOSE, 8, 9, 10, 12>(a, at);
     } else {
-        if (a.cols <= 4096 - kMore) return launch_vectors<T, 128, LOOSE, 5, 8>(a, stream);
-        if (a.cols <= 12282) return launch_vectors<T, 256, LOOSE, 5, 8, 10, 12>(a, stream);
-        return launch_vectors<T, 1024, LOOSE, 5, 6>(a, stream);
+        if (a.cols <= 4096 - kMore) return launch_vectors<T, 128, LOOSE, 5, 8>(a, at);
+        if (a.cols <= 12282) return launch_vectors<T, 256, LOOSE, 5, 8, 10, 12>(a, at);
+        return launch_vectors<T, 1024, LOOSE, 5, 6>(a, at);
     }
 }
 template <typename T>
-cudaError_t launch_t(const RowsI8Args &a, int sm_count, cudaStream_t stream) {
+cudaError_t launch_t(const RowsI8Args &a, const Place &at) {
     if (a.x2 != nullptr && a.norm_w != nullptr && i8_pitch(a.cols) <= 512 * 40) {
-        if (i8_pitch(a.cols) <= 512 * 4) return launch_kernel(gated_norm_kernel<T, 4>, a, 512, stream);
-        if (i8_pitch(a.cols) <= 512 * 16) return launch_kernel(gated_norm_kernel<T, 16>, a, 512, stream);
-        return launch_kernel(gated_norm_kernel<T, 40>, a, 512, stream);
+        if (i8_pitch(a.cols) <= 512 * 4) return launch_kernel(gated_norm_kernel<T, 4>, a, 512, at);
+        if (i8_pitch(a.cols) <= 512 * 16) return launch_kernel(gated_norm_kernel<T, 16>, a, 512, at);
+        return launch_kernel(gated_norm_kernel<T, 40>, a, 512, at);
     }
-    if (a.cols > kMostFast || (a.x2 != nullptr && a.norm_w != nullptr)) return launch_kernel(exact_rows_kernel<T>, a, 512, stream);
-    return a.cols % 4 == 0 ? launch_size<T, false>(a, sm_count, stream) : launch_size<T, true>(a, sm_count, stream);
+    if (a.cols > kMostFast || (a.x2 != nullptr && a.norm_w != nullptr)) return launch_kernel(exact_rows_kernel<T>, a, 512, at);
+    return a.cols % 4 == 0 ? launch_size<T, false>(a, at) : launch_size<T, true>(a, at);
 }
 
 }  // namespace
 
-cudaError_t launch_rows_i8(const RowsI8Args &in, int sm_count, cudaStream_t stream) {
+cudaError_t launch_rows_i8(const RowsI8Args &in, bool overlap, int sm_count, cudaStream_t stream) {
     RowsI8Args a = in;
     a.inv_cols = 1.0 / a.cols;
-    return a.elem == 2 ? launch_t<__half>(a, sm_count, stream) : launch_t<float>(a, sm_count, stream);
+    const Place at{overlap, sm_count, stream};
+    return a.elem == 2 ? launch_t<__half>(a, at) : launch_t<float>(a, at);
 }
 
 }  // namespace vqm

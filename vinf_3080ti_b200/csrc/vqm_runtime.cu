@@ -1639,8 +1639,7 @@ int vqm_convert_i8(vqm_runtime *rt, const char *weight, const char *name) {
             a.cols = from->cols;
             a.ntok = static_cast<int>(n);
             a.elem = 4;
-            a.overlap = rt->overlap_launch != 0;
-            if (err == cudaSuccess) err = vqm::launch_rows_i8(a, rt->sm_count, rt->stream);
+            if (err == cudaSuccess) err = vqm::launch_rows_i8(a, rt->overlap_launch != 0, rt->sm_count, rt->stream);
             if (err == cudaSuccess) count_launch(rt, 2);
         }
         const cudaError_t done = cudaStreamSynchronize(rt->stream);  // (products fetch weights ahead of the stream's order)
@@ -1668,7 +1667,6 @@ int vqm_rows_i8(vqm_runtime *rt, const char *x, const char *q, const char *scale
         a.cols = cols;
         a.ntok = ntok;
         a.eps = eps;
-        a.overlap = rt->overlap_launch != 0;
         if ((a.x = find_real(rt, x, n, &a.elem, &rc)) == nullptr) return rc;
         if ((a.q = find_i8(rt, q, static_cast<size_t>(vqm::i8_pitch(cols)) * ntok, &rc)) == nullptr) return rc;
         if ((a.scales = find_f32(rt, scales, static_cast<size_t>(ntok), &rc)) == nullptr) return rc;
@@ -1695,7 +1693,7 @@ int vqm_rows_i8(vqm_runtime *rt, const char *x, const char *q, const char *scale
         if ((rc = check_apart("the 8-bit rows", eq, {ex, ex2, er, et, eg, es})) != VQM_OK) return rc;
         // (sums may lie where x or the residual does, value for value)
         if ((rc = check_apart("the sums", et, {a.total == a.x ? vqm::kNoExtent : ex, a.total == a.residual ? vqm::kNoExtent : er, eg})) != VQM_OK) return rc;
-        const cudaError_t err = vqm::launch_rows_i8(a, rt->sm_count, rt->stream);
+        const cudaError_t err = vqm::launch_rows_i8(a, rt->overlap_launch != 0, rt->sm_count, rt->stream);
         if (err != cudaSuccess) return cuda_fail("rows_i8 launch", err);
         count_launch(rt);
         return VQM_OK;
@@ -1745,7 +1743,6 @@ int vqm_verify(vqm_runtime *rt, const char *target, const char *draft, const cha
         a.vocab = vocab;
         a.seqs = seqs;
         a.drafts = drafts;
-        a.overlap = rt->overlap_launch != 0;
         if ((a.target = find_real(rt, target, s * (k + 1) * static_cast<size_t>(vocab), &a.elem, &rc)) == nullptr) return rc;
         if (drafts > 0 && draft != nullptr && (a.draft = find_real(rt, draft, s * k * static_cast<size_t>(vocab), &a.elem, &rc)) == nullptr) return rc;
         if (drafts > 0 && (a.tokens = static_cast<const int *>(find_real(rt, tokens, s * k, &word, &rc))) == nullptr) return rc;
@@ -1760,7 +1757,7 @@ int vqm_verify(vqm_runtime *rt, const char *target, const char *draft, const cha
             return rc;
         a.status = rt->status;
         if (out_host != nullptr && (rc = no_capture(rt, "a blocking verify")) != VQM_OK) return rc;
-        cudaError_t err = vqm::launch_verify(a, rt->stream);
+        cudaError_t err = vqm::launch_verify(a, rt->overlap_launch != 0, rt->stream);
         if (err != cudaSuccess) return cuda_fail("verify launch", err);
         count_launch(rt);
         if (out_host != nullptr) {

@@ -608,22 +608,22 @@ struct Launcher {
         }
         return cached[blocks];
     }
-    static cudaError_t launch(const VerifyArgs &a, cudaStream_t stream) {
+    static cudaError_t launch(const VerifyArgs &a, bool overlap, cudaStream_t stream) {
         // As many blocks per sequence as all sequences have room for side by side, of at least 2048 elements each.  (With more, so that a second
         // round of clusters follows the first: 64 sequences of 4 drafts 180 and 249 us instead of 162.)
         int blocks = kVMaxCluster;
         while (blocks > 1 && (a.seqs > fit(blocks) || a.vocab < blocks * 2048)) --blocks;
         cudaLaunchConfig_t cfg{};
         cudaLaunchAttribute attr[2];
-        configure(cfg, attr, a.seqs, blocks, a.overlap, stream);
+        configure(cfg, attr, a.seqs, blocks, overlap, stream);
         return cudaLaunchKernelEx(&cfg, kKernel, a);
     }
 };
 
 }  // namespace
 
-cudaError_t launch_verify(const VerifyArgs &a, cudaStream_t stream) {
-    return a.elem == 2 ? Launcher<__half>::launch(a, stream) : Launcher<float>::launch(a, stream);
+cudaError_t launch_verify(const VerifyArgs &a, bool overlap, cudaStream_t stream) {
+    return a.elem == 2 ? Launcher<__half>::launch(a, overlap, stream) : Launcher<float>::launch(a, overlap, stream);
 }
 
 }  // namespace vqm
