@@ -1,5 +1,5 @@
 """The distance from a half within which rows_i8 rounds in 64 bits covers what fp32 may be off by.  Documented errors, in units of 2^-24 (half a step
-behind a power of two): a product, a sum or a conversion 1; __fdividef 2 steps; ex2.approx 2^-22; rcp.approx one step."""
+behind a power of two): a product, a sum, a conversion or __fdiv_rn 1; ex2.approx 2^-22; rcp.approx one step."""
 from __future__ import annotations
 
 import subprocess
@@ -10,7 +10,7 @@ import pytest
 from vinf_3080ti_b200 import build
 
 UNIT = 2.0**-24
-PRODUCT, DIVISION, EX2, RECIPROCAL = 1, 2 * 2, 4, 2
+PRODUCT, DIVISION, EX2, RECIPROCAL = 1, 1, 4, 2
 
 
 @pytest.fixture(scope="module")
@@ -34,7 +34,7 @@ def test_the_margins_cover_the_documented_errors(off):
 
 @pytest.mark.parametrize("whole", [0, 1, 2, 7, 63, 126])
 def test_values_next_to_a_half_are_seen(off, whole):
-    """t = (e g) (r / s) in fp32 with the division two steps off, to either side, against 64 bits."""
+    """t = (e g) (r / s) in fp32 against 64 bits."""
     f32, rng, n = np.float32, np.random.default_rng(whole), 200_000
     for spread in (4, 4096, 1 << 22):
         def mantissa():
@@ -43,11 +43,6 @@ def test_values_next_to_a_half_are_seen(off, whole):
         e, s, r = mantissa(), mantissa(), mantissa() + rng.uniform(-0.49, 0.49, n) * 2.0**-23
         g = f32((whole + 0.5) * s / (r * e)).astype(np.float64)
         want = np.rint(e * g * r / s)
-        quotient = f32(r).astype(np.float64) / s
-        for side in (-1.0, 1.0):
-            end = quotient + side * 2 * np.spacing(f32(quotient)).astype(np.float64)
-            f = f32(end)
-            f = np.where((f.astype(np.float64) - end) * side > 0, np.nextafter(f, f32(-side * 1e30)), f)
-            t = f32(f32(f32(e) * f32(g)) * f).astype(np.float64)
-            near = np.abs(t - np.rint(t)) > f32(0.5 - np.abs(t) * off[0])
-            assert ((np.rint(t) == want) | near).all()
+        t = f32(f32(f32(e) * f32(g)) * (f32(r) / f32(s))).astype(np.float64)
+        near = np.abs(t - np.rint(t)) > f32(0.5 - np.abs(t) * off[0])
+        assert ((np.rint(t) == want) | near).all()

@@ -221,10 +221,10 @@ struct RowsI8Args {
 // overlap: see launch_attributes
 cudaError_t launch_rows_i8(const RowsI8Args &a, bool overlap, int sm_count, cudaStream_t stream);
 // How far fp32 leaves t = n / s from its value, relative to t: whoever is that near to a half is rounded in 64 bits.  In units of 2^-24: the product with the
-// norm's weights 1, its factor r 1, the division of r by s 4 (2 steps at most, which are 2 units each behind a power of two), the product with that 1, and the
-// rounding of the bound itself, half a unit at |t| = 1/2.  Gated values have two products before the division instead, and the sigmoid: 4 of ex2, 1 of
-// the sum, 2 of the reciprocal, and for each unit of -x (largest of the thread) 1 of the argument and 0.23 of the constant in it.
-constexpr float kI8Off = 8.0f / (1 << 24), kI8GatedOff = 17.0f / (1 << 24), kI8GatedOffPerX = 1.35f / (1 << 24);
+// norm's weights 1, its factor r 1, the division of r by s 1, the product with that 1, and the rounding of the bound itself, half a unit at |t| = 1/2.
+// Gated values have two products before the division instead, and the sigmoid: 4 of ex2, 1 of the sum, 2 of the reciprocal, and for each unit of -x (largest
+// of the thread) 1 of the argument and 0.23 of the constant in it.
+constexpr float kI8Off = 5.0f / (1 << 24), kI8GatedOff = 12.0f / (1 << 24), kI8GatedOffPerX = 1.35f / (1 << 24);
 
 struct QmmI8Args {
     const int8_t *w;       // [rows][w_pitch], 16-byte aligned, w_pitch a multiple of 16

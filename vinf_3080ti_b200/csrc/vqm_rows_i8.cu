@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<T, NV, THREADS>()) rows
         const float scale = wide >= kMostScale ? kUndefined : static_cast<float>(wide);
         s.r = r;
         s.scale = static_cast<double>(scale);
-        s.factor = scale > 1e-37f && r > 1.2e-38 && r < 1e38 ? __fdividef(static_cast<float>(r), scale) : 0.0f;  // (r as a normal fp32 number)
+        s.factor = scale > 1e-37f && r > 1.2e-38 && r < 1e38 ? __fdiv_rn(static_cast<float>(r), scale) : 0.0f;  // (r as a normal fp32 number)
         a.scales[row] = scale;
     }
     __syncthreads();
