@@ -243,13 +243,21 @@ __device__ __forceinline__ void Kept<T, WIDE>::fetch(const T *p) {
     }
 }
 
-// Blocks that an SM holds at least, which bounds the registers: while some rows wait for memory, others are worked on.  Measured, against one block less or
-// more: fp16, 128 threads 35.8 us (6: 37.1; 8, with spills: 41.9; 4001 rows of 5120), 256 threads 19.2 (3: 20.5; 1000 of 8192), 512 threads 27.1 (1: 32.6;
-// 600 of 17408); fp32, 256 threads with 5 vectors 51.2 (3: 53.4; 4001 of 5120), with more of them 3 (5 or 6 spill).
-template <typename T, int NV, int THREADS>
+// Blocks that an SM holds at least, which bounds the registers: while some rows wait for memory, others are worked on.  A bound that makes threads spill some
+// registers still pays where the blocks it gains are a large part, and does not where 100 bytes and more are spilled for a third one of long fp32 rows.
+// Measured, us, against one block less or more; in brackets bytes spilled by plain and gated variants of rows that are multiples of 4 (others spill more):
+//   fp16, 128 threads           7 [48 and 116 at most]: norm 4001 x 5120 36.7 (6: 38.0), gated 38.2 (6: 40.2), 4001 x 4096 gated 34.4 (6: 33.0)
+//   fp16, 256 threads           4 up to 10 vectors [92, 120]: gated 2000 x 8192 30.1 (3: 34.2), 1000 x 10000 23.2 (3: 24.4), norm 26.8 (3: 26.0)
+//                               3 for 12 vectors [0, 84]: gated 1000 x 12000 30.6 (4: 35.3), 400 x 12000 12.8 (4: 19.0); but rows of odd lengths 4: 12001 43.0 (3: 48.4)
+//   fp16, 512 threads           2 [120, 160]: gated 1000 x 17408 36.7 (1: 50.9), norm 39.3 (1: 47.4), 1000 x 14336 31.2 (1: 45.3)
+//   fp32, 256 threads           4 for 5 vectors [12, 0]: norm 4001 x 5120 52.7 (3 took 2 us more); 3 for 8 [24, 0] (4 spills more)
+//                               2 for 10 and 12 [0, 0]: 1000 x 10000 gated 28.9, norm 36, plain 16.2 (3: 33.3, 42.5, 15.1), 1000 x 12000 33.5, 44, 18.2 (3: 46.1, 59, 17.6);
+//                               400 x 10000, which 3 hold at once, gated 15.8 (3: 13.6)
+template <typename T, int NV, int THREADS, bool LOOSE>
 constexpr int blocks_per_sm() {
     if (THREADS == 512) return 2;
-    if (THREADS == 256) return sizeof(T) == 2 || NV <= 5 ? 4 : 3;
+    if (THREADS == 256 && sizeof(T) == 2) return NV <= 10 || LOOSE ? 4 : 3;
+    if (THREADS == 256) return NV <= 5 ? 4 : NV <= 8 ? 3 : 2;
     return THREADS == 128 && sizeof(T) == 2 ? 7 : 1;
 }
 
@@ -257,7 +265,7 @@ constexpr int blocks_per_sm() {
 // from the caches both times.  LOOSE: rows of any length, whose vectors lie on the buffers' grid, not the row's: the first and the last may be
 // partly outside of the row, and the norm's weights and the outputs, which lie on other grids, go one by one.
 template <typename T, int NV, int THREADS, bool GATED, bool LOOSE>
-__global__ void __launch_bounds__(THREADS, blocks_per_sm<T, NV, THREADS>()) rows_i8_kernel(const RowsI8Args a) {
+__global__ void __launch_bounds__(THREADS, blocks_per_sm<T, NV, THREADS, LOOSE>()) rows_i8_kernel(const RowsI8Args a) {
     __shared__ RowShared s;
     constexpr int WARPS = THREADS / 32;
     const size_t row = blockIdx.x, at = row * a.cols;
