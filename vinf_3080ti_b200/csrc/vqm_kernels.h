@@ -238,7 +238,7 @@ struct QmmI8Args {
     bool overlap;          // see launch_attributes
     unsigned *status;      // device word that receives a code if a bounded wait expires
 };
-cudaError_t launch_qmm_i8(const QmmI8Args &a, int sm_count, cudaStream_t stream);
+cudaError_t launch_qmm_i8(const QmmI8Args &a, cudaStream_t stream);
 
 struct VerifyArgs {
     const void *target;        // [seqs][drafts + 1][vocab] of `elem` bytes

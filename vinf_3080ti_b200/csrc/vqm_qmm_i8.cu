@@ -453,7 +453,7 @@ struct Variant {
 
 }  // namespace
 
-cudaError_t launch_qmm_i8(const QmmI8Args &in, int sm_count, cudaStream_t stream) {
+cudaError_t launch_qmm_i8(const QmmI8Args &in, cudaStream_t stream) {
     QmmTc a{};
     a.w_scales = in.w_scales;
     a.q_scales = in.q_scales;

@@ -1724,7 +1724,7 @@ int vqm_qmm_i8(vqm_runtime *rt, const char *weight, const char *q, const char *s
         a.add = (flags & VQM_FUSE_ADD) != 0;
         a.overlap = rt->overlap_launch != 0;
         a.status = rt->status;
-        const cudaError_t err = vqm::launch_qmm_i8(a, rt->sm_count, rt->stream);
+        const cudaError_t err = vqm::launch_qmm_i8(a, rt->stream);
         if (err != cudaSuccess) return cuda_fail("qmm_i8 launch", err);
         count_launch(rt);
         return VQM_OK;
