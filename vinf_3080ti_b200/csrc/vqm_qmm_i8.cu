@@ -18,7 +18,8 @@
 // the exchange of sums.  What it took: the loop that issues the MMAs in one thread, with waits that look at their barrier only (4096 rows: 307 and 299
 // us); outputs loaded 16 columns ahead, scales in shared memory, no choice of types inside (a tile's outputs took 10 us, as long as its MMAs: 299 and
 // 262); two blocks per SM for few rows (5120 x 17408 with 24: 15.6 and 13.9).  Tried: weights fetched into L2 8 or 24 stages ahead of their copies, 16.6
-// and 19.7 or 22.0 us for one row.
+// and 19.7 or 22.0 us for one row.  In between, 17408 x 5120 of one stream: 33 rows 18.0 us, 64 18.4, 128 19.6, 256 25.4: a block's one tile is written
+// after its products.  Products onto what is there read an output behind the one before: 4 rows 18.7, 256 rows 81.
 //
 // Every wait is bounded: on expiry the block records a status code and everybody falls through to the end.
 #include <cuda.h>

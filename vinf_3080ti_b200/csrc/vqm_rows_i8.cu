@@ -5,12 +5,15 @@
 // taken in 64 bits (the mean's square root cancels out of n / s but for the rounding of s), the values in 32, and a value that 32 bits leave next to a
 // half is worked out again in 64.
 //
-// A block per row (of 32 to 1024 threads), its values in registers: memory is read and written once.
-// Rows too long for that, norms of gated values, and rows whose largest value is out of fp32's middle range are worked out in 64 bits throughout.
+// A block per row (of 32 to 1024 threads), its values in registers (but for some that long rows spill, see blocks_per_sm): memory is read and written once.
+// Rows too long for that (more than 24564 values), norms of gated values, and rows whose largest value is out of fp32's middle range are worked out in 64
+// bits throughout, norms of up to 20480 gated values with each value made once.
 //
-// What bounds it: 4001 rows of 5120 with residual and norm take 51 us in fp32 (5200 GB/s of the 6550 that a copy gets) and 36 in fp16 (3980 GB/s): there the
-// instructions, 32 per element, the mean's 64 bits and the norm's weights, and a row's steps one after the other.  1000 gated rows of 17408: 48.5 us in
-// fp32 (3230 GB/s), 36 in fp16; 4001 of 5120: 37 and 38, ex2 and a reciprocal per element and the rows' steps.  One row: 3.4 us.
+// What bounds it: 4001 rows of 5120 with residual and norm take 52 us in fp32 (5080 GB/s of the 6550 that a copy gets) and 34 to 37 in fp16 (3900 GB/s).  There,
+// and in gated rows (4001 x 5120 38 us in both types, 1000 x 17408 49 in fp32 and 37 in fp16), neither the issue slots (32 to 52 %) nor DRAM (23 to 35 %) are
+// at their limit: a row's steps follow one another, with two barriers and one thread's 64-bit work between its two passes over the registers, and the rows
+// that an SM holds cover a part of that.  Lengths that are no multiple of 4 write bytes one by one (4001 x 5121 58 to 77 us).  One row: 3.4 us.  In 64 bits:
+// 1000 gated rows of 28672 458 us in fp32, without a gate 382 with norm and 224 plain; norms of gated rows 371 (4001 x 5120) and 296 (1000 x 17408).
 // What it took: more rows at a time on an SM (below); an error bound of the gate that looks at the values, so that fewer of them are worked out in 64 bits (1000
 // gated rows of 17408 57 and 52 us, 4001 of 5120 in fp16 53 and 38).
 // Tried: rows copied ahead into shared memory by blocks that stay (71 us for 47), four values looked at together for nearness to a half (no gain).
@@ -31,7 +34,7 @@ __device__ __forceinline__ void load4(const float *p, float (&v)[4]) {
     v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
 }
 
-constexpr int kMostFast = 24564;  // columns of a row that 512 threads hold in 12 vectors each, or 1024 in 6, wherever it begins
+constexpr int kMostFast = 24564;  // columns of a row that 512 threads hold in 12 vectors each, or 1024 in 6, wherever it begins; longer ones take 5 to 10 times as long per value
 constexpr float kUndefined = __builtin_nanf("");
 constexpr double kMostScale = 3.4028235677973366e38;  // half a step above fp32's largest: rounds to infinity from here on
 

@@ -14,7 +14,8 @@
 //
 // What bounds it: 64 sequences x 4 drafts x 151936 in fp32 take 142 us of one stream (2460 GB/s; three streams: 73.5 us a call, 4760 GB/s): 60 us are step 1, near
 // the copy bandwidth, the rest the exponentials in 64 bits of two rows (eight instructions of that pipe and some twenty others each: 45 cycles per 32 of them
-// and scheduler, whatever of loads, table or series is left out).  One sequence x 3 drafts: 28 us on 16 SMs, as many as a cluster takes.  Of that, half
+// and scheduler, whatever of loads, table or series is left out).  The same in fp16 114, greedy 38.5, drafts = 0 37; 75 and 149 sequences,
+// a block for each and half of the SMs or two rounds, 256 and 382.  One sequence x 3 drafts: 22 to 28 us on 16 SMs, as many as a cluster takes.  Of that, half
 // is the steps' latency: a vocabulary of 1000 takes 14 us.  Tried: 1024 threads, two blocks of 256 or 512 per SM (spills), a second round of
 // clusters, both rows' weights kept in shared memory between their two passes (no gain).
 #include <cuda_fp16.h>
