@@ -202,6 +202,49 @@ int vqm_qmm_i8(vqm_runtime *rt, const char *weight, const char *q, const char *s
 int vqm_verify(vqm_runtime *rt, const char *target, const char *draft, const char *tokens, const char *lens, const char *uniforms, const char *temperature,
                int vocab, int seqs, int drafts, const char *out, int *out_host);
 
+/* ---- Passes in 8-bit floating point (no counterpart in the reference) ----
+ * A weight tensor of e4m3 values (1 sign, 4 exponent, 3 mantissa bits, largest 448, no infinities) with one fp32 scale for each block of 128 rows by 128
+ * columns: W[r][k] = scales[r / 128][k / 128] * w[r][k], scales [ceil(rows / 128)][ceil(cols / 128)].  Activations are e4m3 rows with one fp32 scale for each
+ * 128 columns: q [ntok] rows round_up(cols, 16) bytes apart, scales [ceil(cols / 128)][round_up(ntok, 4)] - the scales of a block of columns lie side by
+ * side, row after row.  1 <= cols <= 1048576; rows and ntok are at most 2^30.  Buffers of 8-bit values are allocated or bound with elem = 1.  has / free /
+ * tensor_info (type VQM_F8_BLOCKS, row_bytes = pitch) / device_bytes know these tensors; the matvec entry points and qmm_i8 refuse them (VQM_ERR_VALUE).
+ *
+ * vqm_upload_f8   w: rows * cols bytes in host memory, densely packed; scales as above.  Synchronous; re-upload replaces.
+ * vqm_bind_f8     the same in device memory that the caller keeps and has filled (see vqm_bind_i8): 16-byte aligned, `pitch` bytes from row to row (0:
+ *                 round_up(cols, 16)); what lies behind a row's last column is ignored.  Not to replace a tensor while a graph is being captured.
+ * vqm_convert_f8  makes the tensor `name` from any GGUF tensor: a block's scale = its largest |w| / 448, values to the nearest.  Synchronous.
+ */
+#define VQM_F8_BLOCKS 128
+int vqm_upload_f8(vqm_runtime *rt, const char *name, const void *data, size_t nbytes, const float *scales, size_t scale_bytes, int cols, int rows);
+int vqm_bind_f8(vqm_runtime *rt, const char *name, const void *device_ptr, size_t pitch, const float *scales, int cols, int rows);
+int vqm_convert_f8(vqm_runtime *rt, const char *weight, const char *name);
+/* Activation rows in 8-bit floating point: as vqm_rows_i8 (the same v and n, flags and buffers), but for each 128 columns of a row
+ *   scale = max |n| / 448 in fp32, q = n / scale, in fp32, to the nearest e4m3 value, ties to even.
+ * Zeros have scale 0 and q = 0.  128 columns with an infinite or undefined n have an undefined (NaN) scale and q = 0, which makes their row's products
+ * undefined.  v and n are computed in fp32 (norms whose sum of squares is outside of fp32's middle range in 64 bits).  Zeros are written behind a row's last
+ * column, and what lies between the scales of the last row and the next block's is left as it is.  Asynchronous. */
+int vqm_rows_f8(vqm_runtime *rt, const char *x, const char *q, const char *scales, int cols, int ntok, int flags, const char *x2, const char *residual,
+                const char *total, const char *norm_weight, float eps);
+/* y[t][r] = sum over blocks b of 128 columns of scales[b][t] * W scales[r / 128][b] * sum_k q[t][k] w[r][k] (VQM_FUSE_ADD: +=).  Products are exact, a block's
+ * sum is fp32, as is the sum over the blocks, whose grouping depends on the sizes of the call; y is an fp32 or fp16 buffer; a call whose y overlaps q, the scales
+ * or the weights in device memory is refused (VQM_ERR_VALUE).  Asynchronous. */
+int vqm_qmm_f8(vqm_runtime *rt, const char *weight, const char *q, const char *scales, const char *y, int ntok, int flags);
+
+/* Log probabilities of given tokens (no counterpart in the reference): per row of logits [rows][vocab] (fp32 or fp16), with p = softmax(logits / T),
+ *   out [rows] (fp32) = log p(tokens[row]), tokens int32; a token that is masked or outside of [0, vocab) has -inf;
+ *   entropy [rows] (fp32, NULL: not wanted) = - sum p log p;
+ *   top_ids [rows][top] (int32) = the `top` largest logits' places, in descending order, of equal ones the lowest first, and top_out [rows][top] (fp32, NULL: not
+ *   wanted) their log probabilities; -1 and -inf where a row has fewer that are not masked.  0 <= top <= VQM_MAX_TOP.
+ * temperature [rows] (NULL: 1) as in vqm_verify: T <= 0 (or NaN): p is 1 at the row's largest logit, the lowest index on ties; T above 1e30 counts as
+ * infinite: all tokens that are not masked are equally likely.  Logits of -inf and NaN are masked; of a row's infinite logits each is equally likely and all others
+ * have none.  A row with nothing but masked logits has -inf, entropy 0 and ids -1.  Where a kernel of the runtime has given up a bounded wait that nobody has
+ * been told of yet, the logits may not be complete: out, entropy and top_out are NaN, ids -1.
+ * Sums are fp32 (rows with infinite, undefined or extreme values or temperatures: 64 bits).  A call whose outputs overlap one another or its inputs in
+ * device memory is refused (VQM_ERR_VALUE).  vocab <= VQM_MAX_VOCAB.  Asynchronous. */
+#define VQM_MAX_TOP 32
+int vqm_logprobs(vqm_runtime *rt, const char *logits, const char *tokens, const char *temperature, int vocab, int rows, int top, const char *out,
+                 const char *entropy, const char *top_ids, const char *top_out);
+
 /* set_gemm_min_rows(n) - qwen_runtime.cu:2324-2330: passes of n or more activation rows take the tensor-core GEMM
  * (fp16 operands, fp32 accumulation, like the reference's prompt kernel); 0 = never, every pass is fp32 matvecs. */
 int vqm_set_gemm_min_rows(vqm_runtime *rt, int n);

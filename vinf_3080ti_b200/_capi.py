@@ -67,6 +67,12 @@ SIGNATURES: dict[str, list] = {
     "vqm_rows_i8": [c_void_p, c_char_p, c_char_p, c_char_p, c_int, c_int, c_int, c_char_p, c_char_p, c_char_p, c_char_p, ctypes.c_float],
     "vqm_qmm_i8": [c_void_p, c_char_p, c_char_p, c_char_p, c_char_p, c_int, c_int],
     "vqm_verify": [c_void_p, c_char_p, c_char_p, c_char_p, c_char_p, c_char_p, c_char_p, c_int, c_int, c_int, c_char_p, POINTER(c_int)],
+    "vqm_upload_f8": [c_void_p, c_char_p, c_void_p, c_size_t, c_void_p, c_size_t, c_int, c_int],
+    "vqm_bind_f8": [c_void_p, c_char_p, c_void_p, c_size_t, c_void_p, c_int, c_int],
+    "vqm_convert_f8": [c_void_p, c_char_p, c_char_p],
+    "vqm_rows_f8": [c_void_p, c_char_p, c_char_p, c_char_p, c_int, c_int, c_int, c_char_p, c_char_p, c_char_p, c_char_p, ctypes.c_float],
+    "vqm_qmm_f8": [c_void_p, c_char_p, c_char_p, c_char_p, c_char_p, c_int, c_int],
+    "vqm_logprobs": [c_void_p, c_char_p, c_char_p, c_char_p, c_int, c_int, c_int, c_char_p, c_char_p, c_char_p, c_char_p],
     "vqm_set_gemm_min_rows": [c_void_p, c_int],
     "vqm_synchronize": [c_void_p],
     "vqm_mem_info": [POINTER(c_size_t), POINTER(c_size_t)],

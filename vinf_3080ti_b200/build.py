@@ -118,6 +118,9 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False, d
     work.append(("vqm_rows_i8.cu", [], OBJ / "rows_i8.o"))
     work.append(("vqm_qmm_i8.cu", [], OBJ / "qmm_i8.o"))
     work.append(("vqm_verify.cu", [], OBJ / "verify.o"))
+    work.append(("vqm_rows_f8.cu", [], OBJ / "rows_f8.o"))
+    work.append(("vqm_qmm_f8.cu", [], OBJ / "qmm_f8.o"))
+    work.append(("vqm_logprobs.cu", [], OBJ / "logprobs.o"))
     work.append(("vqm_probe.cu", [], OBJ / "probe.o"))
     work.append(("vqm_gemm.cu", [], OBJ / "gemm.o"))
     work.append(("vqm_gemm_tc5.cu", [], OBJ / "gemm_tc5.o"))

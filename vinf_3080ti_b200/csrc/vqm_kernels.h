@@ -260,6 +260,60 @@ cudaError_t launch_verify(const VerifyArgs &a, bool overlap, cudaStream_t stream
 // Beyond 32768 parts (16.7 million logits to a block) nothing is taken for sure.
 __host__ __device__ constexpr double verify_band(long long adds) { return adds > 32768 ? 2.0 : 1e-4 + 1.05 * 12.0 / (1 << 24) * static_cast<double>(adds); }
 
+// ---- Passes in 8-bit floating point (vqm_rows_f8.cu, vqm_qmm_f8.cu) and log probabilities (vqm_logprobs.cu) ----
+
+constexpr int kF8Blocks = 128;       // type id of a weight tensor of e4m3 values with a scale for each block of 128 x 128 (VQM_F8_BLOCKS)
+constexpr int kF8Block = 128;        // columns (and weight rows) that share a scale
+constexpr int kF8MaxCols = 1 << 20;
+constexpr int kF8MaxRows = 1 << 30;
+__host__ __device__ constexpr long long f8_pitch(int cols) { return (static_cast<long long>(cols) + 15) / 16 * 16; }  // bytes from one row of 8-bit values to the next
+__host__ __device__ constexpr int f8_blocks(int n) { return (n + kF8Block - 1) / kF8Block; }
+__host__ __device__ constexpr long long f8_scale_pitch(int ntok) { return (static_cast<long long>(ntok) + 3) / 4 * 4; }  // floats from the scales of one block of columns to those of the next
+
+struct RowsF8Args {
+    const void *x;         // [ntok][cols] of `elem` bytes
+    const void *x2;        // the values are silu(x) * x2; or null
+    const void *residual;  // the values are x + residual, and go to `total` as well (which may be either of them); or null
+    void *total;
+    const float *norm_w;   // rmsnorm over the columns times these; or null
+    uint8_t *q;            // [ntok][f8_pitch(cols)], zeros behind the last column
+    float *scales;         // [f8_blocks(cols)][f8_scale_pitch(ntok)]
+    int cols, ntok, elem;
+    float eps;
+};
+// overlap: see launch_attributes
+cudaError_t launch_rows_f8(const RowsF8Args &a, bool overlap, int sm_count, cudaStream_t stream);
+// e4m3 blocks of 128 x 128 and their scales from fp32 rows: w [rows][cols] -> q [rows][f8_pitch(cols)], scales [f8_blocks(rows)][f8_blocks(cols)]
+cudaError_t launch_blocks_f8(const float *w, uint8_t *q, float *scales, int rows, int cols, cudaStream_t stream);
+
+struct QmmF8Args {
+    const uint8_t *w;      // [rows][w_pitch], 16-byte aligned, w_pitch a multiple of 16
+    const float *w_scales; // [f8_blocks(rows)][f8_blocks(cols)]
+    const uint8_t *q;      // [ntok][f8_pitch(cols)]
+    const float *q_scales; // [f8_blocks(cols)][f8_scale_pitch(ntok)]
+    void *y;               // [ntok][rows] of y_elem bytes
+    long long w_pitch;
+    int rows, cols, ntok, y_elem;
+    bool add;              // y += instead of y =
+    bool overlap;          // see launch_attributes
+    unsigned *status;      // device word that receives a code if a bounded wait expires
+};
+cudaError_t launch_qmm_f8(const QmmF8Args &a, cudaStream_t stream);
+
+constexpr int kMaxTop = 32;  // alternatives of a row (VQM_MAX_TOP)
+struct LogprobsArgs {
+    const void *logits;        // [rows][vocab] of `elem` bytes
+    const int *tokens;         // [rows]
+    const float *temperature;  // [rows]; or null: 1
+    float *out, *entropy;      // [rows]; entropy may be null
+    int *top_ids;              // [rows][top]
+    float *top_out;            // [rows][top]; or null
+    const unsigned *status;    // device word with the code of a wait that has expired: the logits may not be what they should
+    int vocab, rows, top, elem;
+};
+// overlap: see launch_attributes
+cudaError_t launch_logprobs(const LogprobsArgs &a, bool overlap, int sm_count, cudaStream_t stream);
+
 cudaError_t launch_argmax_rows(const float *x, int n, int ntok, int *out, cudaStream_t stream);
 cudaError_t launch_dequant(int type, const uint8_t *w, float *out, long long numel, const uint8_t *codebook,
                            cudaStream_t stream);

@@ -85,7 +85,7 @@ static PyObject *py_rows_i8(PyObject *self, PyObject *const *args, Py_ssize_t n)
     void *fn, *handle;
     const char *name[7];
     int whole[3], status;
-    if (begin(args, n, 13, "rows_i8", &fn, &handle) < 0) return NULL;
+    if (begin(args, n, 13, "a call for 8-bit rows", &fn, &handle) < 0) return NULL;
     for (int i = 0; i < 3; ++i)
         if (name_of(args[2 + i], 0, &name[i]) < 0 || int_of(args[5 + i], &whole[i]) < 0) return NULL;
     for (int i = 0; i < 4; ++i)
@@ -106,7 +106,7 @@ static PyObject *py_qmm_i8(PyObject *self, PyObject *const *args, Py_ssize_t n) 
     void *fn, *handle;
     const char *name[4];
     int whole[2], status;
-    if (begin(args, n, 8, "qmm_i8", &fn, &handle) < 0) return NULL;
+    if (begin(args, n, 8, "a product of 8-bit rows", &fn, &handle) < 0) return NULL;
     for (int i = 0; i < 4; ++i)
         if (name_of(args[2 + i], 0, &name[i]) < 0) return NULL;
     for (int i = 0; i < 2; ++i)
@@ -139,7 +139,31 @@ static PyObject *py_verify(PyObject *self, PyObject *const *args, Py_ssize_t n) 
     return PyLong_FromLong(status);
 }
 
+typedef int (*logprobs_fn)(void *, const char *, const char *, const char *, int, int, int, const char *, const char *, const char *, const char *);
+
+/* logprobs(address, handle, logits, tokens, temperature, vocab, rows, top, out, entropy, top_ids, top_out) */
+static PyObject *py_logprobs(PyObject *self, PyObject *const *args, Py_ssize_t n) {
+    (void)self;
+    void *fn, *handle;
+    const char *name[7];
+    int whole[3], status;
+    if (begin(args, n, 12, "logprobs", &fn, &handle) < 0) return NULL;
+    for (int i = 0; i < 3; ++i)
+        if (name_of(args[2 + i], i == 2, &name[i]) < 0 || int_of(args[5 + i], &whole[i]) < 0) return NULL;
+    for (int i = 0; i < 4; ++i)
+        if (name_of(args[8 + i], i > 0, &name[3 + i]) < 0) return NULL;
+    Py_BEGIN_ALLOW_THREADS
+    status = ((logprobs_fn)fn)(handle, name[0], name[1], name[2], whole[0], whole[1], whole[2], name[3], name[4], name[5], name[6]);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(status);
+}
+
+/* (calls of 8-bit floating point take what those of 8-bit integers take) */
 #define METHOD(name, text) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, text}
-static PyMethodDef methods[] = {METHOD(qmv, "vqm_qmv"), METHOD(rows_i8, "vqm_rows_i8"), METHOD(qmm_i8, "vqm_qmm_i8"), METHOD(verify, "vqm_verify"), {NULL, NULL, 0, NULL}};
+static PyMethodDef methods[] = {METHOD(qmv, "vqm_qmv"), METHOD(rows_i8, "vqm_rows_i8"), METHOD(qmm_i8, "vqm_qmm_i8"), METHOD(verify, "vqm_verify"),
+                                {"rows_f8", (PyCFunction)(void (*)(void))py_rows_i8, METH_FASTCALL, "vqm_rows_f8"},
+                                {"qmm_f8", (PyCFunction)(void (*)(void))py_qmm_i8, METH_FASTCALL, "vqm_qmm_f8"},
+                                METHOD(logprobs, "vqm_logprobs"),
+                                {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_vqm_pycall", NULL, -1, methods, NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit__vqm_pycall(void) { return PyModule_Create(&module); }

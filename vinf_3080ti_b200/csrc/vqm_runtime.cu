@@ -55,7 +55,7 @@ struct Tensor {
     bool owned = true;
     bool mapped = false;
     CUtensorMap maps[8];  // of the tensor-core matvec, if `mapped`
-    const float *scales = nullptr;  // of 8-bit integer rows (kI8Rows), else null
+    const float *scales = nullptr;  // of 8-bit integer rows (kI8Rows) or 8-bit floating point (kF8Blocks), else null
 };
 
 struct Buffer {
@@ -180,13 +180,26 @@ Tensor *find_tensor(vqm_runtime *rt, const char *name, int *status) {
         *status = fail(VQM_ERR_VALUE, "weight tensor %s holds 8-bit integer rows (qmm_i8 multiplies by those)", name);
         return nullptr;
     }
+    if (t != nullptr && t->type == vqm::kF8Blocks) {
+        *status = fail(VQM_ERR_VALUE, "weight tensor %s holds 8-bit floating point (qmm_f8 multiplies by that)", name);
+        return nullptr;
+    }
     return t;
 }
 // ... and one of 8-bit integer rows.
 Tensor *find_i8_tensor(vqm_runtime *rt, const char *name, int *status) {
     Tensor *t = find_any_tensor(rt, name, status);
     if (t != nullptr && t->type != vqm::kI8Rows) {
-        *status = fail(VQM_ERR_VALUE, "weight tensor %s holds GGUF blocks, not 8-bit integer rows (convert_i8 makes those)", name);
+        *status = fail(VQM_ERR_VALUE, "weight tensor %s holds %s, not 8-bit integer rows (convert_i8 makes those)", name, t->type == vqm::kF8Blocks ? "8-bit floating point" : "GGUF blocks");
+        return nullptr;
+    }
+    return t;
+}
+// ... and one of 8-bit floating point.
+Tensor *find_f8_tensor(vqm_runtime *rt, const char *name, int *status) {
+    Tensor *t = find_any_tensor(rt, name, status);
+    if (t != nullptr && t->type != vqm::kF8Blocks) {
+        *status = fail(VQM_ERR_VALUE, "weight tensor %s holds %s, not 8-bit floating point (convert_f8 makes that)", name, t->type == vqm::kI8Rows ? "8-bit integer rows" : "GGUF blocks");
         return nullptr;
     }
     return t;
@@ -1409,6 +1422,7 @@ int vqm_matvec(vqm_runtime *rt, const char *weight, const float *x_host, size_t 
     if (it == rt->tensors.end()) return fail(VQM_ERR_KEY, "%s is not resident on the GPU", weight);
     Tensor &t = it->second;
     if (t.type == vqm::kI8Rows) return fail(VQM_ERR_VALUE, "weight tensor %s holds 8-bit integer rows (qmm_i8 multiplies by those)", weight);
+    if (t.type == vqm::kF8Blocks) return fail(VQM_ERR_VALUE, "weight tensor %s holds 8-bit floating point (qmm_f8 multiplies by that)", weight);
     if (x_bytes != static_cast<size_t>(t.cols) * sizeof(float))
         return fail(VQM_ERR_VALUE, "%s: x has %zu bytes, expected %d float32", weight, x_bytes, t.cols);
     if (y_bytes < static_cast<size_t>(t.rows) * sizeof(float))
@@ -1480,7 +1494,7 @@ int vqm_dequantize(vqm_runtime *rt, const char *weight, const char *out) {
 }
 
 }  // extern "C"
-// ---- 8-bit integer passes and the verification of drafted tokens ---------------------------------------------
+// ---- 8-bit passes, the verification of drafted tokens, log probabilities ---------------------------------------------
 
 namespace {
 
@@ -1540,6 +1554,31 @@ cudaError_t alloc_i8(Tensor &t, int cols, int rows) {
     t.cols = cols;
     t.row_bytes = pitch;
     t.nbytes = values + sizeof(float) * static_cast<size_t>(rows);
+    return cudaSuccess;
+}
+
+int check_f8_shape(const char *name, int cols, int rows) {
+    if (cols < 1 || rows < 1) return fail(VQM_ERR_VALUE, "%s: rows and columns must be positive", name);
+    if (cols > vqm::kF8MaxCols || rows > vqm::kF8MaxRows) return fail(VQM_ERR_VALUE, "%s: at most %d columns and %d rows", name, vqm::kF8MaxCols, vqm::kF8MaxRows);
+    return VQM_OK;
+}
+size_t f8_scale_count(int cols, int rows) { return static_cast<size_t>(vqm::f8_blocks(rows)) * static_cast<size_t>(vqm::f8_blocks(cols)); }
+
+// Rows of f8_pitch(cols) bytes, and behind them the scales of the blocks.
+cudaError_t alloc_f8(Tensor &t, int cols, int rows) {
+    const size_t pitch = static_cast<size_t>(vqm::f8_pitch(cols)), values = pitch * static_cast<size_t>(rows), at = (values + 255) / 256 * 256;
+    const size_t scales = sizeof(float) * f8_scale_count(cols, rows);
+    const cudaError_t err = cudaMalloc(&t.data, at + scales);
+    if (err != cudaSuccess) {
+        t.data = nullptr;
+        return err;
+    }
+    t.scales = reinterpret_cast<const float *>(t.data + at);
+    t.type = vqm::kF8Blocks;
+    t.rows = rows;
+    t.cols = cols;
+    t.row_bytes = pitch;
+    t.nbytes = values + scales;
     return cudaSuccess;
 }
 
@@ -1768,6 +1807,208 @@ int vqm_verify(vqm_runtime *rt, const char *target, const char *draft, const cha
             for (size_t i = 0; i < s; ++i)
                 if (out_host[i * (k + 2)] < 0) return (rc = check_status_word(rt, "verify")) != VQM_OK ? rc : fail(VQM_ERR_CUDA, "verify failed: its logits are not complete");
         }
+        return VQM_OK;
+    });
+}
+
+int vqm_upload_f8(vqm_runtime *rt, const char *name, const void *data, size_t nbytes, const float *scales, size_t scale_bytes, int cols, int rows) {
+    return entry(rt, {name}, [&]() -> int {
+        int rc = check_f8_shape(name, cols, rows);
+        if (rc != VQM_OK) return rc;
+        const size_t want = static_cast<size_t>(cols) * rows, want_scales = sizeof(float) * f8_scale_count(cols, rows);
+        if (data == nullptr || nbytes != want) return fail(VQM_ERR_VALUE, "%s: got %zu bytes, expected %zu", name, data == nullptr ? size_t{0} : nbytes, want);
+        if (scales == nullptr || scale_bytes != want_scales)
+            return fail(VQM_ERR_VALUE, "%s: got %zu bytes of scales, expected %zu", name, scales == nullptr ? size_t{0} : scale_bytes, want_scales);
+        if ((rc = no_capture(rt, "upload_f8")) != VQM_OK) return rc;
+        Tensor t;
+        cudaError_t err = alloc_f8(t, cols, rows);
+        if (err == cudaSuccess && t.row_bytes != static_cast<size_t>(cols)) err = cudaMemset(t.data, 0, t.row_bytes * rows);
+        if (err == cudaSuccess) err = cudaMemcpy2D(t.data, t.row_bytes, data, cols, cols, rows, cudaMemcpyHostToDevice);
+        if (err == cudaSuccess) err = cudaMemcpy(const_cast<float *>(t.scales), scales, scale_bytes, cudaMemcpyHostToDevice);
+        if (err == cudaSuccess) err = cudaStreamSynchronize(nullptr);  // (a copy from pageable memory may return while its last part is on its way)
+        if (err != cudaSuccess) {
+            release(t);
+            return cuda_fail("upload_f8", err);
+        }
+        put_tensor(rt, name, t);
+        return VQM_OK;
+    });
+}
+
+int vqm_bind_f8(vqm_runtime *rt, const char *name, const void *device_ptr, size_t pitch, const float *scales, int cols, int rows) {
+    return entry(rt, {name}, [&]() -> int {
+        int rc = check_f8_shape(name, cols, rows);
+        if (rc != VQM_OK) return rc;
+        if (device_ptr == nullptr || (reinterpret_cast<uintptr_t>(device_ptr) & 15u) != 0)
+            return fail(VQM_ERR_VALUE, "%s: device pointer must be 16-byte aligned", name);
+        if (scales == nullptr || (reinterpret_cast<uintptr_t>(scales) & 3u) != 0)
+            return fail(VQM_ERR_VALUE, "%s: the scales' device pointer must be 4-byte aligned", name);
+        if (pitch == 0) pitch = static_cast<size_t>(vqm::f8_pitch(cols));
+        if (pitch % 16 != 0 || pitch < static_cast<size_t>(cols) || pitch >= (static_cast<size_t>(1) << 40) || pitch > (static_cast<size_t>(1) << 62) / static_cast<size_t>(rows))
+            return fail(VQM_ERR_VALUE, "%s: the rows' pitch must be a multiple of 16 bytes and no less than the columns", name);
+        // (a new name is only noted; for another tensor of that name the stream is waited for, and its memory freed)
+        if (rt->tensors.count(name) != 0 && (rc = no_capture(rt, "to replace a tensor")) != VQM_OK) return rc;
+        Tensor t;
+        t.data = const_cast<uint8_t *>(static_cast<const uint8_t *>(device_ptr));
+        t.owned = false;
+        t.scales = scales;
+        t.type = vqm::kF8Blocks;
+        t.rows = rows;
+        t.cols = cols;
+        t.row_bytes = pitch;
+        t.nbytes = pitch * static_cast<size_t>(rows) + sizeof(float) * f8_scale_count(cols, rows);
+        put_tensor(rt, name, t);
+        return VQM_OK;
+    });
+}
+
+int vqm_convert_f8(vqm_runtime *rt, const char *weight, const char *name) {
+    return entry(rt, {weight, name}, [&]() -> int {
+        int rc = VQM_OK;
+        Tensor *from = find_tensor(rt, weight, &rc);
+        if (from == nullptr) return rc;
+        if ((rc = check_f8_shape(weight, from->cols, from->rows)) != VQM_OK) return rc;
+        const size_t numel = static_cast<size_t>(from->rows) * from->cols;
+        if (numel % 8 != 0) return fail(VQM_ERR_VALUE, "%s: element count must be a multiple of 8", weight);
+        const uint8_t *cb = codebook_for(rt, from->type);
+        if (vqm::grid_is_codebook(from->type) && cb == nullptr)
+            return fail(VQM_ERR_VALUE, "the codebook for GGUF type %d has not been set (vqm_set_codebook)", from->type);
+        if ((rc = no_capture(rt, "convert_f8")) != VQM_OK) return rc;
+        // a part of the rows at a time, a multiple of 128 of them, in 64 MB or so of fp32
+        size_t part = (static_cast<size_t>(1) << 24) / from->cols / vqm::kF8Block * vqm::kF8Block;
+        if (part < vqm::kF8Block) part = vqm::kF8Block;
+        if (part > static_cast<size_t>(from->rows)) part = from->rows;
+        Tensor t;
+        float *values = nullptr;
+        cudaError_t err = alloc_f8(t, from->cols, from->rows);
+        if (err == cudaSuccess) err = cudaMalloc(&values, sizeof(float) * part * from->cols);
+        for (size_t r = 0; r < static_cast<size_t>(from->rows) && err == cudaSuccess; r += part) {
+            const size_t n = part < from->rows - r ? part : from->rows - r;
+            err = vqm::launch_dequant(from->type, from->data + r * from->row_bytes, values, static_cast<long long>(n * from->cols), cb, rt->stream);
+            if (err == cudaSuccess)
+                err = vqm::launch_blocks_f8(values, t.data + r * t.row_bytes, const_cast<float *>(t.scales) + r / vqm::kF8Block * vqm::f8_blocks(from->cols), static_cast<int>(n), from->cols, rt->stream);
+            if (err == cudaSuccess) count_launch(rt, 2);
+        }
+        const cudaError_t done = cudaStreamSynchronize(rt->stream);  // (products fetch weights ahead of the stream's order)
+        if (err == cudaSuccess) err = done;
+        cudaFree(values);
+        if (err != cudaSuccess) {
+            release(t);
+            return cuda_fail("convert_f8", err);
+        }
+        put_tensor(rt, name, t);
+        return VQM_OK;
+    });
+}
+
+int vqm_rows_f8(vqm_runtime *rt, const char *x, const char *q, const char *scales, int cols, int ntok, int flags, const char *x2, const char *residual,
+                const char *total, const char *norm_weight, float eps) {
+    return entry(rt, {x, q, scales}, [&]() -> int {
+        if (ntok < 1 || ntok > vqm::kF8MaxRows) return fail(VQM_ERR_VALUE, "ntok must be in [1, %d]", vqm::kF8MaxRows);
+        if (cols < 1 || cols > vqm::kF8MaxCols) return fail(VQM_ERR_VALUE, "cols must be in [1, %d]", vqm::kF8MaxCols);
+        if ((flags & ~(VQM_FUSE_ADD | VQM_FUSE_NORM | VQM_FUSE_SILU_MUL)) != 0) return fail(VQM_ERR_VALUE, "unknown flag bits %d", flags);
+        if ((flags & VQM_FUSE_ADD) && (flags & VQM_FUSE_SILU_MUL)) return fail(VQM_ERR_VALUE, "a residual is added to x itself, not to silu(x) * x2");
+        const size_t n = static_cast<size_t>(ntok) * cols, n_scales = static_cast<size_t>(vqm::f8_blocks(cols)) * static_cast<size_t>(vqm::f8_scale_pitch(ntok));
+        int rc = VQM_OK;
+        vqm::RowsF8Args a{};
+        a.cols = cols;
+        a.ntok = ntok;
+        a.eps = eps;
+        if ((a.x = find_real(rt, x, n, &a.elem, &rc)) == nullptr) return rc;
+        if ((a.q = reinterpret_cast<uint8_t *>(find_i8(rt, q, static_cast<size_t>(vqm::f8_pitch(cols)) * ntok, &rc))) == nullptr) return rc;
+        if ((a.scales = find_f32(rt, scales, n_scales, &rc)) == nullptr) return rc;
+        if (flags & VQM_FUSE_SILU_MUL) {
+            if (x2 == nullptr) return fail(VQM_ERR_VALUE, "VQM_FUSE_SILU_MUL needs x2");
+            if ((a.x2 = find_real(rt, x2, n, &a.elem, &rc)) == nullptr) return rc;
+        }
+        if (flags & VQM_FUSE_ADD) {
+            if (residual == nullptr) return fail(VQM_ERR_VALUE, "VQM_FUSE_ADD needs the residual");
+            if ((a.residual = find_real(rt, residual, n, &a.elem, &rc)) == nullptr) return rc;
+            if ((a.total = find_real(rt, total != nullptr ? total : residual, n, &a.elem, &rc)) == nullptr) return rc;
+        } else if (total != nullptr) {
+            return fail(VQM_ERR_VALUE, "a buffer for the sums without VQM_FUSE_ADD");
+        }
+        if (flags & VQM_FUSE_NORM) {
+            if (norm_weight == nullptr) return fail(VQM_ERR_VALUE, "VQM_FUSE_NORM needs norm_weight");
+            if ((a.norm_w = find_norm(rt, norm_weight, cols, &rc)) == nullptr) return rc;
+            if (!(eps >= 0.0f)) return fail(VQM_ERR_VALUE, "eps must be >= 0");
+        }
+        const size_t bytes = n * static_cast<size_t>(a.elem);
+        const vqm::Extent ex{a.x, bytes}, ex2{a.x2, bytes}, er{a.residual, bytes}, et{a.total, bytes}, eg{a.norm_w, sizeof(float) * static_cast<size_t>(cols)};
+        const vqm::Extent es{a.scales, sizeof(float) * n_scales}, eq{a.q, static_cast<size_t>(vqm::f8_pitch(cols)) * ntok};
+        if ((rc = check_apart("the scales", es, {ex, ex2, er, et, eg})) != VQM_OK) return rc;
+        if ((rc = check_apart("the 8-bit rows", eq, {ex, ex2, er, et, eg, es})) != VQM_OK) return rc;
+        // (sums may lie where x or the residual does, value for value)
+        if ((rc = check_apart("the sums", et, {a.total == a.x ? vqm::kNoExtent : ex, a.total == a.residual ? vqm::kNoExtent : er, eg})) != VQM_OK) return rc;
+        const cudaError_t err = vqm::launch_rows_f8(a, rt->overlap_launch != 0, rt->sm_count, rt->stream);
+        if (err != cudaSuccess) return cuda_fail("rows_f8 launch", err);
+        count_launch(rt);
+        return VQM_OK;
+    });
+}
+
+int vqm_qmm_f8(vqm_runtime *rt, const char *weight, const char *q, const char *scales, const char *y, int ntok, int flags) {
+    return entry(rt, {weight, q, scales, y}, [&]() -> int {
+        if (ntok < 1 || ntok > vqm::kF8MaxRows) return fail(VQM_ERR_VALUE, "ntok must be in [1, %d]", vqm::kF8MaxRows);
+        if ((flags & ~VQM_FUSE_ADD) != 0) return fail(VQM_ERR_VALUE, "unknown flag bits %d", flags);
+        int rc = VQM_OK;
+        Tensor *t = find_f8_tensor(rt, weight, &rc);
+        if (t == nullptr) return rc;
+        const size_t rows = static_cast<size_t>(t->rows), tok = static_cast<size_t>(ntok), q_bytes = static_cast<size_t>(vqm::f8_pitch(t->cols)) * tok;
+        const size_t n_scales = static_cast<size_t>(vqm::f8_blocks(t->cols)) * static_cast<size_t>(vqm::f8_scale_pitch(ntok));
+        vqm::QmmF8Args a{};
+        if ((a.q = reinterpret_cast<uint8_t *>(find_i8(rt, q, q_bytes, &rc))) == nullptr) return rc;
+        if ((a.q_scales = find_f32(rt, scales, n_scales, &rc)) == nullptr) return rc;
+        if ((a.y = find_real(rt, y, rows * tok, &a.y_elem, &rc)) == nullptr) return rc;
+        const vqm::Extent w{t->data, (rows - 1) * t->row_bytes + static_cast<size_t>(t->cols)}, ws{t->scales, sizeof(float) * f8_scale_count(t->cols, t->rows)};
+        const vqm::Extent eq{a.q, q_bytes}, es{a.q_scales, sizeof(float) * n_scales};
+        if ((rc = check_apart("the outputs", vqm::Extent{a.y, rows * tok * static_cast<size_t>(a.y_elem)}, {eq, es, w, ws})) != VQM_OK) return rc;
+        a.w = t->data;
+        a.w_scales = t->scales;
+        a.w_pitch = static_cast<long long>(t->row_bytes);
+        a.rows = t->rows;
+        a.cols = t->cols;
+        a.ntok = ntok;
+        a.add = (flags & VQM_FUSE_ADD) != 0;
+        a.overlap = rt->overlap_launch != 0;
+        a.status = rt->status;
+        const cudaError_t err = vqm::launch_qmm_f8(a, rt->stream);
+        if (err != cudaSuccess) return cuda_fail("qmm_f8 launch", err);
+        count_launch(rt);
+        return VQM_OK;
+    });
+}
+
+int vqm_logprobs(vqm_runtime *rt, const char *logits, const char *tokens, const char *temperature, int vocab, int rows, int top, const char *out,
+                 const char *entropy, const char *top_ids, const char *top_out) {
+    return entry(rt, {logits, tokens, out}, [&]() -> int {
+        if (vocab < 1 || vocab > VQM_MAX_VOCAB || rows < 1) return fail(VQM_ERR_VALUE, "vocab must be in [1, %d], the number of rows positive", VQM_MAX_VOCAB);
+        if (top < 0 || top > VQM_MAX_TOP) return fail(VQM_ERR_VALUE, "top must be in [0, %d]", VQM_MAX_TOP);
+        if (top > 0 && top_ids == nullptr) return fail(VQM_ERR_VALUE, "alternatives without a buffer for their ids");
+        if (top == 0 && (top_ids != nullptr || top_out != nullptr)) return fail(VQM_ERR_VALUE, "buffers for alternatives, but top is 0");
+        const size_t n = static_cast<size_t>(rows), k = static_cast<size_t>(top);
+        int rc = VQM_OK, word = 4;
+        vqm::LogprobsArgs a{};
+        a.vocab = vocab;
+        a.rows = rows;
+        a.top = top;
+        if ((a.logits = find_real(rt, logits, n * static_cast<size_t>(vocab), &a.elem, &rc)) == nullptr) return rc;
+        if ((a.tokens = static_cast<const int *>(find_real(rt, tokens, n, &word, &rc))) == nullptr) return rc;
+        if (temperature != nullptr && (a.temperature = find_f32(rt, temperature, n, &rc)) == nullptr) return rc;
+        if ((a.out = find_f32(rt, out, n, &rc)) == nullptr) return rc;
+        if (entropy != nullptr && (a.entropy = find_f32(rt, entropy, n, &rc)) == nullptr) return rc;
+        if (top > 0 && (a.top_ids = static_cast<int *>(find_real(rt, top_ids, n * k, &word, &rc))) == nullptr) return rc;
+        if (top_out != nullptr && (a.top_out = find_f32(rt, top_out, n * k, &rc)) == nullptr) return rc;
+        const vqm::Extent el{a.logits, n * static_cast<size_t>(vocab) * static_cast<size_t>(a.elem)}, ek{a.tokens, 4 * n}, et{a.temperature, 4 * n};
+        const vqm::Extent eo{a.out, 4 * n}, ee{a.entropy, 4 * n}, ei{a.top_ids, 4 * n * k}, ev{a.top_out, 4 * n * k};
+        if ((rc = check_apart("the log probabilities", eo, {el, ek, et, ee, ei, ev})) != VQM_OK) return rc;
+        if ((rc = check_apart("the entropies", ee, {el, ek, et, ei, ev})) != VQM_OK) return rc;
+        if ((rc = check_apart("the alternatives", ei, {el, ek, et, ev})) != VQM_OK) return rc;
+        if ((rc = check_apart("the alternatives' log probabilities", ev, {el, ek, et})) != VQM_OK) return rc;
+        a.status = rt->status;
+        const cudaError_t err = vqm::launch_logprobs(a, rt->overlap_launch != 0, rt->sm_count, rt->stream);
+        if (err != cudaSuccess) return cuda_fail("logprobs launch", err);
+        count_launch(rt);
         return VQM_OK;
     });
 }

@@ -21,6 +21,7 @@ from . import _capi
 from .gguf_types import CODEBOOK_BYTES
 
 MAX_DRAFTS = 255  # of a sequence, in one verification
+MAX_TOP = 32  # alternatives of a row's log probabilities
 MAX_ARGMAX_ROWS = 256  # engine/csrc/megakernel/qwen_runtime.cu:573
 
 
@@ -325,6 +326,46 @@ class Runtime:
             return None
         rows = [list(host[i * (drafts + 2):(i + 1) * (drafts + 2)]) for i in range(seqs)]
         return [row[1:row[0] + 2] for row in rows]
+
+    # ---- passes in 8-bit floating point, log probabilities (no reference counterpart; see include/vinf_b200.h) -------------------
+    def upload_f8(self, name: str, data, scales, cols: int, rows: int) -> None:
+        """A weight tensor of e4m3 values: rows * cols bytes, densely packed, and one fp32 scale for each block of 128 rows by 128 columns."""
+        keep, addr, n = _ptr(data)
+        keep_scales, scale_addr, scale_n = _ptr(scales)
+        _capi.check(self._lib.vqm_upload_f8(self._h, _name(name), addr, n, scale_addr, scale_n, int(cols), int(rows)))
+
+    def bind_f8(self, name: str, device_ptr: int, scales_ptr: int, cols: int, rows: int, pitch: int = 0) -> None:
+        """The same in device memory (not freed by the runtime); rows `pitch` bytes apart, 0: cols rounded up to 16."""
+        if pitch < 0:
+            raise ValueError("pitch must not be negative")
+        _capi.check(self._lib.vqm_bind_f8(self._h, _name(name), ctypes.c_void_p(device_ptr), int(pitch), ctypes.c_void_p(scales_ptr), int(cols), int(rows)))
+
+    def convert_f8(self, weight: str, name: str) -> None:
+        """Makes the e4m3 tensor `name` from the GGUF tensor `weight`, a scale for each block of 128 x 128."""
+        _capi.check(self._lib.vqm_convert_f8(self._h, _name(weight), _name(name)))
+
+    def rows_f8(self, x: str, q: str, scales: str, cols: int, ntok: int = 1, *, residual: str | None = None, total: str | None = None,
+                norm: str | None = None, eps: float = 1e-6, silu_mul: str | None = None) -> None:
+        """Activation rows as e4m3 `q` with a scale for each 128 columns (scales: ceil(cols / 128) times ntok rounded up to 4), after the residual's addition
+        (the sum goes to `total`, or back to `residual`) or silu(x) * silu_mul, and the rms norm with the weights `norm`, where given.  Asynchronous."""
+        flags = (1 if residual is not None else 0) | (2 if norm is not None else 0) | (8 if silu_mul is not None else 0)
+        status = _capi.caller("rows_f8")(self._h.value, x, q, scales, cols, ntok, flags, silu_mul, residual, total, norm, eps)
+        if status:
+            _capi.check(status)
+
+    def qmm_f8(self, weight: str, q: str, scales: str, y: str, ntok: int = 1, *, add: bool = False) -> None:
+        """y (+)= W x for a tensor of e4m3 values and activations from rows_f8.  Asynchronous."""
+        status = _capi.caller("qmm_f8")(self._h.value, weight, q, scales, y, ntok, 1 if add else 0)
+        if status:
+            _capi.check(status)
+
+    def logprobs(self, logits: str, tokens: str, vocab: int, rows: int = 1, *, out: str, entropy: str | None = None, top: int = 0, top_ids: str | None = None,
+                 top_out: str | None = None, temperature: str | None = None) -> None:
+        """Log probabilities of `tokens`, one per row of logits, into `out`; entropies, and the `top` likeliest tokens with their log probabilities, where
+        buffers for them are given.  Asynchronous."""
+        status = _capi.caller("logprobs")(self._h.value, logits, tokens, temperature, vocab, rows, top, out, entropy, top_ids, top_out)
+        if status:
+            _capi.check(status)
 
     def set_gemm_min_rows(self, n: int) -> None:
         _capi.check(self._lib.vqm_set_gemm_min_rows(self._h, int(n)))
