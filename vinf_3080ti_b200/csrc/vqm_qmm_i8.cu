@@ -26,12 +26,12 @@
 #include <cuda_fp16.h>
 
 #include "vqm_kernels.h"
-#include "vqm_tcmv.cuh"
+#include "vqm_tiles8.cuh"
 
 namespace vqm {
 namespace {
 
-constexpr int kQRows = 128, kQCols = 128;           // weight rows of a block's tile, columns of a stage
+constexpr int kQRows = 128;                         // weight rows of a block's tile
 constexpr int kQA = kQRows * kQCols;                // bytes of a stage's weights
 constexpr int kQMaxN = 256, kQMaxStages = 12, kQMaxSplit = 8;
 // Shared memory of the stages.  Blocks of few activation rows, which wait for memory, take half an SM: those of the next launch are there already, with
@@ -53,42 +53,6 @@ struct QmmTc {
     int half_sm;                       // two blocks per SM
 };
 
-using tc::bar_arrive, tc::bar_init, tc::bar_try, tc::bar_try_cluster, tc::in_block, tc::s32;
-
-// Bounded; false once this or another wait of the block has given up.  A wait that succeeds looks at nothing but its barrier: the loops below have some
-// 500 cycles per stage.
-template <bool CLUSTER>
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *failed) {
-    unsigned long long began = 0;
-#pragma unroll 1
-    for (uint32_t i = 1;; ++i) {
-        if (CLUSTER ? bar_try_cluster(bar, parity) : bar_try(bar, parity)) return true;
-        if ((i & 255u) == 0 && tc::give_up(&began, failed)) return false;
-    }
-}
-// The same by one lane for its warp.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *failed) {
-    int ok = 1;
-    if ((threadIdx.x & 31) == 0) ok = wait<false>(bar, parity, failed) ? 1 : 0;
-    __syncwarp();
-    return __shfl_sync(0xFFFFFFFFu, ok, 0) != 0;
-}
-
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {  // K-major, 128-byte swizzle, groups of 8 rows 1024 bytes apart
-    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ void copy_tile(uint32_t to, const CUtensorMap *map, int x, int row, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to), "l"(map), "r"(x), "r"(row), "r"(bar)
-                 : "memory");
-}
-__device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void arrive_in(uint32_t cluster_addr) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory"); }
-__device__ __forceinline__ void cluster_sync() {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 template <bool PAIR>
 __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     if constexpr (PAIR)
@@ -97,16 +61,6 @@ __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint3
     else
         asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
                      : "memory");
-}
-// Arrives on the barrier (in both blocks of pair `pair`) once the MMAs issued so far are done.
-template <bool PAIR>
-__device__ __forceinline__ void commit(uint32_t bar, uint32_t pair) {
-    if constexpr (PAIR) {
-        const uint16_t both = static_cast<uint16_t>(3u << (2 * pair));
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(both) : "memory");
-    } else {
-        tc::commit(bar);
-    }
 }
 template <int N>
 __device__ __forceinline__ void load_sums(uint32_t at, int (&v)[N]) {
@@ -399,18 +353,6 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
         else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
         if (lane == 0 && s_failed) atomicExch(a.status, kStatusWaitExpired);
     }
-}
-
-// 8-bit rows as a 2-D tensor; a tile is 128 columns of `box_rows` rows.  Columns and rows beyond the last arrive as zeros.
-cudaError_t encode_rows(CUtensorMap *map, const int8_t *rows_at, int cols, long long pitch, int rows, int box_rows) {
-    TcEncode encode = nullptr;
-    if (const cudaError_t err = tc_encoder(&encode); err != cudaSuccess) return err;
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(pitch)};
-    const cuuint32_t box[2] = {kQCols, static_cast<cuuint32_t>(box_rows)}, elem[2] = {1, 1};
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(rows_at), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
-               ? cudaSuccess
-               : cudaErrorInvalidValue;
 }
 
 template <bool PAIR, bool SPLIT>
