@@ -321,6 +321,17 @@ def test_product_on_shapes_of_models(rt, rows, cols, ntok):
 
 
 @pytest.mark.parametrize("kind", [np.float32, np.float16])
+@pytest.mark.parametrize("rows,cols,ntok", [(40000, 200, 3), (40000, 200, 17), (40000, 200, 40), (40000, 200, 100), (30001, 136, 120), (40000, 200, 300), (20000, 130, 700), (20004, 300, 130)])
+def test_product_of_more_tiles_than_fit_at_once(rt, rows, cols, ntok, kind):
+    """Blocks take several tiles, one after the other; a tile's outputs are still on their way when the next one's are made."""
+    rng = np.random.default_rng(rows + ntok)
+    w, ws, q, qs = make(rng, rows, cols, ntok, whole=True)
+    ws[:] = 1.0
+    qs[:] = 1.0 / 16
+    check_product(rt, w, ws, q, qs, kind=kind, whole=True)
+
+
+@pytest.mark.parametrize("kind", [np.float32, np.float16])
 @pytest.mark.parametrize("rows,cols,ntok", [(1, 1, 1), (257, 300, 4), (1000, 2000, 33), (300, 5120, 1), (129, 129, 128), (257, 512, 200), (999, 700, 300)])
 def test_product_onto_what_is_there(rt, rows, cols, ntok, kind):
     rng = np.random.default_rng(rows)

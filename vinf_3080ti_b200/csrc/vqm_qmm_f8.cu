@@ -8,11 +8,13 @@
 //   warp 1      one thread issues the MMAs (in the second block of a pair: passes "full" on to the first)
 //   warp 2      tensor memory
 //   warps 4-11  sums and outputs: two warps for each 32 lanes of tensor memory, each half of the columns
-// Up to 128 activation rows: the weight rows are the lanes, the activation rows the columns (16, 32, 64 or 128).  A lane's weight scale is the block's, the activation
-// scales are one for each column.
-// PAIR, more than 128: two blocks of a cluster multiply 256 activation rows, which are the lanes, by 256 weight rows together (cta_group::2).  A lane then needs one factor for all
-// of its 128 columns of a block; with the weight rows in the lanes it would need 128 different ones from shared memory, twice what that gives in the time of the MMAs.
-// SPLIT (few tiles): the blocks (pairs) of a cluster share the columns of a tile, and exchange their sums by st.async.
+// Up to 64 activation rows: the weight rows are the lanes, the activation rows the columns (16, 32 or 64).  A lane's weight scale is the block's, the activation scales
+// are one for each column, by shared memory.
+// TURNED, more: the activation rows are the lanes, 128 weight rows the columns, and a lane needs one factor for all of its columns.  (With the weight rows in the lanes
+// it would need 128 different ones, which shared memory gives in twice the time of the MMAs.)  Outputs go out by TMA, where rows are multiples of 16 bytes.
+// PAIR, many rows (pairs_pay): two blocks of a cluster multiply 256 activation rows by 256 weight rows together (cta_group::2), each half of the weight rows by itself, so
+// that four accumulators are in turn.
+// SPLIT (few tiles, single blocks): the blocks of a cluster share the columns of a tile, and exchange their sums by st.async.
 //
 // Every wait is bounded: on expiry the block records a status code and everybody falls through to the end.
 #include <cuda.h>
@@ -27,10 +29,10 @@ namespace {
 constexpr int kRows = 128;                  // rows of a block's first operand, the lanes of tensor memory
 constexpr int kABytes = kRows * kQCols;     // of a stage
 constexpr int kMaxStages = 12, kMaxCluster = 8;
-constexpr int kRing = 216 * 1024, kHalfRing = 106 * 1024, kPairRing = 192 * 1024, kStaging = 4096;  // (a warp's, for outputs of pairs)
+constexpr int kRing = 216 * 1024, kHalfRing = 106 * 1024, kTurnedRing = 160 * 1024, kBox = 4096, kStaging = 2 * kBox;  // (a warp's, for outputs of pairs)
 constexpr int kWriters = 8, kThreads = 128 + 32 * kWriters;
 // Registers of a thread: a pair's writers hold 128 sums and two sets of 32 that come from tensor memory.  The shares add up to what the block is launched with.
-constexpr int kWriterRegs = 224, kOtherRegs = 56, kLaunchRegs = 168;
+constexpr int kWriterRegs = 216, kOtherRegs = 72, kLaunchRegs = 168;
 static_assert(128 * kOtherRegs + 32 * kWriters * kWriterRegs <= kThreads * kLaunchRegs, "registers of a block");
 
 struct QmmF8 {
@@ -45,6 +47,15 @@ struct QmmF8 {
     int exchange;                      // where in the ring's memory they leave sums for one another, if not where the stages are (0)
     int y_elem, add;
     int half_sm;                       // two blocks per SM
+    int tile_out;                      // pairs: outputs go out by TMA
+};
+template <bool TURNED>
+struct Maps {
+    CUtensorMap w, q;
+};
+template <>
+struct Maps<true> {
+    CUtensorMap w, q, y;
 };
 
 template <bool PAIR>
@@ -55,6 +66,11 @@ __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint3
     else
         asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
                      : "memory");
+}
+// A pair's copies, whichever block they go to, are counted on a barrier of the first.
+__device__ __forceinline__ void copy_tile_of_pair(uint32_t to, const CUtensorMap *map, int x, int row, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(to), "l"(map), "r"(x), "r"(row), "r"(bar)
+                 : "memory");
 }
 // N columns of this warp's 32 lanes
 template <int N>
@@ -83,17 +99,11 @@ __device__ __forceinline__ void load_sums(uint32_t at, uint32_t (&v)[N]) {
 }
 __device__ __forceinline__ void loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-using Two = unsigned long long;  // two fp32
-__device__ __forceinline__ Two two(float x, float y) {
-    Two v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
-    return v;
+__device__ __forceinline__ void add_scaled(float &s0, float &s1, uint32_t x, uint32_t y, float a, float b) {
+    asm("{\n\t.reg .b64 v, c, d;\n\tmov.b64 v, {%2, %3};\n\tmov.b64 c, {%4, %5};\n\tmov.b64 d, {%0, %1};\n\tfma.rn.f32x2 d, v, c, d;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "+f"(s0), "+f"(s1)
+        : "r"(x), "r"(y), "f"(a), "f"(b));
 }
-__device__ __forceinline__ void add_scaled(Two &sum, uint32_t x, uint32_t y, Two scales) {
-    asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%1, %2};\n\tfma.rn.f32x2 %0, v, %3, %0;\n\t}" : "+l"(sum) : "r"(x), "r"(y), "l"(scales));
-}
-__device__ __forceinline__ float first(Two v) { return __uint_as_float(static_cast<uint32_t>(v)); }
-__device__ __forceinline__ float second(Two v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
 
 __device__ __forceinline__ float get(const float *y) { return *y; }
 __device__ __forceinline__ float get(const __half *y) { return __half2float(*y); }
@@ -132,16 +142,31 @@ __device__ __forceinline__ void write8_any(const QmmF8 &a, long long at, long lo
     else write8(static_cast<float *>(a.y) + at, stride, left, a.add != 0, v);
 }
 
+// Eight outputs that lie side by side.
+template <typename Y>
+__device__ __forceinline__ void write8_along(Y *y, int row, int rows, bool add, float (&v)[8]) {
+    if (rows % 4 != 0) return write8(y + row, 1, rows - row, add, v);
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+        if (row + i >= rows) break;
+        float four[4] = {};
+        if (add) get4(y + row + i, four);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) four[e] += v[i + e];
+        put4(y + row + i, four);
+    }
+}
+
 // 32 activation rows (of the lanes) by 32 weight rows (of a lane's values), turned in shared memory so that what is written together lies together.  `room`: a
 // warp's 4 KB, rows of 128 bytes whose 16-byte pieces are exchanged against bank conflicts.
 template <typename Y>
-__device__ __forceinline__ void write_turned(const QmmF8 &a, uint32_t room, const Two *sums, int tok0, int row0) {
+__device__ __forceinline__ void write_turned(const QmmF8 &a, uint32_t room, const float *sums, int tok0, int row0) {
     const int lane = threadIdx.x & 31;
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const uint32_t to = room + lane * 128 + ((j ^ (lane & 7)) * 16);
-        asm volatile("st.shared.v2.u64 [%0], {%1, %2};" ::"r"(to), "l"(sums[2 * j]), "l"(sums[2 * j + 1]) : "memory");
+        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(sums[4 * j]), "f"(sums[4 * j + 1]), "f"(sums[4 * j + 2]), "f"(sums[4 * j + 3]) : "memory");
     }
     __syncwarp();
     Y *y = static_cast<Y *>(a.y);
@@ -149,7 +174,7 @@ __device__ __forceinline__ void write_turned(const QmmF8 &a, uint32_t room, cons
         const int piece = lane & 7, row = row0 + piece * 4;
         if (row < a.rows) {
             Y *at = y + static_cast<long long>(tok0 + (lane >> 3)) * a.rows + row;
-#pragma unroll
+#pragma unroll 1
             for (int part = 0; part < 8; part += 4) {
                 float was[4][4];
                 if (a.add)
@@ -179,21 +204,62 @@ __device__ __forceinline__ void write_turned(const QmmF8 &a, uint32_t room, cons
     }
 }
 
+// The same by TMA, a box of 128 bytes of 32 activation rows at a time; two boxes of a warp in turn.
+template <typename Y, int CW>
+__device__ __forceinline__ void write_boxes(const QmmF8 &a, const CUtensorMap *map, uint32_t room, uint32_t &turn, const float *sums, int tok0, int row0) {
+    constexpr int COLS = 128 / sizeof(Y);
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int b = 0; b < CW / COLS; ++b) {
+        const uint32_t box = room + (turn++ & 1) * kBox;
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // (the store before the last one has read its box)
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t to = box + lane * 128 + ((j ^ (lane & 7)) * 16);
+            if constexpr (sizeof(Y) == 4) {
+                const float *v = sums + b * 32 + 4 * j;
+                asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
+            } else {
+                uint32_t h[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const __half2 v = __floats2half2_rn(sums[b * 64 + 8 * j + 2 * i], sums[b * 64 + 8 * j + 2 * i + 1]);
+                    h[i] = *reinterpret_cast<const uint32_t *>(&v);
+                }
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+            // (what is beyond the last row or column is not written; no box begins there)
+            if (tok0 < a.ntok && row0 + b * COLS < a.rows)
+                asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(row0 + b * COLS), "r"(tok0), "r"(box) : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+    }
+}
+
 // CW: columns of tensor memory that a writer warp reads
-template <int CW, bool PAIR, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, !PAIR && CW <= 16 ? 2 : 1) qmm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap q_map, const QmmF8 a) {
-    static_assert(!PAIR || CW == 128);
+__host__ __device__ constexpr bool turned(int cw) { return cw >= 64; }  // the lanes are activation rows
+__host__ __device__ constexpr bool paired(int cw) { return cw == 128; }
+template <int CW, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(const __grid_constant__ Maps<turned(CW)> maps, const QmmF8 a) {
+    constexpr bool PAIR = paired(CW), TURNED = turned(CW);
+    static_assert(!(PAIR && SPLIT));
     constexpr int GROUP = PAIR ? 2 : 1, N = 2 * CW, BUFS = PAIR ? 2 : 4, TMEM = N * BUFS;
+    constexpr int HALVES = PAIR ? 2 : 1;  // parts of an accumulator that are multiplied, and handed on, by themselves
     extern __shared__ uint8_t ring_raw[];
-    __shared__ __align__(8) uint64_t s_full[kMaxStages], s_empty[kMaxStages], s_acc_full[BUFS], s_acc_empty[BUFS], s_sums[kWriters];
-    __shared__ __align__(16) float s_scales[PAIR ? 1 : kWriters][2][PAIR ? 4 : CW];
+    __shared__ __align__(8) uint64_t s_full[kMaxStages], s_empty[kMaxStages], s_acc_full[HALVES][BUFS], s_acc_empty[HALVES][BUFS], s_sums[kWriters];
+    __shared__ __align__(16) float s_scales[TURNED ? 1 : kWriters][2][TURNED ? 4 : CW];
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed, s_issued;
     const uint32_t ring = (s32(ring_raw) + 1023u) & ~1023u;  // (the swizzle works on address bits)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t in_cluster = 0;
     if constexpr (PAIR || SPLIT) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(in_cluster));
-    const int rank = PAIR ? static_cast<int>(in_cluster & 1u) : 0, part = static_cast<int>(in_cluster) / GROUP;  // place in the pair, share of the columns
+    const int rank = PAIR ? static_cast<int>(in_cluster & 1u) : 0, part = SPLIT ? static_cast<int>(in_cluster) : 0;  // place in the pair, share of the columns
     const uint32_t leader = in_cluster & ~1u;
     const int cluster = static_cast<int>(blockIdx.x) / (GROUP * a.split), n_clusters = static_cast<int>(gridDim.x) / (GROUP * a.split);
     const int k0 = SPLIT ? part * a.n_k / a.split : 0, k1 = SPLIT ? (part + 1) * a.n_k / a.split : a.n_k;
@@ -202,13 +268,14 @@ __global__ void __launch_bounds__(kThreads, !PAIR && CW <= 16 ? 2 : 1) qmm_f8_ke
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; ++s) {
-            bar_init(s32(&s_full[s]), PAIR && rank == 0 ? 2 : 1);  // the first block of a pair hears of the second's stage
-            bar_init(s32(&s_empty[s]), 1);
+            bar_init(s32(&s_full[s]), 1);  // (a pair's: the first block's)
+            bar_init(s32(&s_empty[s]), HALVES);
         }
-        for (int b = 0; b < BUFS; ++b) {
-            bar_init(s32(&s_acc_full[b]), 1);
-            bar_init(s32(&s_acc_empty[b]), kWriters * GROUP);
-        }
+        for (int h = 0; h < HALVES; ++h)
+            for (int b = 0; b < BUFS; ++b) {
+                bar_init(s32(&s_acc_full[h][b]), 1);
+                bar_init(s32(&s_acc_empty[h][b]), kWriters / HALVES * GROUP);
+            }
         for (int w = 0; w < kWriters; ++w) bar_init(s32(&s_sums[w]), 1);
         s_failed = s_issued = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -234,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, !PAIR && CW <= 16 ? 2 : 1) qmm_f8_ke
     // Tiles go to clusters in turn; 8 tiles of weight rows by all tiles of activation rows follow one another, so that what is multiplied at one
     // time is a block of both that stays in L2.
     auto place = [&](int tile, int &row_tile, int &tok_tile) {
-        if constexpr (!PAIR) {
+        if constexpr (!TURNED) {
             row_tile = tile, tok_tile = 0;
         } else {
             constexpr int kBand = 8;
@@ -248,11 +315,23 @@ __global__ void __launch_bounds__(kThreads, !PAIR && CW <= 16 ? 2 : 1) qmm_f8_ke
         if constexpr (PAIR) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == 0) {
             if (tc::elect_one()) {
+                const uint32_t full0 = PAIR ? in_block(s32(&s_full[0]), static_cast<int>(leader)) : s32(&s_full[0]);
+                const uint32_t to0 = PAIR ? in_block(ring, static_cast<int>(in_cluster)) : ring;
                 auto copy_w = [&](int stage, int k, int row_tile) {
-                    copy_tile(ring + stage * stage_bytes + (PAIR ? kABytes : 0), &w_map, k * kQCols, (row_tile * GROUP + rank) * kRows, s32(&s_full[stage]));
+                    if constexpr (PAIR) {  // 64 rows of each half
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            copy_tile_of_pair(to0 + stage * stage_bytes + kABytes + h * (kABytes / 2), &maps.w, k * kQCols, (row_tile * 2 + h) * kRows + rank * (kRows / 2), full0 + stage * 8);
+                    } else {
+                        copy_tile(to0 + stage * stage_bytes + (TURNED ? kABytes : 0), &maps.w, k * kQCols, row_tile * kRows, full0 + stage * 8);
+                    }
                 };
                 auto copy_q = [&](int stage, int k, int tok_tile) {
-                    copy_tile(ring + stage * stage_bytes + (PAIR ? 0 : kABytes), &q_map, k * kQCols, PAIR ? (tok_tile * GROUP + rank) * kRows : 0, s32(&s_full[stage]));
+                    if constexpr (PAIR) copy_tile_of_pair(to0 + stage * stage_bytes, &maps.q, k * kQCols, (tok_tile * GROUP + rank) * kRows, full0 + stage * 8);
+                    else copy_tile(to0 + stage * stage_bytes + (TURNED ? 0 : kABytes), &maps.q, k * kQCols, tok_tile * kRows, full0 + stage * 8);
+                };
+                auto expect_stage = [&](int stage) {
+                    if (rank == 0) expect(s32(&s_full[stage]), GROUP * stage_bytes);
                 };
                 int issued = 0, stage = 0;
                 uint32_t parity = 1;  // of the wait for a stage that is being used again
@@ -266,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, !PAIR && CW <= 16 ? 2 : 1) qmm_f8_ke
                         // stream makes, the activations, is waited for.
                         const int ahead = min(a.stages, k1 - k0);
                         for (int i = 0; i < ahead; ++i) {
-                            expect(s32(&s_full[i]), stage_bytes);
+                            expect_stage(i);
                             copy_w(i, k0 + i, row_tile);
                         }
                         asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -281,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, !PAIR && CW <= 16 ? 2 : 1) qmm_f8_ke
                             ok = false;
                             break;
                         }
-                        expect(s32(&s_full[stage]), stage_bytes);
+                        expect_stage(stage);
                         copy_w(stage, k, row_tile);
                         copy_q(stage, k, tok_tile);
                         ++issued;
@@ -291,10 +370,11 @@ __global__ void __launch_bounds__(kThreads, !PAIR && CW <= 16 ? 2 : 1) qmm_f8_ke
                 s_issued = issued;
             }
             __syncwarp();
-        } else if (warp == 1) {
-            if (tc::elect_one()) {
+        } else if (warp == 1 || (PAIR && warp == 3)) {
+            if (rank == 0 && tc::elect_one()) {
+                const int part_of = warp >> 1;  // the half that this warp multiplies
                 // D fp32, A and B e4m3, K-major
-                const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(GROUP * kRows >> 4) << 24);
+                const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(N / HALVES >> 3) << 17) | (static_cast<uint32_t>(GROUP * kRows >> 4) << 24);
                 int stage = 0, done = 0;
                 uint32_t parity = 0;
                 bool ok = true;
@@ -302,20 +382,15 @@ __global__ void __launch_bounds__(kThreads, !PAIR && CW <= 16 ? 2 : 1) qmm_f8_ke
                     for (int k = k0; k < k1; ++k, ++done) {
                         const uint32_t full = s32(&s_full[stage]);
                         const int buf = done % BUFS;
-                        ok = PAIR && rank == 0 ? wait<true>(full, parity, failed) : wait<false>(full, parity, failed);
+                        ok = wait<false>(full, parity, failed);
+                        if (ok && done >= BUFS) ok = wait<false>(s32(&s_acc_empty[part_of][buf]), (done / BUFS - 1) & 1, failed);
                         if (!ok) break;
-                        if (rank == 0) {
-                            if (done >= BUFS) ok = wait<PAIR>(s32(&s_acc_empty[buf]), (done / BUFS - 1) & 1, failed);
-                            if (!ok) break;
-                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                            const uint64_t a_desc = tile_desc(ring + stage * stage_bytes), b_desc = tile_desc(ring + stage * stage_bytes + kABytes);
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint64_t a_desc = tile_desc(ring + stage * stage_bytes), b_desc = tile_desc(ring + stage * stage_bytes + kABytes + part_of * (kABytes / 2));
 #pragma unroll
-                            for (int j = 0; j < kQCols / 32; ++j) mma_f8<PAIR>(tmem + buf * N, a_desc + 2 * j, b_desc + 2 * j, idesc, j > 0 ? 1u : 0u);
-                            commit<PAIR>(s32(&s_empty[stage]), static_cast<uint32_t>(part));
-                            commit<PAIR>(s32(&s_acc_full[buf]), static_cast<uint32_t>(part));
-                        } else {
-                            arrive_in(in_block(full, static_cast<int>(leader)));
-                        }
+                        for (int j = 0; j < kQCols / 32; ++j) mma_f8<PAIR>(tmem + buf * N + part_of * CW, a_desc + 2 * j, b_desc + 2 * j, idesc, j > 0 ? 1u : 0u);
+                        commit<PAIR>(s32(&s_acc_full[part_of][buf]), static_cast<uint32_t>(part));
+                        commit<PAIR>(s32(&s_empty[stage]), static_cast<uint32_t>(part));
                         if (++stage == a.stages) stage = 0, parity ^= 1;
                     }
                 }
@@ -330,100 +405,130 @@ __global__ void __launch_bounds__(kThreads, !PAIR && CW <= 16 ? 2 : 1) qmm_f8_ke
     } else {
         if constexpr (PAIR) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWriterRegs));
         constexpr int PART = CW < 32 ? CW : 32;  // columns of one load
-        const int writer = warp - 4, lanes = warp & 3, half = writer >> 2;  // (a warp may read the 32 lanes (warp % 4) * 32 onwards)
+        const int writer = warp - 4, lanes = warp & 3, half = writer >> 2, part_of = PAIR ? half : 0;  // (a warp may read the 32 lanes (warp % 4) * 32 onwards)
         asm volatile("griddepcontrol.wait;" ::: "memory");
-        int done = 0;
         bool ok = true;
-        Two sums[CW / 2];
-        int row0 = 0, tok0 = 0;  // of this lane's outputs: PAIR: activation row tok0, weight rows from row0 on; else weight row row0, activation rows from tok0 on
-        for (int tile = cluster; tile < n_tiles && ok; tile += n_clusters) {
+        float sums[CW];
+        uint32_t turn = 0, box_turn = 0;  // blocks of columns, boxes of outputs so far
+        const uint32_t emptied = PAIR ? in_block(s32(&s_acc_empty[part_of][0]), static_cast<int>(leader)) : s32(&s_acc_empty[0][0]);
+        int row0 = 0, tok0 = 0;  // of this lane's outputs: TURNED: activation row tok0, weight rows from row0 on; else weight row row0, activation rows from tok0 on
+        for (int tile = cluster; tile < n_tiles; tile += n_clusters) {
             int row_tile, tok_tile;
             place(tile, row_tile, tok_tile);
-            const float *sx, *sw;
-            bool has_x, has_x2 = false, has_w;
-            if constexpr (PAIR) {
+#pragma unroll
+            for (int j = 0; j < CW; ++j) sums[j] = 0.0f;
+            if constexpr (TURNED) {
+                // (what is beyond the last row takes the last one's scales)
+                const float *sx = a.q_scales + min((tok_tile * GROUP + rank) * kRows + lanes * 32 + lane, a.ntok - 1) + k0 * a.q_scale_pitch;
+                const float *sw = a.w_scales + static_cast<size_t>(min(PAIR ? row_tile * 2 + half : row_tile, (a.rows - 1) / kF8Block)) * a.n_k + k0;
+                float x_next = *sx, w_next = __ldg(sw);  // on their way one block ahead
+#pragma unroll 1
+                for (int left = k1 - k0; left > 0; --left, ++turn) {
+                    const int buf = turn % BUFS;
+                    ok &= wait<false>(s32(&s_acc_full[part_of][buf]), (turn / BUFS) & 1, failed);  // (no way out of the loop: the sums would be copied)
+                    __syncwarp();
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t at = tmem + buf * N + half * CW + (static_cast<uint32_t>(lanes * 32) << 16);
+                    uint32_t v[2][PART];
+                    load_sums<PART>(at, v[0]);
+                    const float scale = x_next * w_next;
+                    if (left > 1) {
+                        sx += a.q_scale_pitch, ++sw;
+                        x_next = *sx, w_next = __ldg(sw);
+                    }
+#pragma unroll
+                    for (int p = 0; p < CW / PART; ++p) {
+                        loaded();
+                        if (p + 1 < CW / PART) {
+                            load_sums<PART>(at + (p + 1) * PART, v[(p + 1) & 1]);  // (on its way while these are added)
+                        } else {
+                            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) {
+                                if constexpr (PAIR) arrive_in(emptied + buf * 8);
+                                else bar_arrive(emptied + buf * 8);
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < PART; j += 2) add_scaled(sums[p * PART + j], sums[p * PART + j + 1], v[p & 1][j], v[p & 1][j + 1], scale, scale);
+                    }
+                }
+                place(tile, row_tile, tok_tile);
                 tok0 = (tok_tile * GROUP + rank) * kRows + lanes * 32 + lane;
-                row0 = row_tile * GROUP * kRows + half * CW;
-                sx = a.q_scales + tok0, sw = a.w_scales + static_cast<size_t>(row_tile * GROUP + half) * a.n_k;
-                has_x = tok0 < a.ntok, has_w = row0 < a.rows;
+                row0 = row_tile * 2 * CW + half * CW;
             } else {
                 row0 = row_tile * kRows + lanes * 32 + lane;
                 tok0 = half * CW;
-                sx = a.q_scales + tok0 + lane, sw = a.w_scales + static_cast<size_t>(row_tile) * a.n_k;
-                has_x = lane < CW && tok0 + lane < a.ntok, has_x2 = CW > 32 && tok0 + lane + 32 < a.ntok, has_w = true;
-            }
-#pragma unroll
-            for (int j = 0; j < CW / 2; ++j) sums[j] = 0;
-            // scales are on their way one block ahead
-            float x_next = has_x ? sx[k0 * a.q_scale_pitch] : 0.0f, x2_next = has_x2 ? sx[k0 * a.q_scale_pitch + 32] : 0.0f, w_next = has_w ? __ldg(sw + k0) : 0.0f;
+                const bool has_x = lane < CW && tok0 + lane < a.ntok, has_x2 = CW > 32 && tok0 + lane + 32 < a.ntok;
+                const float *sx = a.q_scales + tok0 + lane + k0 * a.q_scale_pitch, *sw = a.w_scales + static_cast<size_t>(row_tile) * a.n_k + k0;
+                float x_next = has_x ? *sx : 0.0f, x2_next = has_x2 ? sx[32] : 0.0f, w_next = __ldg(sw);
 #pragma unroll 1
-            for (int k = k0; k < k1; ++k, ++done) {
-                const int buf = done % BUFS;
-                const float x = x_next, x2 = x2_next, w = w_next;
-                if (k + 1 < k1) {
-                    if (has_x) x_next = sx[(k + 1) * a.q_scale_pitch];
-                    if (has_x2) x2_next = sx[(k + 1) * a.q_scale_pitch + 32];
-                    if (has_w) w_next = __ldg(sw + k + 1);
-                }
-                if constexpr (!PAIR) {
-                    if (lane < CW) s_scales[writer][buf & 1][lane] = x * w;
-                    if constexpr (CW > 32) s_scales[writer][buf & 1][lane + 32] = x2 * w;
+                for (int left = k1 - k0; left > 0; --left, ++turn) {
+                    const int buf = turn % BUFS;
+                    float *scales = s_scales[writer][buf & 1];
+                    if (lane < CW) scales[lane] = x_next * w_next;
+                    if constexpr (CW > 32) scales[lane + 32] = x2_next * w_next;
                     __syncwarp();  // (and nobody reads what the next block but one replaces)
-                }
-                ok = warp_wait(s32(&s_acc_full[buf]), (done / BUFS) & 1, failed);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t at = tmem + buf * N + half * CW + (static_cast<uint32_t>(lanes * 32) << 16);
-                uint32_t v[2][PART];
-                load_sums<PART>(at, v[0]);
-#pragma unroll
-                for (int p = 0; p < CW / PART; ++p) {
-                    loaded();
-                    if (p + 1 < CW / PART) {
-                        load_sums<PART>(at + (p + 1) * PART, v[(p + 1) & 1]);  // (on its way while these are added)
-                    } else {
-                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                        __syncwarp();
-                        if (lane == 0) {
-                            if constexpr (PAIR) arrive_in(in_block(s32(&s_acc_empty[buf]), static_cast<int>(leader)));
-                            else bar_arrive(s32(&s_acc_empty[buf]));
-                        }
+                    if (left > 1) {
+                        sx += a.q_scale_pitch, ++sw;
+                        if (has_x) x_next = *sx;
+                        if (has_x2) x2_next = sx[32];
+                        w_next = __ldg(sw);
                     }
-                    if constexpr (PAIR) {
-                        const Two s = two(x * w, x * w);
+                    ok &= wait<false>(s32(&s_acc_full[0][buf]), (turn / BUFS) & 1, failed);
+                    __syncwarp();
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t at = tmem + buf * N + half * CW + (static_cast<uint32_t>(lanes * 32) << 16);
+                    uint32_t v[2][PART];
+                    load_sums<PART>(at, v[0]);
 #pragma unroll
-                        for (int j = 0; j < PART / 2; ++j) add_scaled(sums[p * PART / 2 + j], v[p & 1][2 * j], v[p & 1][2 * j + 1], s);
-                    } else {
+                    for (int p = 0; p < CW / PART; ++p) {
+                        loaded();
+                        if (p + 1 < CW / PART) {
+                            load_sums<PART>(at + (p + 1) * PART, v[(p + 1) & 1]);
+                        } else {
+                            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) bar_arrive(emptied + buf * 8);
+                        }
 #pragma unroll
-                        for (int j = 0; j < PART / 4; ++j) {
-                            const float4 s = *reinterpret_cast<const float4 *>(&s_scales[writer][buf & 1][p * PART + 4 * j]);
-                            add_scaled(sums[p * PART / 2 + 2 * j], v[p & 1][4 * j], v[p & 1][4 * j + 1], two(s.x, s.y));
-                            add_scaled(sums[p * PART / 2 + 2 * j + 1], v[p & 1][4 * j + 2], v[p & 1][4 * j + 3], two(s.z, s.w));
+                        for (int j = 0; j < PART; j += 4) {
+                            const float4 s = *reinterpret_cast<const float4 *>(scales + p * PART + j);
+                            float *to = sums + p * PART + j;
+                            add_scaled(to[0], to[1], v[p & 1][j], v[p & 1][j + 1], s.x, s.y);
+                            add_scaled(to[2], to[3], v[p & 1][j + 2], v[p & 1][j + 3], s.z, s.w);
                         }
                     }
                 }
             }
             if constexpr (!SPLIT) {
                 if (tile + n_clusters >= n_tiles) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-                if (!ok) break;
-                if constexpr (PAIR) {
-                    const uint32_t room = ring + a.stages * stage_bytes + writer * kStaging;
+                if (!ok) continue;  // (once a wait has given up the writers go on to the end without writing)
+                if constexpr (TURNED) {
+                    const uint32_t room = ring + kTurnedRing + writer * kStaging;
+                    if (a.tile_out) {
+                        if (a.y_elem == 2) write_boxes<__half, CW>(a, &maps.y, room, box_turn, sums, tok0 - lane, row0);
+                        else write_boxes<float, CW>(a, &maps.y, room, box_turn, sums, tok0 - lane, row0);
+                    } else {
 #pragma unroll
-                    for (int p = 0; p < CW / 32; ++p) {
-                        if (a.y_elem == 2) write_turned<__half>(a, room, sums + p * 16, tok0 - lane, row0 + p * 32);
-                        else write_turned<float>(a, room, sums + p * 16, tok0 - lane, row0 + p * 32);
+                        for (int p = 0; p < CW / 32; ++p) {
+                            if (a.y_elem == 2) write_turned<__half>(a, room, sums + p * 32, tok0 - lane, row0 + p * 32);
+                            else write_turned<float>(a, room, sums + p * 32, tok0 - lane, row0 + p * 32);
+                        }
                     }
                 } else if (row0 < a.rows) {
 #pragma unroll
                     for (int c = 0; c < CW / 8; ++c) {
                         float v[8];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) v[2 * j] = first(sums[4 * c + j]), v[2 * j + 1] = second(sums[4 * c + j]);
+                        for (int j = 0; j < 8; ++j) v[j] = sums[8 * c + j];
                         write8_any(a, static_cast<long long>(tok0 + 8 * c) * a.rows + row0, a.rows, a.ntok - tok0 - 8 * c, v);
                     }
                 }
             }
         }
+        if constexpr (TURNED && !SPLIT)
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         if constexpr (SPLIT) {
             // One tile; its sums go, 8 columns of 32 lanes at a time (a unit), to the block that writes them, and there to the same warp.
             const uint32_t room = ring + a.exchange, bar = s32(&s_sums[writer]);
@@ -440,9 +545,11 @@ __global__ void __launch_bounds__(kThreads, !PAIR && CW <= 16 ? 2 : 1) qmm_f8_ke
                     continue;
                 }
                 // stores that count their bytes on a barrier of the block that they go to
-                const uint32_t to = in_block(room_of(c, part, owner), owner * GROUP + rank), there = in_block(bar, owner * GROUP + rank);
-                asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(to), "l"(sums[4 * c]), "l"(sums[4 * c + 1]), "r"(there) : "memory");
-                asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(to + 512), "l"(sums[4 * c + 2]), "l"(sums[4 * c + 3]), "r"(there) : "memory");
+                const uint32_t to = in_block(room_of(c, part, owner), owner), there = in_block(bar, owner);
+                asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "f"(sums[8 * c + 0]), "f"(sums[8 * c + 1]), "f"(sums[8 * c + 2]), "f"(sums[8 * c + 3]), "r"(there)
+                             : "memory");
+                asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to + 512), "f"(sums[8 * c + 4]), "f"(sums[8 * c + 5]), "f"(sums[8 * c + 6]), "f"(sums[8 * c + 7]), "r"(there)
+                             : "memory");
             }
             __syncwarp();
             asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (its other half is at the end: until then others may still send)
@@ -457,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, !PAIR && CW <= 16 ? 2 : 1) qmm_f8_ke
                         if (owner_of(c) != part) continue;
                         float v[8];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) v[2 * j] = first(sums[4 * c + j]), v[2 * j + 1] = second(sums[4 * c + j]);
+                        for (int j = 0; j < 8; ++j) v[j] = sums[8 * c + j];
                         for (int p = 0; p < a.split; ++p) {
                             if (p == part) continue;
                             const uint32_t from = room_of(c, p, part);
@@ -465,8 +572,11 @@ __global__ void __launch_bounds__(kThreads, !PAIR && CW <= 16 ? 2 : 1) qmm_f8_ke
                             v[0] += __uint_as_float(x.x), v[1] += __uint_as_float(x.y), v[2] += __uint_as_float(x.z), v[3] += __uint_as_float(x.w);
                             v[4] += __uint_as_float(z.x), v[5] += __uint_as_float(z.y), v[6] += __uint_as_float(z.z), v[7] += __uint_as_float(z.w);
                         }
-                        if constexpr (PAIR) {
-                            if (tok0 < a.ntok) write8_any(a, static_cast<long long>(tok0) * a.rows + row0 + 8 * c, 1, a.rows - row0 - 8 * c, v);
+                        if constexpr (TURNED) {
+                            if (tok0 < a.ntok && row0 + 8 * c < a.rows) {
+                                if (a.y_elem == 2) write8_along(static_cast<__half *>(a.y) + static_cast<long long>(tok0) * a.rows, row0 + 8 * c, a.rows, a.add != 0, v);
+                                else write8_along(static_cast<float *>(a.y) + static_cast<long long>(tok0) * a.rows, row0 + 8 * c, a.rows, a.add != 0, v);
+                            }
                         } else {
                             if (row0 < a.rows) write8_any(a, static_cast<long long>(tok0 + 8 * c) * a.rows + row0, a.rows, a.ntok - tok0 - 8 * c, v);
                         }
@@ -477,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, !PAIR && CW <= 16 ? 2 : 1) qmm_f8_ke
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (s_failed && threadIdx.x == 0) {  // whichever wait gave up: the last copies land before the block may leave (this wait has a limit too)
+    if (s_failed && threadIdx.x == 0 && rank == 0) {  // whichever wait gave up: the last copies land before the block (the pair) may leave (this wait has a limit too)
         int left = 1 << 16;
         for (int last = max(0, s_issued - a.stages); last < s_issued; ++last)
             while (!bar_try(s32(&s_full[last % a.stages]), (last / a.stages) & 1) && --left > 0) __nanosleep(64);
@@ -493,12 +603,24 @@ __global__ void __launch_bounds__(kThreads, !PAIR && CW <= 16 ? 2 : 1) qmm_f8_ke
     }
 }
 
-template <int CW, bool PAIR, bool SPLIT>
+// Outputs as a 2-D tensor, written in boxes of 128 bytes of 32 rows.
+cudaError_t encode_outputs(CUtensorMap *map, void *y, int rows, int ntok, int elem_bytes) {
+    TcEncode encode = nullptr;
+    if (const cudaError_t err = tc_encoder(&encode); err != cudaSuccess) return err;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(ntok)}, strides[1] = {static_cast<cuuint64_t>(rows) * static_cast<cuuint64_t>(elem_bytes)};
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / elem_bytes), 32}, elem[2] = {1, 1};
+    return encode(map, elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, y, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? cudaSuccess
+               : cudaErrorInvalidValue;
+}
+
+template <int CW, bool SPLIT>
 struct Variant {
-    static constexpr bool kHalf = !PAIR && CW <= 16;  // two blocks per SM
-    static constexpr int kGroup = PAIR ? 2 : 1, kRoom = PAIR ? kPairRing : kHalf ? kHalfRing : kRing;
-    static constexpr int kSmem = kRoom + 1024 + (PAIR ? kWriters * kStaging : 0);
-    static constexpr auto kKernel = qmm_f8_kernel<CW, PAIR, SPLIT>;
+    static constexpr bool PAIR = paired(CW), TURNED = turned(CW), kHalf = CW <= 16;  // two blocks per SM
+    static constexpr int kGroup = PAIR ? 2 : 1, kRoom = TURNED ? kTurnedRing : kHalf ? kHalfRing : kRing;
+    static constexpr int kSmem = kRoom + 1024 + (TURNED ? kWriters * kStaging : 0);
+    static constexpr auto kKernel = qmm_f8_kernel<CW, SPLIT>;
     static void configure(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int clusters, int split, int smem, bool overlap, cudaStream_t stream) {
         cfg.gridDim = dim3(static_cast<unsigned>(clusters * split * kGroup));
         cfg.blockDim = dim3(kThreads);
@@ -528,31 +650,38 @@ struct Variant {
         }
         return cached[split] < 0 ? 0 : cached[split];
     }
-    static cudaError_t launch(const CUtensorMap &w, const CUtensorMap &q, const QmmF8 &a, bool overlap, cudaStream_t stream) {
+    static cudaError_t launch(const Maps<TURNED> &maps, const QmmF8 &a, bool overlap, cudaStream_t stream) {
         const int fit = clusters(a.split), tiles = a.row_tiles * a.tok_tiles;
         if (fit == 0) return cudaErrorInvalidConfiguration;
         cudaLaunchConfig_t cfg{};
         cudaLaunchAttribute attr[2];
         configure(cfg, attr, SPLIT ? tiles : (tiles < fit ? tiles : fit), a.split, kSmem, overlap, stream);
-        return cudaLaunchKernelEx(&cfg, kKernel, w, q, a);
+        return cudaLaunchKernelEx(&cfg, kKernel, maps, a);
     }
 };
 
-template <int CW, bool PAIR>
+// As many parts of the columns as leave every cluster room beside the others, of two blocks of columns at least.
+template <int CW>
+int split_of(long long tiles, int n_k) {
+    int best = 1;
+    if constexpr (!paired(CW))
+        for (int split = 2; split <= kMaxCluster && n_k >= 2 * split; ++split)
+            if (tiles <= Variant<CW, true>::clusters(split)) best = split;
+    return best;
+}
+
+template <int CW>
 cudaError_t launch(QmmF8 a, const QmmF8Args &in, cudaStream_t stream) {
-    using One = Variant<CW, PAIR, false>;
-    using Many = Variant<CW, PAIR, true>;
-    constexpr int kStage = kABytes + (PAIR ? kRows : 2 * CW) * kQCols;
-    a.tok_tiles = PAIR ? (in.ntok + 2 * kRows - 1) / (2 * kRows) : 1;
-    a.row_tiles = (in.rows + One::kGroup * kRows - 1) / (One::kGroup * kRows);
+    using One = Variant<CW, false>;
+    constexpr bool PAIR = paired(CW), TURNED = turned(CW);
+    constexpr int kStage = kABytes + (TURNED ? kRows : 2 * CW) * kQCols, kTile = One::kGroup * kRows;
+    a.tok_tiles = TURNED ? (in.ntok + kTile - 1) / kTile : 1;
+    a.row_tiles = (in.rows + kTile - 1) / kTile;
     a.half_sm = One::kHalf;
     a.b_bytes = kStage - kABytes;
-    // As many parts of the columns as leave every cluster room beside the others, of two blocks of columns at least.
-    a.split = 1;
     const long long tiles = static_cast<long long>(a.row_tiles) * a.tok_tiles;
     if (tiles > (1ll << 30)) return cudaErrorInvalidValue;
-    for (int split = 2; split <= kMaxCluster / One::kGroup && a.n_k >= 2 * split; ++split)
-        if (tiles <= Many::clusters(split)) a.split = split;
+    a.split = split_of<CW>(tiles, a.n_k);
     const bool brief = a.n_k <= 8 * a.split;  // a few stages for each block: what counts is how soon it begins and ends
     // Sums have memory of their own where that costs no stage or the stages are few, else they go where the stages were, one barrier of the cluster later.
     const int room = a.split > 1 ? CW / 8 * ((kWriters + a.split - 1) / a.split) * (a.split - 1) * 1024 : 0;
@@ -560,11 +689,27 @@ cudaError_t launch(QmmF8 a, const QmmF8Args &in, cudaStream_t stream) {
     const int beside = (One::kRoom - room) / kStage;
     if (a.split > 1 && (beside == a.stages || (brief && beside >= 3))) a.exchange = One::kRoom - room, a.stages = beside;
     if (a.stages > kMaxStages) a.stages = kMaxStages;
-    CUtensorMap w, q;
-    cudaError_t err = encode_rows(&w, in.w, in.cols, in.w_pitch, in.rows, kRows);
-    if (err == cudaSuccess) err = encode_rows(&q, in.q, in.cols, f8_pitch(in.cols), in.ntok, PAIR ? kRows : 2 * CW);
+    Maps<TURNED> maps{};
+    cudaError_t err = encode_rows(&maps.w, in.w, in.cols, in.w_pitch, in.rows, PAIR ? kRows / 2 : kRows);
+    if (err == cudaSuccess) err = encode_rows(&maps.q, in.q, in.cols, f8_pitch(in.cols), in.ntok, TURNED ? kRows : 2 * CW);
+    if constexpr (TURNED) {
+        a.tile_out = !in.add && static_cast<long long>(in.rows) * in.y_elem % 16 == 0;
+        if (a.tile_out && err == cudaSuccess) err = encode_outputs(&maps.y, in.y, in.rows, in.ntok, in.y_elem);
+    }
     if (err != cudaSuccess) return err;
-    return a.split > 1 ? Many::launch(w, q, a, in.overlap, stream) : One::launch(w, q, a, in.overlap, stream);
+    if constexpr (!PAIR)
+        if (a.split > 1) return Variant<CW, true>::launch(maps, a, in.overlap, stream);
+    return One::launch(maps, a, in.overlap, stream);
+}
+
+// Whether pairs of blocks finish before single ones do.  A pair takes 0.55 us for a block of columns of 256 x 256 outputs, a single block 0.39 for 128 x 128, and what
+// leaves SMs without work can be split by columns as clusters of single blocks only.  (6144 x 5120 with 256 rows: 30.9 and 15.5 us, with 512 21.6 and 27.1.)
+bool pairs_pay(int rows, int ntok, int n_k) {
+    const long long single = static_cast<long long>((rows + kRows - 1) / kRows) * ((ntok + kRows - 1) / kRows), pairs = static_cast<long long>((rows + 2 * kRows - 1) / (2 * kRows)) * ((ntok + 2 * kRows - 1) / (2 * kRows));
+    const int fit = Variant<64, false>::clusters(1), pair_fit = Variant<128, false>::clusters(1);
+    if (fit == 0 || pair_fit == 0) return pair_fit != 0;
+    const int split = single > fit ? 1 : split_of<64>(single, n_k);
+    return (pairs + pair_fit - 1) / pair_fit * n_k * 10 < (single + fit - 1) / fit * ((n_k + split - 1) / split) * 7;
 }
 
 }  // namespace
@@ -581,10 +726,10 @@ cudaError_t launch_qmm_f8(const QmmF8Args &in, cudaStream_t stream) {
     a.n_k = f8_blocks(in.cols);
     a.y_elem = in.y_elem;
     a.add = in.add;
-    if (in.ntok > 128) return launch<128, true>(a, in, stream);
-    if (in.ntok > 64) return launch<64, false>(a, in, stream);
-    if (in.ntok > 32) return launch<32, false>(a, in, stream);
-    return in.ntok > 16 ? launch<16, false>(a, in, stream) : launch<8, false>(a, in, stream);
+    if (in.ntok > 128 && pairs_pay(in.rows, in.ntok, a.n_k)) return launch<128>(a, in, stream);
+    if (in.ntok > 64) return launch<64>(a, in, stream);
+    if (in.ntok > 32) return launch<32>(a, in, stream);
+    return in.ntok > 16 ? launch<16>(a, in, stream) : launch<8>(a, in, stream);
 }
 
 }  // namespace vqm
