@@ -1,9 +1,10 @@
 """Log probabilities on the GPU against their definition in 64 bits (tests/f8_formulas.py).  Places are whole numbers: they are equal.
 
 Tolerances, in units u = 2^-24.  With S the sum of e = exp((l - m) / T): the argument d / T of an exponential is off by 4 of itself (difference, reciprocal of T, its
-product with log2(e), product) and the exponential by 4 more; weighted by p, |d| / T comes to the entropy H at most.  A lane adds its values up 8 at a time and those sums one after the
-other, at most vocab / 2048 + 8 of them, each addition 1; joins of lanes, warps and blocks 5 exponentials and products of each 6 steps, 60.  So S, and log S, is off by
-    sums = (4 H + 4 + vocab / 2048 + 8 + 60) u,
+product with log2(e), product) and the exponential by 4 more; weighted by p, |d| / T comes to the entropy H at most.  A lane adds up 8192 / 512 values of fp32 (16-bit ones: twice
+as many, in two sums) in 16 additions, and those sums one after the other: for each an addition, and where it brings a new largest an exponential and a product, 7 together for at
+most vocab / 8192 + 1 of them.  Lanes, warps and blocks take two such scalings and 10 additions more, 22.  So S, and log S, is off by
+    sums = (4 H + 4 + 16 + 7 (vocab / 8192 + 1) + 22) u,
 a log probability by that and 3 of itself, and the entropy, log S + U / S, by sums (1 + 3 H).
 """
 from __future__ import annotations
@@ -56,7 +57,7 @@ def check(rt, logits, tokens, top=0, temperature=None, **kw):
     out, ent, ids, best = run(rt, logits, tokens, top, at, **kw)
     want_out, want_ent, want_ids, want_best = F.logprobs(logits, tokens, top, at)
     assert np.array_equal(ids, want_ids), np.argwhere(ids != want_ids)[:5]
-    sums = (4 * want_ent + 4 + logits.shape[1] / 2048 + 8 + 60) * F.U
+    sums = (4 * want_ent + 4 + 16 + 7 * (logits.shape[1] / 8192 + 1) + 22) * F.U
 
     def near(got, want, off):
         # answers are fp32: what is a half step or more beyond its largest, 2^128 - 2^104, is infinite there

@@ -1,25 +1,128 @@
 // Log probabilities of given tokens, the entropy of the distribution they are drawn from, and its likeliest tokens:  p = softmax(l / T),
 //   out = log p(token),   entropy = - sum p log p,   the `top` largest logits, of equal ones the lowest place first.
-// Simple form: a block of threads per row; a pass for the largest logit, one for the sums in 64 bits, one for each alternative.
+//
+// One pass over a row, in vectors of 16 bytes: each thread keeps the largest logit m it has seen, S = sum exp((l - m) / T) and U = sum exp((l - m) / T) (l - m); a new largest
+// scales both.  Then  log p(t) = (l_t - m) / T - log S  and  entropy = log S - U / (S T).  A row is a block's, or shared by the blocks of a cluster where there are few rows;
+// sums and alternatives meet in distributed shared memory, and nothing is kept in device memory.
+// The alternatives need no second pass: the `top`-th largest of the maxima of 32 groups of threads is no more than the `top`-th largest logit, because so many groups each hold
+// one that is no less.  Only threads whose own largest reaches it (31 of 512 on average for 20 alternatives) hold candidates, and what they have read is read again.  Of
+// n candidates each finds its own place, by counting those before it.  Rows where more tie than the list holds take a pass for each alternative.
+// Rows of infinite or extreme logits, and extreme temperatures, are summed in 64 bits by one block.
 #include <cuda_fp16.h>
 
 #include "vqm_kernels.h"
+#include "vqm_logits.cuh"
 
 namespace vqm {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxBlocks = 16, kGroups = 32;
+constexpr int kUnroll = 4;       // vectors of a thread in flight
+constexpr int kList = 1024;      // candidates
+constexpr float kLow = -1e30f;   // what is below counts as that in differences, so that they and their products stay finite
+constexpr float kMostT = 1e20f, kLeastT = 1e-30f;  // temperatures that fp32 works with: a masked logit, at -1e30 or less, still comes to nothing
 
-__device__ __forceinline__ float as_float(float v) { return v; }
-__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
-
+using Key = unsigned long long;
 // A logit and its place as one number, larger for what comes first: by value, then by the lower place.  0: nothing (masked).
-__device__ __forceinline__ unsigned long long key_of(float v, int i) {
+__device__ __forceinline__ Key key_of(float v, int i) {
     if (!(v > -INFINITY)) return 0;
     const uint32_t b = __float_as_uint(v == 0.0f ? 0.0f : v);  // (the zeros are equal)
-    return static_cast<unsigned long long>((b & 0x80000000u) != 0 ? ~b : b | 0x80000000u) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(i));
+    return static_cast<Key>((b & 0x80000000u) != 0 ? ~b : b | 0x80000000u) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(i));
 }
-__device__ __forceinline__ int place_of(unsigned long long key) { return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(key)); }
+__device__ __forceinline__ int place_of(Key key) { return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(key)); }
+__device__ __forceinline__ float value_of(Key key) {
+    const uint32_t b = static_cast<uint32_t>(key >> 32);
+    return __uint_as_float((b & 0x80000000u) != 0 ? b & 0x7FFFFFFFu : ~b);
+}
+__device__ __forceinline__ float undefined() { return __uint_as_float(0x7FFFFFFFu); }
+
+// Two fp32 at a time.
+using Two = unsigned long long;
+__device__ __forceinline__ Two two(float x, float y) {
+    Two v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ void both(Two v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    Two v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    Two v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+
+// The largest of some vectors (NaN counts as nothing).
+__device__ __forceinline__ float largest(const uint4 (&w)[kUnroll], const float *) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i)
+        m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(w[i].x), __uint_as_float(w[i].y)), fmaxf(__uint_as_float(w[i].z), __uint_as_float(w[i].w))));
+    return m;
+}
+__device__ __forceinline__ float largest(const uint4 (&w)[kUnroll], const __half *) {
+    auto half2_of = [](uint32_t v) { return *reinterpret_cast<const __half2 *>(&v); };
+    __half2 m = half2_of(0xFC00FC00u);
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) m = __hmax2(m, __hmax2(__hmax2(half2_of(w[i].x), half2_of(w[i].y)), __hmax2(half2_of(w[i].z), half2_of(w[i].w))));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+
+struct Sums {
+    float m, s, u;  // the largest so far (kLow: none), S and U
+};
+template <typename T>
+__device__ __forceinline__ void add_vectors(Sums &a, const uint4 (&w)[kUnroll], float c) {
+    const float most = largest(w, static_cast<const T *>(nullptr));
+    if (most > a.m) {
+        const float d = a.m - most, f = ex2(d * c);
+        a.u = f * fmaf(d, a.s, a.u);
+        a.s *= f;
+        a.m = most;
+    }
+    const Two minus = two(-a.m, -a.m), cc = two(c, c);
+    Two s = 0, u = 0;
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+        float x[kVec<T>];
+        values_of(w[i], x);
+#pragma unroll
+        for (int e = 0; e < kVec<T>; e += 2) {
+            float d0, d1, t0, t1;
+            both(add2(two(x[e], x[e + 1]), minus), d0, d1);
+            const Two d = two(fmaxf(d0, kLow), fmaxf(d1, kLow));
+            both(mul2(d, cc), t0, t1);
+            const Two p = two(ex2(t0), ex2(t1));
+            s = add2(s, p);
+            u = fma2(p, d, u);
+        }
+    }
+    float s0, s1, u0, u1;
+    both(s, s0, s1);
+    both(u, u0, u1);
+    a.s += s0 + s1;
+    a.u += u0 + u1;
+}
+
+struct Shared {
+    float group[kGroups];           // largest logits of groups of 16 threads
+    float part[2][kWarps];
+    Key list[kList];                // candidates
+    Key best[kMaxTop];              // this block's alternatives, in order
+    Key key[kWarps];
+    double wide[kWarps];
+    float sums[3];                  // this block's m, S and U
+    int count;
+    unsigned status;
+};
 
 template <typename V, typename F>
 __device__ V over_block(V v, V (&room)[kWarps], F &&join) {
@@ -31,76 +134,296 @@ __device__ V over_block(V v, V (&room)[kWarps], F &&join) {
     for (int w = 1; w < kWarps; ++w) v = join(v, room[w]);
     return v;
 }
-
+// The first `want` of s.list[0, n) in order, by the whole block, to s.best; zeros behind the last.
+__device__ __forceinline__ void rank_list(Shared &s, int n, int want) {
+    if (threadIdx.x < kMaxTop) s.best[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const Key mine = s.list[i];
+        int before = 0;
+        for (int j = 0; j < n; ++j) before += s.list[j] > mine;
+        if (mine != 0 && before < want) s.best[before] = mine;
+    }
+    __syncthreads();
+}
+// The same of all of a slice [begin, end), a pass for each.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobsArgs a) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    __shared__ double s_sum[kWarps];
-    __shared__ unsigned long long s_key[kWarps];
-    const size_t row = blockIdx.x;
-    const T *x = static_cast<const T *>(a.logits) + row * a.vocab;
-    const float given = a.temperature != nullptr ? a.temperature[row] : 1.0f;
-    const bool greedy = !(given > 0.0f), broken = *a.status != 0;
-    auto larger = [](unsigned long long p, unsigned long long q) { return p > q ? p : q; };
-    auto plus = [](double p, double q) { return p + q; };
-    auto next = [&](unsigned long long below) {  // the largest key under that
-        unsigned long long most = 0;
-        for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
-            const unsigned long long k = key_of(as_float(x[i]), i);
-            if (k < below && k > most) most = k;
-        }
-        return over_block(most, s_key, larger);
-    };
-    const unsigned long long first = next(~0ull);
-    const float top = first != 0 ? as_float(x[place_of(first)]) : 0.0f;
-    const bool flat = given > 1e30f && top < INFINITY;
-    const double inv = 1.0 / static_cast<double>(given);
-    auto less = [&](float v, int i) -> double {  // (logit - largest) / T, -inf where p is nothing
-        if (!(v > -INFINITY)) return -INFINITY;
-        if (greedy) return i == place_of(first) ? 0.0 : -INFINITY;
-        if (v == top || flat) return 0.0;
-        return top == INFINITY ? -INFINITY : (static_cast<double>(v) - static_cast<double>(top)) * inv;
-    };
+static __device__ __noinline__ void rank_by_passes(Shared &s, const T *x, int begin, int end, int want) {
+    Key last = ~0ull;
+    for (int k = 0; k < want; ++k) {
+        Key most = 0;
+        if (last != 0)
+            for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += kThreads) {
+                const Key key = key_of(as_float(x[i]), i);
+                if (key < last && key > most) most = key;
+            }
+        last = over_block(most, s.key, [](Key p, Key q) { return p > q ? p : q; });
+        if (threadIdx.x == 0) s.best[k] = last;
+    }
+    __syncthreads();
+}
+// log S and the entropy in 64 bits, by the whole block.
+template <typename T>
+static __device__ __noinline__ void wide_sums(Shared &s, const T *x, int n, float top, double inverse, bool flat, double &log_sum, double &entropy) {
     double sum = 0.0, weighted = 0.0;
-    for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
-        const double d = less(as_float(x[i]), i), e = exp(d);
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const float v = as_float(x[i]);
+        if (!(v > -INFINITY)) continue;
+        const double d = v == top || flat ? 0.0 : top == INFINITY ? -INFINITY : (static_cast<double>(v) - static_cast<double>(top)) * inverse, e = exp(d);
         sum += e;
         if (e > 0.0) weighted -= e * d;
     }
-    sum = over_block(sum, s_sum, plus);
-    weighted = over_block(weighted, s_sum, plus);
-    const double log_sum = sum > 0.0 ? log(sum) : 0.0;
-    auto answer = [&](float v, int i) { return broken ? __uint_as_float(0x7FFFFFFFu) : static_cast<float>(less(v, i) - log_sum); };
+    auto plus = [](double p, double q) { return p + q; };
+    sum = over_block(sum, s.wide, plus);
+    weighted = over_block(weighted, s.wide, plus);
+    log_sum = sum > 0.0 ? log(sum) : 0.0;
+    entropy = sum > 0.0 ? log_sum + weighted / sum : 0.0;
+}
+
+__device__ __forceinline__ uint32_t in_cluster(const void *p, int block) {
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(block));
+    return at;
+}
+__device__ __forceinline__ float load_float(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ Key load_key(uint32_t at) {
+    Key v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sync_cluster() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const LogprobsArgs a, const int n_blocks) {
+    __shared__ Shared s;
+    constexpr int VEC = kVec<T>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = a.vocab;
+    const int row = static_cast<int>(blockIdx.x) / n_blocks, block = static_cast<int>(blockIdx.x) % n_blocks;
+    const T *x = static_cast<const T *>(a.logits) + static_cast<size_t>(row) * n;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const float given = a.temperature != nullptr ? a.temperature[row] : 1.0f;
+    const bool greedy = !(given > 0.0f);
+    const bool ordinary = given >= kLeastT && given <= kMostT;  // of the temperature
+    const float c = ordinary ? 1.4426950408889634f / given : 1.0f;
     if (threadIdx.x == 0) {
-        const int token = a.tokens[row];
-        const bool inside = token >= 0 && token < a.vocab;
-        a.out[row] = answer(inside ? as_float(x[token]) : -INFINITY, token);
-        if (a.entropy != nullptr) a.entropy[row] = broken ? __uint_as_float(0x7FFFFFFFu) : sum > 0.0 ? static_cast<float>(log_sum + weighted / sum) : 0.0f;
+        s.count = 0;
+        s.status = *a.status;
     }
-    unsigned long long k = first;
-    for (int j = 0; j < a.top; ++j) {
-        if (threadIdx.x == 0) {
-            const size_t to = row * a.top + j;
-            a.top_ids[to] = k != 0 && !broken ? place_of(k) : -1;
-            if (a.top_out != nullptr) a.top_out[to] = answer(k != 0 ? as_float(x[place_of(k)]) : -INFINITY, place_of(k));
+
+    // this block's vectors
+    const int first = first_of(x);  // index of vector 0's first element
+    const int vectors = (n - first + VEC - 1) / VEC;
+    const int begin = static_cast<int>(static_cast<long long>(vectors) * block / n_blocks), end = static_cast<int>(static_cast<long long>(vectors) * (block + 1) / n_blocks);
+    Sums sums{kLow, 0.0f, 0.0f};
+#pragma unroll 1
+    for (int v = begin + static_cast<int>(threadIdx.x); v < end; v += kUnroll * kThreads) {
+        uint4 w[kUnroll];
+#pragma unroll
+        for (int i = 0; i < kUnroll; ++i) {
+            if (v + i * kThreads < end) load_vec(x, n, first, v + i * kThreads, w[i]);
+            else w[i] = make_uint4(kNothing<T>, kNothing<T>, kNothing<T>, kNothing<T>);
         }
-        if (k != 0 && j + 1 < a.top) k = next(k);
+        add_vectors<T>(sums, w, c);
+    }
+
+    // the largest of each group of 16 threads, and the block's
+    float most = sums.m;
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, off));
+    if ((lane & 15) == 0) s.group[warp * 2 + (lane >> 4)] = most;
+    __syncthreads();
+    const float mine = s.group[lane];
+    float all = mine;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, off));
+    const float f = ex2((sums.m - all) * c);
+    float sum = sums.s * f, weighted = f * fmaf(sums.m - all, sums.s, sums.u);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
+        weighted += __shfl_xor_sync(0xFFFFFFFFu, weighted, off);
+    }
+    if (lane == 0) s.part[0][warp] = sum, s.part[1][warp] = weighted;
+
+    const int want = a.top > 0 ? a.top : greedy ? 1 : 0;
+    if (want > 0) {
+        // the want-th largest group; where that is out of what the sums tell apart, all logits are candidates
+        int before = 0;
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) {
+            const float other = __shfl_sync(0xFFFFFFFFu, mine, j);
+            before += other > mine || (other == mine && j < lane);
+        }
+        float least = __shfl_sync(0xFFFFFFFFu, mine, __ffs(__ballot_sync(0xFFFFFFFFu, before == want - 1)) - 1);
+        const bool any = !(least > kLow);
+        if (any) least = -INFINITY;
+        auto offer = [&](int v) {
+            uint4 w;
+            load_vec(x, n, first, v, w);
+            float value[VEC];
+            values_of(w, value);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (value[e] >= least && value[e] > -INFINITY) {
+                    const int at = atomicAdd(&s.count, 1);
+                    if (at < kList) s.list[at] = key_of(value[e], first + v * VEC + e);
+                }
+        };
+        unsigned holders = __ballot_sync(0xFFFFFFFFu, any || sums.m >= least);
+        if (any) {
+            for (int v = begin + static_cast<int>(threadIdx.x); v < end && s.count <= kList; v += kThreads) offer(v);  // (a count beyond the list's size is all that is asked then)
+        } else {
+            for (; holders != 0; holders &= holders - 1) {  // a warp reads a thread's vectors again
+                const int thread = warp * 32 + __ffs(holders) - 1;
+                for (int v = begin + thread + lane * kThreads; v < end; v += 32 * kThreads) offer(v);
+            }
+        }
+        __syncthreads();
+        const int found = s.count;
+        if (found <= kList) rank_list(s, found, want);
+        else rank_by_passes(s, x, max(0, first + begin * VEC), min(n, first + end * VEC), want);
+    } else {
+        __syncthreads();
+    }
+    if (warp == 0) {
+        float p = lane < kWarps ? s.part[0][lane] : 0.0f, q = lane < kWarps ? s.part[1][lane] : 0.0f;
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) {
+            p += __shfl_xor_sync(0xFFFFFFFFu, p, off);
+            q += __shfl_xor_sync(0xFFFFFFFFu, q, off);
+        }
+        if (lane == 0) s.sums[0] = all, s.sums[1] = p, s.sums[2] = q;
+    }
+    if (n_blocks > 1) {
+        sync_cluster();
+        if (block != 0) {
+            sync_cluster();  // (until then the first block reads what is here)
+            return;
+        }
+    } else {
+        __syncthreads();
+    }
+
+    // The first block joins the others' sums (every warp for itself) and alternatives.
+    float top = kLow;
+    double total = 0.0, product = 0.0;
+    {
+        float m = kLow, p = 0.0f, q = 0.0f;
+        if (lane < n_blocks) {
+            const uint32_t at = in_cluster(s.sums, lane);
+            m = load_float(at), p = load_float(at + 4), q = load_float(at + 8);
+        }
+        top = m;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
+        const float g = ex2((m - top) * c);
+        total = static_cast<double>(p * g), product = static_cast<double>(g * fmaf(m - top, p, q));
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) {
+            total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
+            product += __shfl_xor_sync(0xFFFFFFFFu, product, off);
+        }
+    }
+    if (want > 0 && n_blocks > 1) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < n_blocks * want; i += kThreads) {  // (at most 512)
+            const Key key = load_key(in_cluster(s.best, i / want) + static_cast<uint32_t>(i % want) * 8);
+            s.list[i] = key;
+        }
+        __syncthreads();
+        rank_list(s, n_blocks * want, want);
+    }
+    if (n_blocks > 1) sync_cluster();  // nothing of the others is read any more
+
+    double log_sum = 0.0, entropy = 0.0, inverse = 1.0 / static_cast<double>(given);
+    const bool flat = given > 1e30f;
+    const bool in_reach = top > kLow && top < -kLow;
+    bool none = false;
+    if (greedy) {
+        none = s.best[0] == 0;
+    } else if (in_reach && ordinary) {
+        log_sum = log(total);
+        entropy = log_sum - product / (total * static_cast<double>(given));
+    } else {
+        if (!in_reach) {  // the largest as it is
+            float m = -INFINITY;
+            for (int i = threadIdx.x; i < n; i += kThreads) m = fmaxf(m, as_float(x[i]));
+            top = over_block(m, s.part[0], [](float p, float q) { return fmaxf(p, q); });
+        }
+        none = top == -INFINITY;
+        wide_sums(s, x, n, top, inverse, flat && top < INFINITY, log_sum, entropy);
+    }
+    auto answer = [&](float v, int place) -> float {
+        if (s.status != 0) return undefined();
+        if (none || !(v > -INFINITY)) return -INFINITY;
+        if (greedy) return place == place_of(s.best[0]) ? 0.0f : -INFINITY;
+        if (v == top || (flat && top < INFINITY)) return static_cast<float>(-log_sum);
+        return top == INFINITY ? -INFINITY : static_cast<float>((static_cast<double>(v) - static_cast<double>(top)) * inverse - log_sum);
+    };
+    if (threadIdx.x == 32) {
+        const int token = a.tokens[row];
+        a.out[row] = answer(token >= 0 && token < n ? as_float(x[token]) : -INFINITY, token);
+        if (a.entropy != nullptr) a.entropy[row] = s.status != 0 ? undefined() : none || greedy ? 0.0f : static_cast<float>(entropy > 0.0 ? entropy : 0.0);
+    }
+    if (threadIdx.x < static_cast<unsigned>(a.top)) {
+        const Key key = s.best[threadIdx.x];
+        const size_t to = static_cast<size_t>(row) * a.top + threadIdx.x;
+        a.top_ids[to] = key != 0 && s.status == 0 ? place_of(key) : -1;
+        if (a.top_out != nullptr) a.top_out[to] = answer(key != 0 ? value_of(key) : -INFINITY, place_of(key));
     }
 }
+
+template <typename T>
+struct Launcher {
+    static constexpr auto kKernel = logprobs_kernel<T>;
+    static void configure(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int rows, int blocks, bool overlap, cudaStream_t stream) {
+        cfg.gridDim = dim3(static_cast<unsigned>(rows) * static_cast<unsigned>(blocks));
+        cfg.blockDim = dim3(kThreads);
+        cfg.stream = stream;
+        cfg.attrs = attr;
+        cfg.numAttrs = launch_attributes(attr, overlap, blocks > 1 ? blocks : 0);
+    }
+    // clusters of so many blocks that fit on the GPU at once (cached; one device per process)
+    static int fit(int blocks) {
+        static int cached[kMaxBlocks + 1] = {};
+        if (cached[blocks] == 0) {
+            int n = 0;
+            cudaLaunchConfig_t cfg{};
+            cudaLaunchAttribute attr[2];
+            configure(cfg, attr, 1024, blocks, true, nullptr);
+            if ((blocks > 8 && cudaFuncSetAttribute(kKernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
+                cudaOccupancyMaxActiveClusters(&n, kKernel, &cfg) != cudaSuccess) {
+                (void)cudaGetLastError();
+                n = 0;
+            }
+            cached[blocks] = n > 0 ? n : -1;
+        }
+        return cached[blocks];
+    }
+    static cudaError_t launch(const LogprobsArgs &a, bool overlap, cudaStream_t stream) {
+        // As many blocks per row as all rows have room for side by side, of at least 4096 elements each.
+        int blocks = kMaxBlocks;
+        while (blocks > 1 && (a.vocab < blocks * 4096 || a.rows > fit(blocks))) blocks /= 2;
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute attr[2];
+        configure(cfg, attr, a.rows, blocks, overlap, stream);
+        return cudaLaunchKernelEx(&cfg, kKernel, a, blocks);
+    }
+};
 
 }  // namespace
 
 cudaError_t launch_logprobs(const LogprobsArgs &a, bool overlap, int sm_count, cudaStream_t stream) {
     (void)sm_count;
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[2];
-    cfg.gridDim = dim3(static_cast<unsigned>(a.rows));
-    cfg.blockDim = dim3(kThreads);
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = launch_attributes(attr, overlap, 0);
-    return a.elem == 2 ? cudaLaunchKernelEx(&cfg, logprobs_kernel<__half>, a) : cudaLaunchKernelEx(&cfg, logprobs_kernel<float>, a);
+    return a.elem == 2 ? Launcher<__half>::launch(a, overlap, stream) : Launcher<float>::launch(a, overlap, stream);
 }
 
 }  // namespace vqm
