@@ -16,9 +16,10 @@
 namespace vqm {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxBlocks = 16, kGroups = 32;
+constexpr int kMostWarps = 16, kMaxBlocks = 16;
 constexpr int kUnroll = 4;       // vectors of a thread in flight
 constexpr int kList = 1024;      // candidates
+constexpr int kParts = 16;       // of what a thread reads, whose largest logits are kept
 constexpr float kLow = -1e30f;   // what is below counts as that in differences, so that they and their products stay finite
 constexpr float kMostT = 1e20f, kLeastT = 1e-30f;  // temperatures that fp32 works with: a masked logit, at -1e30 or less, still comes to nothing
 
@@ -80,7 +81,7 @@ struct Sums {
     float m, s, u;  // the largest so far (kLow: none), S and U
 };
 template <typename T>
-__device__ __forceinline__ void add_vectors(Sums &a, const uint4 (&w)[kUnroll], float c) {
+__device__ __forceinline__ float add_vectors(Sums &a, const uint4 (&w)[kUnroll], float c) {  // returns their largest
     const float most = largest(w, static_cast<const T *>(nullptr));
     if (most > a.m) {
         const float d = a.m - most, f = ex2(d * c);
@@ -110,63 +111,70 @@ __device__ __forceinline__ void add_vectors(Sums &a, const uint4 (&w)[kUnroll], 
     both(u, u0, u1);
     a.s += s0 + s1;
     a.u += u0 + u1;
+    return most;
 }
 
 struct Shared {
-    float group[kGroups];           // largest logits of groups of 16 threads
-    float part[2][kWarps];
-    Key list[kList];                // candidates
-    Key best[kMaxTop];              // this block's alternatives, in order
-    Key key[kWarps];
-    double wide[kWarps];
+    float most[kMostWarps][32];     // largest logits of the threads
+    float part[2][kMostWarps];
+    alignas(16) Key list[kList];    // candidates
+    Key theirs[kMaxBlocks][kMaxTop];  // the blocks' alternatives
+    Key best[kMaxTop];              // this block's, in order
+    Key key[kMostWarps];
+    double wide[kMostWarps];
     float sums[3];                  // this block's m, S and U
     int count;
     unsigned status;
 };
 
-template <typename V, typename F>
-__device__ V over_block(V v, V (&room)[kWarps], F &&join) {
+template <int THREADS, typename V, typename F>
+__device__ V over_block(V v, V (&room)[kMostWarps], F &&join) {
     for (int off = 16; off > 0; off >>= 1) v = join(v, __shfl_xor_sync(0xFFFFFFFFu, v, off));
     __syncthreads();
     if ((threadIdx.x & 31) == 0) room[threadIdx.x >> 5] = v;
     __syncthreads();
     v = room[0];
-    for (int w = 1; w < kWarps; ++w) v = join(v, room[w]);
+    for (int w = 1; w < THREADS / 32; ++w) v = join(v, room[w]);
     return v;
 }
-// The first `want` of s.list[0, n) in order, by the whole block, to s.best; zeros behind the last.
+// The first `want` of s.list[0, n) in order, by the whole block, to s.best; zeros behind the last.  s.list has room for zeros up to a multiple of 4.
+template <int THREADS>
 __device__ __forceinline__ void rank_list(Shared &s, int n, int want) {
     if (threadIdx.x < kMaxTop) s.best[threadIdx.x] = 0;
+    if (threadIdx.x < 4 && n % 4 != 0 && threadIdx.x >= static_cast<unsigned>(n % 4)) s.list[n / 4 * 4 + threadIdx.x] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) {
+    for (int i = threadIdx.x; i < n; i += THREADS) {
         const Key mine = s.list[i];
         int before = 0;
-        for (int j = 0; j < n; ++j) before += s.list[j] > mine;
+        for (int j = 0; j < n; j += 4) {
+            const ulonglong2 p = *reinterpret_cast<const ulonglong2 *>(s.list + j), q = *reinterpret_cast<const ulonglong2 *>(s.list + j + 2);
+            before += (p.x > mine) + (p.y > mine) + (q.x > mine) + (q.y > mine);
+        }
         if (mine != 0 && before < want) s.best[before] = mine;
     }
     __syncthreads();
 }
 // The same of all of a slice [begin, end), a pass for each.
-template <typename T>
+template <typename T, int THREADS>
 static __device__ __noinline__ void rank_by_passes(Shared &s, const T *x, int begin, int end, int want) {
     Key last = ~0ull;
     for (int k = 0; k < want; ++k) {
         Key most = 0;
         if (last != 0)
-            for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += kThreads) {
+            for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += THREADS) {
                 const Key key = key_of(as_float(x[i]), i);
                 if (key < last && key > most) most = key;
             }
-        last = over_block(most, s.key, [](Key p, Key q) { return p > q ? p : q; });
+        last = over_block<THREADS>(most, s.key, [](Key p, Key q) { return p > q ? p : q; });
         if (threadIdx.x == 0) s.best[k] = last;
     }
     __syncthreads();
 }
 // log S and the entropy in 64 bits, by the whole block.
-template <typename T>
+template <typename T, int THREADS>
 static __device__ __noinline__ void wide_sums(Shared &s, const T *x, int n, float top, double inverse, bool flat, double &log_sum, double &entropy) {
     double sum = 0.0, weighted = 0.0;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
+    for (int i = threadIdx.x; i < n; i += THREADS) {
         const float v = as_float(x[i]);
         if (!(v > -INFINITY)) continue;
         const double d = v == top || flat ? 0.0 : top == INFINITY ? -INFINITY : (static_cast<double>(v) - static_cast<double>(top)) * inverse, e = exp(d);
@@ -174,8 +182,8 @@ static __device__ __noinline__ void wide_sums(Shared &s, const T *x, int n, floa
         if (e > 0.0) weighted -= e * d;
     }
     auto plus = [](double p, double q) { return p + q; };
-    sum = over_block(sum, s.wide, plus);
-    weighted = over_block(weighted, s.wide, plus);
+    sum = over_block<THREADS>(sum, s.wide, plus);
+    weighted = over_block<THREADS>(weighted, s.wide, plus);
     log_sum = sum > 0.0 ? log(sum) : 0.0;
     entropy = sum > 0.0 ? log_sum + weighted / sum : 0.0;
 }
@@ -200,10 +208,11 @@ __device__ __forceinline__ void sync_cluster() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const LogprobsArgs a, const int n_blocks) {
+template <typename T, int THREADS, int PER_SM>
+__global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const LogprobsArgs a, const int n_blocks) {
     __shared__ Shared s;
-    constexpr int VEC = kVec<T>;
+    __shared__ float part_room[kParts * THREADS];
+    constexpr int VEC = kVec<T>, WARPS = THREADS / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = a.vocab;
     const int row = static_cast<int>(blockIdx.x) / n_blocks, block = static_cast<int>(blockIdx.x) % n_blocks;
     const T *x = static_cast<const T *>(a.logits) + static_cast<size_t>(row) * n;
@@ -222,25 +231,35 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const LogprobsArg
     const int first = first_of(x);  // index of vector 0's first element
     const int vectors = (n - first + VEC - 1) / VEC;
     const int begin = static_cast<int>(static_cast<long long>(vectors) * block / n_blocks), end = static_cast<int>(static_cast<long long>(vectors) * (block + 1) / n_blocks);
+    const int per_part = (end - begin + kParts * kUnroll * THREADS - 1) / (kParts * kUnroll * THREADS);  // turns of the loop
+    const int want = a.top > 0 ? a.top : greedy ? 1 : 0;
+    float(*const part_most)[THREADS] = reinterpret_cast<float(*)[THREADS]>(part_room);
     Sums sums{kLow, 0.0f, 0.0f};
+    float in_part = -INFINITY;
+    int part = 0, turn = 0;
 #pragma unroll 1
-    for (int v = begin + static_cast<int>(threadIdx.x); v < end; v += kUnroll * kThreads) {
+    for (int v = begin + static_cast<int>(threadIdx.x); v < end; v += kUnroll * THREADS) {
         uint4 w[kUnroll];
 #pragma unroll
         for (int i = 0; i < kUnroll; ++i) {
-            if (v + i * kThreads < end) load_vec(x, n, first, v + i * kThreads, w[i]);
+            if (v + i * THREADS < end) load_vec(x, n, first, v + i * THREADS, w[i]);
             else w[i] = make_uint4(kNothing<T>, kNothing<T>, kNothing<T>, kNothing<T>);
         }
-        add_vectors<T>(sums, w, c);
+        in_part = fmaxf(in_part, add_vectors<T>(sums, w, c));
+        if (want > 0 && ++turn == per_part) {
+            part_most[part++][threadIdx.x] = in_part;
+            in_part = -INFINITY;
+            turn = 0;
+        }
     }
+    if (turn > 0) part_most[part++][threadIdx.x] = in_part;
 
-    // the largest of each group of 16 threads, and the block's
-    float most = sums.m;
-#pragma unroll
-    for (int off = 8; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, off));
-    if ((lane & 15) == 0) s.group[warp * 2 + (lane >> 4)] = most;
+    // the largest of each group, the threads of one place in their warps, and the block's
+    s.most[warp][lane] = sums.m;
     __syncthreads();
-    const float mine = s.group[lane];
+    float mine = s.most[0][lane];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) mine = fmaxf(mine, s.most[w][lane]);
     float all = mine;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, off));
@@ -253,21 +272,18 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const LogprobsArg
     }
     if (lane == 0) s.part[0][warp] = sum, s.part[1][warp] = weighted;
 
-    const int want = a.top > 0 ? a.top : greedy ? 1 : 0;
     if (want > 0) {
         // the want-th largest group; where that is out of what the sums tell apart, all logits are candidates
         int before = 0;
 #pragma unroll
-        for (int j = 0; j < kGroups; ++j) {
+        for (int j = 0; j < 32; ++j) {
             const float other = __shfl_sync(0xFFFFFFFFu, mine, j);
             before += other > mine || (other == mine && j < lane);
         }
         float least = __shfl_sync(0xFFFFFFFFu, mine, __ffs(__ballot_sync(0xFFFFFFFFu, before == want - 1)) - 1);
         const bool any = !(least > kLow);
         if (any) least = -INFINITY;
-        auto offer = [&](int v) {
-            uint4 w;
-            load_vec(x, n, first, v, w);
+        auto offer = [&](const uint4 &w, int v) {
             float value[VEC];
             values_of(w, value);
 #pragma unroll
@@ -277,24 +293,41 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const LogprobsArg
                     if (at < kList) s.list[at] = key_of(value[e], first + v * VEC + e);
                 }
         };
-        unsigned holders = __ballot_sync(0xFFFFFFFFu, any || sums.m >= least);
         if (any) {
-            for (int v = begin + static_cast<int>(threadIdx.x); v < end && s.count <= kList; v += kThreads) offer(v);  // (a count beyond the list's size is all that is asked then)
+            for (int v = begin + static_cast<int>(threadIdx.x); v < end && s.count <= kList; v += THREADS) {  // (a count beyond the list's size is all that is asked then)
+                uint4 w;
+                load_vec(x, n, first, v, w);
+                offer(w, v);
+            }
         } else {
-            for (; holders != 0; holders &= holders - 1) {  // a warp reads a thread's vectors again
-                const int thread = warp * 32 + __ffs(holders) - 1;
-                for (int v = begin + thread + lane * kThreads; v < end; v += 32 * kThreads) offer(v);
+            // a thread reads those parts again that hold one
+            unsigned parts = 0;
+            if (sums.m >= least)
+                for (int p = 0; p < part; ++p) parts |= part_most[p][threadIdx.x] >= least ? 1u << p : 0u;
+            for (; parts != 0; parts &= parts - 1) {
+                const int from = begin + static_cast<int>(threadIdx.x) + (__ffs(parts) - 1) * per_part * kUnroll * THREADS;
+                for (int t = 0; t < per_part; ++t) {
+                    uint4 w[kUnroll];
+#pragma unroll
+                    for (int i = 0; i < kUnroll; ++i) {
+                        const int v = from + (t * kUnroll + i) * THREADS;
+                        if (v < end) load_vec(x, n, first, v, w[i]);
+                        else w[i] = make_uint4(kNothing<T>, kNothing<T>, kNothing<T>, kNothing<T>);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kUnroll; ++i) offer(w[i], from + (t * kUnroll + i) * THREADS);
+                }
             }
         }
         __syncthreads();
         const int found = s.count;
-        if (found <= kList) rank_list(s, found, want);
-        else rank_by_passes(s, x, max(0, first + begin * VEC), min(n, first + end * VEC), want);
+        if (found <= kList) rank_list<THREADS>(s, found, want);
+        else rank_by_passes<T, THREADS>(s, x, max(0, first + begin * VEC), min(n, first + end * VEC), want);
     } else {
         __syncthreads();
     }
     if (warp == 0) {
-        float p = lane < kWarps ? s.part[0][lane] : 0.0f, q = lane < kWarps ? s.part[1][lane] : 0.0f;
+        float p = lane < WARPS ? s.part[0][lane] : 0.0f, q = lane < WARPS ? s.part[1][lane] : 0.0f;
 #pragma unroll
         for (int off = 8; off > 0; off >>= 1) {
             p += __shfl_xor_sync(0xFFFFFFFFu, p, off);
@@ -333,19 +366,38 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const LogprobsArg
         }
     }
     if (want > 0 && n_blocks > 1) {
+        // Of lists in order, if r of them have a q-th key no less than some key, and r q is `want` at least, what is under that key is not asked for.
+        for (int i = threadIdx.x; i < n_blocks * want; i += THREADS) s.theirs[i / want][i % want] = load_key(in_cluster(s.best, i / want) + static_cast<uint32_t>(i % want) * 8);
+        if (threadIdx.x == 0) s.count = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < n_blocks * want; i += kThreads) {  // (at most 512)
-            const Key key = load_key(in_cluster(s.best, i / want) + static_cast<uint32_t>(i % want) * 8);
-            s.list[i] = key;
+        const int q = warp + 1, r = (want + q - 1) / q;
+        Key least = 0;
+        if (q <= want && r <= n_blocks) {
+            const Key key = lane < n_blocks ? s.theirs[lane][q - 1] : 0;
+            int before = 0;
+#pragma unroll
+            for (int j = 0; j < kMaxBlocks; ++j) {
+                const Key other = __shfl_sync(0xFFFFFFFFu, key, j);
+                before += other > key || (other == key && j < lane);
+            }
+            least = __shfl_sync(0xFFFFFFFFu, key, __ffs(__ballot_sync(0xFFFFFFFFu, before == r - 1)) - 1);
+        }
+        if (lane == 0) s.key[warp] = least;
+        __syncthreads();
+        for (int w = 0; w < WARPS; ++w) least = s.key[w] > least ? s.key[w] : least;
+        for (int i = threadIdx.x; i < n_blocks * want; i += THREADS) {
+            const Key key = s.theirs[i / want][i % want];
+            if (key != 0 && key >= least) s.list[atomicAdd(&s.count, 1)] = key;
         }
         __syncthreads();
-        rank_list(s, n_blocks * want, want);
+        rank_list<THREADS>(s, s.count, want);
     }
     if (n_blocks > 1) sync_cluster();  // nothing of the others is read any more
 
+    const bool in_reach = top > kLow && top < -kLow;
+    if (warp > 1 && (greedy || (in_reach && ordinary))) return;
     double log_sum = 0.0, entropy = 0.0, inverse = 1.0 / static_cast<double>(given);
     const bool flat = given > 1e30f;
-    const bool in_reach = top > kLow && top < -kLow;
     bool none = false;
     if (greedy) {
         none = s.best[0] == 0;
@@ -355,11 +407,11 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const LogprobsArg
     } else {
         if (!in_reach) {  // the largest as it is
             float m = -INFINITY;
-            for (int i = threadIdx.x; i < n; i += kThreads) m = fmaxf(m, as_float(x[i]));
-            top = over_block(m, s.part[0], [](float p, float q) { return fmaxf(p, q); });
+            for (int i = threadIdx.x; i < n; i += THREADS) m = fmaxf(m, as_float(x[i]));
+            top = over_block<THREADS>(m, s.part[0], [](float p, float q) { return fmaxf(p, q); });
         }
         none = top == -INFINITY;
-        wide_sums(s, x, n, top, inverse, flat && top < INFINITY, log_sum, entropy);
+        wide_sums<T, THREADS>(s, x, n, top, inverse, flat && top < INFINITY, log_sum, entropy);
     }
     auto answer = [&](float v, int place) -> float {
         if (s.status != 0) return undefined();
@@ -381,15 +433,17 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const LogprobsArg
     }
 }
 
-template <typename T>
+// A block of 256 threads for each row; where there are few rows, the blocks of a cluster, of 512.
+template <typename T, bool SHARED>
 struct Launcher {
-    static constexpr auto kKernel = logprobs_kernel<T>;
+    static constexpr int kThreads = SHARED ? 512 : 256;
+    static constexpr auto kKernel = logprobs_kernel<T, kThreads, SHARED ? 2 : 5>;
     static void configure(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int rows, int blocks, bool overlap, cudaStream_t stream) {
         cfg.gridDim = dim3(static_cast<unsigned>(rows) * static_cast<unsigned>(blocks));
         cfg.blockDim = dim3(kThreads);
         cfg.stream = stream;
         cfg.attrs = attr;
-        cfg.numAttrs = launch_attributes(attr, overlap, blocks > 1 ? blocks : 0);
+        cfg.numAttrs = launch_attributes(attr, overlap, SHARED ? blocks : 0);
     }
     // clusters of so many blocks that fit on the GPU at once (cached; one device per process)
     static int fit(int blocks) {
@@ -408,22 +462,27 @@ struct Launcher {
         }
         return cached[blocks];
     }
-    static cudaError_t launch(const LogprobsArgs &a, bool overlap, cudaStream_t stream) {
-        // As many blocks per row as all rows have room for side by side, of at least 4096 elements each.
-        int blocks = kMaxBlocks;
-        while (blocks > 1 && (a.vocab < blocks * 4096 || a.rows > fit(blocks))) blocks /= 2;
+    static cudaError_t launch(const LogprobsArgs &a, int blocks, bool overlap, cudaStream_t stream) {
         cudaLaunchConfig_t cfg{};
         cudaLaunchAttribute attr[2];
         configure(cfg, attr, a.rows, blocks, overlap, stream);
         return cudaLaunchKernelEx(&cfg, kKernel, a, blocks);
     }
 };
+template <typename T>
+cudaError_t launch(const LogprobsArgs &a, bool overlap, cudaStream_t stream) {
+    // As many blocks of 512 threads per row as all rows have room for side by side, of at least 4096 elements each.  With more rows, or short ones, what counts is how many
+    // rows at different steps an SM holds: five blocks of 256 threads.  (151936, fp32, 20 alternatives: 149 rows 33 us and 48, 300 rows 59 and 56; 300 rows of 5000 11 and 7.)
+    for (int blocks = kMaxBlocks; blocks > 0; blocks /= 2)
+        if (a.vocab >= (blocks > 1 ? blocks : 2) * 4096 && a.rows <= Launcher<T, true>::fit(blocks)) return Launcher<T, true>::launch(a, blocks, overlap, stream);
+    return Launcher<T, false>::launch(a, 1, overlap, stream);
+}
 
 }  // namespace
 
 cudaError_t launch_logprobs(const LogprobsArgs &a, bool overlap, int sm_count, cudaStream_t stream) {
     (void)sm_count;
-    return a.elem == 2 ? Launcher<__half>::launch(a, overlap, stream) : Launcher<float>::launch(a, overlap, stream);
+    return a.elem == 2 ? launch<__half>(a, overlap, stream) : launch<float>(a, overlap, stream);
 }
 
 }  // namespace vqm
