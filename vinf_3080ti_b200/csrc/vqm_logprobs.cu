@@ -12,6 +12,7 @@
 
 #include "vqm_kernels.h"
 #include "vqm_logits.cuh"
+#include "vqm_packed.cuh"
 
 namespace vqm {
 namespace {
@@ -36,30 +37,6 @@ __device__ __forceinline__ float value_of(Key key) {
     return __uint_as_float((b & 0x80000000u) != 0 ? b & 0x7FFFFFFFu : ~b);
 }
 __device__ __forceinline__ float undefined() { return __uint_as_float(0x7FFFFFFFu); }
-
-// Two fp32 at a time.
-using Two = unsigned long long;
-__device__ __forceinline__ Two two(float x, float y) {
-    Two v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
-    return v;
-}
-__device__ __forceinline__ void both(Two v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ Two add2(Two a, Two b) {
-    Two v;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-    return v;
-}
-__device__ __forceinline__ Two mul2(Two a, Two b) {
-    Two v;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-    return v;
-}
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
-    Two v;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
-    return v;
-}
 
 // The largest of some vectors (NaN counts as nothing).
 __device__ __forceinline__ float largest(const uint4 (&w)[kUnroll], const float *) {

@@ -4,6 +4,7 @@
 #include <cuda_fp16.h>
 
 #include "vqm_kernels.h"
+#include "vqm_packed.cuh"
 
 namespace vqm {
 namespace {
@@ -11,15 +12,15 @@ namespace {
 constexpr float kMost = 448.0f;  // of e4m3
 
 // silu(x) * x2.  With h = exp(-|x| / 2) neither a far negative x, whose silu is exp(x) x, nor a large x2 leaves fp32 on the way.  h = 2^t (1 + d), where t is the
-// argument in fp32 and d what its rounding has left, times ln 2.
+// argument in fp32 and d what its rounding has left, times ln 2.  (x below -174 counts as gated off; what is undefined comes back with x itself.)
 __device__ __forceinline__ float gated(float x, float x2) {
     constexpr float kHalfLog2e = 0.72134752044448170f, kRest = static_cast<float>(0.72134752044448170368 - static_cast<double>(kHalfLog2e)), kLn2 = 0.69314718055994531f;
-    const float y = -fabsf(x), t = y * kHalfLog2e, d = fmaf(y, kRest, fmaf(y, kHalfLog2e, -t));
+    const float y = fmaxf(-fabsf(x), -400.0f), t = y * kHalfLog2e, d = fmaf(y, kRest, fmaf(y, kHalfLog2e, -t));
     float h, r;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(h) : "f"(t));
-    h = x == x && y >= -400.0f ? fmaf(h, d * kLn2, h) : x == x ? 0.0f : x;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(t));
+    h = fmaf(h, d * kLn2, h);
     const float g = x < 0.0f ? h : 1.0f;
-    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(fmaf(h, h, 1.0f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(h, h, 1.0f)));
     return x * g * r * (x2 * g);
 }
 
@@ -30,47 +31,37 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return out;
 }
 
+constexpr int kEach = 16;                 // values of a thread
+constexpr int kLanes = kF8Block / kEach;  // threads of a block of columns
+// They are groups of as many as 16 bytes hold; a group of each of the kLanes threads, then the next group of each: what is read or written together lies together.
+template <typename T>
+constexpr int kGroup = 16 / static_cast<int>(sizeof(T));
+template <typename T>
+__device__ __forceinline__ int column(int e) {  // of a thread's value e, in its block of columns
+    constexpr int G = kGroup<T>;
+    return e / G * G * kLanes + static_cast<int>(threadIdx.x % kLanes) * G + e % G;
+}
+
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float rounded(float v, const float *) { return v; }
 __device__ __forceinline__ __half rounded(float v, const __half *) { return __float2half_rn(v); }
-
-// Eight columns from `c` on, zeros from the last on; vec: rows begin on 16 bytes.
-__device__ __forceinline__ void load8(const float *p, int left, bool vec, float (&v)[8]) {
-    if (vec && left >= 8) {
-        const float4 x = *reinterpret_cast<const float4 *>(p), y = *reinterpret_cast<const float4 *>(p + 4);
-        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = e < left ? p[e] : 0.0f;
-    }
+__device__ __forceinline__ void load(const float *p, float *v) {
+    const float4 x = *reinterpret_cast<const float4 *>(p);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
 }
-__device__ __forceinline__ void load8(const __half *p, int left, bool vec, float (&v)[8]) {
-    if (vec && left >= 8) {
-        const uint4 w = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+__device__ __forceinline__ void load(const __half *p, float *v) {
+    const uint4 w = *reinterpret_cast<const uint4 *>(p);
+    const uint32_t r[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r[e]));
-            v[2 * e] = f.x, v[2 * e + 1] = f.y;
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = e < left ? __half2float(p[e]) : 0.0f;
+    for (int e = 0; e < 4; ++e) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r[e]));
+        v[2 * e] = f.x, v[2 * e + 1] = f.y;
     }
 }
 // Rounds the values to the buffer's type, and stores them.
-__device__ __forceinline__ void store8(float *p, int left, bool vec, const float (&v)[8]) {
-    if (vec && left >= 8) {
-        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e < left) p[e] = v[e];
-    }
-}
-__device__ __forceinline__ void store8(__half *p, int left, bool vec, float (&v)[8]) {
+__device__ __forceinline__ void store(float *p, float *v) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store(__half *p, float *v) {
     uint32_t r[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -79,67 +70,83 @@ __device__ __forceinline__ void store8(__half *p, int left, bool vec, float (&v)
         const float2 f = __half22float2(h);
         v[2 * e] = f.x, v[2 * e + 1] = f.y;
     }
-    if (vec && left >= 8) {
-        *reinterpret_cast<uint4 *>(p) = make_uint4(r[0], r[1], r[2], r[3]);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e < left) p[e] = __ushort_as_half(static_cast<unsigned short>(r[e / 2] >> (16 * (e & 1))));
-    }
+    *reinterpret_cast<uint4 *>(p) = make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// The values of eight columns of a row from c on, before the norm, zeros behind the last; the sums are stored.  By all lanes of a warp, of which 16 side by side have 128 columns;
-// c < 0: none.  Rows that do not begin on 16 bytes are read (and sums written) 16 columns after 16 columns, and turned in shared memory.
-constexpr int kTurn = 128 + 16;  // floats of 16 lanes (half a warp's banks apart)
+// A thread's values of the block of columns from c0 on, before the norm, zeros behind the row's last; the sums are stored.  By all lanes of a warp; c0 < 0: none.
+// VEC: rows begin on 16 bytes, so groups are whole.  Others are read (and sums written) kLanes columns after kLanes columns, and turned in shared memory.
+constexpr int kTurn = kF8Block + kLanes;  // floats of a block of columns (the others' in other banks)
 template <typename T, bool VEC>
-__device__ __forceinline__ void values8(const RowsF8Args &a, size_t row, int c, float *room, float (&v)[8]) {
+__device__ __forceinline__ void values(const RowsF8Args &a, size_t row, int c0, float *room, float (&v)[kEach]) {
+    const size_t at = row * a.cols;
+    const T *x = static_cast<const T *>(a.x) + at, *second = static_cast<const T *>(a.residual != nullptr ? a.residual : a.x2) + at;
+    T *total = static_cast<T *>(a.total) + at;
     if constexpr (VEC) {
-        const size_t at = row * a.cols + c;
-        const int left = c < 0 ? 0 : a.cols - c;
-        if (left <= 0) {
+        constexpr int G = kGroup<T>;
+        float more[kEach];
+        int c[kEach / G];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-            return;
+        for (int g = 0; g < kEach / G; ++g) {
+            c[g] = c0 >= 0 && c0 + column<T>(g * G) < a.cols ? c0 + column<T>(g * G) : -1;
+#pragma unroll
+            for (int e = 0; e < G; ++e) v[g * G + e] = more[g * G + e] = 0.0f;
+            if (c[g] >= 0) load(x + c[g], v + g * G);
         }
-        load8(static_cast<const T *>(a.x) + at, left, true, v);
+        if (a.residual != nullptr || a.x2 != nullptr)
+#pragma unroll
+            for (int g = 0; g < kEach / G; ++g)
+                if (c[g] >= 0) load(second + c[g], more + g * G);
         if (a.residual != nullptr) {
-            float r[8];
-            load8(static_cast<const T *>(a.residual) + at, left, true, r);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += r[e];
-            store8(static_cast<T *>(a.total) + at, left, true, v);
+            for (int e = 0; e < kEach; ++e) v[e] += more[e];
+#pragma unroll
+            for (int g = 0; g < kEach / G; ++g)
+                if (c[g] >= 0) store(total + c[g], v + g * G);
         } else if (a.x2 != nullptr) {
-            float x2[8];
-            load8(static_cast<const T *>(a.x2) + at, left, true, x2);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = gated(v[e], x2[e]);
+            for (int e = 0; e < kEach; ++e) v[e] = gated(v[e], more[e]);
         }
     } else {
-        const int lane16 = static_cast<int>(threadIdx.x & 15), c0 = (c < 0 ? a.cols : c - lane16 * 8) + lane16;
-        const size_t at = row * a.cols + c0;
-        float *const turn = room + threadIdx.x / 16 * kTurn;
-        float more[8] = {};
-        const T *second = static_cast<const T *>(a.residual != nullptr ? a.residual : a.x2);
+        const int lane = static_cast<int>(threadIdx.x % kLanes), c = (c0 < 0 ? a.cols : c0) + lane;
+        float *const turn = room + threadIdx.x / kLanes * kTurn;
+        float more[kEach] = {};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = c0 + e * 16 < a.cols ? as_float(static_cast<const T *>(a.x)[at + e * 16]) : 0.0f;
-        if (second != nullptr)
+        for (int e = 0; e < kEach; ++e) v[e] = c + e * kLanes < a.cols ? as_float(x[c + e * kLanes]) : 0.0f;
+        if (a.residual != nullptr || a.x2 != nullptr)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) more[e] = c0 + e * 16 < a.cols ? as_float(second[at + e * 16]) : 0.0f;
+            for (int e = 0; e < kEach; ++e) more[e] = c + e * kLanes < a.cols ? as_float(second[c + e * kLanes]) : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < kEach; ++e) {
             if (a.residual != nullptr) {
-                const T total = rounded(v[e] + more[e], static_cast<const T *>(nullptr));
-                if (c0 + e * 16 < a.cols) static_cast<T *>(a.total)[at + e * 16] = total;
-                v[e] = as_float(total);
+                const T sum = rounded(v[e] + more[e], static_cast<const T *>(nullptr));
+                if (c + e * kLanes < a.cols) total[c + e * kLanes] = sum;
+                v[e] = as_float(sum);
             } else if (a.x2 != nullptr) {
                 v[e] = gated(v[e], more[e]);
             }
-            turn[lane16 + e * 16] = v[e];
+            turn[lane + e * kLanes] = v[e];
         }
         __syncwarp();
-        const float4 p = *reinterpret_cast<const float4 *>(turn + lane16 * 8), q = *reinterpret_cast<const float4 *>(turn + lane16 * 8 + 4);
+#pragma unroll
+        for (int e = 0; e < kEach; e += 4) {
+            const float4 p = *reinterpret_cast<const float4 *>(turn + column<T>(e));
+            v[e] = p.x, v[e + 1] = p.y, v[e + 2] = p.z, v[e + 3] = p.w;
+        }
         __syncwarp();
-        v[0] = p.x, v[1] = p.y, v[2] = p.z, v[3] = p.w, v[4] = q.x, v[5] = q.y, v[6] = q.z, v[7] = q.w;
+    }
+}
+// The norm's weights of a thread's values, zeros behind the last.
+template <typename T, bool VEC>
+__device__ __forceinline__ void weights(const RowsF8Args &a, int c0, float (&g)[kEach]) {
+#pragma unroll
+    for (int e = 0; e < kEach; e += 4) {
+        const int c = c0 + column<T>(e);
+        if (VEC ? c < a.cols : c + 4 <= a.cols) {  // (buffers and tensors are 16-byte aligned)
+            load(a.norm_w + c, g + e);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) g[e + i] = !VEC && c + i < a.cols ? a.norm_w[c + i] : 0.0f;
+        }
     }
 }
 // v / scale as fp32 rounds it.  With y = 1 / scale rounded, q = v y and the remainder v - q scale (which one fused multiply and add gives exactly), q + remainder y rounds
@@ -148,49 +155,75 @@ __device__ __forceinline__ float quotient(float v, float scale, float y) {
     const float q = v * y;
     return fmaf(fmaf(-q, scale, v), y, q);
 }
-// Eight columns of a row to 8 bits; 16 lanes side by side have a block of columns.  All lanes of the warp; on: the columns are in the row's pitch.
-__device__ __forceinline__ void quantise8(const RowsF8Args &a, size_t row, int c, bool on, const float (&n)[8]) {
-    uint32_t most = 0;
+__device__ __forceinline__ Two quotients(Two v, Two minus_scale, Two y) {
+    const Two q = mul2(v, y);
+    return fma2(fma2(q, minus_scale, v), y, q);
+}
+// The largest magnitude; what is undefined stays so.
+__device__ __forceinline__ float most_of(float a, float b) {
+    float v;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return v;
+}
+// A thread's values of the block of columns from c0 on to 8 bits.  All lanes of the warp; c0 < 0, or beyond the row's last: none.
+template <typename T>
+__device__ __forceinline__ void quantise(const RowsF8Args &a, size_t row, int c0, const float (&n)[kEach]) {
+    float m[kEach / 2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(n[e]) & 0x7FFFFFFFu);  // (what is undefined is larger than what is infinite)
+    for (int e = 0; e < kEach / 2; ++e) m[e] = most_of(n[e], n[e + kEach / 2]);
 #pragma unroll
-    for (int off = 8; off > 0; off >>= 1) most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, off));
-    const bool fine = most < 0x7F800000u;
-    const float scale = fine ? __uint_as_float(most) / kMost : __uint_as_float(0x7FFFFFFFu);
-    if (!on) return;
-    if (c % kF8Block == 0) a.scales[static_cast<size_t>(c / kF8Block) * f8_scale_pitch(a.ntok) + row] = scale;
-    uint2 q = make_uint2(0, 0);
+    for (int w = kEach / 4; w > 0; w /= 2)
+#pragma unroll
+        for (int e = 0; e < w; ++e) m[e] = most_of(m[e], m[e + w]);
+    float most = m[0];
+#pragma unroll
+    for (int off = kLanes / 2; off > 0; off >>= 1) most = most_of(most, __shfl_xor_sync(0xFFFFFFFFu, most, off));
+    if (c0 < 0 || c0 >= a.cols) return;
+    float scale = quotient(most, kMost, 1.0f / kMost);
+    uint32_t q[kEach / 4] = {};
     if (scale >= 0x1p-80f && scale <= 0x1p100f) {
         const float y = 1.0f / scale;
-        q.x = pack2(quotient(n[0], scale, y), quotient(n[1], scale, y)) | pack2(quotient(n[2], scale, y), quotient(n[3], scale, y)) << 16;
-        q.y = pack2(quotient(n[4], scale, y), quotient(n[5], scale, y)) | pack2(quotient(n[6], scale, y), quotient(n[7], scale, y)) << 16;
-    } else if (fine && scale > 0.0f) {
-        q.x = pack2(n[0] / scale, n[1] / scale) | pack2(n[2] / scale, n[3] / scale) << 16;
-        q.y = pack2(n[4] / scale, n[5] / scale) | pack2(n[6] / scale, n[7] / scale) << 16;
+        const Two yy = two(y, y), minus = two(-scale, -scale);
+#pragma unroll
+        for (int i = 0; i < kEach / 4; ++i) {
+            float t[4];
+            both(quotients(two(n[4 * i], n[4 * i + 1]), minus, yy), t[0], t[1]);
+            both(quotients(two(n[4 * i + 2], n[4 * i + 3]), minus, yy), t[2], t[3]);
+            q[i] = pack2(t[0], t[1]) | pack2(t[2], t[3]) << 16;
+        }
+    } else {
+        scale = most < INFINITY ? most / kMost : __uint_as_float(0x7FFFFFFFu);
+        if (scale > 0.0f)
+#pragma unroll
+            for (int i = 0; i < kEach / 4; ++i)
+                q[i] = pack2(n[4 * i] / scale, n[4 * i + 1] / scale) | pack2(n[4 * i + 2] / scale, n[4 * i + 3] / scale) << 16;
     }
-    *reinterpret_cast<uint2 *>(a.q + row * f8_pitch(a.cols) + c) = q;
+    if (threadIdx.x % kLanes == 0) a.scales[static_cast<size_t>(c0 / kF8Block) * f8_scale_pitch(a.ntok) + row] = scale;
+    uint8_t *const to = a.q + row * f8_pitch(a.cols) + c0;
+    const int left = static_cast<int>(f8_pitch(a.cols)) - c0;  // (a multiple of 16)
+    if constexpr (kGroup<T> == 8) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+            if (column<T>(8 * g) < left) *reinterpret_cast<uint2 *>(to + column<T>(8 * g)) = make_uint2(q[2 * g], q[2 * g + 1]);
+    } else {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            if (column<T>(4 * g) < left) *reinterpret_cast<uint32_t *>(to + column<T>(4 * g)) = q[g];
+    }
 }
 
-// Without a norm the blocks of columns have nothing to do with one another: 16 lanes each, UNITS of them, wherever they lie.
-template <typename T, int UNITS, bool VEC>
-__global__ void __launch_bounds__(256) blocks_kernel(const RowsF8Args a, unsigned n_units, int row0) {
+constexpr int kBlocksThreads = 256;
+// Without a norm the blocks of columns have nothing to do with one another: kLanes threads each, wherever they lie.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kBlocksThreads, 5) blocks_kernel(const RowsF8Args a, unsigned n_units, int row0) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    __shared__ __align__(16) float s_turn[VEC ? 1 : 16 * kTurn];
-    const unsigned n_blocks = static_cast<unsigned>(f8_blocks(a.cols)), step = gridDim.x * 16u, at = blockIdx.x * 16u + threadIdx.x / 16;
-    float v[UNITS][8];
-    unsigned row[UNITS];
-    int c[UNITS];
-#pragma unroll
-    for (int i = 0; i < UNITS; ++i) {
-        const unsigned unit = at + i * step;
-        row[i] = unit / n_blocks;
-        c[i] = unit < n_units ? static_cast<int>(unit - row[i] * n_blocks) * kF8Block + static_cast<int>(threadIdx.x & 15) * 8 : -1;
-        row[i] += row0;
-        values8<T, VEC>(a, row[i], c[i], s_turn, v[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < UNITS; ++i) quantise8(a, row[i], c[i], c[i] >= 0 && c[i] < f8_pitch(a.cols), v[i]);
+    __shared__ __align__(16) float s_turn[VEC ? 1 : kBlocksThreads / kLanes * kTurn];
+    const unsigned n_blocks = static_cast<unsigned>(f8_blocks(a.cols)), unit = blockIdx.x * (kBlocksThreads / kLanes) + threadIdx.x / kLanes, row = unit / n_blocks;
+    const int c0 = unit < n_units ? static_cast<int>(unit - row * n_blocks) * kF8Block : -1;
+    float v[kEach];
+    values<T, VEC>(a, row0 + row, c0, s_turn, v);
+    quantise<T>(a, row0 + row, c0, v);
 }
 
 __device__ __forceinline__ double over_block(double v, double *room) {  // (a warp, or all warps of the block)
@@ -206,26 +239,31 @@ __device__ __forceinline__ double over_block(double v, double *room) {  // (a wa
     return v;
 }
 
-// With a norm: a row by a block, or (ONE_WARP) by each warp; values stay in registers, PARTS times eight of a thread.
+// With a norm: a row by a block, or (ONE_WARP) by each warp; values stay in registers, PARTS times kEach of a thread.
 template <typename T, int PARTS, bool ONE_WARP, bool VEC, int THREADS, int PER_SM>
 __global__ void __launch_bounds__(THREADS, PER_SM) norm_kernel(const RowsF8Args a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __shared__ float s_sum[32];
     __shared__ double s_wide[32];
-    __shared__ __align__(16) float s_turn[VEC ? 1 : THREADS / 16 * kTurn];
+    __shared__ __align__(16) float s_turn[VEC ? 1 : THREADS / kLanes * kTurn];
     const int lane = threadIdx.x & 31, threads = ONE_WARP ? 32 : static_cast<int>(blockDim.x), mine = ONE_WARP ? lane : static_cast<int>(threadIdx.x);
     const size_t row = ONE_WARP ? static_cast<size_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
     if (ONE_WARP && row >= static_cast<size_t>(a.ntok)) return;
-    float v[PARTS][8];
-    float sum = 0.0f;
+    float v[PARTS][kEach];
+    Two squares = 0;
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) {
-        const int c = (i * threads + mine) * 8;
-        values8<T, VEC>(a, row, c, s_turn, v[i]);
+        values<T, VEC>(a, row, (i * threads + mine) / kLanes * kF8Block, s_turn, v[i]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(v[i][e], v[i][e], sum);
+        for (int e = 0; e < kEach; e += 2) {
+            const Two x = two(v[i][e], v[i][e + 1]);
+            squares = fma2(x, x, squares);
+        }
     }
+    float sum, other;
+    both(squares, sum, other);
+    sum += other;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
     if constexpr (!ONE_WARP) {
@@ -234,29 +272,38 @@ __global__ void __launch_bounds__(THREADS, PER_SM) norm_kernel(const RowsF8Args 
         sum = 0.0f;
         for (int w = 0; w < threads / 32; ++w) sum += s_sum[w];
     }
-    float factor = 0.0f;
-    double wide_factor = 0.0;
-    const bool wide = !(sum > 1e-30f && sum < 1e37f);  // squares that fp32 may not hold: in 64 bits
-    if (wide) {
+    if (sum > 1e-30f && sum < 1e37f) {
+        const float factor = 1.0f / sqrtf(sum / static_cast<float>(a.cols) + a.eps);
+        const Two f = two(factor, factor);
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+            const int c0 = (i * threads + mine) / kLanes * kF8Block;
+            if (c0 < a.cols) {
+                float g[kEach];
+                weights<T, VEC>(a, c0, g);
+#pragma unroll
+                for (int e = 0; e < kEach; e += 2) both(mul2(mul2(two(v[i][e], v[i][e + 1]), f), two(g[e], g[e + 1])), v[i][e], v[i][e + 1]);
+            }
+            quantise<T>(a, row, c0, v[i]);
+        }
+    } else {  // squares that fp32 may not hold: in 64 bits
         double total = 0.0;
 #pragma unroll
         for (int i = 0; i < PARTS; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) total = fma(static_cast<double>(v[i][e]), static_cast<double>(v[i][e]), total);
-        wide_factor = 1.0 / sqrt(over_block(total, ONE_WARP ? nullptr : s_wide) / a.cols + static_cast<double>(a.eps));
-    } else {
-        factor = 1.0f / sqrtf(sum / static_cast<float>(a.cols) + a.eps);
-    }
+            for (int e = 0; e < kEach; ++e) total = fma(static_cast<double>(v[i][e]), static_cast<double>(v[i][e]), total);
+        const double factor = 1.0 / sqrt(over_block(total, ONE_WARP ? nullptr : s_wide) / a.cols + static_cast<double>(a.eps));
 #pragma unroll
-    for (int i = 0; i < PARTS; ++i) {
-        const int c = (i * threads + mine) * 8;
-        if (c < a.cols) {
-            float g[8];
-            load8(a.norm_w + c, a.cols - c, a.cols % 4 == 0, g);
+        for (int i = 0; i < PARTS; ++i) {
+            const int c0 = (i * threads + mine) / kLanes * kF8Block;
+            if (c0 < a.cols) {
+                float g[kEach];
+                weights<T, VEC>(a, c0, g);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] = c + e >= a.cols ? 0.0f : wide ? static_cast<float>(static_cast<double>(v[i][e]) * wide_factor * static_cast<double>(g[e])) : v[i][e] * factor * g[e];
+                for (int e = 0; e < kEach; ++e) v[i][e] = c0 + column<T>(e) < a.cols ? static_cast<float>(static_cast<double>(v[i][e]) * factor * static_cast<double>(g[e])) : 0.0f;
+            }
+            quantise<T>(a, row, c0, v[i]);
         }
-        quantise8(a, row, c, c < f8_pitch(a.cols), v[i]);
     }
 }
 
@@ -266,28 +313,29 @@ __global__ void __launch_bounds__(1024) long_norm_kernel(const RowsF8Args a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __shared__ double s_wide[32];
-    __shared__ __align__(16) float s_turn[VEC ? 1 : 64 * kTurn];
+    extern __shared__ __align__(16) float s_long_turn[];
     const size_t row = blockIdx.x;
+    const int step = static_cast<int>(blockDim.x) * kEach, first = static_cast<int>(threadIdx.x) / kLanes * kF8Block;
     double sum = 0.0;
-    float v[8];
-    for (int c0 = 0; c0 < a.cols; c0 += 8192) {
-        values8<T, VEC>(a, row, c0 + static_cast<int>(threadIdx.x) * 8, s_turn, v);
+    float v[kEach];
+    for (int c = 0; c < a.cols; c += step) {
+        values<T, VEC>(a, row, c + first, s_long_turn, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fma(static_cast<double>(v[e]), static_cast<double>(v[e]), sum);
+        for (int e = 0; e < kEach; ++e) sum = fma(static_cast<double>(v[e]), static_cast<double>(v[e]), sum);
     }
     const double factor = 1.0 / sqrt(over_block(sum, s_wide) / a.cols + static_cast<double>(a.eps));
     RowsF8Args again = a;
     if (a.residual != nullptr) again.x = a.total, again.residual = nullptr;  // (what this thread has stored, as it reads them)
-    for (int c0 = 0; c0 < a.cols; c0 += 8192) {
-        const int c = c0 + static_cast<int>(threadIdx.x) * 8;
-        values8<T, VEC>(again, row, c, s_turn, v);
-        if (c < a.cols) {
-            float g[8];
-            load8(a.norm_w + c, a.cols - c, a.cols % 4 == 0, g);
+    for (int c = 0; c < a.cols; c += step) {
+        const int c0 = c + first;
+        values<T, VEC>(again, row, c0, s_long_turn, v);
+        if (c0 < a.cols) {
+            float g[kEach];
+            weights<T, VEC>(a, c0, g);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = c + e >= a.cols ? 0.0f : static_cast<float>(static_cast<double>(v[e]) * factor * static_cast<double>(g[e]));
+            for (int e = 0; e < kEach; ++e) v[e] = c0 + column<T>(e) < a.cols ? static_cast<float>(static_cast<double>(v[e]) * factor * static_cast<double>(g[e])) : 0.0f;
         }
-        quantise8(a, row, c, c < f8_pitch(a.cols), v);
+        quantise<T>(a, row, c0, v);
     }
 }
 
@@ -315,9 +363,6 @@ __global__ void __launch_bounds__(256) blocks_f8_kernel(const float *w, uint8_t 
             some ? pack2(value(r, 0) / scale, value(r, 1) / scale) | pack2(value(r, 2) / scale, value(r, 3) / scale) << 16 : 0u;
 }
 
-#ifndef NPARTS
-#define NPARTS 1
-#endif
 template <typename T, bool VEC>
 cudaError_t launch(const RowsF8Args &a, bool overlap, int sm_count, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
@@ -325,34 +370,42 @@ cudaError_t launch(const RowsF8Args &a, bool overlap, int sm_count, cudaStream_t
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = launch_attributes(attr, overlap, 0);
-    const int eights = static_cast<int>(f8_pitch(a.cols) / 8), n_blocks = f8_blocks(a.cols);
+    const int n_blocks = f8_blocks(a.cols), pieces = n_blocks * kLanes;
     if (a.norm_w == nullptr) {
         // (so many rows at a time that their blocks of columns can be counted in 32 bits)
         const int most = (1 << 30) / n_blocks;
         for (int row = 0; row < a.ntok; row += most) {
-            const unsigned units = static_cast<unsigned>(most < a.ntok - row ? most : a.ntok - row) * static_cast<unsigned>(n_blocks), each = units >= 64u * static_cast<unsigned>(sm_count) ? 2 : 1;
-            cfg.blockDim = dim3(256);
-            cfg.gridDim = dim3((units + 16 * each - 1) / (16 * each));
-            const cudaError_t err = each == 2 ? cudaLaunchKernelEx(&cfg, blocks_kernel<T, 2, VEC>, a, units, row) : cudaLaunchKernelEx(&cfg, blocks_kernel<T, 1, VEC>, a, units, row);
+            const unsigned units = static_cast<unsigned>(most < a.ntok - row ? most : a.ntok - row) * static_cast<unsigned>(n_blocks);
+            constexpr unsigned kAtOnce = kBlocksThreads / kLanes;
+            cfg.blockDim = dim3(kBlocksThreads);
+            cfg.gridDim = dim3((units + kAtOnce - 1) / kAtOnce);
+            const cudaError_t err = cudaLaunchKernelEx(&cfg, blocks_kernel<T, VEC>, a, units, row);
             if (err != cudaSuccess) return err;
         }
         return cudaSuccess;
     }
-    if (eights <= 32) {
+    if (pieces <= 32) {
         cfg.blockDim = dim3(128);
         cfg.gridDim = dim3(static_cast<unsigned>((a.ntok + 3ll) / 4));
         return cudaLaunchKernelEx(&cfg, norm_kernel<T, 1, true, VEC, 128, 8>, a);
     }
     cfg.gridDim = dim3(static_cast<unsigned>(a.ntok));
-    auto threads = [&](int parts) { return static_cast<unsigned>(((eights + parts - 1) / parts + 31) / 32 * 32); };
-    int parts = a.ntok > 2 * sm_count ? NPARTS : 1;
-    while (parts < 4 && threads(parts) > 1024) parts *= 2;
-    cfg.blockDim = dim3(threads(parts));
-    if (parts == 1) return threads(1) <= 640 ? cudaLaunchKernelEx(&cfg, norm_kernel<T, 1, false, VEC, 640, 2>, a) : cudaLaunchKernelEx(&cfg, norm_kernel<T, 1, false, VEC, 1024, 2>, a);
-    if (parts == 2) return threads(2) <= 640 ? cudaLaunchKernelEx(&cfg, norm_kernel<T, 2, false, VEC, 640, 2>, a) : cudaLaunchKernelEx(&cfg, norm_kernel<T, 2, false, VEC, 1024, 1>, a);
-    if (threads(4) <= 576) return cudaLaunchKernelEx(&cfg, norm_kernel<T, 4, false, VEC, 576, 2>, a);
-    if (threads(4) <= 1024) return cudaLaunchKernelEx(&cfg, norm_kernel<T, 4, false, VEC, 1024, 1>, a);
-    cfg.blockDim = dim3(1024);
+    auto threads = [&](int parts) { return static_cast<unsigned>(((pieces + parts - 1) / parts + 31) / 32 * 32); };
+    auto norm = [&](auto kernel, int parts) {
+        cfg.blockDim = dim3(threads(parts));
+        return cudaLaunchKernelEx(&cfg, kernel, a);
+    };
+    // Blocks per SM: as many as leave the values in registers, 16-bit ones, which wait for less, one more (4001 x 5120 with residual: fp32 41 us with three, 43 with four and 44 with
+    // two; fp16 35, 32 and 45).  Few rows do not fill the SMs anyhow.
+    constexpr int kPerSm = VEC && sizeof(T) == 2 ? 4 : 3;
+    const bool few = a.ntok <= 2 * sm_count;
+    if (threads(1) <= 384 && !few) return norm(norm_kernel<T, 1, false, VEC, 384, kPerSm>, 1);
+    if (threads(1) <= 512 && few) return norm(norm_kernel<T, 1, false, VEC, 512, 1>, 1);
+    if (threads(2) <= 512) return norm(norm_kernel<T, 2, false, VEC, 512, 2>, 2);
+    if (threads(3) <= 384) return norm(norm_kernel<T, 3, false, VEC, 384, 2>, 3);
+    if (threads(4) <= 512) return norm(norm_kernel<T, 4, false, VEC, 512, 1>, 4);
+    cfg.blockDim = dim3(512);
+    cfg.dynamicSmemBytes = VEC ? 0 : 512 / kLanes * kTurn * sizeof(float);
     return cudaLaunchKernelEx(&cfg, long_norm_kernel<T, VEC>, a);
 }
 template <typename T>
