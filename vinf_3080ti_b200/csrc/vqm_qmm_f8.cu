@@ -31,8 +31,8 @@ constexpr int kABytes = kRows * kQCols;     // of a stage
 constexpr int kMaxStages = 12, kMaxCluster = 8;
 constexpr int kRing = 216 * 1024, kHalfRing = 106 * 1024, kTurnedRing = 160 * 1024, kBox = 4096, kStaging = 2 * kBox;  // (a warp's, for outputs of pairs)
 constexpr int kWriters = 8, kThreads = 128 + 32 * kWriters;
-// Registers of a thread: a pair's writers hold 128 sums and two sets of 32 that come from tensor memory.  The shares add up to what the block is launched with.
-constexpr int kWriterRegs = 216, kOtherRegs = 72, kLaunchRegs = 168;
+// Registers of a thread: a pair's writers hold 128 sums and two sets of 16 that come from tensor memory.  The shares add up to what the block is launched with.
+constexpr int kWriterRegs = 224, kOtherRegs = 56, kLaunchRegs = 168;
 static_assert(128 * kOtherRegs + 32 * kWriters * kWriterRegs <= kThreads * kLaunchRegs, "registers of a block");
 
 struct QmmF8 {
@@ -72,6 +72,8 @@ __device__ __forceinline__ void copy_tile_of_pair(uint32_t to, const CUtensorMap
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(to), "l"(map), "r"(x), "r"(row), "r"(bar)
                  : "memory");
 }
+// Tensor memory has been read (and a fence says so): nothing else is handed over, so that loads on their way are not waited for.
+__device__ __forceinline__ void arrive_relaxed(uint32_t cluster_addr) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory"); }
 // N columns of this warp's 32 lanes
 template <int N>
 __device__ __forceinline__ void load_sums(uint32_t at, uint32_t (&v)[N]) {
@@ -103,6 +105,13 @@ __device__ __forceinline__ void add_scaled(float &s0, float &s1, uint32_t x, uin
     asm("{\n\t.reg .b64 v, c, d;\n\tmov.b64 v, {%2, %3};\n\tmov.b64 c, {%4, %5};\n\tmov.b64 d, {%0, %1};\n\tfma.rn.f32x2 d, v, c, d;\n\tmov.b64 {%0, %1}, d;\n\t}"
         : "+f"(s0), "+f"(s1)
         : "r"(x), "r"(y), "f"(a), "f"(b));
+}
+
+// Whether the barrier's phase is over, without waiting.
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
 }
 
 __device__ __forceinline__ float get(const float *y) { return *y; }
@@ -404,12 +413,12 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
         }
     } else {
         if constexpr (PAIR) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWriterRegs));
-        constexpr int PART = CW < 32 ? CW : 32;  // columns of one load
         const int writer = warp - 4, lanes = warp & 3, half = writer >> 2, part_of = PAIR ? half : 0;  // (a warp may read the 32 lanes (warp % 4) * 32 onwards)
         asm volatile("griddepcontrol.wait;" ::: "memory");
         bool ok = true;
         float sums[CW];
         uint32_t turn = 0, box_turn = 0;  // blocks of columns, boxes of outputs so far
+        bool ready = false;               // the accumulator of this turn is known to be there
         const uint32_t emptied = PAIR ? in_block(s32(&s_acc_empty[part_of][0]), static_cast<int>(leader)) : s32(&s_acc_empty[0][0]);
         int row0 = 0, tok0 = 0;  // of this lane's outputs: TURNED: activation row tok0, weight rows from row0 on; else weight row row0, activation rows from tok0 on
         for (int tile = cluster; tile < n_tiles; tile += n_clusters) {
@@ -425,32 +434,34 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
 #pragma unroll 1
                 for (int left = k1 - k0; left > 0; --left, ++turn) {
                     const int buf = turn % BUFS;
-                    ok &= wait<false>(s32(&s_acc_full[part_of][buf]), (turn / BUFS) & 1, failed);  // (no way out of the loop: the sums would be copied)
+                    if (!ready) ok &= wait<false>(s32(&s_acc_full[part_of][buf]), (turn / BUFS) & 1, failed);  // (no way out of the loop: the sums would be copied)
                     __syncwarp();
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t at = tmem + buf * N + half * CW + (static_cast<uint32_t>(lanes * 32) << 16);
-                    uint32_t v[2][PART];
-                    load_sums<PART>(at, v[0]);
+                    constexpr int PW = 16;  // columns of one load
+                    uint32_t v[2][PW];
+                    load_sums<PW>(at, v[0]);
+                    load_sums<PW>(at + PW, v[1]);
                     const float scale = x_next * w_next;
                     if (left > 1) {
                         sx += a.q_scale_pitch, ++sw;
                         x_next = *sx, w_next = __ldg(sw);
                     }
 #pragma unroll
-                    for (int p = 0; p < CW / PART; ++p) {
-                        loaded();
-                        if (p + 1 < CW / PART) {
-                            load_sums<PART>(at + (p + 1) * PART, v[(p + 1) & 1]);  // (on its way while these are added)
-                        } else {
+                    for (int p = 0; p < CW / PW; ++p) {
+                        if (p % 2 == 0) loaded();
+                        if (p + 2 == CW / PW) {  // the accumulator may be used again, and whether the next one is there shows while these are added
                             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                             __syncwarp();
                             if (lane == 0) {
-                                if constexpr (PAIR) arrive_in(emptied + buf * 8);
+                                if constexpr (PAIR) arrive_relaxed(emptied + buf * 8);
                                 else bar_arrive(emptied + buf * 8);
                             }
+                            ready = bar_test(s32(&s_acc_full[part_of][(turn + 1) % BUFS]), ((turn + 1) / BUFS) & 1);
                         }
 #pragma unroll
-                        for (int j = 0; j < PART; j += 2) add_scaled(sums[p * PART + j], sums[p * PART + j + 1], v[p & 1][j], v[p & 1][j + 1], scale, scale);
+                        for (int j = 0; j < PW; j += 2) add_scaled(sums[p * PW + j], sums[p * PW + j + 1], v[p & 1][j], v[p & 1][j + 1], scale, scale);
+                        if (p + 2 < CW / PW) load_sums<PW>(at + (p + 2) * PW, v[p & 1]);
                     }
                 }
                 place(tile, row_tile, tok_tile);
@@ -475,29 +486,21 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
                         if (has_x2) x2_next = sx[32];
                         w_next = __ldg(sw);
                     }
-                    ok &= wait<false>(s32(&s_acc_full[0][buf]), (turn / BUFS) & 1, failed);
+                    if (!ready) ok &= wait<false>(s32(&s_acc_full[0][buf]), (turn / BUFS) & 1, failed);
                     __syncwarp();
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t at = tmem + buf * N + half * CW + (static_cast<uint32_t>(lanes * 32) << 16);
-                    uint32_t v[2][PART];
-                    load_sums<PART>(at, v[0]);
+                    uint32_t v[CW];
+                    load_sums<CW>(tmem + buf * N + half * CW + (static_cast<uint32_t>(lanes * 32) << 16), v);
+                    loaded();
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(emptied + buf * 8);
+                    ready = bar_test(s32(&s_acc_full[0][(turn + 1) % BUFS]), ((turn + 1) / BUFS) & 1);
 #pragma unroll
-                    for (int p = 0; p < CW / PART; ++p) {
-                        loaded();
-                        if (p + 1 < CW / PART) {
-                            load_sums<PART>(at + (p + 1) * PART, v[(p + 1) & 1]);
-                        } else {
-                            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                            __syncwarp();
-                            if (lane == 0) bar_arrive(emptied + buf * 8);
-                        }
-#pragma unroll
-                        for (int j = 0; j < PART; j += 4) {
-                            const float4 s = *reinterpret_cast<const float4 *>(scales + p * PART + j);
-                            float *to = sums + p * PART + j;
-                            add_scaled(to[0], to[1], v[p & 1][j], v[p & 1][j + 1], s.x, s.y);
-                            add_scaled(to[2], to[3], v[p & 1][j + 2], v[p & 1][j + 3], s.z, s.w);
-                        }
+                    for (int j = 0; j < CW; j += 4) {
+                        const float4 s = *reinterpret_cast<const float4 *>(scales + j);
+                        add_scaled(sums[j], sums[j + 1], v[j], v[j + 1], s.x, s.y);
+                        add_scaled(sums[j + 2], sums[j + 3], v[j + 2], v[j + 3], s.z, s.w);
                     }
                 }
             }
