@@ -688,9 +688,9 @@ cudaError_t launch(QmmF8 a, const QmmF8Args &in, cudaStream_t stream) {
     const bool brief = a.n_k <= 8 * a.split;  // a few stages for each block: what counts is how soon it begins and ends
     // Sums have memory of their own where that costs no stage or the stages are few, else they go where the stages were, one barrier of the cluster later.
     const int room = a.split > 1 ? CW / 8 * ((kWriters + a.split - 1) / a.split) * (a.split - 1) * 1024 : 0;
-    a.stages = One::kRoom / kStage;
-    const int beside = (One::kRoom - room) / kStage;
-    if (a.split > 1 && (beside == a.stages || (brief && beside >= 3))) a.exchange = One::kRoom - room, a.stages = beside;
+    const int whole = a.split > 1 ? One::kSmem - 1024 : One::kRoom, beside = (whole - room) / kStage;  // (what is split has no outputs on their way)
+    a.stages = whole / kStage;
+    if (a.split > 1 && (beside == a.stages || (brief && beside >= 3))) a.exchange = whole - room, a.stages = beside;
     if (a.stages > kMaxStages) a.stages = kMaxStages;
     Maps<TURNED> maps{};
     cudaError_t err = encode_rows(&maps.w, in.w, in.cols, in.w_pitch, in.rows, PAIR ? kRows / 2 : kRows);
