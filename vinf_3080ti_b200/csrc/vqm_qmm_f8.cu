@@ -151,10 +151,9 @@ __device__ __forceinline__ void write8_any(const QmmF8 &a, long long at, long lo
     else write8(static_cast<float *>(a.y) + at, stride, left, a.add != 0, v);
 }
 
-// Eight outputs that lie side by side.
+// Eight outputs that lie side by side, of an activation row; rows begin on four outputs.
 template <typename Y>
 __device__ __forceinline__ void write8_along(Y *y, int row, int rows, bool add, float (&v)[8]) {
-    if (rows % 4 != 0) return write8(y + row, 1, rows - row, add, v);
 #pragma unroll
     for (int i = 0; i < 8; i += 4) {
         if (row + i >= rows) break;
@@ -164,6 +163,15 @@ __device__ __forceinline__ void write8_along(Y *y, int row, int rows, bool add, 
         for (int e = 0; e < 4; ++e) four[e] += v[i + e];
         put4(y + row + i, four);
     }
+}
+// Rows that do not: eight outputs of each of 32 activation rows, which lie in shared memory, by the whole warp, four rows at a time.  (A store of two bytes in each of 32 rows
+// takes as long as one of 16: 1001 x 4999 with 177 rows, fp16, 12.2 us that way and 10.7.)
+__device__ __forceinline__ void write8_odd(const QmmF8 &a, uint32_t room, int tok0, int row) {
+    const int lane = threadIdx.x & 31, t = tok0 + (lane >> 3), col = row + (lane & 7);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[i]) : "r"(room + i * 128 + lane * 4));
+    if (col < a.rows) write8_any(a, static_cast<long long>(t) * a.rows + col, 4ll * a.rows, (a.ntok - t + 3) / 4, v);
 }
 
 // 32 activation rows (of the lanes) by 32 weight rows (of a lane's values), turned in shared memory so that what is written together lies together.  `room`: a
@@ -470,20 +478,18 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
             } else {
                 row0 = row_tile * kRows + lanes * 32 + lane;
                 tok0 = half * CW;
-                const bool has_x = lane < CW && tok0 + lane < a.ntok, has_x2 = CW > 32 && tok0 + lane + 32 < a.ntok;
+                const bool has_x = lane < CW && tok0 + lane < a.ntok;
                 const float *sx = a.q_scales + tok0 + lane + k0 * a.q_scale_pitch, *sw = a.w_scales + static_cast<size_t>(row_tile) * a.n_k + k0;
-                float x_next = has_x ? *sx : 0.0f, x2_next = has_x2 ? sx[32] : 0.0f, w_next = __ldg(sw);
+                float x_next = has_x ? *sx : 0.0f, w_next = __ldg(sw);
 #pragma unroll 1
                 for (int left = k1 - k0; left > 0; --left, ++turn) {
                     const int buf = turn % BUFS;
                     float *scales = s_scales[writer][buf & 1];
                     if (lane < CW) scales[lane] = x_next * w_next;
-                    if constexpr (CW > 32) scales[lane + 32] = x2_next * w_next;
                     __syncwarp();  // (and nobody reads what the next block but one replaces)
                     if (left > 1) {
                         sx += a.q_scale_pitch, ++sw;
                         if (has_x) x_next = *sx;
-                        if (has_x2) x2_next = sx[32];
                         w_next = __ldg(sw);
                     }
                     if (!ready) ok &= wait<false>(s32(&s_acc_full[0][buf]), (turn / BUFS) & 1, failed);
@@ -506,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
             }
             if constexpr (!SPLIT) {
                 if (tile + n_clusters >= n_tiles) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-                if (!ok) continue;  // (once a wait has given up the writers go on to the end without writing)
+                if (!__all_sync(0xFFFFFFFFu, ok)) continue;  // (once a wait has given up the writers go on to the end without writing)
                 if constexpr (TURNED) {
                     const uint32_t room = ring + kTurnedRing + writer * kStaging;
                     if (a.tile_out) {
@@ -536,13 +542,19 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
             // One tile; its sums go, 8 columns of 32 lanes at a time (a unit), to the block that writes them, and there to the same warp.
             const uint32_t room = ring + a.exchange, bar = s32(&s_sums[writer]);
             const int of_column = (kWriters + a.split - 1) / a.split;  // units of 8 columns that a block may have
-            auto owner_of = [&](int c) { return (c * 9 + writer) % a.split; };
+            const int first_owner = writer % a.split;
+            auto free_room = [&](int c) { return room + static_cast<uint32_t>((c * of_column + writer / a.split) * (a.split - 1)) * 1024; };  // (once this warp has read what came)
             auto room_of = [&](int c, int from, int owner) { return room + static_cast<uint32_t>((c * of_column + writer / a.split) * (a.split - 1) + (from < owner ? from : from - 1)) * 1024 + lane * 16; };
             if (a.exchange == 0) cluster_sync();  // every block's MMAs are done with its stages, where the sums go
-            int mine = 0;
+            int mine = 0, next = first_owner;
+            auto owner_next = [&] {  // of unit 0, 1, ...
+                const int owner = next;
+                next = next + 1 == a.split ? 0 : next + 1;
+                return owner;
+            };
 #pragma unroll
             for (int c = 0; c < CW / 8; ++c) {
-                const int owner = owner_of(c);
+                const int owner = owner_next();
                 if (owner == part) {
                     ++mine;
                     continue;
@@ -561,10 +573,11 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
                 if (lane == 0) expect(bar, static_cast<uint32_t>(mine * (a.split - 1)) * 1024);
                 const bool there = wait<true>(bar, 0, failed);  // (by every lane: it reads what others have stored)
                 __syncwarp();
-                if (there && ok && !*failed) {
+                if (__all_sync(0xFFFFFFFFu, there && ok && !*failed)) {
+                    next = first_owner;
 #pragma unroll
                     for (int c = 0; c < CW / 8; ++c) {
-                        if (owner_of(c) != part) continue;
+                        if (owner_next() != part) continue;
                         float v[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) v[j] = sums[8 * c + j];
@@ -576,13 +589,23 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
                             v[4] += __uint_as_float(z.x), v[5] += __uint_as_float(z.y), v[6] += __uint_as_float(z.z), v[7] += __uint_as_float(z.w);
                         }
                         if constexpr (TURNED) {
-                            if (tok0 < a.ntok && row0 + 8 * c < a.rows) {
+                            if (a.rows % 4 != 0) {
+                                const uint32_t to = free_room(c) + lane * 32;
+                                __syncwarp();
+#pragma unroll
+                                for (int i = 0; i < 8; i += 4) asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + i * 4), "f"(v[i]), "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3]) : "memory");
+                            } else if (tok0 < a.ntok) {
                                 if (a.y_elem == 2) write8_along(static_cast<__half *>(a.y) + static_cast<long long>(tok0) * a.rows, row0 + 8 * c, a.rows, a.add != 0, v);
                                 else write8_along(static_cast<float *>(a.y) + static_cast<long long>(tok0) * a.rows, row0 + 8 * c, a.rows, a.add != 0, v);
                             }
                         } else {
                             if (row0 < a.rows) write8_any(a, static_cast<long long>(tok0 + 8 * c) * a.rows + row0, a.rows, a.ntok - tok0 - 8 * c, v);
                         }
+                    }
+                    if (TURNED && a.rows % 4 != 0) {
+                        __syncwarp();
+#pragma unroll 1
+                        for (int c = (part + a.split - first_owner) % a.split; c < CW / 8; c += a.split) write8_odd(a, free_room(c), tok0 - lane, row0 + 8 * c);
                     }
                 }
             }
@@ -663,13 +686,18 @@ struct Variant {
     }
 };
 
-// As many parts of the columns as leave every cluster room beside the others, of two blocks of columns at least.
+// Parts of a tile's columns, of two blocks of columns at least, where every cluster has room beside the others.  Up to 64 activation rows: as many as that leaves
+// (1024 x 5120 with 4 rows: 12.4, 8.1, 6.6, 5.9 and 5.1 us with 1, 2, 3, 4 and 8 parts).  With more, the exchange of 128 x 128 sums takes as long as 12 blocks of columns,
+// and clusters beside which the next launch's have no room delay its beginning: as many as take least by that, at 0.27 us for a block of columns
+// (1024 x 2048, 128 rows: 7.4, 8.1, 7.6, 7.0, 7.2, 8.1 and 8.5 us with 1, 2, 3, 4, 5, 6 and 8; 1024 x 17408: 40.4, 24.7, 18.8, 15.5, 14.2, 14.1 and 13.1).
 template <int CW>
 int split_of(long long tiles, int n_k) {
-    int best = 1;
+    int best = 1, least = n_k * 27;  // 10 ns
     if constexpr (!paired(CW))
-        for (int split = 2; split <= kMaxCluster && n_k >= 2 * split; ++split)
-            if (tiles <= Variant<CW, true>::clusters(split)) best = split;
+        for (int split = 2; split <= kMaxCluster && n_k >= 2 * split; ++split) {
+            const int fit = Variant<CW, true>::clusters(split), takes = n_k * 27 / split + 330 + (2 * tiles > fit ? 220 : 3 * tiles > fit ? 80 : 0);
+            if (tiles <= fit && (!turned(CW) || takes <= least)) best = split, least = takes;
+        }
     return best;
 }
 
