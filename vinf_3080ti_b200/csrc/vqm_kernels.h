@@ -312,7 +312,7 @@ struct LogprobsArgs {
     int vocab, rows, top, elem;
 };
 // overlap: see launch_attributes
-cudaError_t launch_logprobs(const LogprobsArgs &a, bool overlap, int sm_count, cudaStream_t stream);
+cudaError_t launch_logprobs(const LogprobsArgs &a, bool overlap, cudaStream_t stream);
 
 cudaError_t launch_argmax_rows(const float *x, int n, int ntok, int *out, cudaStream_t stream);
 cudaError_t launch_dequant(int type, const uint8_t *w, float *out, long long numel, const uint8_t *codebook,

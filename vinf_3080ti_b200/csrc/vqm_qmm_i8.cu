@@ -53,6 +53,14 @@ struct QmmTc {
     int half_sm;                       // two blocks per SM
 };
 
+// A wait by one lane for its warp.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *failed) {
+    int ok = 1;
+    if ((threadIdx.x & 31) == 0) ok = wait<false>(bar, parity, failed) ? 1 : 0;
+    __syncwarp();
+    return __shfl_sync(0xFFFFFFFFu, ok, 0) != 0;
+}
+__device__ __forceinline__ void arrive_in(uint32_t cluster_addr) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory"); }
 template <bool PAIR>
 __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     if constexpr (PAIR)

@@ -2006,7 +2006,7 @@ int vqm_logprobs(vqm_runtime *rt, const char *logits, const char *tokens, const 
         if ((rc = check_apart("the alternatives", ei, {el, ek, et, ev})) != VQM_OK) return rc;
         if ((rc = check_apart("the alternatives' log probabilities", ev, {el, ek, et})) != VQM_OK) return rc;
         a.status = rt->status;
-        const cudaError_t err = vqm::launch_logprobs(a, rt->overlap_launch != 0, rt->sm_count, rt->stream);
+        const cudaError_t err = vqm::launch_logprobs(a, rt->overlap_launch != 0, rt->stream);
         if (err != cudaSuccess) return cuda_fail("logprobs launch", err);
         count_launch(rt);
         return VQM_OK;

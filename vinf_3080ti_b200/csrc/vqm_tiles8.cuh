@@ -25,13 +25,6 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
         if ((i & 255u) == 0 && tc::give_up(&began, failed)) return false;
     }
 }
-// The same by one lane for its warp.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *failed) {
-    int ok = 1;
-    if ((threadIdx.x & 31) == 0) ok = wait<false>(bar, parity, failed) ? 1 : 0;
-    __syncwarp();
-    return __shfl_sync(0xFFFFFFFFu, ok, 0) != 0;
-}
 
 __device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {  // K-major, 128-byte swizzle, groups of 8 rows 1024 bytes apart
     return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
@@ -43,7 +36,6 @@ __device__ __forceinline__ void copy_tile(uint32_t to, const CUtensorMap *map, i
 __device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void arrive_in(uint32_t cluster_addr) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory"); }
 __device__ __forceinline__ void cluster_sync() {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
