@@ -332,6 +332,15 @@ def test_product_of_more_tiles_than_fit_at_once(rt, rows, cols, ntok, kind):
 
 
 @pytest.mark.parametrize("kind", [np.float32, np.float16])
+@pytest.mark.parametrize("rows,cols,ntok", [(5120, 8192, 256), (4993, 8200, 200), (4994, 8100, 129), (4996, 8300, 255), (5900, 14300, 140), (3300, 4400, 250), (2049, 5120, 500), (129, 17408, 257)])
+def test_product_of_wide_tiles_whose_columns_are_shared(rt, rows, cols, ntok, kind):
+    """Tiles of 256 x 256 by two and three parts of the columns, and sizes beside those that have them."""
+    rng = np.random.default_rng(rows + cols)
+    check_product(rt, *make(rng, rows, cols, ntok, whole=cols <= 5120), kind=kind, whole=cols <= 5120)
+    check_product(rt, *make(rng, rows, cols, ntok), kind=kind, before=rng.standard_normal((ntok, rows)).astype(kind))
+
+
+@pytest.mark.parametrize("kind", [np.float32, np.float16])
 @pytest.mark.parametrize("rows,cols,ntok", [(1, 1, 1), (257, 300, 4), (1000, 2000, 33), (300, 5120, 1), (129, 129, 128), (257, 512, 200), (999, 700, 300)])
 def test_product_onto_what_is_there(rt, rows, cols, ntok, kind):
     rng = np.random.default_rng(rows)

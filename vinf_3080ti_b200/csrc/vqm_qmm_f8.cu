@@ -12,9 +12,9 @@
 // are one for each column, by shared memory.
 // TURNED, more: the activation rows are the lanes, 128 weight rows the columns, and a lane needs one factor for all of its columns.  (With the weight rows in the lanes
 // it would need 128 different ones, which shared memory gives in twice the time of the MMAs.)  Outputs go out by TMA, where rows are multiples of 16 bytes.
-// PAIR, many rows (pairs_pay): two blocks of a cluster multiply 256 activation rows by 256 weight rows together (cta_group::2), each half of the weight rows by itself, so
+// PAIR, many rows: two blocks of a cluster multiply 256 activation rows by 256 weight rows together (cta_group::2), each half of the weight rows by itself, so
 // that four accumulators are in turn.
-// SPLIT (few tiles, single blocks): the blocks of a cluster share the columns of a tile, and exchange their sums by st.async, so that no memory of the runtime is involved.
+// SPLIT (few tiles): the blocks, or pairs, of a cluster share the columns of a tile, and exchange their sums by st.async, so that no memory of the runtime is involved.
 //
 // What bounds it.  Few rows: memory.  17408 x 5120, one launch behind the other: 1 row 17.7 us (5.0 TB/s), 16 18.0, 32 19.9, 64 21.3, of which 3 to 4 are the start and the
 // end of a launch; among others 13.5 (6.6 TB/s).  Many: the writers, then power.  A pair's MMAs take 512 cycles for a block of columns, its writers 626 without a wait
@@ -25,6 +25,8 @@
 // Every wait is bounded: on expiry the block records a status code and everybody falls through to the end.
 #include <cuda.h>
 #include <cuda_fp16.h>
+
+#include <climits>
 
 #include "vqm_kernels.h"
 #include "vqm_tiles8.cuh"
@@ -152,22 +154,46 @@ __device__ __forceinline__ void write8(Y *y, long long stride, int left, bool ad
     for (int j = 0; j < 8; ++j)
         if (j < left) put(y + j * stride, v[j]);
 }
-__device__ __forceinline__ void write8_any(const QmmF8 &a, long long at, long long stride, int left, float (&v)[8]) {
-    if (a.y_elem == 2) write8(static_cast<__half *>(a.y) + at, stride, left, a.add != 0, v);
-    else write8(static_cast<float *>(a.y) + at, stride, left, a.add != 0, v);
+__device__ __forceinline__ void write8_any(const QmmF8 &a, long long at, long long stride, int left, bool add, float (&v)[8]) {
+    if (a.y_elem == 2) write8(static_cast<__half *>(a.y) + at, stride, left, add, v);
+    else write8(static_cast<float *>(a.y) + at, stride, left, add, v);
 }
 
-// Eight outputs that lie side by side, of an activation row; rows begin on four outputs.
+// Eight outputs that lie side by side, of an activation row; rows begin on four outputs.  What they are added to comes first, as it is.
 template <typename Y>
-__device__ __forceinline__ void write8_along(Y *y, int row, int rows, bool add, float (&v)[8]) {
+__device__ __forceinline__ void read8_along(const Y *y, int row, int rows, float (&was)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-        if (row + i >= rows) break;
-        float four[4] = {};
-        if (add) get4(y + row + i, four);
+    for (int i = 0; i < 2; ++i)
+        if (row + 4 * i < rows) {
+            if constexpr (sizeof(Y) == 4) {
+                const float4 w = *reinterpret_cast<const float4 *>(y + row + 4 * i);
+                was[4 * i] = w.x, was[4 * i + 1] = w.y, was[4 * i + 2] = w.z, was[4 * i + 3] = w.w;
+            } else {
+                const float2 w = *reinterpret_cast<const float2 *>(y + row + 4 * i);
+                was[4 * i] = w.x, was[4 * i + 1] = w.y;
+            }
+        }
+}
+template <typename Y>
+__device__ __forceinline__ void write8_along(Y *y, int row, int rows, bool add, const float (&was)[8], float (&v)[8]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) four[e] += v[i + e];
-        put4(y + row + i, four);
+    for (int i = 0; i < 2; ++i) {
+        if (row + 4 * i >= rows) break;
+        float four[4] = {v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+        if (add) {
+            if constexpr (sizeof(Y) == 4) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) four[e] += was[4 * i + e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t bits = __float_as_uint(was[4 * i + e]);
+                    const float2 w = __half22float2(*reinterpret_cast<const __half2 *>(&bits));
+                    four[2 * e] += w.x, four[2 * e + 1] += w.y;
+                }
+            }
+        }
+        put4(y + row + 4 * i, four);
     }
 }
 // Rows that do not: eight outputs of each of 32 activation rows, which lie in shared memory, by the whole warp, four rows at a time.  (A store of two bytes in each of 32 rows
@@ -177,14 +203,21 @@ __device__ __forceinline__ void write8_odd(const QmmF8 &a, uint32_t room, int to
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[i]) : "r"(room + i * 128 + lane * 4));
-    if (col < a.rows) write8_any(a, static_cast<long long>(t) * a.rows + col, 4ll * a.rows, (a.ntok - t + 3) / 4, v);
+    if (col < a.rows) write8_any(a, static_cast<long long>(t) * a.rows + col, 4ll * a.rows, (a.ntok - t + 3) / 4, a.add != 0, v);
 }
 
 // 32 activation rows (of the lanes) by 32 weight rows (of a lane's values), turned in shared memory so that what is written together lies together.  `room`: a
 // warp's 4 KB, rows of 128 bytes whose 16-byte pieces are exchanged against bank conflicts.
 template <typename Y>
 __device__ __forceinline__ void write_turned(const QmmF8 &a, uint32_t room, const float *sums, int tok0, int row0) {
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, piece = lane & 7, row = row0 + piece * 4;
+    Y *const y = static_cast<Y *>(a.y), *const at = y + static_cast<long long>(tok0 + (lane >> 3)) * a.rows + row;
+    const bool whole = a.rows % 4 == 0;  // (buffers are 16-byte aligned)
+    float was[8][4];                     // on its way before anything else
+    if (whole && a.add && row < a.rows)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (tok0 + i * 4 + (lane >> 3) < a.ntok) get4(at + i * 4ll * a.rows, was[i]);
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -192,28 +225,17 @@ __device__ __forceinline__ void write_turned(const QmmF8 &a, uint32_t room, cons
         asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(sums[4 * j]), "f"(sums[4 * j + 1]), "f"(sums[4 * j + 2]), "f"(sums[4 * j + 3]) : "memory");
     }
     __syncwarp();
-    Y *y = static_cast<Y *>(a.y);
-    if (a.rows % 4 == 0) {  // (buffers are 16-byte aligned)
-        const int piece = lane & 7, row = row0 + piece * 4;
+    if (whole) {
         if (row < a.rows) {
-            Y *at = y + static_cast<long long>(tok0 + (lane >> 3)) * a.rows + row;
-#pragma unroll 1
-            for (int part = 0; part < 8; part += 4) {
-                float was[4][4];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int t = i * 4 + (lane >> 3);
+                const uint4 w = lds128u(room + t * 128 + ((piece ^ (t & 7)) * 16));
+                float v[4] = {__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)};
                 if (a.add)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (tok0 + (part + i) * 4 + (lane >> 3) < a.ntok) get4(at + (part + i) * 4ll * a.rows, was[i]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int t = (part + i) * 4 + (lane >> 3);
-                    const uint4 w = lds128u(room + t * 128 + ((piece ^ (t & 7)) * 16));
-                    float v[4] = {__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)};
-                    if (a.add)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] += was[i][e];
-                    if (tok0 + t < a.ntok) put4(at + (part + i) * 4ll * a.rows, v);
-                }
+                    for (int e = 0; e < 4; ++e) v[e] += was[i][e];
+                if (tok0 + t < a.ntok) put4(at + i * 4ll * a.rows, v);
             }
         }
     } else if (row0 + lane < a.rows) {
@@ -270,7 +292,6 @@ __host__ __device__ constexpr bool paired(int cw) { return cw == 128; }
 template <int CW, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(const __grid_constant__ Maps<turned(CW)> maps, const QmmF8 a) {
     constexpr bool PAIR = paired(CW), TURNED = turned(CW);
-    static_assert(!(PAIR && SPLIT));
     constexpr int GROUP = PAIR ? 2 : 1, N = 2 * CW, BUFS = PAIR ? 2 : 4, TMEM = N * BUFS;
     constexpr int HALVES = PAIR ? 2 : 1;  // parts of an accumulator that are multiplied, and handed on, by themselves
     extern __shared__ uint8_t ring_raw[];
@@ -282,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t in_cluster = 0;
     if constexpr (PAIR || SPLIT) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(in_cluster));
-    const int rank = PAIR ? static_cast<int>(in_cluster & 1u) : 0, part = SPLIT ? static_cast<int>(in_cluster) : 0;  // place in the pair, share of the columns
+    const int rank = PAIR ? static_cast<int>(in_cluster & 1u) : 0, part = SPLIT ? static_cast<int>(in_cluster) / GROUP : 0;  // place in the pair, share of the columns
     const uint32_t leader = in_cluster & ~1u;
     const int cluster = static_cast<int>(blockIdx.x) / (GROUP * a.split), n_clusters = static_cast<int>(gridDim.x) / (GROUP * a.split);
     const int k0 = SPLIT ? part * a.n_k / a.split : 0, k1 = SPLIT ? (part + 1) * a.n_k / a.split : a.n_k;
@@ -537,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
                         float v[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) v[j] = sums[8 * c + j];
-                        write8_any(a, static_cast<long long>(tok0 + 8 * c) * a.rows + row0, a.rows, a.ntok - tok0 - 8 * c, v);
+                        write8_any(a, static_cast<long long>(tok0 + 8 * c) * a.rows + row0, a.rows, a.ntok - tok0 - 8 * c, a.add != 0, v);
                     }
                 }
             }
@@ -566,11 +587,38 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
                     continue;
                 }
                 // stores that count their bytes on a barrier of the block that they go to
-                const uint32_t to = in_block(room_of(c, part, owner), owner), there = in_block(bar, owner);
+                const int block = owner * GROUP + rank;
+                const uint32_t to = in_block(room_of(c, part, owner), block), there = in_block(bar, block);
                 asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "f"(sums[8 * c + 0]), "f"(sums[8 * c + 1]), "f"(sums[8 * c + 2]), "f"(sums[8 * c + 3]), "r"(there)
                              : "memory");
                 asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to + 512), "f"(sums[8 * c + 4]), "f"(sums[8 * c + 5]), "f"(sums[8 * c + 6]), "f"(sums[8 * c + 7]), "r"(there)
                              : "memory");
+            }
+            // What outputs are added to is on its way while the others' sums are waited for: a unit's is kept where the sums of its neighbour were (the other one of two, which
+            // has another owner and has been sent).
+            [[maybe_unused]] float onto[TURNED ? 1 : CW];
+            if (a.add) {
+                next = first_owner;
+#pragma unroll
+                for (int c = 0; c < CW / 8; ++c) {
+                    if (owner_next() != part) continue;
+                    if constexpr (TURNED) {
+                        float was[8] = {};
+                        if (a.rows % 4 == 0 && tok0 < a.ntok) {
+                            if (a.y_elem == 2) read8_along(static_cast<const __half *>(a.y) + static_cast<long long>(tok0) * a.rows, row0 + 8 * c, a.rows, was);
+                            else read8_along(static_cast<const float *>(a.y) + static_cast<long long>(tok0) * a.rows, row0 + 8 * c, a.rows, was);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) sums[8 * (c ^ 1) + j] = was[j];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const int t = tok0 + 8 * c + j;
+                            const long long at = static_cast<long long>(t) * a.rows + row0;
+                            onto[8 * c + j] = row0 >= a.rows || t >= a.ntok ? 0.0f : a.y_elem == 2 ? get(static_cast<const __half *>(a.y) + at) : get(static_cast<const float *>(a.y) + at);
+                        }
+                    }
+                }
             }
             __syncwarp();
             asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (its other half is at the end: until then others may still send)
@@ -601,11 +649,17 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
 #pragma unroll
                                 for (int i = 0; i < 8; i += 4) asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + i * 4), "f"(v[i]), "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3]) : "memory");
                             } else if (tok0 < a.ntok) {
-                                if (a.y_elem == 2) write8_along(static_cast<__half *>(a.y) + static_cast<long long>(tok0) * a.rows, row0 + 8 * c, a.rows, a.add != 0, v);
-                                else write8_along(static_cast<float *>(a.y) + static_cast<long long>(tok0) * a.rows, row0 + 8 * c, a.rows, a.add != 0, v);
+                                float was[8];
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) was[j] = sums[8 * (c ^ 1) + j];
+                                if (a.y_elem == 2) write8_along(static_cast<__half *>(a.y) + static_cast<long long>(tok0) * a.rows, row0 + 8 * c, a.rows, a.add != 0, was, v);
+                                else write8_along(static_cast<float *>(a.y) + static_cast<long long>(tok0) * a.rows, row0 + 8 * c, a.rows, a.add != 0, was, v);
                             }
                         } else {
-                            if (row0 < a.rows) write8_any(a, static_cast<long long>(tok0 + 8 * c) * a.rows + row0, a.rows, a.ntok - tok0 - 8 * c, v);
+                            if (a.add)
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) v[j] += onto[8 * c + j];
+                            if (row0 < a.rows) write8_any(a, static_cast<long long>(tok0 + 8 * c) * a.rows + row0, a.rows, a.ntok - tok0 - 8 * c, false, v);
                         }
                     }
                     if (TURNED && a.rows % 4 != 0) {
@@ -693,17 +747,22 @@ struct Variant {
 };
 
 // Parts of a tile's columns, of two blocks of columns at least, where every cluster has room beside the others.  Up to 64 activation rows: as many as that leaves
-// (1024 x 5120 with 4 rows: 12.4, 8.1, 6.6, 5.9 and 5.1 us with 1, 2, 3, 4 and 8 parts).  With more, the exchange of 128 x 128 sums takes as long as 12 blocks of columns,
-// and clusters beside which the next launch's have no room delay its beginning: as many as take least by that, at 0.27 us for a block of columns
-// (1024 x 2048, 128 rows: 7.4, 8.1, 7.6, 7.0, 7.2, 8.1 and 8.5 us with 1, 2, 3, 4, 5, 6 and 8; 1024 x 17408: 40.4, 24.7, 18.8, 15.5, 14.2, 14.1 and 13.1).
+// (1024 x 5120 with 4 rows: 12.4, 8.1, 6.6, 5.9 and 5.1 us with 1, 2, 3, 4 and 8 parts).  With more, the exchange of 128 x 128 sums takes as long as 12 blocks of columns, that
+// of a pair 12 us, and clusters beside which the next launch's have no room delay its beginning: as many as take least by that, at 0.27 us (0.55) for a block of columns.
+// (128 rows, 1024 x 2048: 7.4, 8.1, 7.6, 7.0, 7.2, 8.1 and 8.5 us with 1, 2, 3, 4, 5, 6 and 8; 1024 x 17408: 40.4, 24.7, 18.8, 15.5, 14.2, 14.1 and 13.1.  Pairs, 256 rows,
+// 5120 x 17408: 59.5, 48.0 and 38.2 with 1, 2 and 3, and single blocks, which cannot be split there, 54.0; 5120 x 5120: 18.6, 21.8 and 20.0, and 15.6.)
+template <int CW>
+constexpr int kExchange = paired(CW) ? 1200 : 330;  // 10 ns
+template <int CW>
+constexpr int kMaxSplit = paired(CW) ? 3 : kMaxCluster;  // (four pairs gain from 290 blocks of columns on)
 template <int CW>
 int split_of(long long tiles, int n_k) {
-    int best = 1, least = n_k * 27;  // 10 ns
-    if constexpr (!paired(CW))
-        for (int split = 2; split <= kMaxCluster && n_k >= 2 * split; ++split) {
-            const int fit = Variant<CW, true>::clusters(split), takes = n_k * 27 / split + 330 + (2 * tiles > fit ? 220 : 3 * tiles > fit ? 80 : 0);
-            if (tiles <= fit && (!turned(CW) || takes <= least)) best = split, least = takes;
-        }
+    constexpr int kEach = paired(CW) ? 55 : 27;  // 10 ns
+    int best = 1, least = n_k * kEach;
+    for (int split = 2; split <= (kMaxSplit<CW>) && n_k >= 2 * split; ++split) {
+        const int fit = Variant<CW, true>::clusters(split), takes = n_k * kEach / split + kExchange<CW> + (2 * tiles > fit ? 220 : 3 * tiles > fit ? 80 : 0);
+        if (tiles <= fit && (!turned(CW) || takes <= least)) best = split, least = takes;
+    }
     return best;
 }
 
@@ -734,19 +793,18 @@ cudaError_t launch(QmmF8 a, const QmmF8Args &in, cudaStream_t stream) {
         if (a.tile_out && err == cudaSuccess) err = encode_outputs(&maps.y, in.y, in.rows, in.ntok, in.y_elem);
     }
     if (err != cudaSuccess) return err;
-    if constexpr (!PAIR)
-        if (a.split > 1) return Variant<CW, true>::launch(maps, a, in.overlap, stream);
+    if (a.split > 1) return Variant<CW, true>::launch(maps, a, in.overlap, stream);
     return One::launch(maps, a, in.overlap, stream);
 }
 
-// Whether pairs of blocks finish before single ones do.  A pair takes 0.55 us for a block of columns of 256 x 256 outputs, a single block 0.39 for 128 x 128, and what
-// leaves SMs without work can be split by columns as clusters of single blocks only.  (6144 x 5120 with 256 rows: 30.9 and 15.5 us, with 512 21.6 and 27.1.)
-bool pairs_pay(int rows, int ntok, int n_k) {
-    const long long single = static_cast<long long>((rows + kRows - 1) / kRows) * ((ntok + kRows - 1) / kRows), pairs = static_cast<long long>((rows + 2 * kRows - 1) / (2 * kRows)) * ((ntok + 2 * kRows - 1) / (2 * kRows));
-    const int fit = Variant<64, false>::clusters(1), pair_fit = Variant<128, false>::clusters(1);
-    if (fit == 0 || pair_fit == 0) return pair_fit != 0;
-    const int split = single > fit ? 1 : split_of<64>(single, n_k);
-    return (pairs + pair_fit - 1) / pair_fit * n_k * 10 < (single + fit - 1) / fit * ((n_k + split - 1) / split) * 7;
+// What blocks (pairs) of all tiles take, in 10 ns: a pair 0.55 us for a block of columns of 256 x 256 outputs, a single block 0.39 for 128 x 128, where all have work.
+template <int CW>
+long long takes(int rows, int ntok, int n_k) {
+    constexpr int kTile = Variant<CW, false>::kGroup * kRows, kEach = paired(CW) ? 55 : 39;
+    const long long tiles = static_cast<long long>((rows + kTile - 1) / kTile) * ((ntok + kTile - 1) / kTile);
+    const int fit = Variant<CW, false>::clusters(1), split = split_of<CW>(tiles, n_k);
+    if (fit == 0) return LLONG_MAX;
+    return split > 1 ? n_k * kEach / split + kExchange<CW> : (tiles + fit - 1) / fit * n_k * kEach;
 }
 
 }  // namespace
@@ -763,7 +821,8 @@ cudaError_t launch_qmm_f8(const QmmF8Args &in, cudaStream_t stream) {
     a.n_k = f8_blocks(in.cols);
     a.y_elem = in.y_elem;
     a.add = in.add;
-    if (in.ntok > 128 && pairs_pay(in.rows, in.ntok, a.n_k)) return launch<128>(a, in, stream);
+    // (6144 x 5120 with 256 rows: pairs 30.9 us, single blocks 15.9; with 512 21.6 and 27.1)
+    if (in.ntok > 128 && takes<128>(in.rows, in.ntok, a.n_k) < takes<64>(in.rows, in.ntok, a.n_k)) return launch<128>(a, in, stream);
     if (in.ntok > 64) return launch<64>(a, in, stream);
     if (in.ntok > 32) return launch<32>(a, in, stream);
     return in.ntok > 16 ? launch<16>(a, in, stream) : launch<8>(a, in, stream);
