@@ -9,8 +9,8 @@
 // n candidates each finds its own place, by counting those before it.  Rows where more tie than the list holds take a pass for each alternative.
 // Rows of infinite or extreme logits, and extreme temperatures, are summed in 64 bits by one block.
 //
-// What bounds it.  Many rows: memory, and for fp16 the instructions as well (issue slots 61 %; the exponentials, 16 a cycle of an SM, 69 us of the 131).  2048 x 151936: fp32 190 us without
-// alternatives (6.5 TB/s) and 221 with 20, fp16 115 (5.4) and 131 with one.  Few rows: the steps, each of which waits for the one before: 1 x 151936 5.8 us, 10.3 with 20
+// What bounds it.  Many rows: memory, and for fp16 the instructions as well (issue slots 61 %; the exponentials, 16 a cycle of an SM, 69 us of the 126).  2048 x 151936: fp32 185 us without
+// alternatives (6.7 TB/s) and 219 with 20, fp16 109 (5.7) and 126 with one.  Few rows: the steps, each of which waits for the one before: 1 x 151936 5.2 us, 10.3 with 20
 // alternatives, by one cluster of 16 blocks (more would have to meet in device memory).
 #include <cuda_fp16.h>
 
@@ -95,11 +95,12 @@ __device__ __forceinline__ float add_vectors(Sums &a, const uint4 (&w)[kUnroll],
     return most;
 }
 
+static_assert(sizeof(float) * kMostWarps * 32 <= sizeof(Key) * kMaxBlocks * kMaxTop);
 struct Shared {
     float most[kMostWarps][32];     // largest logits of the threads
     float part[2][kMostWarps];
     alignas(16) Key list[kList];    // candidates
-    Key theirs[kMaxBlocks][kMaxTop];  // the blocks' alternatives
+    alignas(16) Key theirs[kMaxBlocks][kMaxTop];  // the blocks' alternatives; before that, the warps' copies of the groups' largest
     Key best[kMaxTop];              // this block's, in order
     Key key[kMostWarps];
     double wide[kMostWarps];
@@ -208,10 +209,22 @@ __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const Logprob
         s.status = *a.status;
     }
 
+    // What the answer needs besides is read ahead of the row, where rows are few (1 x 151936 5.3 and 5.0 us); the registers cost many rows more than that (108.6 and 109.8).
+    constexpr bool kAhead = THREADS == 512;
+    auto token_at = [&](int &token, float &v) {
+        token = a.tokens[row];
+        v = token >= 0 && token < n ? as_float(x[token]) : -INFINITY;
+    };
+    int token = -1;
+    float asked = -INFINITY;
+    if (kAhead && threadIdx.x == 32 && block == 0) token_at(token, asked);
+
     // this block's vectors
     const int first = first_of(x);  // index of vector 0's first element
     const int vectors = (n - first + VEC - 1) / VEC;
     const int begin = static_cast<int>(static_cast<long long>(vectors) * block / n_blocks), end = static_cast<int>(static_cast<long long>(vectors) * (block + 1) / n_blocks);
+    const uint4 *const vector0 = reinterpret_cast<const uint4 *>(x + first);
+    const int whole = min(end, vectors - 1);  // vectors before it (but for the row's first) hold nothing else
     const int per_part = (end - begin + kParts * kUnroll * THREADS - 1) / (kParts * kUnroll * THREADS);  // turns of the loop
     const int want = a.top > 0 ? a.top : greedy ? 1 : 0;
     float(*const part_most)[THREADS] = reinterpret_cast<float(*)[THREADS]>(part_room);
@@ -221,10 +234,15 @@ __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const Logprob
 #pragma unroll 1
     for (int v = begin + static_cast<int>(threadIdx.x); v < end; v += kUnroll * THREADS) {
         uint4 w[kUnroll];
+        if (v > 0 && v + (kUnroll - 1) * THREADS < whole) {
 #pragma unroll
-        for (int i = 0; i < kUnroll; ++i) {
-            if (v + i * THREADS < end) load_vec(x, n, first, v + i * THREADS, w[i]);
-            else w[i] = make_uint4(kNothing<T>, kNothing<T>, kNothing<T>, kNothing<T>);
+            for (int i = 0; i < kUnroll; ++i) w[i] = vector0[v + i * THREADS];
+        } else {
+#pragma unroll
+            for (int i = 0; i < kUnroll; ++i) {
+                if (v + i * THREADS < end) load_vec(x, n, first, v + i * THREADS, w[i]);
+                else w[i] = make_uint4(kNothing<T>, kNothing<T>, kNothing<T>, kNothing<T>);
+            }
         }
         in_part = fmaxf(in_part, add_vectors<T>(sums, w, c));
         if (want > 0 && ++turn == per_part) {
@@ -254,14 +272,22 @@ __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const Logprob
     if (lane == 0) s.part[0][warp] = sum, s.part[1][warp] = weighted;
 
     if (want > 0) {
-        // the want-th largest group; where that is out of what the sums tell apart, all logits are candidates
-        int before = 0;
+        // The want-th largest group: the largest value that so many reach.  Where that is out of what the sums tell apart, all logits are candidates.
+        float least = all;
+        if (want > 1) {
+            float *const group = reinterpret_cast<float *>(s.theirs) + warp * 32;
+            group[lane] = mine;
+            __syncwarp();
+            int reach = 0;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            const float other = __shfl_sync(0xFFFFFFFFu, mine, j);
-            before += other > mine || (other == mine && j < lane);
+            for (int j = 0; j < 32; j += 4) {
+                const float4 g = *reinterpret_cast<const float4 *>(group + j);
+                reach += (g.x >= mine) + (g.y >= mine) + (g.z >= mine) + (g.w >= mine);
+            }
+            least = reach >= want ? mine : -INFINITY;
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) least = fmaxf(least, __shfl_xor_sync(0xFFFFFFFFu, least, off));
         }
-        float least = __shfl_sync(0xFFFFFFFFu, mine, __ffs(__ballot_sync(0xFFFFFFFFu, before == want - 1)) - 1);
         const bool any = !(least > kLow);
         if (any) least = -INFINITY;
         auto offer = [&](const uint4 &w, int v) {
@@ -402,8 +428,8 @@ __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const Logprob
         return top == INFINITY ? -INFINITY : static_cast<float>((static_cast<double>(v) - static_cast<double>(top)) * inverse - log_sum);
     };
     if (threadIdx.x == 32) {
-        const int token = a.tokens[row];
-        a.out[row] = answer(token >= 0 && token < n ? as_float(x[token]) : -INFINITY, token);
+        if (!kAhead) token_at(token, asked);
+        a.out[row] = answer(asked, token);
         if (a.entropy != nullptr) a.entropy[row] = s.status != 0 ? undefined() : none || greedy ? 0.0f : static_cast<float>(entropy > 0.0 ? entropy : 0.0);
     }
     if (threadIdx.x < static_cast<unsigned>(a.top)) {
@@ -453,7 +479,7 @@ struct Launcher {
 template <typename T>
 cudaError_t launch(const LogprobsArgs &a, bool overlap, cudaStream_t stream) {
     // As many blocks of 512 threads per row as all rows have room for side by side, of at least 4096 elements each.  With more rows, or short ones, what counts is how many
-    // rows at different steps an SM holds: five blocks of 256 threads.  (151936, fp32, 20 alternatives: 149 rows 33 us and 48, 300 rows 59 and 56; 300 rows of 5000 11 and 7.)
+    // rows at different steps an SM holds: five blocks of 256 threads.  (151936, fp32, 20 alternatives: 149 rows 30 us and 48, 300 rows 59 and 56; 300 rows of 5000 11 and 7.)
     for (int blocks = kMaxBlocks; blocks > 0; blocks /= 2)
         if (a.vocab >= (blocks > 1 ? blocks : 2) * 4096 && a.rows <= Launcher<T, true>::fit(blocks)) return Launcher<T, true>::launch(a, blocks, overlap, stream);
     return Launcher<T, false>::launch(a, 1, overlap, stream);
