@@ -9,7 +9,7 @@
 // n candidates each finds its own place, by counting those before it.  Rows where more tie than the list holds take a pass for each alternative.
 // Rows of infinite or extreme logits, and extreme temperatures, are summed in 64 bits by one block.
 //
-// What bounds it.  Many rows: memory, and for fp16 the instructions as well (issue slots 61 %; the exponentials, 16 a cycle of an SM, 69 us of the 126).  2048 x 151936: fp32 185 us without
+// What bounds it.  Many rows: memory, and for fp16 the instructions as well (issue slots 51 %; the exponentials, 16 a cycle of an SM, 69 us of the 126).  2048 x 151936: fp32 185 us without
 // alternatives (6.7 TB/s) and 219 with 20, fp16 109 (5.7) and 126 with one.  Few rows: the steps, each of which waits for the one before: 1 x 151936 5.2 us, 10.3 with 20
 // alternatives, by one cluster of 16 blocks (more would have to meet in device memory).
 #include <cuda_fp16.h>
