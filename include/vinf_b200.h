@@ -239,7 +239,8 @@ int vqm_qmm_f8(vqm_runtime *rt, const char *weight, const char *q, const char *s
  * infinite: all tokens that are not masked are equally likely.  Logits of -inf and NaN are masked; of a row's infinite logits each is equally likely and all others
  * have none.  A row with nothing but masked logits has -inf, entropy 0 and ids -1.  Where a kernel of the runtime has given up a bounded wait that nobody has
  * been told of yet, the logits may not be complete: out, entropy and top_out are NaN, ids -1.
- * Sums are fp32 (rows with infinite, undefined or extreme values or temperatures: 64 bits).  A call whose outputs overlap one another or its inputs in
+ * Sums are fp32 (rows with infinite, undefined or extreme values or temperatures: 64 bits); the likeliest token's own part of a row's sum is kept apart, so that next to
+ * certainty log probabilities and entropies are as exact, relative to themselves, as elsewhere.  Exponentials below 2^-126 count as nothing.  A call whose outputs overlap one another or its inputs in
  * device memory is refused (VQM_ERR_VALUE).  vocab <= VQM_MAX_VOCAB.  Asynchronous. */
 #define VQM_MAX_TOP 32
 int vqm_logprobs(vqm_runtime *rt, const char *logits, const char *tokens, const char *temperature, int vocab, int rows, int top, const char *out,

@@ -2,16 +2,18 @@
 //   out = log p(token),   entropy = - sum p log p,   the `top` largest logits, of equal ones the lowest place first.
 //
 // One pass over a row, in vectors of 16 bytes: each thread keeps the largest logit m it has seen, S = sum exp((l - m) / T) and U = sum exp((l - m) / T) (l - m); a new largest
-// scales both.  Then  log p(t) = (l_t - m) / T - log S  and  entropy = log S - U / (S T).  A row is a block's, or shared by the blocks of a cluster where there are few rows;
+// scales both.  Then  log p(t) = (l_t - m) / T - log S  and  entropy = log S - U / (S T).  The exponential of m itself, 1, is never added to the others: of a token that is all
+// but certain the answers are what the others come to, log S = log(1 + (S - 1)).  So a thread keeps what came with its m (16 or 32 logits) apart from the rest of S, and the
+// warp that has the row's m reads those logits again.  A row is a block's, or shared by the blocks of a cluster where there are few rows;
 // sums and alternatives meet in distributed shared memory, and nothing is kept in device memory.
 // The alternatives need no second pass: the `top`-th largest of the maxima of 32 groups of threads is no more than the `top`-th largest logit, because so many groups each hold
 // one that is no less.  Only threads whose own largest reaches it (31 of 512 on average for 20 alternatives) hold candidates, and what they have read is read again.  Of
 // n candidates each finds its own place, by counting those before it.  Rows where more tie than the list holds take a pass for each alternative.
 // Rows of infinite or extreme logits, and extreme temperatures, are summed in 64 bits by one block.
 //
-// What bounds it.  Many rows: memory, and for fp16 the instructions as well (issue slots 51 %; the exponentials, 16 a cycle of an SM, 69 us of the 126).  2048 x 151936: fp32 185 us without
-// alternatives (6.7 TB/s) and 219 with 20, fp16 109 (5.7) and 126 with one.  Few rows: the steps, each of which waits for the one before: 1 x 151936 5.2 us, 10.3 with 20
-// alternatives, by one cluster of 16 blocks (more would have to meet in device memory).
+// What bounds it.  Many rows: memory, and for fp16 the instructions as well (issue slots 51 %; the exponentials, 16 a cycle of an SM, 69 us of the 130).  2048 x 151936: fp32 189 us without
+// alternatives (6.6 TB/s) and 223 with 20, fp16 113 (5.5) and 130 with one; 4 and 5 us less with the largest logit's 1 among the others.  Few rows: the steps, each of which waits
+// for the one before: 1 x 151936 5.7 us, 10.2 with 20 alternatives, by one cluster of 16 blocks (more would have to meet in device memory).
 #include <cuda_fp16.h>
 
 #include "vqm_kernels.h"
@@ -59,16 +61,19 @@ __device__ __forceinline__ float largest(const uint4 (&w)[kUnroll], const __half
 }
 
 struct Sums {
-    float m, s, u;  // the largest so far (kLow: none), S and U
+    float m, u;       // the largest so far (kLow: none), and U
+    float s, with_m;  // S in two parts, the second from the vectors that brought m: those hold a 1, next to which small terms lose their digits
 };
-template <typename T>
-__device__ __forceinline__ float add_vectors(Sums &a, const uint4 (&w)[kUnroll], float c) {  // returns their largest
+template <typename T, int THREADS>
+__device__ __forceinline__ float add_vectors(Sums &a, const uint4 (&w)[kUnroll], int at, float c, int *brought) {  // returns their largest
     const float most = largest(w, static_cast<const T *>(nullptr));
-    if (most > a.m) {
-        const float d = a.m - most, f = ex2(d * c);
-        a.u = f * fmaf(d, a.s, a.u);
-        a.s *= f;
+    const bool more = most > a.m;
+    if (more) {
+        const float d = a.m - most, f = ex2(d * c), s = a.s + a.with_m;
+        a.u = f * fmaf(d, s, a.u);
+        a.s = f * s;
         a.m = most;
+        brought[threadIdx.x] = at;
     }
     const Two minus = two(-a.m, -a.m), cc = two(c, c);
     Two s = 0, u = 0;
@@ -90,25 +95,39 @@ __device__ __forceinline__ float add_vectors(Sums &a, const uint4 (&w)[kUnroll],
     float s0, s1, u0, u1;
     both(s, s0, s1);
     both(u, u0, u1);
-    a.s += s0 + s1;
+    const float here = s0 + s1;
+    if (more) a.with_m = here;
+    else a.s += here;
     a.u += u0 + u1;
     return most;
 }
 
-static_assert(sizeof(float) * kMostWarps * 32 <= sizeof(Key) * kMaxBlocks * kMaxTop);
+template <int THREADS>
 struct Shared {
-    float most[kMostWarps][32];     // largest logits of the threads
+    float most[THREADS / 32][32];   // largest logits of the threads
     float part[2][kMostWarps];
+    int ones[kMostWarps];           // exponentials that are 1
     alignas(16) Key list[kList];    // candidates
-    alignas(16) Key theirs[kMaxBlocks][kMaxTop];  // the blocks' alternatives; before that, the warps' copies of the groups' largest
+    union {
+        struct {
+            alignas(16) float groups[THREADS / 32][32];  // the warps' copies of the groups' largest
+            int brought[THREADS];                        // the first of the vectors that each thread's largest logit came with
+        };
+        Key theirs[THREADS == 512 ? kMaxBlocks : 1][kMaxTop];  // later on: the alternatives of a cluster's blocks
+    };
     Key best[kMaxTop];              // this block's, in order
     Key key[kMostWarps];
     double wide[kMostWarps];
-    float sums[3];                  // this block's m, S and U
+    float sums[4];                  // this block's m, S but for what is 1, U, and how many are 1
     int count;
     unsigned status;
 };
 
+__device__ __forceinline__ float warp_largest(float v) {
+    float m;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xFFFFFFFF;" : "=f"(m) : "f"(v));
+    return m;
+}
 template <int THREADS, typename V, typename F>
 __device__ V over_block(V v, V (&room)[kMostWarps], F &&join) {
     for (int off = 16; off > 0; off >>= 1) v = join(v, __shfl_xor_sync(0xFFFFFFFFu, v, off));
@@ -121,7 +140,7 @@ __device__ V over_block(V v, V (&room)[kMostWarps], F &&join) {
 }
 // The first `want` of s.list[0, n) in order, by the whole block, to s.best; zeros behind the last.  s.list has room for zeros up to a multiple of 4.
 template <int THREADS>
-__device__ __forceinline__ void rank_list(Shared &s, int n, int want) {
+__device__ __forceinline__ void rank_list(Shared<THREADS> &s, int n, int want) {
     if (threadIdx.x < kMaxTop) s.best[threadIdx.x] = 0;
     if (threadIdx.x < 4 && n % 4 != 0 && threadIdx.x >= static_cast<unsigned>(n % 4)) s.list[n / 4 * 4 + threadIdx.x] = 0;
     __syncthreads();
@@ -138,7 +157,7 @@ __device__ __forceinline__ void rank_list(Shared &s, int n, int want) {
 }
 // The same of all of a slice [begin, end), a pass for each.
 template <typename T, int THREADS>
-static __device__ __noinline__ void rank_by_passes(Shared &s, const T *x, int begin, int end, int want) {
+static __device__ __noinline__ void rank_by_passes(Shared<THREADS> &s, const T *x, int begin, int end, int want) {
     Key last = ~0ull;
     for (int k = 0; k < want; ++k) {
         Key most = 0;
@@ -154,20 +173,26 @@ static __device__ __noinline__ void rank_by_passes(Shared &s, const T *x, int be
 }
 // log S and the entropy in 64 bits, by the whole block.
 template <typename T, int THREADS>
-static __device__ __noinline__ void wide_sums(Shared &s, const T *x, int n, float top, double inverse, bool flat, double &log_sum, double &entropy) {
-    double sum = 0.0, weighted = 0.0;
+static __device__ __noinline__ void wide_sums(Shared<THREADS> &s, const T *x, int n, float top, double inverse, bool flat, double &log_sum, double &entropy) {
+    double sum = 0.0, weighted = 0.0, ones = 0.0;
     for (int i = threadIdx.x; i < n; i += THREADS) {
         const float v = as_float(x[i]);
         if (!(v > -INFINITY)) continue;
-        const double d = v == top || flat ? 0.0 : top == INFINITY ? -INFINITY : (static_cast<double>(v) - static_cast<double>(top)) * inverse, e = exp(d);
+        if (v == top || flat) {
+            ones += 1.0;
+            continue;
+        }
+        const double d = top == INFINITY ? -INFINITY : (static_cast<double>(v) - static_cast<double>(top)) * inverse, e = exp(d);
         sum += e;
         if (e > 0.0) weighted -= e * d;
     }
     auto plus = [](double p, double q) { return p + q; };
     sum = over_block<THREADS>(sum, s.wide, plus);
     weighted = over_block<THREADS>(weighted, s.wide, plus);
-    log_sum = sum > 0.0 ? log(sum) : 0.0;
-    entropy = sum > 0.0 ? log_sum + weighted / sum : 0.0;
+    ones = over_block<THREADS>(ones, s.wide, plus);
+    const double rest = ones - 1.0 + sum;
+    log_sum = ones > 0.0 ? log1p(rest) : 0.0;
+    entropy = ones > 0.0 ? log_sum + weighted / (1.0 + rest) : 0.0;
 }
 
 __device__ __forceinline__ uint32_t in_cluster(const void *p, int block) {
@@ -192,7 +217,7 @@ __device__ __forceinline__ void sync_cluster() {
 
 template <typename T, int THREADS, int PER_SM>
 __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const LogprobsArgs a, const int n_blocks) {
-    __shared__ Shared s;
+    __shared__ Shared<THREADS> s;
     __shared__ float part_room[kParts * THREADS];
     constexpr int VEC = kVec<T>, WARPS = THREADS / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = a.vocab;
@@ -228,7 +253,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const Logprob
     const int per_part = (end - begin + kParts * kUnroll * THREADS - 1) / (kParts * kUnroll * THREADS);  // turns of the loop
     const int want = a.top > 0 ? a.top : greedy ? 1 : 0;
     float(*const part_most)[THREADS] = reinterpret_cast<float(*)[THREADS]>(part_room);
-    Sums sums{kLow, 0.0f, 0.0f};
+    Sums sums{kLow, 0.0f, 0.0f, 0.0f};
     float in_part = -INFINITY;
     int part = 0, turn = 0;
 #pragma unroll 1
@@ -244,7 +269,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const Logprob
                 else w[i] = make_uint4(kNothing<T>, kNothing<T>, kNothing<T>, kNothing<T>);
             }
         }
-        in_part = fmaxf(in_part, add_vectors<T>(sums, w, c));
+        in_part = fmaxf(in_part, add_vectors<T, THREADS>(sums, w, v, c, s.brought));
         if (want > 0 && ++turn == per_part) {
             part_most[part++][threadIdx.x] = in_part;
             in_part = -INFINITY;
@@ -259,23 +284,32 @@ __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const Logprob
     float mine = s.most[0][lane];
 #pragma unroll
     for (int w = 1; w < WARPS; ++w) mine = fmaxf(mine, s.most[w][lane]);
-    float all = mine;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, off));
-    const float f = ex2((sums.m - all) * c);
-    float sum = sums.s * f, weighted = f * fmaf(sums.m - all, sums.s, sums.u);
+    const float all = warp_largest(mine);
+    // The largest logit's 1 is counted, not added; its thread's warp adds up again what it came with.
+    const bool largest_here = sums.m == all && all > kLow;
+    const float f = ex2((sums.m - all) * c), held = sums.s + sums.with_m;
+    float sum = largest_here ? sums.s : held * f, weighted = f * fmaf(sums.m - all, held, sums.u);
+    int ones = 0;
+    for (unsigned with = __ballot_sync(0xFFFFFFFFu, largest_here); with != 0; with &= with - 1)
+        if (lane < kUnroll * VEC) {
+            const int vector = s.brought[warp * 32 + __ffs(with) - 1] + lane / VEC * THREADS, i = first + vector * VEC + lane % VEC;
+            const float v = vector < end && i >= 0 && i < n ? as_float(x[i]) : -INFINITY;
+            if (v == all) ++ones;
+            else sum += ex2(fmaxf(v - all, kLow) * c);
+        }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
         sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
         weighted += __shfl_xor_sync(0xFFFFFFFFu, weighted, off);
     }
-    if (lane == 0) s.part[0][warp] = sum, s.part[1][warp] = weighted;
+    ones = __reduce_add_sync(0xFFFFFFFFu, ones);
+    if (lane == 0) s.part[0][warp] = sum, s.part[1][warp] = weighted, s.ones[warp] = ones;
 
     if (want > 0) {
         // The want-th largest group: the largest value that so many reach.  Where that is out of what the sums tell apart, all logits are candidates.
         float least = all;
         if (want > 1) {
-            float *const group = reinterpret_cast<float *>(s.theirs) + warp * 32;
+            float *const group = s.groups[warp];
             group[lane] = mine;
             __syncwarp();
             int reach = 0;
@@ -284,9 +318,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const Logprob
                 const float4 g = *reinterpret_cast<const float4 *>(group + j);
                 reach += (g.x >= mine) + (g.y >= mine) + (g.z >= mine) + (g.w >= mine);
             }
-            least = reach >= want ? mine : -INFINITY;
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) least = fmaxf(least, __shfl_xor_sync(0xFFFFFFFFu, least, off));
+            least = warp_largest(reach >= want ? mine : -INFINITY);
         }
         const bool any = !(least > kLow);
         if (any) least = -INFINITY;
@@ -335,12 +367,13 @@ __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const Logprob
     }
     if (warp == 0) {
         float p = lane < WARPS ? s.part[0][lane] : 0.0f, q = lane < WARPS ? s.part[1][lane] : 0.0f;
+        const int o = __reduce_add_sync(0xFFFFFFFFu, lane < WARPS ? s.ones[lane] : 0);
 #pragma unroll
         for (int off = 8; off > 0; off >>= 1) {
             p += __shfl_xor_sync(0xFFFFFFFFu, p, off);
             q += __shfl_xor_sync(0xFFFFFFFFu, q, off);
         }
-        if (lane == 0) s.sums[0] = all, s.sums[1] = p, s.sums[2] = q;
+        if (lane == 0) s.sums[0] = all, s.sums[1] = p, s.sums[2] = q, s.sums[3] = static_cast<float>(o);
     }
     if (n_blocks > 1) {
         sync_cluster();
@@ -354,23 +387,25 @@ __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const Logprob
 
     // The first block joins the others' sums (every warp for itself) and alternatives.
     float top = kLow;
-    double total = 0.0, product = 0.0;
+    double rest = 0.0, product = 0.0;  // S - 1, U
     {
-        float m = kLow, p = 0.0f, q = 0.0f;
+        float m = kLow, p = 0.0f, q = 0.0f, o = 0.0f;
         if (lane < n_blocks) {
             const uint32_t at = in_cluster(s.sums, lane);
-            m = load_float(at), p = load_float(at + 4), q = load_float(at + 8);
+            m = load_float(at), p = load_float(at + 4), q = load_float(at + 8), o = load_float(at + 12);
         }
         top = m;
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
         const float g = ex2((m - top) * c);
-        total = static_cast<double>(p * g), product = static_cast<double>(g * fmaf(m - top, p, q));
+        product = static_cast<double>(g * fmaf(m - top, p + o, q));
+        rest = m == top ? static_cast<double>(p) : static_cast<double>((p + o) * g);
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) {
-            total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
+            rest += __shfl_xor_sync(0xFFFFFFFFu, rest, off);
             product += __shfl_xor_sync(0xFFFFFFFFu, product, off);
         }
+        rest += static_cast<double>(static_cast<int>(__reduce_add_sync(0xFFFFFFFFu, m == top ? static_cast<int>(o) : 0)) - 1);
     }
     if (want > 0 && n_blocks > 1) {
         // Of lists in order, if r of them have a q-th key no less than some key, and r q is `want` at least, what is under that key is not asked for.
@@ -409,8 +444,8 @@ __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const Logprob
     if (greedy) {
         none = s.best[0] == 0;
     } else if (in_reach && ordinary) {
-        log_sum = log(total);
-        entropy = log_sum - product / (total * static_cast<double>(given));
+        log_sum = log1p(rest);
+        entropy = log_sum - product / ((1.0 + rest) * static_cast<double>(given));
     } else {
         if (!in_reach) {  // the largest as it is
             float m = -INFINITY;
