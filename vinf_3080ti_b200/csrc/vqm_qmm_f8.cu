@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
     __shared__ __align__(8) uint64_t s_full[kMaxStages], s_empty[kMaxStages], s_acc_full[HALVES][BUFS], s_acc_empty[HALVES][BUFS], s_sums[kWriters];
     __shared__ __align__(16) float s_scales[TURNED ? 1 : kWriters][2][TURNED ? 4 : CW];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_failed, s_issued;
+    __shared__ int s_failed;
     const uint32_t ring = (s32(ring_raw) + 1023u) & ~1023u;  // (the swizzle works on address bits)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t in_cluster = 0;
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
                 bar_init(s32(&s_acc_empty[h][b]), kWriters / HALVES * GROUP);
             }
         for (int w = 0; w < kWriters; ++w) bar_init(s32(&s_sums[w]), 1);
-        s_failed = s_issued = 0;
+        s_failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 2) {
@@ -411,7 +411,13 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
                         if (++stage == a.stages) stage = 0, parity ^= 1;
                     }
                 }
-                s_issued = issued;
+                // The last copies land before the block goes on to its end, or in a cluster says that others may: whatever waits have given up, none comes to memory that is
+                // somebody else's by then.  In the second block of a pair, whose copies are counted in the first, the MMAs' having read them says so; where those have given
+                // up, the time that this takes to give up too.
+                const uint32_t landed = rank == 0 ? s32(&s_full[0]) : s32(&s_empty[0]);
+                int left = 1 << 16;
+                for (int last = max(0, issued - a.stages); last < issued; ++last)
+                    while (!bar_test(landed + last % a.stages * 8, (last / a.stages) & 1) && --left > 0) __nanosleep(64);
             }
             __syncwarp();
         } else if (warp == 1 || (PAIR && warp == 3)) {
@@ -426,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
                     for (int k = k0; k < k1; ++k, ++done) {
                         const uint32_t full = s32(&s_full[stage]);
                         const int buf = done % BUFS;
-                        ok = wait<false>(full, parity, failed);
+                        ok = !stalled(part, done) && wait<false>(full, parity, failed);
                         if (ok && done >= BUFS) ok = wait<false>(s32(&s_acc_empty[part_of][buf]), (done / BUFS - 1) & 1, failed);
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -572,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
             const int first_owner = writer % a.split;
             auto free_room = [&](int c) { return room + static_cast<uint32_t>((c * of_column + writer / a.split) * (a.split - 1)) * 1024; };  // (once this warp has read what came)
             auto room_of = [&](int c, int from, int owner) { return room + static_cast<uint32_t>((c * of_column + writer / a.split) * (a.split - 1) + (from < owner ? from : from - 1)) * 1024 + lane * 16; };
-            if (a.exchange == 0) cluster_sync();  // every block's MMAs are done with its stages, where the sums go
+            if (a.exchange == 0) cluster_sync();  // every block's MMAs are done with its stages, where the sums go (in one that has given up, no copy is on its way)
             int mine = 0, next = first_owner;
             auto owner_next = [&] {  // of unit 0, 1, ...
                 const int owner = next;
@@ -673,12 +679,6 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (s_failed && threadIdx.x == 0 && rank == 0) {  // whichever wait gave up: the last copies land before the block (the pair) may leave (this wait has a limit too)
-        int left = 1 << 16;
-        for (int last = max(0, s_issued - a.stages); last < s_issued; ++last)
-            while (!bar_try(s32(&s_full[last % a.stages]), (last / a.stages) & 1) && --left > 0) __nanosleep(64);
-    }
-    __syncwarp();
     // no block's shared or tensor memory goes away under another
     if constexpr (SPLIT) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     else if constexpr (PAIR) cluster_sync();

@@ -14,6 +14,13 @@ constexpr int kQCols = 128;  // columns of a stage
 
 using tc::bar_arrive, tc::bar_init, tc::bar_try, tc::bar_try_cluster, tc::in_block, tc::s32;
 
+// A test has one part of a tile's columns multiply no more than the first block of them, so that waits run out.
+#ifdef VQM_STALLED_PART
+__device__ __forceinline__ bool stalled(int part, int done) { return part == VQM_STALLED_PART && done >= 1; }
+#else
+__device__ __forceinline__ constexpr bool stalled(int, int) { return false; }
+#endif
+
 // Bounded; false once this or another wait of the block has given up.  A wait that succeeds looks at nothing but its barrier: the loops below have some
 // 500 cycles per stage.
 template <bool CLUSTER>
