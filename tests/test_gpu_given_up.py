@@ -80,10 +80,21 @@ def results(tmp_path, kernel, stalled, sizes):
 F8_SIZES = [(1024, 5120, 4, 1), (1024, 17408, 4, 0), (1000, 5120, 30, 1), (1024, 17408, 50, 1), (1024, 17408, 128, 1), (1001, 17408, 128, 0), (5120, 17408, 256, 1)]
 
 
-def test_a_launch_that_gives_up_ends_and_leaves_the_next_as_it_is(tmp_path):
-    for (rows, ntok), first, second in results(tmp_path, "vqm_qmm_f8.cu", 1, F8_SIZES):
+@pytest.fixture(scope="module")
+def second_part_stalls(tmp_path_factory):
+    return results(tmp_path_factory.mktemp("f8"), "vqm_qmm_f8.cu", 1, F8_SIZES)
+
+
+def test_a_launch_that_gives_up_ends_and_leaves_the_next_as_it_is(second_part_stalls):
+    for (rows, ntok), first, second in second_part_stalls:
         assert first[:2] == (0, 1)
         assert second == (0, 0, 0, 40000 * ntok, 0)
+
+
+def test_sums_that_a_part_has_given_up_reach_no_output(second_part_stalls):
+    """Every output needs that part's: all of them are as they were."""
+    for (rows, ntok), first, _ in second_part_stalls:
+        assert first == (0, 1, rows * ntok, 0, 0), (rows, ntok)
 
 
 def test_blocks_that_share_no_columns_write_nothing_once_they_have_given_up(tmp_path):

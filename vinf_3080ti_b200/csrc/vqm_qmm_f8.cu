@@ -579,6 +579,7 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
             auto free_room = [&](int c) { return room + static_cast<uint32_t>((c * of_column + writer / a.split) * (a.split - 1)) * 1024; };  // (once this warp has read what came)
             auto room_of = [&](int c, int from, int owner) { return room + static_cast<uint32_t>((c * of_column + writer / a.split) * (a.split - 1) + (from < owner ? from : from - 1)) * 1024 + lane * 16; };
             if (a.exchange == 0) cluster_sync();  // every block's MMAs are done with its stages, where the sums go (in one that has given up, no copy is on its way)
+            const bool whole = __all_sync(0xFFFFFFFFu, ok);  // else nothing is sent, and who waits for it gives up too
             int mine = 0, next = first_owner;
             auto owner_next = [&] {  // of unit 0, 1, ...
                 const int owner = next;
@@ -592,6 +593,7 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
                     ++mine;
                     continue;
                 }
+                if (!whole) continue;
                 // stores that count their bytes on a barrier of the block that they go to
                 const int block = owner * GROUP + rank;
                 const uint32_t to = in_block(room_of(c, part, owner), block), there = in_block(bar, block);
@@ -633,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, CW <= 16 ? 2 : 1) qmm_f8_kernel(cons
                 if (lane == 0) expect(bar, static_cast<uint32_t>(mine * (a.split - 1)) * 1024);
                 const bool there = wait<true>(bar, 0, failed);  // (by every lane: it reads what others have stored)
                 __syncwarp();
-                if (__all_sync(0xFFFFFFFFu, there && ok && !*failed)) {
+                if (__all_sync(0xFFFFFFFFu, there && whole && !*failed)) {
                     next = first_owner;
 #pragma unroll
                     for (int c = 0; c < CW / 8; ++c) {
