@@ -101,3 +101,9 @@ def test_blocks_that_share_no_columns_write_nothing_once_they_have_given_up(tmp_
     for (rows, ntok), first, second in results(tmp_path, "vqm_qmm_f8.cu", 0, [(1024, 5120, 4, 1), (1024, 17408, 128, 1), (5120, 17408, 256, 1)]):
         assert first[:2] == (0, 1)
         assert second == (0, 1, 40000 * ntok, 0, 0)
+
+
+def test_the_same_of_8_bit_integers(tmp_path):
+    for (rows, ntok), first, second in results(tmp_path, "vqm_qmm_i8.cu", 1, [(1024, 5120, 4, 1), (1000, 17408, 50, 1), (1024, 17408, 200, 0), (1024, 17408, 300, 1)]):
+        assert first == (0, 1, rows * ntok, 0, 0), (rows, ntok)
+        assert second == (0, 0, 0, 40000 * ntok, 0)

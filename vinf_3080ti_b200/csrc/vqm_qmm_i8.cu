@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
                 const uint32_t acc = tmem + buf * a.acc_cols;
                 for (int k = k0; k < k1; ++k) {
                     const uint32_t full = s32(&s_full[stage]);
-                    ok = PAIR && rank == 0 ? wait<true>(full, parity, failed) : wait<false>(full, parity, failed);
+                    ok = !stalled(part, k - k0) && (PAIR && rank == 0 ? wait<true>(full, parity, failed) : wait<false>(full, parity, failed));
                     if (!ok) break;
                     if (rank == 0) {
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -296,11 +296,12 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
         place(cluster, row_tile, tok_tile);
         const int row = (row_tile * GROUP + rank) * kQRows + lanes * 32 + lane;
         float w_scale = 0.0f;
+        bool whole = false;  // else nothing is sent, and who waits for it gives up too
         if (warp >= 4) {
             if (row < a.rows) w_scale = __ldg(a.w_scales + row);
             asm volatile("griddepcontrol.wait;" ::: "memory");
             fetch_scales(a, tok_tile * a.n, s_scales[0]);
-            (void)warp_wait(s32(&s_acc_full[0]), 0, failed);
+            whole = warp_wait(s32(&s_acc_full[0]), 0, failed);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
         const uint32_t sums = s32(&s_sums), room = ring + a.exchange;
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
         if (warp >= 4) {
             for (int c = half; c < a.n / 8; c += 2) {
                 const int unit = c * 4 + lanes, owner = unit % a.split;
-                if (owner == part) continue;
+                if (owner == part || !whole) continue;
                 int v[8];
                 load_sums(at + c * 8, v);
                 loaded();
@@ -341,7 +342,7 @@ __global__ void __launch_bounds__(kQThreads, PAIR ? 1 : 2) qmm_i8_kernel(const _
                     const uint4 x = lds128u(from), z = lds128u(from + 512);
                     v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += z.x, v[5] += z.y, v[6] += z.z, v[7] += z.w;
                 }
-                if (ok && !*failed) write_any(a, v, row, tok_tile * a.n + c * 8, w_scale, s_scales[0] + c * 8);
+                if (ok && whole && !*failed) write_any(a, v, row, tok_tile * a.n + c * 8, w_scale, s_scales[0] + c * 8);
             }
         }
     }
