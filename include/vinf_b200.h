@@ -226,7 +226,8 @@ int vqm_convert_f8(vqm_runtime *rt, const char *weight, const char *name);
 int vqm_rows_f8(vqm_runtime *rt, const char *x, const char *q, const char *scales, int cols, int ntok, int flags, const char *x2, const char *residual,
                 const char *total, const char *norm_weight, float eps);
 /* y[t][r] = sum over blocks b of 128 columns of scales[b][t] * W scales[r / 128][b] * sum_k q[t][k] w[r][k] (VQM_FUSE_ADD: +=).  Products are exact, a block's
- * sum is fp32, as is the sum over the blocks, whose grouping depends on the sizes of the call; y is an fp32 or fp16 buffer; a call whose y overlaps q, the scales
+ * sum is fp32, as is the sum over the blocks, whose grouping depends on the sizes of the call.  The two scales are multiplied with one another first, in fp32: every block's
+ * product of scales is to be 0 or between 2^-126 and 2^128; what is smaller loses digits, what is larger is infinite (undefined for a block whose sum is 0).  y is an fp32 or fp16 buffer; a call whose y overlaps q, the scales
  * or the weights in device memory is refused (VQM_ERR_VALUE).  Asynchronous. */
 int vqm_qmm_f8(vqm_runtime *rt, const char *weight, const char *q, const char *scales, const char *y, int ntok, int flags);
 
