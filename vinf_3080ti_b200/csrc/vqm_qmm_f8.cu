@@ -38,7 +38,7 @@ namespace {
 constexpr int kRows = 128;                  // rows of a block's first operand, the lanes of tensor memory
 constexpr int kABytes = kRows * kQCols;     // of a stage
 constexpr int kMaxStages = 12, kMaxCluster = 8;
-constexpr int kRing = 216 * 1024, kHalfRing = 106 * 1024, kTurnedRing = 160 * 1024, kBox = 4096, kStaging = 2 * kBox;  // (a warp's, for outputs of pairs)
+constexpr int kRing = 216 * 1024, kHalfRing = 106 * 1024, kTurnedRing = 160 * 1024, kBox = 4096, kStaging = 2 * kBox;  // (a warp's, for outputs on their way)
 constexpr int kWriters = 8, kThreads = 128 + 32 * kWriters;
 // Registers of a thread: a pair's writers hold 128 sums and two sets of 16 that come from tensor memory.  The shares add up to what the block is launched with.
 constexpr int kWriterRegs = 224, kOtherRegs = 56, kLaunchRegs = 168;
@@ -56,7 +56,7 @@ struct QmmF8 {
     int exchange;                      // where in the ring's memory they leave sums for one another, if not where the stages are (0)
     int y_elem, add;
     int half_sm;                       // two blocks per SM
-    int tile_out;                      // pairs: outputs go out by TMA
+    int tile_out;                      // TURNED: outputs go out by TMA
 };
 template <bool TURNED>
 struct Maps {
@@ -792,7 +792,7 @@ cudaError_t launch(QmmF8 a, const QmmF8Args &in, cudaStream_t stream) {
     cudaError_t err = encode_rows(&maps.w, in.w, in.cols, in.w_pitch, in.rows, PAIR ? kRows / 2 : kRows);
     if (err == cudaSuccess) err = encode_rows(&maps.q, in.q, in.cols, f8_pitch(in.cols), in.ntok, TURNED ? kRows : 2 * CW);
     if constexpr (TURNED) {
-        a.tile_out = !in.add && static_cast<long long>(in.rows) * in.y_elem % 16 == 0;
+        a.tile_out = a.split == 1 && !in.add && static_cast<long long>(in.rows) * in.y_elem % 16 == 0;
         if (a.tile_out && err == cudaSuccess) err = encode_outputs(&maps.y, in.y, in.rows, in.ntok, in.y_elem);
     }
     if (err != cudaSuccess) return err;
