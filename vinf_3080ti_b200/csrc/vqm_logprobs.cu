@@ -285,18 +285,17 @@ __global__ void __launch_bounds__(THREADS, PER_SM) logprobs_kernel(const Logprob
 #pragma unroll
     for (int w = 1; w < WARPS; ++w) mine = fmaxf(mine, s.most[w][lane]);
     const float all = warp_largest(mine);
-    // The largest logit's 1 is counted, not added; its thread's warp adds up again what it came with.
-    const bool largest_here = sums.m == all && all > kLow;
+    // The largest logit's 1 is counted, not added; its thread's warp adds up again what it came with.  (Of several such threads one in each warp: with two ones nothing is certain.)
+    const int owner = __ffs(__ballot_sync(0xFFFFFFFFu, sums.m == all && all > kLow)) - 1;
     const float f = ex2((sums.m - all) * c), held = sums.s + sums.with_m;
-    float sum = largest_here ? sums.s : held * f, weighted = f * fmaf(sums.m - all, held, sums.u);
+    float sum = lane == owner ? sums.s : held * f, weighted = f * fmaf(sums.m - all, held, sums.u);
     int ones = 0;
-    for (unsigned with = __ballot_sync(0xFFFFFFFFu, largest_here); with != 0; with &= with - 1)
-        if (lane < kUnroll * VEC) {
-            const int vector = s.brought[warp * 32 + __ffs(with) - 1] + lane / VEC * THREADS, i = first + vector * VEC + lane % VEC;
-            const float v = vector < end && i >= 0 && i < n ? as_float(x[i]) : -INFINITY;
-            if (v == all) ++ones;
-            else sum += ex2(fmaxf(v - all, kLow) * c);
-        }
+    if (owner >= 0 && lane < kUnroll * VEC) {
+        const int vector = s.brought[warp * 32 + owner] + lane / VEC * THREADS, i = first + vector * VEC + lane % VEC;
+        const float v = vector < end && i >= 0 && i < n ? as_float(x[i]) : -INFINITY;
+        if (v == all) ones = 1;
+        else sum += ex2(fmaxf(v - all, kLow) * c);
+    }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
         sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
