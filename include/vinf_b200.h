@@ -237,7 +237,8 @@ int vqm_qmm_f8(vqm_runtime *rt, const char *weight, const char *q, const char *s
  *   top_ids [rows][top] (int32) = the `top` largest logits' places, in descending order, of equal ones the lowest first, and top_out [rows][top] (fp32, NULL: not
  *   wanted) their log probabilities; -1 and -inf where a row has fewer that are not masked.  0 <= top <= VQM_MAX_TOP.
  * temperature [rows] (NULL: 1) as in vqm_verify: T <= 0 (or NaN): p is 1 at the row's largest logit, the lowest index on ties; T above 1e30 counts as
- * infinite: all tokens that are not masked are equally likely.  Logits of -inf and NaN are masked; of a row's infinite logits each is equally likely and all others
+ * infinite: all tokens that are not masked are equally likely.  Logits of -inf and NaN are masked, finite ones never (where fewer than `top`
+ * others are left, that takes a pass over the row for each alternative); of a row's infinite logits each is equally likely and all others
  * have none.  A row with nothing but masked logits has -inf, entropy 0 and ids -1.  Where a kernel of the runtime has given up a bounded wait that nobody has
  * been told of yet, the logits may not be complete: out, entropy and top_out are NaN, ids -1.
  * Sums are fp32 (rows with infinite, undefined or extreme values or temperatures: 64 bits); the likeliest token's own part of a row's sum is kept apart, so that next to
